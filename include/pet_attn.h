@@ -344,6 +344,40 @@ PET_ATTN_API int pet_norm_rows_bwd(int rows, int width, float* in_adj, int64_t l
                                    const float* out_adj, int64_t ldg, const float* in, int64_t ldi,
                                    const float* weight, int ln, void* stream);
 
+/* ---- the norm for training: rows in 16 bits, the parameters' gradients ------ */
+
+/* An element type of rows, and of tensors of gradients. */
+enum { PET_DTYPE_F32 = 0, PET_DTYPE_BF16 = 1, PET_DTYPE_F16 = 2 };
+
+#define PET_NORM_MAX_WIDTH 16384
+
+/* pet_norm_rows with rows in fp32, bf16 or fp16 (dtype, in's and out's; the
+ * weights fp32, the sums in fp32, one rounding to the type at the end), up to
+ * PET_NORM_MAX_WIDTH wide; any alignment of an element (fp32 to 2048 columns is
+ * pet_norm_rows itself). No counterpart in the reference. */
+PET_ATTN_API int pet_norm_rows_typed(int dtype, int rows, int width, void* out, int64_t ldo, const void* in,
+                                     int64_t ldi, const float* weight, const float* bias, void* stream);
+
+/* Bytes of device workspace pet_norm_rows_grads needs for a weight's or bias's
+ * gradient (none without). */
+PET_ATTN_API size_t pet_norm_rows_grads_workspace(int rows, int width);
+
+/* pet_norm_rows_bwd for training, rows as pet_norm_rows_typed's (in_adj,
+ * out_adj and in of one dtype): in_adj = beta in_adj + the norm's adjoint, and
+ * with it the parameters' gradients,
+ *   weight_adj[d] = beta_w weight_adj[d] + sum over rows of out_adj[r][d] xhat[r][d],
+ *   bias_adj[d]   = beta_w bias_adj[d]   + sum over rows of out_adj[r][d]  (LayerNorm),
+ * in fp32, each sum in a fixed order. in_adj, weight_adj and bias_adj may each
+ * be NULL (not all; bias_adj only with ln nonzero); in_adj may be out_adj or in
+ * (with its leading dimension), and nothing else may overlap. live (device, may
+ * be NULL): only rows < *live count, the rows after are neither read nor written.
+ * workspace 16-byte aligned, its contents nobody's after the call. No
+ * counterpart in the reference, which has no gradients of parameters. */
+PET_ATTN_API int pet_norm_rows_grads(int dtype, int rows, int width, void* in_adj, int64_t lda, float beta,
+                                     const void* out_adj, int64_t ldg, const void* in, int64_t ldi,
+                                     const float* weight, int ln, float* weight_adj, float* bias_adj, float beta_w,
+                                     const int* live, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Bytes of device workspace pet_attention_layer / _layer_bwd need: the
  * normed tokens [T, D] and qkv [T, 3D], with pet_attention_bwd_workspace's,
  * each 256-byte aligned. */
@@ -375,6 +409,32 @@ PET_ATTN_API int pet_attention_layer_bwd(const pet_attn_shape* shape, float* tok
                                          const float* w_in, const float* b_in, const float* cf_seq, int64_t ldc,
                                          const float* w_out, const int* off, const float* merged, const float* ml,
                                          void* workspace, size_t workspace_bytes, void* stream);
+
+/* Where the gradients of an attention layer's parameters go (device, the
+ * parameters' own shapes, fp32, contiguous; NULL: not made, a bias's not
+ * without its weight's), each onto beta times itself. */
+typedef struct pet_layer_grads {
+  float *norm_w, *norm_b; /* [D] (norm_b with a LayerNorm only) */
+  float *w_in, *b_in;     /* [3D, D], [3D] */
+  float *w_out, *b_out;   /* [D, D], [D] */
+  float beta;
+} pet_layer_grads;
+
+/* Bytes of device workspace pet_attention_layer_grads needs. */
+PET_ATTN_API size_t pet_attention_layer_grads_workspace(const pet_attn_shape* shape);
+
+/* pet_attention_layer_bwd with the gradients of the layer's parameters
+ * (pet_linear_grads of the two linears, pet_norm_rows_grads of the norm) over
+ * the live rows: the layer's training backward. tokens_adj and cf_seq_adj as
+ * pet_attention_layer_bwd's (to fp32 roundings: qkv's adjoint is kept in fp32
+ * for w_in's gradient). No counterpart in the reference. */
+PET_ATTN_API int pet_attention_layer_grads(const pet_attn_shape* shape, const pet_layer_grads* grads,
+                                           float* tokens_adj, int64_t lda, float* cf_seq_adj, int64_t ldca,
+                                           const float* out_adj, int64_t ldo, const float* tokens, int64_t ldt,
+                                           const float* norm_w, const float* norm_b, const float* w_in,
+                                           const float* b_in, const float* cf_seq, int64_t ldc, const float* w_out,
+                                           const int* off, const float* merged, const float* ml, void* workspace,
+                                           size_t workspace_bytes, void* stream);
 
 /* ---- the consumer of cf_seq_adj: the forces' edge term --------------------- */
 

@@ -230,6 +230,54 @@ PET_ATTN_API int pet_linear_fused_blocks(int M, int N, int K, const void* Ablock
                                          const float* cin, int64_t ldcin, float beta, float* pre, int64_t ldpre,
                                          int act, void* stream);
 
+/* ---- a dense layer's gradients, a model's gradient norm --------------------- */
+
+/* Bytes of device workspace pet_linear_grads needs. */
+PET_ATTN_API size_t pet_linear_grads_workspace(int dtype, int M, int N, int K);
+
+/* The parameters' gradients of a dense layer out = in W^T + b (W [N, K]) from
+ * its input rows in [M, K] (ld ldi) and its output's adjoint out_adj [M, N] (ld
+ * ldo), both of one dtype (PET_DTYPE_*), at any alignment of an element:
+ *   w_adj[n][k] = beta w_adj[n][k] + sum over m of out_adj[m][n] in[m][k],
+ *   b_adj[n]    = beta b_adj[n]    + sum over m of out_adj[m][n]  (b_adj may be NULL),
+ * fp32 (w_adj ld ldw); beta 0 overwrites. fp32 rows at fp32 accuracy, 16-bit
+ * rows' products exact, the sums in fp32 and in a fixed order. live (device, may
+ * be NULL): only rows m < *live count, the rows after are not read. w_adj and
+ * b_adj overlap nothing; workspace 16-byte aligned, its contents nobody's after
+ * the call. No counterpart in the reference, which has no gradients of parameters. */
+PET_ATTN_API int pet_linear_grads(int dtype, int M, int N, int K, const void* out_adj, int64_t ldo, const void* in,
+                                  int64_t ldi, const int* live, float* w_adj, int64_t ldw, float* b_adj, float beta,
+                                  void* workspace, size_t workspace_bytes, void* stream);
+
+/* One tensor of a list of gradients: rows x cols elements in rows of ld
+ * (consecutive: rows 1), of type dtype (PET_DTYPE_*), at any alignment of an
+ * element. At most 2^36 elements. */
+typedef struct pet_grad_tensor {
+  void* data;
+  int64_t rows, cols, ld;
+  int dtype;
+} pet_grad_tensor;
+
+/* Bytes of device workspace pet_grad_norm and pet_grad_clip need for n tensors. */
+PET_ATTN_API size_t pet_grad_workspace(int n);
+
+/* *norm (device) = |scale| (sum of |g|^p over all elements of the n tensors)^(1/p),
+ * p 1 or 2, or p 0 for the largest |g|; summed in double in a fixed order. The
+ * list is host memory, read before the call returns. A NaN anywhere gives NaN;
+ * no tensors, or empty ones, give 0. workspace 16-byte aligned. No counterpart
+ * in the reference. */
+PET_ATTN_API int pet_grad_norm(const pet_grad_tensor* grads, int n, int p, double scale, float* norm, void* workspace,
+                               size_t workspace_bytes, void* stream);
+
+/* pet_grad_norm, and every g *= scale min(1, max_norm / (norm + eps)) in place,
+ * the factor made on the device in double and rounded to fp32, the product
+ * rounded once to g's type: scale undoes a loss's scale or averages over
+ * micro-batches. An infinite norm scales by 0 (0 for a finite g, NaN for an
+ * infinite one), a NaN by NaN; max_norm infinity does not clip. No two tensors
+ * may overlap. max_norm and eps at least 0, scale finite. */
+PET_ATTN_API int pet_grad_clip(const pet_grad_tensor* grads, int n, int p, double scale, double max_norm, double eps,
+                               float* norm, void* workspace, size_t workspace_bytes, void* stream);
+
 /* FLOPs (2 M N K per product) of the dense products this library's kernels
  * have launched in this process, by the instructions that run them:
  * flops[0] the fp32 fused kernel (fp32 matrix cores), [1] split-fp32 as bf16

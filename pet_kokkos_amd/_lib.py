@@ -63,6 +63,16 @@ EXPORTS = (
     "pet_linear_fused_blocks",
     "pet_norm_rows_pairs",
     "pet_gemm_flop_tally",
+    "pet_norm_rows_typed",
+    "pet_norm_rows_grads_workspace",
+    "pet_norm_rows_grads",
+    "pet_linear_grads_workspace",
+    "pet_linear_grads",
+    "pet_grad_workspace",
+    "pet_grad_norm",
+    "pet_grad_clip",
+    "pet_attention_layer_grads_workspace",
+    "pet_attention_layer_grads",
 )
 
 OK, EINVAL, EHEADDIM, ESLOTS, EALIGN, ELAUNCH, EBLAS, EWORKSPACE, EINDEX, ESCRATCH = range(10)
@@ -114,6 +124,18 @@ class ModelEdges(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int) for n in ("n_atoms", "n_edges", "max_neighbors", "n_struct")] + \
                [(n, ctypes.c_void_p) for n in ("struct_off", "species", "off", "center", "neigh_species", "reverse",
                                                "vec", "dist", "pcut", "cut")]
+
+
+class GradTensor(ctypes.Structure):
+    """pet_grad_tensor (include/pet_model.h)."""
+    _fields_ = [("data", ctypes.c_void_p), ("rows", ctypes.c_int64), ("cols", ctypes.c_int64), ("ld", ctypes.c_int64),
+                ("dtype", ctypes.c_int)]
+
+
+class LayerGrads(ctypes.Structure):
+    """pet_layer_grads (include/pet_attn.h)."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("norm_w", "norm_b", "w_in", "b_in", "w_out", "b_out")] + \
+               [("beta", ctypes.c_float)]
 
 
 class PetAttnError(RuntimeError):
@@ -255,6 +277,29 @@ def load() -> ctypes.CDLL:
     lib.pet_model_pairs_scratch_bytes.argtypes = [_P]
     lib.pet_model_last_tier.restype = ctypes.c_int
     lib.pet_model_last_tier.argtypes = [_P]
+    _Z = ctypes.c_size_t
+    lib.pet_norm_rows_typed.restype = ctypes.c_int
+    lib.pet_norm_rows_typed.argtypes = [_I, _I, _I, _P, _I64, _P, _I64, _P, _P, _P]
+    lib.pet_norm_rows_grads_workspace.restype = _Z
+    lib.pet_norm_rows_grads_workspace.argtypes = [_I, _I]
+    lib.pet_norm_rows_grads.restype = ctypes.c_int
+    lib.pet_norm_rows_grads.argtypes = [_I, _I, _I, _P, _I64, _F, _P, _I64, _P, _I64, _P, _I, _P, _P, _F, _P, _P, _Z,
+                                        _P]
+    lib.pet_linear_grads_workspace.restype = _Z
+    lib.pet_linear_grads_workspace.argtypes = [_I, _I, _I, _I]
+    lib.pet_linear_grads.restype = ctypes.c_int
+    lib.pet_linear_grads.argtypes = [_I, _I, _I, _I, _P, _I64, _P, _I64, _P, _P, _I64, _P, _F, _P, _Z, _P]
+    lib.pet_grad_workspace.restype = _Z
+    lib.pet_grad_workspace.argtypes = [_I]
+    lib.pet_grad_norm.restype = ctypes.c_int
+    lib.pet_grad_norm.argtypes = [ctypes.POINTER(GradTensor), _I, _I, _D, _P, _P, _Z, _P]
+    lib.pet_grad_clip.restype = ctypes.c_int
+    lib.pet_grad_clip.argtypes = [ctypes.POINTER(GradTensor), _I, _I, _D, _D, _D, _P, _P, _Z, _P]
+    lib.pet_attention_layer_grads_workspace.restype = _Z
+    lib.pet_attention_layer_grads_workspace.argtypes = [sp]
+    lib.pet_attention_layer_grads.restype = ctypes.c_int
+    lib.pet_attention_layer_grads.argtypes = [sp, ctypes.POINTER(LayerGrads), _P, _I64, _P, _I64, _P, _I64, _P, _I64,
+                                              _P, _P, _P, _P, _P, _I64, _P, _P, _P, _P, _P, _Z, _P]
     _lib = lib
     return lib
 

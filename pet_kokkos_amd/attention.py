@@ -94,6 +94,68 @@ def _stream() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # PET_DTYPE_*
+
+
+def _typed(t: torch.Tensor, name: str, rows: int, width: int, dtype: torch.dtype, device) -> int:
+    """The leading dimension of a row-major [rows, width] view of the dtype on the device."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: a torch tensor is needed")
+    if t.device != device or t.device.type != "cuda":
+        raise ValueError(f"{name}: on {t.device}, the operands' device is {device}")
+    if t.dtype != dtype or t.dtype not in DTYPES:
+        raise ValueError(f"{name}: {t.dtype}, the rows' type is {dtype} (float32, bfloat16 or float16)")
+    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != width:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {(rows, width)}")
+    if width > 1 and rows > 0 and t.stride(1) != 1:
+        raise ValueError(f"{name} must be a row-major 2-D view")
+    if rows <= 1:
+        return width
+    if t.stride(0) < width:
+        raise ValueError(f"{name}: rows overlap (stride {t.stride(0)} < width {width})")
+    return t.stride(0)
+
+
+def _vector(t: torch.Tensor, name: str, n: int, device) -> int:
+    """The address of a contiguous float32 [n] on the device."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: a torch tensor is needed")
+    if t.device != device or t.dtype != torch.float32 or tuple(t.shape) != (n,) or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous float32 [{n}] on {device}")
+    return t.data_ptr()
+
+
+def _live(t, device):
+    """The address of the device's count of live rows (one int32), None for all."""
+    if t is None:
+        return None
+    if not isinstance(t, torch.Tensor):
+        raise TypeError("live: a torch tensor is needed")
+    if t.device != device or t.dtype != torch.int32 or t.numel() != 1:
+        raise ValueError(f"live must be one int32 on {device}")
+    return t.data_ptr()
+
+
+def _scratch(t, nbytes: int, device) -> torch.Tensor:
+    """A caller's scratch of at least nbytes, or one of this call's own."""
+    if t is None:
+        return torch.empty(max(nbytes, 1), dtype=torch.uint8, device=device)
+    if not isinstance(t, torch.Tensor):
+        raise TypeError("scratch: a torch tensor is needed")
+    if t.device != device or not t.is_contiguous():
+        raise ValueError(f"scratch: a contiguous tensor on {device}")
+    return t
+
+
+def _call_on(device, what: str, fn, *args) -> None:
+    """fn(*args, stream) with the device's current stream, the device current."""
+    if device.index == torch.cuda.current_device():
+        _lib.check(fn(*args, torch.cuda.current_stream(device).cuda_stream), what)
+    else:
+        with torch.cuda.device(device):
+            _lib.check(fn(*args, torch.cuda.current_stream(device).cuda_stream), what)
+
+
 def shape(N: int, T: int, S: int, heads: int, head_dim: int, temperature: float = 1.0,
           dead: bool = False) -> _lib.Shape:
     # pet_attn_scale's own arithmetic, rounded to float by the struct: a call of the

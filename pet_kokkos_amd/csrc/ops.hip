@@ -186,6 +186,15 @@ using namespace pet_attn;
 int pet_rows_norm_bwd_sink(int rows, int width, float* in_adj, int64_t lda, const float* out_adj, int64_t ldg,
                            const float* in, int64_t ldi, const float* weight, int ln, int n_node, float beta_node,
                            float beta_edge, const int* live_off, hipStream_t st);
+// norm_grads.hip: the same with the parameters' gradients; wgrad.hip: the linears'
+int pet_norm_grads_sink(int dtype, int rows, int width, void* in_adj, int64_t lda, const void* out_adj, int64_t ldg,
+                        const void* in, int64_t ldi, const float* weight, int ln, float* w_adj, float* b_adj,
+                        float beta_w, int n_node, float beta_node, float beta_edge, int live_base, const int* live,
+                        void* ws, hipStream_t st);
+size_t pet_linear_grads_bytes(int dtype, int M, int N, int K);
+int pet_linear_grads_run(int dtype, int M, int N, int K, const void* out_adj, int64_t ldo, const void* in, int64_t ldi,
+                         int live_base, const int* live, float* w_adj, int64_t ldw, float* b_adj, float beta, void* ws,
+                         hipStream_t st);
 int pet_rows_rms_inv(int rows, int width, const float* in, int64_t ldi, float* inv, hipStream_t st);
 int pet_rows_fold_cols(float* out, const float* w, const float* s, int rows, int cols, hipStream_t st);
 
@@ -240,12 +249,12 @@ int output_linear(const pet_attn_shape* sh, float* out, int64_t ldo, const float
 }
 
 // attention_bwd with qkv given raw + (rs, b) (pet_attn_bwd_xf), workspace as
-// pet_attention_bwd's.
+// pet_attention_bwd's; keep_qkv_adj: qkv_adj left in it as fp32.
 int attention_bwd_xf(const pet_attn_shape* sh, float* in_adj, int64_t ldi, int d_in, float* cf_seq_adj, int64_t ldca,
                      const float* out_adj, int64_t ldo, const float* qkv, int64_t ldq, const float* rs,
                      const float* b, const float* cf_seq, int64_t ldc, const float* w_in, const float* w_out,
                      const int* off, const float* merged, const float* ml, float beta, char* ws, hipStream_t st,
-                     void* split_out_t, void* split_in_t, bool parts) {
+                     void* split_out_t, void* split_in_t, bool parts, bool keep_qkv_adj = false) {
   const int D = sh->heads * sh->head_dim, T = sh->n_rows;
   float* dmerged = reinterpret_cast<float*>(ws);
   float* qkv_adj = reinterpret_cast<float*>(ws + align256(sizeof(float) * size_t(T) * D));
@@ -260,7 +269,7 @@ int attention_bwd_xf(const pet_attn_shape* sh, float* in_adj, int64_t ldi, int d
   // kernel, with no fp32 qkv_adj and no split pass of it, where the fp16-pair
   // backward takes the shape and the product is large enough for the split
   // kernel (C3 op level on MI355X: see pet_attention_bwd)
-  if (split_in_t && 3 * D >= 256 && (3 * D) % 32 == 0 && double(T) * d_in * 3 * D >= 4294967296.0 && ldi % 4 == 0 &&
+  if (split_in_t && !keep_qkv_adj && 3 * D >= 256 && (3 * D) % 32 == 0 && double(T) * d_in * 3 * D >= 4294967296.0 && ldi % 4 == 0 &&
       (reinterpret_cast<uintptr_t>(in_adj) & 15) == 0) {
     const int rc = pet_attn_bwd_xf_blocks(sh, qkv, ldq, rs, b, off, dmerged, D, merged, D, ml, cf_seq, ldc, qkv_adj,
                                           cfh, cf_seq_adj, ldca, st);
@@ -277,6 +286,75 @@ int attention_bwd_xf(const pet_attn_shape* sh, float* in_adj, int64_t ldi, int d
   se = split_dense(in_adj, ldi, qkv_adj, 3 * D, w_in, d_in, true, T, d_in, 3 * D, nullptr, beta, split_in_t, parts, st);
   if (se >= 0) return se;
   return gemm_nn(in_adj, ldi, qkv_adj, 3 * D, w_in, T, 3 * D, d_in, beta, st);
+}
+
+// The room of a layer's parameters' gradients past pet_attention_layer_workspace: the
+// linears' or the norm's, one after the other.
+size_t layer_grads_bytes(const pet_attn_shape* sh) {
+  const int D = sh->heads * sh->head_dim, T = sh->n_rows;
+  return align256(std::max({pet_linear_grads_bytes(PET_DTYPE_F32, T, D, D),
+                            pet_linear_grads_bytes(PET_DTYPE_F32, T, 3 * D, D), pet_norm_rows_grads_workspace(T, D)}));
+}
+
+// The layer's backward, with its parameters' gradients where asked for (pg).
+int layer_bwd(const pet_attn_shape* sh, const pet_layer_grads* pg, float* tokens_adj, int64_t lda, float* cf_seq_adj,
+              int64_t ldca, const float* out_adj, int64_t ldo, const float* tokens, int64_t ldt, const float* norm_w,
+              const float* norm_b, const float* w_in, const float* b_in, const float* cf_seq, int64_t ldc,
+              const float* w_out, const int* off, const float* merged, const float* ml, void* workspace,
+              size_t workspace_bytes, hipStream_t st) {
+  if (!sh || !tokens_adj || !tokens || !norm_w || !w_in || !off) return PET_ATTN_EINVAL;
+  const int D = sh->heads * sh->head_dim, T = sh->n_rows;
+  if (ldt < D || lda < D) return PET_ATTN_EINVAL;
+  if (pg && (!out_adj || !merged || ldo < D)) return PET_ATTN_EINVAL;
+  const size_t need = pet_attention_layer_workspace(sh);
+  if (!workspace || workspace_bytes < need + (pg ? layer_grads_bytes(sh) : 0)) return PET_ATTN_EWORKSPACE;
+  if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0) return PET_ATTN_EALIGN;
+  char* ws = static_cast<char*>(workspace);
+  const size_t a0 = align256(sizeof(float) * size_t(T) * D), a1 = align256(sizeof(float) * size_t(T) * 3 * D),
+               a2 = align256(sizeof(float) * size_t(T)), a3 = align256(sizeof(float) * 3 * size_t(D) * D);
+  float* normed = reinterpret_cast<float*>(ws);
+  float* qkv = reinterpret_cast<float*>(ws + a0);
+  char* bwd = ws + a0 + a1 + a2 + a3;  // attention_bwd_xf's: dmerged, qkv_adj, ...
+  if (T > 0) {
+    float* inv = nullptr;
+    const float* bq = nullptr;
+    // a weight's split copy at a time (as the forward's), past the backward's workspace
+    char* sp = bwd + pet_attention_bwd_workspace(sh);
+    if (!norm_b) {  // RMSNorm: the fused projection (as the forward's)
+      inv = reinterpret_cast<float*>(ws + a0 + a1);
+      if (int e = layer_input_rms(sh, inv, reinterpret_cast<float*>(ws + a0 + a1 + a2), qkv, tokens, ldt, norm_w, w_in,
+                                  st, sp))
+        return e;
+      bq = b_in;
+    } else if (int e = layer_input(sh, normed, qkv, tokens, ldt, norm_w, norm_b, w_in, b_in, st)) {
+      return e;
+    }
+    // the normed tokens' adjoint overwrites them: the backward reads only qkv
+    if (int e = attention_bwd_xf(sh, normed, D, D, cf_seq_adj, ldca, out_adj, ldo, qkv, 3 * D, inv, bq, cf_seq, ldc,
+                                 w_in, w_out, off, merged, ml, 0.0f, bwd, st, sp, sp, true, pg != nullptr))
+      return e;
+  }
+  if (!pg)
+    return T == 0 ? int(PET_ATTN_OK)
+                  : pet_rows_norm_bwd_sink(T, D, tokens_adj, lda, normed, D, tokens, ldt, norm_w, norm_b != nullptr,
+                                           sh->n_atoms, 0.0f, 1.0f, off, st);
+  const int N = sh->n_atoms;
+  const int* live = off + N;  // rows N + off[N] .. T-1: a capacity's
+  void* gws = ws + need;
+  if (pg->w_out)
+    if (int e = pet_linear_grads_run(PET_DTYPE_F32, T, D, D, out_adj, ldo, merged, D, N, live, pg->w_out, D, pg->b_out,
+                                     pg->beta, gws, st))
+      return e;
+  if (pg->w_in) {
+    // the normed tokens again, in dmerged's place
+    float* again = reinterpret_cast<float*>(bwd);
+    if (int e = pet_norm_rows(T, D, again, D, tokens, ldt, norm_w, norm_b, st)) return e;
+    if (int e = pet_linear_grads_run(PET_DTYPE_F32, T, 3 * D, D, bwd + a0, 3 * D, again, D, N, live, pg->w_in, D,
+                                     pg->b_in, pg->beta, gws, st))
+      return e;
+  }
+  return pet_norm_grads_sink(PET_DTYPE_F32, T, D, tokens_adj, lda, normed, D, tokens, ldt, norm_w, norm_b != nullptr,
+                             pg->norm_w, pg->norm_b, pg->beta, N, 0.0f, 1.0f, N, live, gws, st);
 }
 
 }  // namespace
@@ -474,37 +552,26 @@ int pet_attention_layer_bwd(const pet_attn_shape* sh, float* tokens_adj, int64_t
                             const float* norm_b, const float* w_in, const float* b_in, const float* cf_seq,
                             int64_t ldc, const float* w_out, const int* off, const float* merged, const float* ml,
                             void* workspace, size_t workspace_bytes, void* stream) {
-  if (!sh || !tokens_adj || !tokens || !norm_w || !w_in || !off) return PET_ATTN_EINVAL;
-  const int D = sh->heads * sh->head_dim, T = sh->n_rows;
-  if (ldt < D || lda < D) return PET_ATTN_EINVAL;
-  if (!workspace || workspace_bytes < pet_attention_layer_workspace(sh)) return PET_ATTN_EWORKSPACE;
-  if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0) return PET_ATTN_EALIGN;
-  if (T == 0) return PET_ATTN_OK;
-  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  char* ws = static_cast<char*>(workspace);
-  const size_t a0 = align256(sizeof(float) * size_t(T) * D), a1 = align256(sizeof(float) * size_t(T) * 3 * D),
-               a2 = align256(sizeof(float) * size_t(T)), a3 = align256(sizeof(float) * 3 * size_t(D) * D);
-  float* normed = reinterpret_cast<float*>(ws);
-  float* qkv = reinterpret_cast<float*>(ws + a0);
-  float* inv = nullptr;
-  const float* bq = nullptr;
-  // a weight's split copy at a time (as the forward's), past the backward's workspace
-  char* sp = ws + a0 + a1 + a2 + a3 + pet_attention_bwd_workspace(sh);
-  if (!norm_b) {  // RMSNorm: the fused projection (as the forward's)
-    inv = reinterpret_cast<float*>(ws + a0 + a1);
-    if (int e = layer_input_rms(sh, inv, reinterpret_cast<float*>(ws + a0 + a1 + a2), qkv, tokens, ldt, norm_w, w_in,
-                                st, sp))
-      return e;
-    bq = b_in;
-  } else if (int e = layer_input(sh, normed, qkv, tokens, ldt, norm_w, norm_b, w_in, b_in, st)) {
-    return e;
-  }
-  // the normed tokens' adjoint overwrites them: the backward reads only qkv
-  if (int e = attention_bwd_xf(sh, normed, D, D, cf_seq_adj, ldca, out_adj, ldo, qkv, 3 * D, inv, bq, cf_seq, ldc,
-                               w_in, w_out, off, merged, ml, 0.0f, ws + a0 + a1 + a2 + a3, st, sp, sp, true))
-    return e;
-  return pet_rows_norm_bwd_sink(T, D, tokens_adj, lda, normed, D, tokens, ldt, norm_w, norm_b != nullptr,
-                                sh->n_atoms, 0.0f, 1.0f, off, st);
+  return layer_bwd(sh, nullptr, tokens_adj, lda, cf_seq_adj, ldca, out_adj, ldo, tokens, ldt, norm_w, norm_b, w_in,
+                   b_in, cf_seq, ldc, w_out, off, merged, ml, workspace, workspace_bytes,
+                   reinterpret_cast<hipStream_t>(stream));
+}
+
+size_t pet_attention_layer_grads_workspace(const pet_attn_shape* sh) {
+  return sh ? pet_attention_layer_workspace(sh) + layer_grads_bytes(sh) : 0;
+}
+
+int pet_attention_layer_grads(const pet_attn_shape* sh, const pet_layer_grads* grads, float* tokens_adj, int64_t lda,
+                              float* cf_seq_adj, int64_t ldca, const float* out_adj, int64_t ldo, const float* tokens,
+                              int64_t ldt, const float* norm_w, const float* norm_b, const float* w_in,
+                              const float* b_in, const float* cf_seq, int64_t ldc, const float* w_out, const int* off,
+                              const float* merged, const float* ml, void* workspace, size_t workspace_bytes,
+                              void* stream) {
+  if (!grads || (grads->norm_b && !norm_b) || (grads->b_in && !grads->w_in) || (grads->b_out && !grads->w_out))
+    return PET_ATTN_EINVAL;
+  return layer_bwd(sh, grads, tokens_adj, lda, cf_seq_adj, ldca, out_adj, ldo, tokens, ldt, norm_w, norm_b, w_in, b_in,
+                   cf_seq, ldc, w_out, off, merged, ml, workspace, workspace_bytes,
+                   reinterpret_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"

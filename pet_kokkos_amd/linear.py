@@ -8,6 +8,9 @@ by the same names: linear_fused (out = in W^T + b + beta out), silu_in_fused
 W's rows interleaved value/gate, h = v sigmoid(g)). W is torch Linear's
 [N, K]; every call raises on a bad shape or alignment instead of returning
 false, since there is no other path here to fall back to.
+
+For training, which the reference does not do, ``linear_grads`` makes a dense
+layer's weight and bias gradients (pet_linear_grads).
 """
 from __future__ import annotations
 
@@ -16,6 +19,7 @@ import ctypes
 import torch
 
 from . import _lib
+from .attention import DTYPES, _call_on, _live, _scratch, _typed, _vector
 
 
 class SplitWeights:
@@ -283,3 +287,29 @@ def swiglu_in_fused(pre, h, inp, W, b):
         _call(inp, W, pre, bias=b)
     else:
         _call(inp, W, h, bias=b, pre=pre, act=2)
+
+
+def linear_grads(out_adj, inp, w_adj, b_adj=None, beta=0.0, live=None, scratch=None):
+    """The parameters' gradients of out = inp W^T + b: w_adj [N, K] = beta *
+    w_adj + out_adj^T inp and b_adj [N] (None: not made) = beta * b_adj + the
+    sum of out_adj's rows, from inp [M, K] and out_adj [M, N] of one type
+    (float32, bfloat16 or float16); the gradients are float32. ``live`` (one
+    int32 on the device): only rows before it count, the rows after are not read.
+    ``scratch``: pet_linear_grads_workspace(dtype, M, N, K) bytes, else
+    allocated."""
+    lib = _lib.load()
+    for t, name in ((out_adj, "out_adj"), (inp, "inp"), (w_adj, "w_adj")):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name}: a torch tensor is needed")
+        if t.dim() != 2:
+            raise ValueError(f"{name}: 2-D is needed, not shape {tuple(t.shape)}")
+    (M, N), K, dev, dt = out_adj.shape, inp.shape[1], inp.device, inp.dtype
+    if N < 1 or K < 1:
+        raise ValueError(f"a weight of {N} x {K}")
+    ldo, ldi = _typed(out_adj, "out_adj", M, N, dt, dev), _typed(inp, "inp", M, K, dt, dev)
+    ldw = _typed(w_adj, "w_adj", N, K, torch.float32, dev)
+    b = None if b_adj is None else _vector(b_adj, "b_adj", N, dev)
+    scratch = _scratch(scratch, lib.pet_linear_grads_workspace(DTYPES[dt], M, N, K), dev)
+    _call_on(dev, "pet_linear_grads", lib.pet_linear_grads, DTYPES[dt], M, N, K, out_adj.data_ptr(), ldo,
+             inp.data_ptr(), ldi, _live(live, dev), w_adj.data_ptr(), ldw, b, float(beta), scratch.data_ptr(),
+             scratch.numel() * scratch.element_size())

@@ -1,0 +1,153 @@
+"""The training operators' refusals, without a GPU: every bad argument is
+turned away before any device work (the addresses here are stand-ins)."""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import pytest
+import torch
+
+from pet_kokkos_amd import _lib, grads, layer, linear
+
+A, B, C, W, WS = (4096 * (i + 1) for i in range(5))
+F32, BF16, F16 = 0, 1, 2
+
+
+def norm(dtype=BF16, rows=4, width=8, out=A, ldo=8, inp=B, ldi=8, w=W, b=None):
+    return _lib.load().pet_norm_rows_typed(dtype, rows, width, out, ldo, inp, ldi, w, b, None)
+
+
+def test_norm_refusals():
+    assert norm(dtype=3) == norm(dtype=-1) == _lib.EINVAL
+    assert norm(rows=-1) == norm(width=0) == norm(width=16385, ldo=16385, ldi=16385) == _lib.EINVAL
+    assert norm(out=None) == norm(inp=None) == norm(w=None) == _lib.EINVAL
+    assert norm(ldo=7) == norm(ldi=7) == _lib.EINVAL
+    assert norm(out=A + 1) == norm(inp=B + 1) == _lib.EALIGN  # half an element off
+    assert norm(dtype=F32, out=A + 2) == norm(dtype=F32, inp=B + 1) == _lib.EALIGN
+
+
+def norm_grads(dtype=F32, rows=4, width=8, in_adj=A, lda=8, g=B, ldg=8, x=C, ldx=8, w=W, ln=1, wa=WS, ba=WS, ws=WS,
+               nbytes=1 << 30):
+    return _lib.load().pet_norm_rows_grads(dtype, rows, width, in_adj, lda, 0.0, g, ldg, x, ldx, w, ln, wa, ba, 0.0,
+                                           None, ws, nbytes, None)
+
+
+def test_norm_grads_refusals():
+    lib = _lib.load()
+    assert norm_grads(dtype=7) == norm_grads(rows=-1) == norm_grads(width=0) == _lib.EINVAL
+    assert norm_grads(width=16385, lda=16385, ldg=16385, ldx=16385) == _lib.EINVAL
+    assert norm_grads(g=None) == norm_grads(x=None) == norm_grads(w=None) == _lib.EINVAL
+    assert norm_grads(lda=7) == norm_grads(ldg=7) == norm_grads(ldx=7) == _lib.EINVAL
+    assert norm_grads(in_adj=None, wa=None, ba=None) == _lib.EINVAL  # nothing to make
+    assert norm_grads(ln=0) == _lib.EINVAL  # an RMSNorm's bias
+    assert norm_grads(in_adj=A + 2) == norm_grads(g=B + 1) == norm_grads(x=C + 2) == norm_grads(ws=WS + 4) == _lib.EALIGN
+    assert norm_grads(wa=WS + 2) == norm_grads(w=W + 1) == _lib.EALIGN
+    need = lib.pet_norm_rows_grads_workspace(4, 8)
+    assert need > 0 and norm_grads(ws=None) == norm_grads(nbytes=need - 1) == _lib.EWORKSPACE
+    assert lib.pet_norm_rows_grads_workspace(-1, 8) == lib.pet_norm_rows_grads_workspace(4, 0) == 0
+
+
+def linear_grads(dtype=F32, M=4, N=8, K=16, g=A, ldg=8, x=B, ldx=16, wa=C, ldw=16, ba=W, ws=WS, nbytes=1 << 40):
+    return _lib.load().pet_linear_grads(dtype, M, N, K, g, ldg, x, ldx, None, wa, ldw, ba, 0.0, ws, nbytes, None)
+
+
+def test_linear_grads_refusals():
+    lib = _lib.load()
+    assert linear_grads(dtype=3) == linear_grads(M=-1) == linear_grads(N=0) == linear_grads(K=0) == _lib.EINVAL
+    assert linear_grads(g=None) == linear_grads(x=None) == linear_grads(wa=None) == _lib.EINVAL
+    assert linear_grads(ldg=7) == linear_grads(ldx=15) == linear_grads(ldw=15) == _lib.EINVAL
+    big = 1 << 16
+    assert linear_grads(N=big, K=big, ldg=big, ldx=big, ldw=big) == _lib.EINDEX
+    assert linear_grads(g=A + 2) == linear_grads(x=B + 1) == linear_grads(wa=C + 2) == linear_grads(ba=W + 1) == _lib.EALIGN
+    assert linear_grads(dtype=F16, g=A + 1) == linear_grads(ws=WS + 8) == _lib.EALIGN
+    need = lib.pet_linear_grads_workspace(F32, 4, 8, 16)
+    assert need > 0 and linear_grads(ws=None) == linear_grads(nbytes=need - 1) == _lib.EWORKSPACE
+    assert lib.pet_linear_grads_workspace(3, 4, 8, 16) == lib.pet_linear_grads_workspace(F32, -1, 8, 16) == 0
+
+
+def clip(entries=((A, 2, 3, 3, F32),), p=2, scale=1.0, max_norm=1.0, eps=1e-6, out=B, ws=WS, nbytes=1 << 30, n=None,
+         norm_only=False):
+    lib = _lib.load()
+    array = (_lib.GradTensor * max(1, len(entries)))(*[_lib.GradTensor(*e) for e in entries])
+    n = len(entries) if n is None else n
+    if norm_only:
+        return lib.pet_grad_norm(array, n, p, scale, out, ws, nbytes, None)
+    return lib.pet_grad_clip(array, n, p, scale, max_norm, eps, out, ws, nbytes, None)
+
+
+@pytest.mark.parametrize("norm_only", [True, False])
+def test_gradient_list_refusals(norm_only):
+    def call(**a):
+        return clip(norm_only=norm_only, **a)
+    assert call(p=3) == call(p=-1) == call(n=-1) == call(out=None) == _lib.EINVAL
+    assert call(scale=math.nan) == call(scale=math.inf) == _lib.EINVAL
+    assert call(entries=((A, -1, 3, 3, F32),)) == call(entries=((A, 2, -3, 3, F32),)) == _lib.EINVAL
+    assert call(entries=((A, 2, 3, 2, F32),)) == call(entries=((None, 2, 3, 3, F32),)) == _lib.EINVAL
+    assert call(entries=((A, 2, 3, 3, 3),)) == _lib.EINVAL
+    assert call(entries=((A, 1 << 20, 1 << 17, 1 << 17, BF16),)) == _lib.EINDEX
+    assert call(entries=((A + 2, 2, 3, 3, F32),)) == call(entries=((A + 1, 2, 3, 3, F16),)) == _lib.EALIGN
+    assert call(ws=None) == call(nbytes=_lib.load().pet_grad_workspace(1) - 1) == _lib.EWORKSPACE
+    assert call(ws=WS + 4) == call(out=B + 2) == _lib.EALIGN
+    assert _lib.load().pet_grad_workspace(-1) == 0 < _lib.load().pet_grad_workspace(0)
+
+
+def test_clip_refusals():
+    for bad in (-1.0, math.nan):
+        assert clip(max_norm=bad) == clip(eps=bad) == _lib.EINVAL
+    assert clip(eps=math.inf) == _lib.EINVAL
+
+
+def test_layer_grads_refusals():
+    lib = _lib.load()
+    sh = _lib.Shape(2, 6, 4, 1, 16, 0, 0.25)
+    need = lib.pet_attention_layer_grads_workspace(ctypes.byref(sh))
+    assert need > lib.pet_attention_layer_workspace(ctypes.byref(sh))
+    assert lib.pet_attention_layer_grads_workspace(None) == 0
+
+    def call(pg, norm_b=None, nbytes=need, tokens=A, out_adj=A, ldo=16, merged=A, ws=1 << 20):
+        return lib.pet_attention_layer_grads(ctypes.byref(sh), None if pg is None else ctypes.byref(pg), A, 16, A, 4,
+                                             out_adj, ldo, tokens, 16, A, norm_b, A, None, A, 4, A, A, merged, A, ws,
+                                             nbytes, None)
+    assert call(None) == _lib.EINVAL
+    assert call(_lib.LayerGrads(norm_b=A)) == _lib.EINVAL  # an RMSNorm's bias
+    assert call(_lib.LayerGrads(b_in=A)) == call(_lib.LayerGrads(b_out=A)) == _lib.EINVAL
+    assert call(_lib.LayerGrads(), tokens=None) == call(_lib.LayerGrads(), out_adj=None) == _lib.EINVAL
+    assert call(_lib.LayerGrads(), merged=None) == call(_lib.LayerGrads(), ldo=15) == _lib.EINVAL
+    assert call(_lib.LayerGrads(), nbytes=need - 1) == call(_lib.LayerGrads(), ws=None) == _lib.EWORKSPACE
+    assert call(_lib.LayerGrads(), ws=(1 << 20) + 16) == _lib.EALIGN
+
+
+def test_host_tensors_are_refused():
+    """There is no CPU path: tensors in host memory raise before the library is called."""
+    x, w = torch.zeros(4, 8), torch.zeros(8)
+    with pytest.raises(ValueError):
+        layer.norm_rows(x.bfloat16(), x.bfloat16(), w, None)
+    with pytest.raises(ValueError):
+        layer.norm_rows_bwd(x.half(), x.half(), x.half(), w, False)
+    with pytest.raises(ValueError):
+        layer.norm_rows_grads(x, w, None, x, x, w, False)
+    with pytest.raises(ValueError):
+        linear.linear_grads(x, x, torch.zeros(8, 8))
+    with pytest.raises(TypeError):
+        linear.linear_grads(x, None, torch.zeros(8, 8))
+    with pytest.raises(ValueError):
+        grads.GradList([x])
+    with pytest.raises(TypeError):
+        grads.GradList([3.0])
+
+
+def test_layouts_of_gradients():
+    """Which strides count as consecutive, as rows of a wider matrix, or as neither."""
+    t = torch.zeros(4, 6, 8)
+    assert grads._layout(t, 0) == (1, 192, 192)
+    assert grads._layout(t.permute(2, 0, 1), 0) == (1, 192, 192)
+    assert grads._layout(t[:, :, :5][0], 0) == (6, 5, 8)
+    assert grads._layout(t[0].t()[:5], 0) == (6, 5, 8)
+    assert grads._layout(t[0, :, 3:4], 0) == (6, 1, 8) == grads._layout(t[0, :, 3], 0)
+    assert grads._layout(torch.zeros(()), 0) == (1, 1, 1)
+    for bad in (t[:, ::2, :5], t[0, :, ::2], torch.zeros(3, 1).expand(3, 4), t[:, :5, :]):
+        with pytest.raises(ValueError):
+            grads._layout(bad, 0)
+    a, b = t[0][:, :5], t[0][:, 5:]
+    assert grads._side_by_side(a, b) and not grads._side_by_side(a, t[0][:, 4:])
