@@ -19,94 +19,170 @@
 #include <type_traits>
 
 #include "../../include/pet_attn.h"
+#include "gemm_common.h"
 #include "typed.h"
 
 namespace pet_norm {
 
 using pet_typed::kVec;
 using pet_typed::live_rows;
+using pet_typed::u4e;
 
 constexpr float kRmsEps = 1.1920928955078125e-07f;  // float32 epsilon
 constexpr float kLnEps = 1e-5f;
 
 constexpr int threads_of(int TPR) { return TPR > 256 ? TPR : 256; }
-
-// A row's sum over its TPR threads, the same bits in each of them: a butterfly
-// over the lanes and, where a row is the whole workgroup's, the waves' sums in
-// order through LDS (`red`, one slot a wave; two barriers, so a call may follow a
-// call).
-template <int TPR>
-__device__ __forceinline__ float row_sum(float x, float* red) {
-#pragma unroll
-  for (int o = (TPR < 64 ? TPR : 64) / 2; o > 0; o >>= 1) x += __shfl_xor(x, o);
-  if constexpr (TPR > 64) {
-    constexpr int W = TPR / 64;
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
-    __syncthreads();
-    x = 0.f;
-#pragma unroll
-    for (int i = 0; i < W; ++i) x += red[i];
-    __syncthreads();
-  }
-  return x;
+// Waves a SIMD of the backward, by the elements a lane holds (x, g, the weight and
+// the two sums, and the next row's raw ones): the registers are held to it, so
+// that a grid of it fills the chip in one round. (1024 workgroups of which 768
+// fitted took two: 65536 x 1024 in bf16 131 us.)
+constexpr int waves_of(int E) { return E <= 4 ? 8 : E <= 8 ? 5 : E <= 16 ? 3 : 2; }
+// 1 / sqrt(x): the hardware's estimate and a Newton step.
+__device__ __forceinline__ float rsqrt_nr(float x) {
+  const float y = __builtin_amdgcn_rsqf(x);
+  return y * fmaf(-0.5f * x * y, y, 1.5f);
 }
 
-// A thread's share of a row: C chunks of kVec elements, chunk j at kVec (t + TPR j).
+// A lane's value from the lane that a DPP control names.
+template <int ctrl>
+__device__ __forceinline__ float dpp(float x) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), ctrl, 0xf, 0xf, true));
+}
+// A row's sums over its TPR threads, the same bits in each of them: in registers
+// over the lanes (quads, halves and whole rows of 16 by DPP, then the rows of 16
+// exchanged) and, where a row is the whole workgroup's, the waves' sums in order
+// through LDS (`red`, double-buffered by `turn`, so that a sum costs one barrier).
+template <int TPR, int n>
+__device__ __forceinline__ void row_sums(float (&x)[n], float (*red)[2][3], int& turn) {
+#pragma unroll
+  for (int i = 0; i < n; ++i) {
+    x[i] += dpp<0xb1>(x[i]);   // quad_perm 1, 0, 3, 2
+    x[i] += dpp<0x4e>(x[i]);   // quad_perm 2, 3, 0, 1
+    x[i] += dpp<0x141>(x[i]);  // the half row mirrored
+    x[i] += dpp<0x140>(x[i]);  // the row mirrored
+  }
+  if constexpr (TPR >= 32) {
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x[i]), __float_as_uint(x[i]), false, false);
+      x[i] = __uint_as_float(b[0]) + __uint_as_float(b[1]);
+    }
+  }
+  if constexpr (TPR >= 64) {
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x[i]), __float_as_uint(x[i]), false, false);
+      x[i] = __uint_as_float(b[0]) + __uint_as_float(b[1]);
+    }
+  }
+  if constexpr (TPR > 64) {
+    if ((threadIdx.x & 63) == 0)
+#pragma unroll
+      for (int i = 0; i < n; ++i) red[threadIdx.x >> 6][turn][i] = x[i];
+    pet_gemm::ring_barrier();
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      x[i] = 0.f;
+#pragma unroll
+      for (int w = 0; w < TPR / 64; ++w) x[i] += red[w][turn][i];
+    }
+    turn ^= 1;
+  }
+}
+
+// A thread's share of a row as it lies in memory: C chunks of kVec elements, chunk
+// j at kVec (t + TPR j), zeros past the width.
 template <class T, int TPR, int C>
-__device__ __forceinline__ void load_row(const T* row, int width, int t, float (&x)[C][kVec<T>]) {
+__device__ __forceinline__ void load_row(const T* row, int width, int t, u4e (&q)[C]) {
 #pragma unroll
   for (int j = 0; j < C; ++j) {
-    const int d = kVec<T> * (t + TPR * j);
-    pet_typed::load<T>(row + (d < width ? d : 0), d < width ? width - d : 0, x[j]);
+    const int d = kVec<T> * (t + TPR * j), left = width - d;
+    q[j] = u4e{0u, 0u, 0u, 0u};
+    if (left >= kVec<T>) {
+      q[j] = *reinterpret_cast<const u4e*>(row + d);
+    } else if (left > 0) {  // every load in flight, then those past the row's end dropped
+      T v[kVec<T>];
+#pragma unroll
+      for (int e = 0; e < kVec<T>; ++e) v[e] = row[d + min(e, left - 1)];
+#pragma unroll
+      for (int e = 0; e < kVec<T>; ++e)
+        if constexpr (sizeof(T) == 4) q[j][e] = e < left ? __float_as_uint(v[e]) : 0u;
+        else q[j][e / 2] |= e < left ? unsigned(__builtin_bit_cast(unsigned short, v[e])) << (16 * (e & 1)) : 0u;
+    }
   }
 }
-// 1 / sqrt(mean((x - mu)^2) + eps) of the row, mu returned.
-template <class T, int TPR, int C>
-__device__ __forceinline__ float row_inv(const float (&x)[C][kVec<T>], int width, int t, bool ln, float& mu, float* red) {
-  constexpr int V = kVec<T>;
-  mu = 0.f;
-  if (ln) {
-    float s = 0.f;
+// n floats of a vector at d, zeros past the width.
+template <int n>
+__device__ __forceinline__ void load_vec(const float* p, int d, int width, float (&x)[n]) {
+  if (d + n <= width) {
 #pragma unroll
-    for (int j = 0; j < C; ++j)
+    for (int e = 0; e < n; e += 4) {
+      const u4e q = *reinterpret_cast<const u4e*>(p + d + e);
 #pragma unroll
-      for (int e = 0; e < V; ++e) s += x[j][e];
-    mu = row_sum<TPR>(s, red) / width;
-  }
-  float v = 0.f;
-#pragma unroll
-  for (int j = 0; j < C; ++j)
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const float a = x[j][e] - mu;
-      v += V * (t + TPR * j) + e < width ? a * a : 0.f;
+      for (int i = 0; i < 4; ++i) x[e + i] = __uint_as_float(q[i]);
     }
-  v = row_sum<TPR>(v, red);
-  return 1.0f / sqrtf(v / width + (ln ? kLnEps : kRmsEps));
+  } else {
+#pragma unroll
+    for (int e = 0; e < n; ++e) x[e] = d + e < width ? p[d + e] : 0.f;
+  }
+}
+
+// x - mu for the `left` elements that are the row's, 0 for those past it.
+template <int n>
+__device__ __forceinline__ void center(float (&x)[n], float mu, int left) {
+  if (left >= n) {
+#pragma unroll
+    for (int e = 0; e < n; ++e) x[e] -= mu;
+  } else {
+#pragma unroll
+    for (int e = 0; e < n; ++e) x[e] = e < left ? x[e] - mu : 0.f;
+  }
 }
 
 template <class T, int TPR, int C>
-__global__ void __launch_bounds__(threads_of(TPR)) norm_typed_fwd_kernel(int rows, int width, T* __restrict__ out,
+__global__ void __launch_bounds__(threads_of(TPR)) norm_typed_fwd_kernel(int rows, int width, float per, T* __restrict__ out,
                                                                          int64_t ldo, const T* __restrict__ in,
                                                                          int64_t ldi, const float* __restrict__ weight,
                                                                          const float* __restrict__ bias) {
   constexpr int V = kVec<T>, RPB = threads_of(TPR) / TPR;
-  __shared__ float red[TPR > 64 ? TPR / 64 : 1];
+  __shared__ float red[TPR > 64 ? TPR / 64 : 1][2][3];
   const int t = threadIdx.x % TPR;
   const int64_t r = int64_t(blockIdx.x) * RPB + threadIdx.x / TPR;
   if (r >= rows) return;  // (a row's threads leave together)
-  float x[C][V], mu;
-  load_row<T, TPR, C>(in + r * ldi, width, t, x);
-  const float inv = row_inv<T, TPR, C>(x, width, t, bias != nullptr, mu, red);
+  int turn = 0;
+  u4e q[C];
+  float x[C][V];
+  load_row<T, TPR, C>(in + r * ldi, width, t, q);
+  float mu = 0.f;
+#pragma unroll
+  for (int j = 0; j < C; ++j) pet_typed::unpack<T>(q[j], x[j]);
+  if (bias) {
+    float s[1] = {0.f};
+#pragma unroll
+    for (int j = 0; j < C; ++j)
+#pragma unroll
+      for (int e = 0; e < V; ++e) s[0] += x[j][e];
+    row_sums<TPR>(s, red, turn);
+    mu = s[0] * per;
+  }
+  float v[1] = {0.f};
+#pragma unroll
+  for (int j = 0; j < C; ++j) {
+    center<V>(x[j], mu, width - V * (t + TPR * j));
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[0] = fmaf(x[j][e], x[j][e], v[0]);
+  }
+  row_sums<TPR>(v, red, turn);
+  const float inv = rsqrt_nr(fmaf(v[0], per, bias ? kLnEps : kRmsEps));
 #pragma unroll
   for (int j = 0; j < C; ++j) {
     const int d = V * (t + TPR * j);
     if (d < width) {
+      float w[V], b[V];
+      load_vec<V>(weight, d, width, w);
+      if (bias) load_vec<V>(bias, d, width, b);
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const int k = min(d + e, width - 1);
-        x[j][e] = (x[j][e] - mu) * inv * weight[k] + (bias ? bias[k] : 0.f);
-      }
+      for (int e = 0; e < V; ++e) x[j][e] = x[j][e] * inv * w[e] + (bias ? b[e] : 0.f);
       pet_typed::store<T>(out + r * ldo + d, width - d, x[j]);
     }
   }
@@ -116,42 +192,69 @@ __global__ void __launch_bounds__(threads_of(TPR)) norm_typed_fwd_kernel(int row
 // beta_edge; in_adj null: the parameters' gradients alone. part [gridDim.x][2][width]:
 // this workgroup's sums (null: in_adj alone).
 template <class T, int TPR, int C, bool LN>
-__global__ void __launch_bounds__(threads_of(TPR))
-    norm_grads_kernel(int rows, int width, T* __restrict__ in_adj, int64_t lda, const T* __restrict__ out_adj,
-                      int64_t ldg, const T* __restrict__ in, int64_t ldi, const float* __restrict__ weight, int n_node,
+__global__ void __launch_bounds__(threads_of(TPR), waves_of(C * kVec<T>))
+    norm_grads_kernel(int rows, int width, float per, T* __restrict__ in_adj, int64_t lda,
+                      const T* __restrict__ out_adj, int64_t ldg, const T* __restrict__ in, int64_t ldi, const float* __restrict__ weight, int n_node,
                       float beta_node, float beta_edge, int live_base, const int* __restrict__ live,
                       float* __restrict__ part) {
   constexpr int V = kVec<T>, RPB = threads_of(TPR) / TPR;
-  __shared__ float red[TPR > 64 ? TPR / 64 : 1];
+  __shared__ float red[TPR > 64 ? TPR / 64 : 1][2][3];
   const int t = threadIdx.x % TPR, g0 = threadIdx.x / TPR;
   const int end = live_rows(rows, live_base, live);
+  int turn = 0;
   float w[C][V], dw[C][V], db[C][V];
 #pragma unroll
-  for (int j = 0; j < C; ++j)
+  for (int j = 0; j < C; ++j) {
+    load_vec<V>(weight, V * (t + TPR * j), width, w[j]);
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const int d = V * (t + TPR * j) + e;
-      w[j][e] = d < width ? weight[d] : 0.f, dw[j][e] = 0.f, db[j][e] = 0.f;
+    for (int e = 0; e < V; ++e) dw[j][e] = 0.f, db[j][e] = 0.f;
+  }
+  const int64_t step = int64_t(gridDim.x) * RPB;
+  int64_t r = int64_t(blockIdx.x) * RPB + g0;
+  constexpr bool AHEAD = C * V <= 16;  // (a lane of 32 elements has no registers for the next row's)
+  u4e qx[C], qg[C];
+  if (AHEAD && r < end) {
+    load_row<T, TPR, C>(in + r * ldi, width, t, qx);
+    load_row<T, TPR, C>(out_adj + r * ldg, width, t, qg);
+  }
+  for (; r < end; r += step) {
+    float x[C][V], g[C][V], mu = 0.f;
+    if (!AHEAD) {
+      load_row<T, TPR, C>(in + r * ldi, width, t, qx);
+      load_row<T, TPR, C>(out_adj + r * ldg, width, t, qg);
     }
-  for (int64_t r = int64_t(blockIdx.x) * RPB + g0; r < end; r += int64_t(gridDim.x) * RPB) {
-    float x[C][V], g[C][V], mu;
-    load_row<T, TPR, C>(in + r * ldi, width, t, x);
-    load_row<T, TPR, C>(out_adj + r * ldg, width, t, g);
-    const float inv = row_inv<T, TPR, C>(x, width, t, LN, mu, red);
-    float sg = 0.f, sgx = 0.f;
 #pragma unroll
-    for (int j = 0; j < C; ++j)
+    for (int j = 0; j < C; ++j) pet_typed::unpack<T>(qx[j], x[j]), pet_typed::unpack<T>(qg[j], g[j]);
+    if (AHEAD && r + step < end) {  // the next row, while this one is worked on
+      load_row<T, TPR, C>(in + (r + step) * ldi, width, t, qx);
+      load_row<T, TPR, C>(out_adj + (r + step) * ldg, width, t, qg);
+    }
+    if (LN) {
+      float s[1] = {0.f};
+#pragma unroll
+      for (int j = 0; j < C; ++j)
+#pragma unroll
+        for (int e = 0; e < V; ++e) s[0] += x[j][e];
+      row_sums<TPR>(s, red, turn);
+      mu = s[0] * per;
+    }
+    // sum (x - mu)^2, g w (x - mu), g w
+    float s[LN ? 3 : 2] = {};
+#pragma unroll
+    for (int j = 0; j < C; ++j) {
+      if (LN) center<V>(x[j], mu, width - V * (t + TPR * j));
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        // (past the width g is 0, and x - mu times it)
-        const float xh = (x[j][e] - mu) * inv, gw = g[j][e] * w[j][e];
-        if (LN) sg += gw;
-        sgx += gw * xh;
-        dw[j][e] = fmaf(g[j][e], xh, dw[j][e]);
         if (LN) db[j][e] += g[j][e];
+        const float gw = g[j][e] * w[j][e];
+        s[0] = fmaf(x[j][e], x[j][e], s[0]);
+        s[1] = fmaf(gw, x[j][e], s[1]);
+        if (LN) s[2] += gw;
       }
-    if (!in_adj) continue;
-    const float mg = LN ? row_sum<TPR>(sg, red) / width : 0.f, mgx = row_sum<TPR>(sgx, red) / width;
+    }
+    row_sums<TPR>(s, red, turn);
+    const float inv = rsqrt_nr(fmaf(s[0], per, LN ? kLnEps : kRmsEps));
+    const float mgx = s[1] * inv * per, mg = LN ? s[LN ? 2 : 0] * per : 0.f;
     const float beta = r < n_node ? beta_node : beta_edge;
     T* a_row = in_adj + r * lda;
 #pragma unroll
@@ -159,14 +262,15 @@ __global__ void __launch_bounds__(threads_of(TPR))
       const int d = V * (t + TPR * j);
       if (d < width) {
         float o[V];
-        if (beta != 0.f) pet_typed::load<T>(a_row + d, width - d, o);
+        if (in_adj && beta != 0.f) pet_typed::load<T>(a_row + d, width - d, o);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          const float xh = (x[j][e] - mu) * inv;
+          const float xh = x[j][e] * inv;
+          dw[j][e] = fmaf(g[j][e], xh, dw[j][e]);
           const float v = inv * fmaf(-xh, mgx, fmaf(g[j][e], w[j][e], -mg));
           o[e] = beta != 0.f ? fmaf(beta, o[e], v) : v;
         }
-        pet_typed::store<T>(a_row + d, width - d, o);
+        if (in_adj) pet_typed::store<T>(a_row + d, width - d, o);
       }
     }
   }
@@ -191,55 +295,76 @@ __global__ void __launch_bounds__(threads_of(TPR))
     } else {
 #pragma unroll
       for (int j = 0; j < C; ++j)
-        if (V * (t + TPR * j) < width) {
 #pragma unroll
-          for (int e = 0; e < V; ++e)
-            if (V * (t + TPR * j) + e < width) to[V * (t + TPR * j) + e] = a[j][e];
-        }
+        for (int e = 0; e < V; ++e)
+          if (V * (t + TPR * j) + e < width) to[V * (t + TPR * j) + e] = a[j][e];
     }
   };
   put(dw, p);
   if (LN) put(db, p + width);
 }
 
-// adj = beta adj + the sum of the parts, in double: 32 columns by 32 strips of parts a workgroup.
+// adj = beta adj + the sum of the parts, in double: 16 columns by 64 strips of
+// parts a workgroup, a strip's loads eight at a time. (32 columns by 32 strips, one
+// load after the other: 11 us for 1024 parts.)
 __global__ void __launch_bounds__(1024) norm_parts_kernel(int parts, int width, const float* __restrict__ part,
                                                           float* __restrict__ w_adj, float* __restrict__ b_adj,
                                                           float beta) {
-  __shared__ double s[32][33];
-  const int c = threadIdx.x & 31, strip = threadIdx.x >> 5;
-  const int d = blockIdx.x * 32 + c, which = blockIdx.y;
+  __shared__ double s[64][17];
+  const int c = threadIdx.x & 15, strip = threadIdx.x >> 4;
+  const int d = blockIdx.x * 16 + c, which = blockIdx.y;
   float* adj = which ? b_adj : w_adj;
   if (!adj) return;
   double a = 0.0;
-  if (d < width)
-    for (int q = strip; q < parts; q += 32) a += part[(int64_t(q) * 2 + which) * width + d];
+  if (d < width) {
+    const float* p = part + int64_t(which) * width + d;
+    int q = strip;
+    for (; q + 7 * 64 < parts; q += 8 * 64) {
+      float x[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) x[u] = p[int64_t(q + 64 * u) * 2 * width];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) a += x[u];
+    }
+    for (; q < parts; q += 64) a += p[int64_t(q) * 2 * width];
+  }
   s[strip][c] = a;
   __syncthreads();
-  if (threadIdx.x < 32 && d < width) {
+  if (threadIdx.x < 256) {  // four strips' quarters, then those
+    const int cc = threadIdx.x & 15, f = threadIdx.x >> 4;
     double v = 0.0;
-    for (int q = 0; q < 32; ++q) v += s[q][c];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) v += s[4 * f + q][cc];
+    s[4 * f][cc] = v;
+  }
+  __syncthreads();
+  if (threadIdx.x < 16 && d < width) {
+    double v = 0.0;
+#pragma unroll
+    for (int q = 0; q < 16; ++q) v += s[4 * q][c];
     adj[d] = beta != 0.f ? float(double(beta) * adj[d] + v) : float(v);
   }
 }
 
-// f(threads a row, chunks a thread) for rows of the width.
+// f(threads a row, chunks a thread) for rows of the width: a wave's or a part of
+// one while a lane holds at most 16 elements (of the backward's four values each,
+// in registers), the workgroup's past that.
 template <class T, class F>
 int with_row(int width, F&& f) {
-  constexpr int V = kVec<T>;
+  constexpr int V = kVec<T>, S = V == 4 ? 2 : 1;  // S: the chunks of 8 elements
   using std::integral_constant;
   if (width <= 16 * V) return f(integral_constant<int, 16>{}, integral_constant<int, 1>{});
   if (width <= 32 * V) return f(integral_constant<int, 32>{}, integral_constant<int, 1>{});
   if (width <= 64 * V) return f(integral_constant<int, 64>{}, integral_constant<int, 1>{});
-  if (width <= 128 * V) return f(integral_constant<int, 64>{}, integral_constant<int, 2>{});
-  if (width <= 256 * V) return f(integral_constant<int, 64>{}, integral_constant<int, 4>{});
-  if (width <= 512 * V) return f(integral_constant<int, 256>{}, integral_constant<int, 2>{});
-  if (width <= 1024 * V) return f(integral_constant<int, 256>{}, integral_constant<int, 4>{});
-  if (V == 8 || width <= 2048 * V) return f(integral_constant<int, 512>{}, integral_constant<int, 4>{});
-  return f(integral_constant<int, 512>{}, integral_constant<int, 8>{});
+  if (width <= 512) return f(integral_constant<int, 64>{}, integral_constant<int, S>{});
+  if (width <= 1024) return f(integral_constant<int, 64>{}, integral_constant<int, 2 * S>{});
+  if (width <= 2048) return f(integral_constant<int, 256>{}, integral_constant<int, S>{});
+  if (width <= 4096) return f(integral_constant<int, 256>{}, integral_constant<int, 2 * S>{});
+  if (width <= 8192) return f(integral_constant<int, 1024>{}, integral_constant<int, S>{});
+  return f(integral_constant<int, 512>{}, integral_constant<int, 4 * S>{});
 }
 
-constexpr int kMaxParts = 1024;
+constexpr int kCus = 256, kMaxParts = 2048;
 
 }  // namespace pet_norm
 
@@ -259,10 +384,14 @@ int pet_norm_grads_sink(int dtype, int rows, int width, void* in_adj, int64_t ld
     using T = decltype(tv);
     return with_row<T>(width, [&](auto lc, auto cc) {
       constexpr int TPR = decltype(lc)::value, C = decltype(cc)::value, TH = threads_of(TPR), RPB = TH / TPR;
-      blocks = int(std::max<int64_t>(1, std::min<int64_t>((int64_t(rows) + RPB - 1) / RPB, kMaxParts)));
+      // as many workgroups as the chip holds at once, each with the same rows to within one
+      constexpr int most = kCus * (waves_of(C * kVec<T>) * 256 / TH);
+      static_assert(most <= kMaxParts, "the workspace's rows");
+      const int64_t groups = std::max<int64_t>(1, (int64_t(rows) + RPB - 1) / RPB), each = (groups + most - 1) / most;
+      blocks = int((groups + each - 1) / each);
       auto run = [&](auto lnc) {
         hipLaunchKernelGGL((norm_grads_kernel<T, TPR, C, decltype(lnc)::value>), dim3(unsigned(blocks)), dim3(TH), 0, st,
-                           rows, width, static_cast<T*>(in_adj), lda, static_cast<const T*>(out_adj), ldg,
+                           rows, width, 1.0f / width, static_cast<T*>(in_adj), lda, static_cast<const T*>(out_adj), ldg,
                            static_cast<const T*>(in), ldi, weight, n_node, beta_node, beta_edge, live_base, live, part);
       };
       if (ln) run(std::true_type{});
@@ -271,7 +400,7 @@ int pet_norm_grads_sink(int dtype, int rows, int width, void* in_adj, int64_t ld
     });
   });
   if (e || !parts) return e;
-  hipLaunchKernelGGL(norm_parts_kernel, dim3(unsigned((width + 31) / 32), ln ? 2 : 1), dim3(1024), 0, st, blocks, width,
+  hipLaunchKernelGGL(norm_parts_kernel, dim3(unsigned((width + 15) / 16), ln ? 2 : 1), dim3(1024), 0, st, blocks, width,
                      part, w_adj, b_adj, beta_w);
   return hipGetLastError() == hipSuccess ? int(PET_ATTN_OK) : int(PET_ATTN_ELAUNCH);
 }
@@ -294,7 +423,7 @@ int pet_norm_rows_typed(int dtype, int rows, int width, void* out, int64_t ldo, 
     return with_row<T>(width, [&](auto lc, auto cc) {
       constexpr int TPR = decltype(lc)::value, C = decltype(cc)::value, TH = threads_of(TPR), RPB = TH / TPR;
       hipLaunchKernelGGL((norm_typed_fwd_kernel<T, TPR, C>), dim3(unsigned((int64_t(rows) + RPB - 1) / RPB)), dim3(TH),
-                         0, reinterpret_cast<hipStream_t>(stream), rows, width, static_cast<T*>(out), ldo,
+                         0, reinterpret_cast<hipStream_t>(stream), rows, width, 1.0f / width, static_cast<T*>(out), ldo,
                          static_cast<const T*>(in), ldi, weight, bias);
       return hipGetLastError() == hipSuccess ? int(PET_ATTN_OK) : int(PET_ATTN_ELAUNCH);
     });

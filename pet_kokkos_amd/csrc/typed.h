@@ -48,14 +48,16 @@ __device__ __forceinline__ u4e pack(const float (&x)[kVec<T>]) {
   }
   return q;
 }
-// n elements at p (n at least the vector: all of it), zeros past them.
+// n elements at p (at least one; from the vector's on: all of it), zeros past them.
 template <class T>
 __device__ __forceinline__ void load(const T* p, int64_t n, float (&x)[kVec<T>]) {
   if (n >= kVec<T>) {
     unpack<T>(*reinterpret_cast<const u4e*>(p), x);
   } else {
 #pragma unroll
-    for (int i = 0; i < kVec<T>; ++i) x[i] = i < n ? float(p[i]) : 0.f;
+    for (int i = 0; i < kVec<T>; ++i) x[i] = float(p[min(int64_t(i), n - 1)]);  // (all in flight)
+#pragma unroll
+    for (int i = 0; i < kVec<T>; ++i) x[i] = i < n ? x[i] : 0.f;
   }
 }
 template <class T>

@@ -62,9 +62,12 @@ struct Tile {
   static constexpr int STAGE = ROWS * 8;            // 16-byte chunks
 };
 
-// The slot of chunk q in LDS row r: a read or a write of 16 rows by four chunks
-// runs at the rate of consecutive lanes.
-__device__ __forceinline__ int slot(int q, int r) { return r * 8 + (q ^ (((r >> 1) & 1) | ((r >> 1) & 4))); }
+// The slot of half h (hi and lo, or a step's first and last 32 rows) of chunk q in
+// LDS row r: a read or a write of 16 rows by four chunks runs at the rate of
+// consecutive lanes.
+__device__ __forceinline__ int slot(int q, int h, int r) {
+  return r * 8 + ((2 * q + h) ^ (((r >> 1) & 1) | ((r >> 1) & 4)));
+}
 
 // The largest |x| of eight (a NaN is passed over: it makes its column NaN by itself).
 __device__ __forceinline__ float amax8(const unsigned (&x)[8]) {
@@ -225,8 +228,8 @@ __global__ void __launch_bounds__(64 * WN * WK, TN * TK >= 16 ? 2 : 4)
       for (int j = 0; j < V; ++j) {
         u4 hi, lo;
         split8(x[j], neg ? -scale[j] : scale[j], hi, lo);
-        to[slot(oct, row0 + 16 * j)] = hi;
-        to[slot(4 + oct, row0 + 16 * j)] = lo;
+        to[slot(g, 0, row0 + 16 * j)] = hi;
+        to[slot(g, 1, row0 + 16 * j)] = lo;
         if (bias) {
           float t[8];
 #pragma unroll
@@ -244,8 +247,8 @@ __global__ void __launch_bounds__(64 * WN * WK, TN * TK >= 16 ? 2 : 4)
           even[d] = __builtin_amdgcn_perm(raw[2 * d + 1][w], raw[2 * d][w], 0x05040100u) ^ flip;
           odd[d] = __builtin_amdgcn_perm(raw[2 * d + 1][w], raw[2 * d][w], 0x07060302u) ^ flip;
         }
-        to[slot(oct, row0 + 32 * w)] = even;
-        to[slot(oct, row0 + 32 * w + 16)] = odd;
+        to[slot(g, oq, row0 + 32 * w)] = even;
+        to[slot(g, oq, row0 + 32 * w + 16)] = odd;
         if (bias) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -292,11 +295,11 @@ __global__ void __launch_bounds__(64 * WN * WK, TN * TK >= 16 ? 2 : 4)
 #pragma unroll
     for (int j = 0; j < TK; ++j)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) b[j][h] = from[slot(4 * h + g, rk + 16 * j + c)];
+      for (int h = 0; h < 2; ++h) b[j][h] = from[slot(g, h, rk + 16 * j + c)];
     const float sg = s & 1 ? -1.f : 1.f;
 #pragma unroll
     for (int i = 0; i < TN; ++i) {
-      const u4 x = from[slot(g, rn + 16 * i + c)], y = from[slot(4 + g, rn + 16 * i + c)];
+      const u4 x = from[slot(g, 0, rn + 16 * i + c)], y = from[slot(g, 1, rn + 16 * i + c)];
 #pragma unroll
       for (int j = 0; j < TK; ++j) {
         f4 t = {0.f, 0.f, 0.f, 0.f};
@@ -430,23 +433,59 @@ __global__ void __launch_bounds__(64 * WN * WK, TN * TK >= 16 ? 2 : 4)
     }
 }
 
-// adj = beta adj + the pieces' sums, in order and in double.
-__global__ void __launch_bounds__(256) wgrad_sum_kernel(int N, int K, int pieces, int wpieces,
-                                                        const float* __restrict__ part,
+// adj = beta adj + the pieces' sums in double: a thread sums every STRIPS-th
+// piece of four elements, eight loads at a time, the strips are joined in order.
+// (One thread an element, its loads one after the other: 24 us for 80 pieces of
+// 768 x 256 against 8.)
+constexpr int kStrips = 8;
+__global__ void __launch_bounds__(256) wgrad_sum_kernel(int N, int K, int pieces, const float* __restrict__ part,
                                                         const double* __restrict__ bpart, float* __restrict__ w_adj,
                                                         int64_t ldw, float* __restrict__ b_adj, float beta) {
-  const int64_t nk = wpieces > 1 ? int64_t(N) * K : 0, i = int64_t(blockIdx.x) * 256 + threadIdx.x;
-  if (i >= nk + (b_adj ? N : 0)) return;
-  double v = 0.0;
-  float* o;
-  if (i < nk) {
-    for (int s = 0; s < pieces; ++s) v += part[int64_t(s) * nk + i];
-    o = w_adj + i / K * ldw + i % K;
+  __shared__ double sums[kStrips][32][4];
+  const int64_t nk = part ? int64_t(N) * K : 0, wblocks = (nk + 127) / 128;
+  const int q = threadIdx.x & 31, strip = threadIdx.x >> 5;
+  const bool bias = int64_t(blockIdx.x) >= wblocks;
+  const int64_t i = (int64_t(blockIdx.x) - (bias ? wblocks : 0)) * 128 + 4 * q, n = bias ? N : nk;
+  double v[4] = {0.0, 0.0, 0.0, 0.0};
+  if (bias) {
+    for (int s = strip; s < pieces; s += kStrips)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (i + e < n) v[e] += bpart[int64_t(s) * N + i + e];
+  } else if (i + 4 <= n) {
+    int s = strip;
+    for (; s + 7 * kStrips < pieces; s += 8 * kStrips) {
+      f4u x[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) x[u] = *reinterpret_cast<const f4u*>(part + int64_t(s + u * kStrips) * nk + i);
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] += x[u][e];
+    }
+#pragma unroll 2
+    for (; s < pieces; s += kStrips) {
+      const f4u x = *reinterpret_cast<const f4u*>(part + int64_t(s) * nk + i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] += x[e];
+    }
   } else {
-    for (int s = 0; s < pieces; ++s) v += bpart[int64_t(s) * N + (i - nk)];
-    o = b_adj + (i - nk);
+    for (int s = strip; s < pieces; s += kStrips)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (i + e < n) v[e] += part[int64_t(s) * nk + i + e];
   }
-  *o = beta != 0.f ? float(double(beta) * *o + v) : float(v);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) sums[strip][q][e] = v[e];
+  __syncthreads();
+  const int t = threadIdx.x;
+  const int64_t j = i - 4 * q + t;
+  if (t >= 128 || j >= n) return;
+  double r = 0.0;
+#pragma unroll
+  for (int s = 0; s < kStrips; ++s) r += sums[s][t >> 2][t & 3];
+  float* o = bias ? b_adj + j : w_adj + j / K * ldw + j % K;
+  *o = beta != 0.f ? float(double(beta) * *o + r) : float(r);
 }
 
 // How a product is cut: the tile and the pieces.
@@ -506,10 +545,10 @@ int pet_linear_grads_run(int dtype, int M, int N, int K, const void* out_adj, in
     return hipGetLastError() == hipSuccess ? int(PET_ATTN_OK) : int(PET_ATTN_ELAUNCH);
   });
   if (e) return e;
-  const int64_t total = (p.pieces > 1 ? int64_t(N) * K : 0) + (b_adj ? N : 0);
-  if (total == 0) return PET_ATTN_OK;
-  hipLaunchKernelGGL(wgrad_sum_kernel, dim3(unsigned((total + 255) / 256)), dim3(256), 0, st, N, K, p.pieces, p.pieces,
-                     part, bpart, w_adj, ldw, b_adj, beta);
+  const int64_t blocks = (p.pieces > 1 ? (int64_t(N) * K + 127) / 128 : 0) + (b_adj ? (int64_t(N) + 127) / 128 : 0);
+  if (blocks == 0) return PET_ATTN_OK;
+  hipLaunchKernelGGL(wgrad_sum_kernel, dim3(unsigned(blocks)), dim3(256), 0, st, N, K, p.pieces,
+                     p.pieces > 1 ? part : nullptr, bpart, w_adj, ldw, b_adj, beta);
   return hipGetLastError() == hipSuccess ? int(PET_ATTN_OK) : int(PET_ATTN_ELAUNCH);
 }
 
