@@ -24,6 +24,13 @@
 // them, so it finds the new scale by itself and hands the factor on through LDS
 // (rare). A value below 2^-14 of the column's largest is held to 2^-36 of that.
 //
+// What bounds it: the matrix unit under the clock that its power leaves. For
+// 486946 x 2048 x 512 in bf16 (1.25 ms, 815 TFLOP/s; a library's product of that
+// shape 2.0 ms, of 8192 cubed 1131 TFLOP/s) the products alone take 0.73 ms, the
+// rows' way into LDS alone 0.71, the loads alone 0.60; together the clock falls from
+// 2.2 to 1.8 GHz, and the matrix unit is busy 42% of the cycles. 122688 x 768 x 256
+// in fp32 takes 198 us, of which writing and adding the pieces is 30.
+//
 // The matrix instruction rounds toward minus infinity, an error with a mean that
 // half a million rows would add up. So a step is summed from zero, the sums of
 // the steps are added in fp32 to nearest, and g's odd steps are negated and
@@ -97,11 +104,13 @@ __device__ __forceinline__ f4 mfma(const u4& a, const u4& b, const f4& c) {
   if constexpr (std::is_same<T, __bf16>::value) return pet_split::mfma_bf(a, b, c);
   else return pet_split::mfma_h(a, b, c);
 }
+// c + both halves of x times those of y (ones, of either sign), rounded once.
 template <class T>
-__device__ __forceinline__ float half_of(unsigned w, int h) {
-  if constexpr (std::is_same<T, __bf16>::value) return __uint_as_float(h ? w & 0xffff0000u : w << 16);
-  const unsigned short s = static_cast<unsigned short>(h ? w >> 16 : w);
-  return float(__builtin_bit_cast(_Float16, s));
+__device__ __forceinline__ float dot2(unsigned x, unsigned y, float c) {
+  typedef T t2 __attribute__((ext_vector_type(2)));
+  if constexpr (std::is_same<T, __bf16>::value)
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(t2, x), __builtin_bit_cast(t2, y), c, false);
+  else return __builtin_amdgcn_fdot2(__builtin_bit_cast(t2, x), __builtin_bit_cast(t2, y), c, false);
 }
 
 typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
@@ -117,7 +126,7 @@ struct Args {
   int pieces, tiles_n, tiles_k;
   float* out;      // [pieces][N][K], or with one piece w_adj
   int64_t ldo;
-  double* bout;    // [pieces][N], null: no bias
+  double* bout;    // [pieces][tiles_k][N], null: no bias
   float beta;      // with one piece
 };
 
@@ -132,6 +141,7 @@ __global__ void __launch_bounds__(64 * WN * WK, TN * TK >= 16 ? 2 : 4)
   __shared__ int changed[2][C::WAVES];                          // a wave's unit set some
   __shared__ int expo[PAIRS ? C::ROWS : 1];
   __shared__ int special[C::WAVES];
+  __shared__ double bsum[4 * C::OQ][C::BN];  // g's sums, a slot a thread and column
 
   // The pieces go round the XCDs, a piece's tiles to one of them, whose L2 then
   // holds the rows that they share.
@@ -151,51 +161,103 @@ __global__ void __launch_bounds__(64 * WN * WK, TN * TK >= 16 ? 2 : 4)
   const int group = (is_g ? wave : wave - C::GA * C::OQ) / C::OQ, oq = wave % C::OQ;  // (GA OQ is a multiple of OQ)
   const int col = (is_g ? n0 : k0) + group * 16 * V + V * c, left = (is_g ? a.N : a.K) - col;
   const int64_t ld = is_g ? a.ldg : a.ldx;
-  const int oct = 4 * oq + g;  // this thread's eight rows of a step
+  // (16 consecutive lanes write two octets' chunks, as a read's groups of lanes meet them: no bank twice)
+  const int gs = g ^ (((c >> 2) + 1) >> 1 & 1), oct = 4 * oq + gs;  // this thread's eight rows of a step
   const int row0 = (is_g ? 0 : C::BN) + group * 16 * V + c;  // its LDS rows: row0 + 16 j
-  const T* src = (is_g ? G : X) + (int64_t(first) + 8 * oct) * ld + col;
+  // Every load lands in the operand: columns past its last are read as its last V
+  // (`mend` moves and drops them), or where it has fewer than V one by one; rows
+  // past the piece's last as that one.
+  const int cols = is_g ? a.N : a.K;
+  const bool narrow = cols < V, whole = col - V * c + 16 * V <= cols;  // of the unit: wave-uniform
+  const T* src = (is_g ? G : X) + (int64_t(first) + 8 * oct) * ld + (narrow ? 0 : min(col, cols - V));
+  const int64_t ahead = int64_t(C::STEP) * ld;
   unsigned raw[8][W];
   auto load = [&](int s) {
-    const int rows = last - first - s * C::STEP - 8 * oct;
-    const T* p = src + int64_t(s) * C::STEP * ld;
+    if (!reads) return;
+    const T* p = src;
+    src += ahead;
+    int rows = 8;
+    if ((s + 1) * C::STEP > last - first) {  // the piece's last, partial step
+      rows = last - first - s * C::STEP - 8 * oct;
+      if (rows < 1) p -= (1 - rows) * ld, rows = 1;
+    }
+    if (narrow) {
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+          if constexpr (PAIRS) raw[r][w] = __float_as_uint(p[min(col + w, cols - 1)]);
+          else
+            raw[r][w] = unsigned(__builtin_bit_cast(unsigned short, p[min(col + 2 * w, cols - 1)])) |
+                        unsigned(__builtin_bit_cast(unsigned short, p[min(col + 2 * w + 1, cols - 1)])) << 16;
+        }
+        p += r + 1 < rows ? ld : 0;
+      }
+      return;
+    }
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
-#pragma unroll
-      for (int w = 0; w < W; ++w) raw[r][w] = 0;
-      if (reads && r < rows) {
-        if (left >= V) {
-          if constexpr (W == 4) {
-            const u4u q = *reinterpret_cast<const u4u*>(p + r * ld);
-            raw[r][0] = q[0], raw[r][1] = q[1], raw[r][2] = q[2], raw[r][3] = q[3];
-          } else {
-            const u2u q = *reinterpret_cast<const u2u*>(p + r * ld);
-            raw[r][0] = q[0], raw[r][1] = q[1];
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < V; ++j)
-            if (j < left) {
-              if constexpr (PAIRS) raw[r][j] = __float_as_uint(p[r * ld + j]);
-              else raw[r][j / 2] |= unsigned(__builtin_bit_cast(unsigned short, p[r * ld + j])) << (16 * (j & 1));
-            }
-        }
+      if constexpr (W == 4) {
+        const u4u q = *reinterpret_cast<const u4u*>(p);
+        raw[r][0] = q[0], raw[r][1] = q[1], raw[r][2] = q[2], raw[r][3] = q[3];
+      } else {
+        const u2u q = *reinterpret_cast<const u2u*>(p);
+        raw[r][0] = q[0], raw[r][1] = q[1];
       }
+      p += r + 1 < rows ? ld : 0;
     }
   };
+  // Zeros for the rows and columns that are not the piece's.
+  auto mend = [&](int s) {
+    const int rows = last - first - s * C::STEP - 8 * oct;
+    constexpr int PER = V / W;  // elements a word
+    if (!whole) {
+      const int up = narrow ? 0 : min(max(V - left, 0), V - 1);  // elements to move down
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+          unsigned x[W + 1];
+#pragma unroll
+          for (int i = 0; i <= W; ++i) x[i] = w + i < W ? raw[r][w + i] : 0u;
+          unsigned lo = 0, hi = 0;
+#pragma unroll
+          for (int i = 0; i < W; ++i)
+            if (up / PER == i) lo = x[i], hi = x[i + 1];
+          unsigned v = PER == 2 && (up & 1) ? lo >> 16 | hi << 16 : lo;
+          const int n = left - w * PER;  // elements of the word that are the operand's
+          raw[r][w] = n >= PER ? v : PER == 2 && n == 1 ? v & 0xffffu : 0u;
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+#pragma unroll
+      for (int w = 0; w < W; ++w) raw[r][w] = r < rows ? raw[r][w] : 0u;
+  };
 
-  float scale[PAIRS ? V : 1], limit[PAIRS ? V : 1];
+  float scale[PAIRS ? V : 1];  // of each column, 2^126 until a value is too large for that
 #pragma unroll
-  for (int j = 0; j < (PAIRS ? V : 1); ++j) scale[j] = 1.f, limit[j] = 0.f;
-  double bsum[V];
+  for (int j = 0; j < (PAIRS ? V : 1); ++j) scale[j] = 0x1p126f;
+  // (a column's tiles share out the steps whose g they sum)
+  const bool bias = a.bout && is_g && reads;
+  const int kt = tile % a.tiles_k;
+  int turn = 0;
+  double* mine = &bsum[oct][(is_g ? group : 0) * 16 * V + c];  // LDS rows' order, as row0
+  float few[V];  // of sixteen steps, then added there (every step: a tenth of the whole time)
 #pragma unroll
-  for (int j = 0; j < V; ++j) bsum[j] = 0.0;
-  const bool bias = a.bout && is_g && k0 == 0 && reads;
+  for (int j = 0; j < V; ++j) few[j] = 0.f;
+  if (bias)
+#pragma unroll
+    for (int j = 0; j < V; ++j) mine[16 * j] = 0.0;
   int inf = 0;
 
   // the step that `load` read, into LDS
   auto put = [&](int s) {
     if (!reads) return;
+    if (!whole || (s + 1) * C::STEP > last - first) mend(s);
     u4* to = stage + (s & 1) * C::STAGE;
+    const bool sums = bias && turn == kt;
+    turn = turn + 1 == a.tiles_k ? 0 : turn + 1;
     if constexpr (PAIRS) {
       unsigned x[V][8];
 #pragma unroll
@@ -205,18 +267,17 @@ __global__ void __launch_bounds__(64 * WN * WK, TN * TK >= 16 ? 2 : 4)
       float m[V];
       bool grew = false;
 #pragma unroll
-      for (int j = 0; j < V; ++j) m[j] = amax8(x[j]), grew |= m[j] > limit[j];
+      for (int j = 0; j < V; ++j) m[j] = amax8(x[j]), grew |= m[j] * scale[j] > 32768.f;
       const bool any = __builtin_amdgcn_ballot_w64(grew) != 0;
       if (any) {
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           const float top = max_g(m[j]);
           float f = 1.f;
-          if (top > limit[j]) {
-            const int k = min(12 - __builtin_amdgcn_frexp_expf(fminf(top, kFltMax)), 126);
-            f = limit[j] > 0.f ? __builtin_amdgcn_ldexpf(limit[j], k - 15) : 0.f;
+          if (top * scale[j] > 32768.f) {
+            const int k = 12 - __builtin_amdgcn_frexp_expf(fminf(top, kFltMax));
+            f = __builtin_amdgcn_ldexpf(1.f, k + 1 - __builtin_amdgcn_frexp_expf(scale[j]));
             scale[j] = __builtin_amdgcn_ldexpf(1.f, k);
-            limit[j] = fminf(__builtin_amdgcn_ldexpf(1.f, 15 - k), kFltMax);
           }
           inf |= top > kFltMax;
           if (g == 0) factor[s & 1][row0 + 16 * j] = f;
@@ -228,17 +289,18 @@ __global__ void __launch_bounds__(64 * WN * WK, TN * TK >= 16 ? 2 : 4)
       for (int j = 0; j < V; ++j) {
         u4 hi, lo;
         split8(x[j], neg ? -scale[j] : scale[j], hi, lo);
-        to[slot(g, 0, row0 + 16 * j)] = hi;
-        to[slot(g, 1, row0 + 16 * j)] = lo;
-        if (bias) {
+        to[slot(gs, 0, row0 + 16 * j)] = hi;
+        to[slot(gs, 1, row0 + 16 * j)] = lo;
+        if (sums) {
           float t[8];
 #pragma unroll
           for (int r = 0; r < 8; ++r) t[r] = __uint_as_float(x[j][r]);
-          bsum[j] += ((t[0] + t[1]) + (t[2] + t[3])) + ((t[4] + t[5]) + (t[6] + t[7]));
+          few[j] += ((t[0] + t[1]) + (t[2] + t[3])) + ((t[4] + t[5]) + (t[6] + t[7]));
         }
       }
     } else {
       const unsigned flip = is_g && (s & 1) ? 0x80008000u : 0u;
+      const unsigned one = (std::is_same<T, __bf16>::value ? 0x3f803f80u : 0x3c003c00u) ^ flip;
 #pragma unroll
       for (int w = 0; w < W; ++w) {
         u4 even, odd;
@@ -247,19 +309,19 @@ __global__ void __launch_bounds__(64 * WN * WK, TN * TK >= 16 ? 2 : 4)
           even[d] = __builtin_amdgcn_perm(raw[2 * d + 1][w], raw[2 * d][w], 0x05040100u) ^ flip;
           odd[d] = __builtin_amdgcn_perm(raw[2 * d + 1][w], raw[2 * d][w], 0x07060302u) ^ flip;
         }
-        to[slot(g, oq, row0 + 32 * w)] = even;
-        to[slot(g, oq, row0 + 32 * w + 16)] = odd;
-        if (bias) {
+        if (sums)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float t[8];
-#pragma unroll
-            for (int r = 0; r < 8; ++r) t[r] = half_of<T>(raw[r][w], h);
-            bsum[2 * w + h] += ((t[0] + t[1]) + (t[2] + t[3])) + ((t[4] + t[5]) + (t[6] + t[7]));
+          for (int d = 0; d < 4; ++d) {
+            few[2 * w] = dot2<T>(even[d], one, few[2 * w]);
+            few[2 * w + 1] = dot2<T>(odd[d], one, few[2 * w + 1]);
           }
-        }
+        to[slot(gs, oq, row0 + 32 * w)] = even;
+        to[slot(gs, oq, row0 + 32 * w + 16)] = odd;
       }
     }
+    if (bias && ((s & 15) == 15 || (s + 1) * C::STEP >= last - first))
+#pragma unroll
+      for (int j = 0; j < V; ++j) mine[16 * j] += double(few[j]), few[j] = 0.f;
   };
 
   // ---- this wave's products
@@ -291,15 +353,18 @@ __global__ void __launch_bounds__(64 * WN * WK, TN * TK >= 16 ? 2 : 4)
           }
       }
     }
+    __builtin_amdgcn_s_setprio(1);
     u4 b[TK][2];
 #pragma unroll
     for (int j = 0; j < TK; ++j)
 #pragma unroll
       for (int h = 0; h < 2; ++h) b[j][h] = from[slot(g, h, rk + 16 * j + c)];
     const float sg = s & 1 ? -1.f : 1.f;
+    u4 x = from[slot(g, 0, rn + c)], y = from[slot(g, 1, rn + c)];
 #pragma unroll
     for (int i = 0; i < TN; ++i) {
-      const u4 x = from[slot(g, 0, rn + 16 * i + c)], y = from[slot(g, 1, rn + 16 * i + c)];
+      const int ahead = rn + 16 * (i + 1 < TN ? i + 1 : i) + c;
+      const u4 nx = from[slot(g, 0, ahead)], ny = from[slot(g, 1, ahead)];
 #pragma unroll
       for (int j = 0; j < TK; ++j) {
         f4 t = {0.f, 0.f, 0.f, 0.f};
@@ -314,19 +379,38 @@ __global__ void __launch_bounds__(64 * WN * WK, TN * TK >= 16 ? 2 : 4)
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(t[e], sg, acc[i][j][e]);
       }
+      x = nx, y = ny;
     }
+    __builtin_amdgcn_s_setprio(0);
   };
 
   if (steps > 0) {
     load(0);
-    put(0);
-    if (steps > 1) load(1);
-    ring_barrier();
-    for (int s = 0; s < steps; ++s) {
-      if (s + 1 < steps) put(s + 1);
-      if (s + 2 < steps) load(s + 2);
-      products(s);
+    if constexpr (C::WAVES == 8) {
+      // Two waves a SIMD, half a step apart: while one of them splits its rows
+      // into LDS the other has the matrix unit. (All in step: 1289 us against 1227
+      // for 486946 x 2048 x 512 in bf16, 1197 with the products' priority raised.)
+      const bool late = wave >= 4;
+      if (late) ring_barrier();
+      for (int i = 0; i < steps + !late; ++i) {
+        if (i < steps) put(i);
+        if (i + 1 < steps) load(i + 1);
+        ring_barrier();
+        const int p = late ? i : i - 1;
+        if (p >= 0) products(p);
+        ring_barrier();
+      }
+      if (late) ring_barrier();
+    } else {
+      put(0);
+      if (steps > 1) load(1);
       ring_barrier();
+      for (int s = 0; s < steps; ++s) {
+        if (s + 1 < steps) put(s + 1);
+        if (s + 2 < steps) load(s + 2);
+        products(s);
+        ring_barrier();
+      }
     }
   }
 
@@ -338,18 +422,16 @@ __global__ void __launch_bounds__(64 * WN * WK, TN * TK >= 16 ? 2 : 4)
       for (int j = 0; j < V; ++j) expo[row0 + 16 * j] = 1 - __builtin_amdgcn_frexp_expf(scale[j]);
     if (__builtin_amdgcn_ballot_w64(inf) != 0 && l == 0) special[wave] = 1;
   }
-  double* bs = reinterpret_cast<double*>(stage);  // [8 rows' groups][BN]
-  if (bias)
-#pragma unroll
-    for (int j = 0; j < V; ++j) bs[oct * C::BN + group * 16 * V + V * c + j] = bsum[j];
   __syncthreads();
-  if (a.bout && k0 == 0)
-    for (int i = threadIdx.x; i < C::BN; i += 64 * C::WAVES)
-      if (n0 + i < a.N) {
+  if (a.bout)
+    for (int r = threadIdx.x; r < C::BN; r += 64 * C::WAVES) {
+      const int n = n0 + r / (16 * V) * 16 * V + r % 16 * V + r / 16 % V;
+      if (n < a.N) {
         double v = 0.0;
-        for (int q = 0; q < 4 * C::OQ; ++q) v += bs[q * C::BN + i];
-        a.bout[int64_t(piece) * a.N + n0 + i] = v;
+        for (int q = 0; q < 4 * C::OQ; ++q) v += bsum[q][r];
+        a.bout[(int64_t(piece) * a.tiles_k + kt) * a.N + n] = v;
       }
+    }
 
   // columns of LDS rows: row 16 j + i of a group is column V i + j
   auto n_of = [&](int i, int e) {
@@ -438,7 +520,7 @@ __global__ void __launch_bounds__(64 * WN * WK, TN * TK >= 16 ? 2 : 4)
 // (One thread an element, its loads one after the other: 24 us for 80 pieces of
 // 768 x 256 against 8.)
 constexpr int kStrips = 8;
-__global__ void __launch_bounds__(256) wgrad_sum_kernel(int N, int K, int pieces, const float* __restrict__ part,
+__global__ void __launch_bounds__(256) wgrad_sum_kernel(int N, int K, int pieces, int bpieces, const float* __restrict__ part,
                                                         const double* __restrict__ bpart, float* __restrict__ w_adj,
                                                         int64_t ldw, float* __restrict__ b_adj, float beta) {
   __shared__ double sums[kStrips][32][4];
@@ -448,7 +530,7 @@ __global__ void __launch_bounds__(256) wgrad_sum_kernel(int N, int K, int pieces
   const int64_t i = (int64_t(blockIdx.x) - (bias ? wblocks : 0)) * 128 + 4 * q, n = bias ? N : nk;
   double v[4] = {0.0, 0.0, 0.0, 0.0};
   if (bias) {
-    for (int s = strip; s < pieces; s += kStrips)
+    for (int s = strip; s < bpieces; s += kStrips)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         if (i + e < n) v[e] += bpart[int64_t(s) * N + i + e];
@@ -496,25 +578,31 @@ struct Plan {
 constexpr int kEdge[3] = {256, 128, 64};
 constexpr int kResident[3] = {256, 512, 1024};  // workgroups that the chip holds at once
 
+// The largest tile that the result fills and the work feeds. MI355X, us a call:
+//   256 against 128 wide: 122688 x 768 x 256 in fp32 198 and 249, 8192 x 1024 x 1024 93 and 102, 62001 x
+//     500 x 333 156 and 158, 20011 x 1000 x 330 in fp16 64 and 66;
+//   128 against 64 wide: 26670 x 1024 x 128 62 and 72, 27318 x 128 x 128 (4.5e8 products) 34 and 42, but
+//     648 x 1024 x 256 (1.7e8) 23.6 and 20.5: its few steps wait on memory, not on the tile.
+// Pieces fill the chip, in whole eights (an XCD each in turn), of at least four
+// steps (27318 x 128 x 128: 34 us, 41 with two and 46 with sixteen).
 Plan plan_of(int dtype, int M, int N, int K) {
   const int step = dtype == PET_DTYPE_F32 ? 32 : 64;
+  const double work = double(M) * N * K;
   Plan p{};
-  auto tiles = [&](int t) {
-    return ((int64_t(N) + kEdge[t] - 1) / kEdge[t]) * ((int64_t(K) + kEdge[t] - 1) / kEdge[t]);
-  };
-  p.tile = 2;
-  if (N > 64 && K > 64) p.tile = 1;
-  if (N > 128 && K > 128 && double(M) * N * K >= 4e9) p.tile = 0;
-  const int64_t t = tiles(p.tile), steps = std::max<int64_t>(1, (int64_t(M) + step - 1) / step);
-  int64_t pieces = std::max<int64_t>(1, std::min<int64_t>(kResident[p.tile] / t, (steps + 3) / 4));
+  p.tile = N > 128 && K > 128 && work >= 4e9 ? 0 : N > 64 && K > 64 && work >= 3e8 ? 1 : 2;
+  const int64_t edge = kEdge[p.tile], tn = (int64_t(N) + edge - 1) / edge, tk = (int64_t(K) + edge - 1) / edge;
+  const int64_t steps = std::max<int64_t>(1, (int64_t(M) + step - 1) / step);
+  int64_t pieces = std::max<int64_t>(1, std::min<int64_t>(kResident[p.tile] / (tn * tk), (steps + 3) / 4));
   if (pieces > 8) pieces &= ~int64_t(7);
   p.chunk = (steps + pieces - 1) / pieces * step;
   p.pieces = int(std::max<int64_t>(1, (int64_t(M) + p.chunk - 1) / p.chunk));
-  if (p.pieces > 8) p.pieces = int(std::min<int64_t>(pieces, (p.pieces + 7) & ~7));
-  p.tiles_n = (N + kEdge[p.tile] - 1) / kEdge[p.tile], p.tiles_k = (K + kEdge[p.tile] - 1) / kEdge[p.tile];
+  if (p.pieces > 8) p.pieces = (p.pieces + 7) & ~7;
+  p.tiles_n = int(tn), p.tiles_k = int(tk);
   return p;
 }
-size_t bias_bytes(const Plan& p, int N) { return (size_t(p.pieces) * N * sizeof(double) + 15) & ~size_t(15); }
+size_t bias_bytes(const Plan& p, int N) {
+  return (size_t(p.pieces) * p.tiles_k * N * sizeof(double) + 15) & ~size_t(15);
+}
 
 }  // namespace pet_wgrad
 
@@ -548,7 +636,7 @@ int pet_linear_grads_run(int dtype, int M, int N, int K, const void* out_adj, in
   const int64_t blocks = (p.pieces > 1 ? (int64_t(N) * K + 127) / 128 : 0) + (b_adj ? (int64_t(N) + 127) / 128 : 0);
   if (blocks == 0) return PET_ATTN_OK;
   hipLaunchKernelGGL(wgrad_sum_kernel, dim3(unsigned(blocks)), dim3(256), 0, st, N, K, p.pieces,
-                     p.pieces > 1 ? part : nullptr, bpart, w_adj, ldw, b_adj, beta);
+                     p.pieces * p.tiles_k, p.pieces > 1 ? part : nullptr, bpart, w_adj, ldw, b_adj, beta);
   return hipGetLastError() == hipSuccess ? int(PET_ATTN_OK) : int(PET_ATTN_ELAUNCH);
 }
 
