@@ -101,6 +101,10 @@ def _typed(t: torch.Tensor, name: str, rows: int, width: int, dtype: torch.dtype
     """The leading dimension of a row-major [rows, width] view of the dtype on the device."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name}: a torch tensor is needed")
+    if t.dtype is dtype and t.shape == (rows, width) and t.device == device and rows > 1 and width > 1:
+        ld, step = t.stride()  # (what a small call's host side waits for: the checks below again, in one go)
+        if step == 1 and ld >= width and device.type == "cuda" and dtype in DTYPES:
+            return ld
     if t.device != device or t.device.type != "cuda":
         raise ValueError(f"{name}: on {t.device}, the operands' device is {device}")
     if t.dtype != dtype or t.dtype not in DTYPES:
@@ -149,11 +153,15 @@ def _scratch(t, nbytes: int, device) -> torch.Tensor:
 
 def _call_on(device, what: str, fn, *args) -> None:
     """fn(*args, stream) with the device's current stream, the device current."""
-    if device.index == torch.cuda.current_device():
-        _lib.check(fn(*args, torch.cuda.current_stream(device).cuda_stream), what)
+    index = device.index
+    stream = torch._C._cuda_getCurrentRawStream(index)  # torch.cuda.current_stream(device).cuda_stream, 2 us less
+    if index == torch.cuda.current_device():
+        code = fn(*args, stream)
     else:
-        with torch.cuda.device(device):
-            _lib.check(fn(*args, torch.cuda.current_stream(device).cuda_stream), what)
+        with torch.cuda.device(index):
+            code = fn(*args, stream)
+    if code != _lib.OK:
+        raise _lib.PetAttnError(code, what)
 
 
 def shape(N: int, T: int, S: int, heads: int, head_dim: int, temperature: float = 1.0,

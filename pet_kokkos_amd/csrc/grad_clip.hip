@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(256) grad_norm_kernel(Batch b, double* __restr
       using T = decltype(tv);
       chunk_each<T>(b, i, q, [&](T* at, int64_t left) {
         float x[pet_typed::kVec<T>];
-        pet_typed::load<T>(at, left, x);
+        pet_typed::load<T>(at, 0, left, x);
 #pragma unroll
         for (int e = 0; e < pet_typed::kVec<T>; ++e) v[e & 3] = take<p>(v[e & 3], x[e]);
       });
@@ -160,7 +160,7 @@ __global__ void __launch_bounds__(256) grad_clip_kernel(Batch b, Ends a, const d
       using T = decltype(tv);
       chunk_each<T>(b, i, q, [&](T* at, int64_t left) {
         float x[pet_typed::kVec<T>];
-        pet_typed::load<T>(at, left, x);
+        pet_typed::load<T>(at, 0, left, x);
 #pragma unroll
         for (int e = 0; e < pet_typed::kVec<T>; ++e) x[e] *= f;
         pet_typed::store<T>(at, left, x);

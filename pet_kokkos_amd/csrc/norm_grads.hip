@@ -36,7 +36,7 @@ constexpr int threads_of(int TPR) { return TPR > 256 ? TPR : 256; }
 // the two sums, and the next row's raw ones): the registers are held to it, so
 // that a grid of it fills the chip in one round. (1024 workgroups of which 768
 // fitted took two: 65536 x 1024 in bf16 131 us.)
-constexpr int waves_of(int E) { return E <= 4 ? 8 : E <= 8 ? 5 : E <= 16 ? 3 : 2; }
+constexpr int waves_of(int E, int TPR) { return TPR == 1024 ? 4 : E <= 4 ? 8 : E <= 8 ? 5 : E <= 16 ? 3 : 2; }
 // 1 / sqrt(x): the hardware's estimate and a Newton step.
 __device__ __forceinline__ float rsqrt_nr(float x) {
   const float y = __builtin_amdgcn_rsqf(x);
@@ -92,24 +92,10 @@ __device__ __forceinline__ void row_sums(float (&x)[n], float (*red)[2][3], int&
 
 // A thread's share of a row as it lies in memory: C chunks of kVec elements, chunk
 // j at kVec (t + TPR j), zeros past the width.
-template <class T, int TPR, int C>
+template <class T, int TPR, int C, bool WHOLE>
 __device__ __forceinline__ void load_row(const T* row, int width, int t, u4e (&q)[C]) {
 #pragma unroll
-  for (int j = 0; j < C; ++j) {
-    const int d = kVec<T> * (t + TPR * j), left = width - d;
-    q[j] = u4e{0u, 0u, 0u, 0u};
-    if (left >= kVec<T>) {
-      q[j] = *reinterpret_cast<const u4e*>(row + d);
-    } else if (left > 0) {  // every load in flight, then those past the row's end dropped
-      T v[kVec<T>];
-#pragma unroll
-      for (int e = 0; e < kVec<T>; ++e) v[e] = row[d + min(e, left - 1)];
-#pragma unroll
-      for (int e = 0; e < kVec<T>; ++e)
-        if constexpr (sizeof(T) == 4) q[j][e] = e < left ? __float_as_uint(v[e]) : 0u;
-        else q[j][e / 2] |= e < left ? unsigned(__builtin_bit_cast(unsigned short, v[e])) << (16 * (e & 1)) : 0u;
-    }
-  }
+  for (int j = 0; j < C; ++j) q[j] = pet_typed::load_raw<T, WHOLE, TPR == 16>(row, kVec<T> * (t + TPR * j), width);
 }
 // n floats of a vector at d, zeros past the width.
 template <int n>
@@ -139,7 +125,7 @@ __device__ __forceinline__ void center(float (&x)[n], float mu, int left) {
   }
 }
 
-template <class T, int TPR, int C>
+template <class T, int TPR, int C, bool WHOLE>
 __global__ void __launch_bounds__(threads_of(TPR)) norm_typed_fwd_kernel(int rows, int width, float per, T* __restrict__ out,
                                                                          int64_t ldo, const T* __restrict__ in,
                                                                          int64_t ldi, const float* __restrict__ weight,
@@ -152,7 +138,7 @@ __global__ void __launch_bounds__(threads_of(TPR)) norm_typed_fwd_kernel(int row
   int turn = 0;
   u4e q[C];
   float x[C][V];
-  load_row<T, TPR, C>(in + r * ldi, width, t, q);
+  load_row<T, TPR, C, WHOLE>(in + r * ldi, width, t, q);
   float mu = 0.f;
 #pragma unroll
   for (int j = 0; j < C; ++j) pet_typed::unpack<T>(q[j], x[j]);
@@ -190,13 +176,14 @@ __global__ void __launch_bounds__(threads_of(TPR)) norm_typed_fwd_kernel(int row
 
 // in_adj for rows < n_node onto beta_node times itself, for the rows after onto
 // beta_edge; in_adj null: the parameters' gradients alone. part [gridDim.x][2][width]:
-// this workgroup's sums (null: in_adj alone).
-template <class T, int TPR, int C, bool LN>
-__global__ void __launch_bounds__(threads_of(TPR), waves_of(C * kVec<T>))
+// this workgroup's sums (null: in_adj alone); of one workgroup they are the
+// gradients, and go onto beta_w times w_adj and b_adj themselves.
+template <class T, int TPR, int C, bool WHOLE, bool LN>
+__global__ void __launch_bounds__(threads_of(TPR), waves_of(C * kVec<T>, TPR))
     norm_grads_kernel(int rows, int width, float per, T* __restrict__ in_adj, int64_t lda,
                       const T* __restrict__ out_adj, int64_t ldg, const T* __restrict__ in, int64_t ldi, const float* __restrict__ weight, int n_node,
                       float beta_node, float beta_edge, int live_base, const int* __restrict__ live,
-                      float* __restrict__ part) {
+                      float* __restrict__ part, float* __restrict__ w_adj, float* __restrict__ b_adj, float beta_w) {
   constexpr int V = kVec<T>, RPB = threads_of(TPR) / TPR;
   __shared__ float red[TPR > 64 ? TPR / 64 : 1][2][3];
   const int t = threadIdx.x % TPR, g0 = threadIdx.x / TPR;
@@ -214,20 +201,20 @@ __global__ void __launch_bounds__(threads_of(TPR), waves_of(C * kVec<T>))
   constexpr bool AHEAD = C * V <= 16;  // (a lane of 32 elements has no registers for the next row's)
   u4e qx[C], qg[C];
   if (AHEAD && r < end) {
-    load_row<T, TPR, C>(in + r * ldi, width, t, qx);
-    load_row<T, TPR, C>(out_adj + r * ldg, width, t, qg);
+    load_row<T, TPR, C, WHOLE>(in + r * ldi, width, t, qx);
+    load_row<T, TPR, C, WHOLE>(out_adj + r * ldg, width, t, qg);
   }
   for (; r < end; r += step) {
     float x[C][V], g[C][V], mu = 0.f;
     if (!AHEAD) {
-      load_row<T, TPR, C>(in + r * ldi, width, t, qx);
-      load_row<T, TPR, C>(out_adj + r * ldg, width, t, qg);
+      load_row<T, TPR, C, WHOLE>(in + r * ldi, width, t, qx);
+      load_row<T, TPR, C, WHOLE>(out_adj + r * ldg, width, t, qg);
     }
 #pragma unroll
     for (int j = 0; j < C; ++j) pet_typed::unpack<T>(qx[j], x[j]), pet_typed::unpack<T>(qg[j], g[j]);
     if (AHEAD && r + step < end) {  // the next row, while this one is worked on
-      load_row<T, TPR, C>(in + (r + step) * ldi, width, t, qx);
-      load_row<T, TPR, C>(out_adj + (r + step) * ldg, width, t, qg);
+      load_row<T, TPR, C, WHOLE>(in + (r + step) * ldi, width, t, qx);
+      load_row<T, TPR, C, WHOLE>(out_adj + (r + step) * ldg, width, t, qg);
     }
     if (LN) {
       float s[1] = {0.f};
@@ -262,7 +249,8 @@ __global__ void __launch_bounds__(threads_of(TPR), waves_of(C * kVec<T>))
       const int d = V * (t + TPR * j);
       if (d < width) {
         float o[V];
-        if (in_adj && beta != 0.f) pet_typed::load<T>(a_row + d, width - d, o);
+        if (in_adj && beta != 0.f)
+          pet_typed::unpack<T>(pet_typed::load_raw<T, WHOLE, TPR == 16>(a_row, d, width), o);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           const float xh = x[j][e] * inv;
@@ -302,6 +290,12 @@ __global__ void __launch_bounds__(threads_of(TPR), waves_of(C * kVec<T>))
   };
   put(dw, p);
   if (LN) put(db, p + width);
+  if (gridDim.x > 1) return;
+  __syncthreads();
+  for (int d = threadIdx.x; d < width; d += threads_of(TPR)) {
+    if (w_adj) w_adj[d] = beta_w != 0.f ? fmaf(beta_w, w_adj[d], p[d]) : p[d];
+    if (LN && b_adj) b_adj[d] = beta_w != 0.f ? fmaf(beta_w, b_adj[d], p[width + d]) : p[width + d];
+  }
 }
 
 // adj = beta adj + the sum of the parts, in double: 16 columns by 64 strips of
@@ -385,21 +379,26 @@ int pet_norm_grads_sink(int dtype, int rows, int width, void* in_adj, int64_t ld
     return with_row<T>(width, [&](auto lc, auto cc) {
       constexpr int TPR = decltype(lc)::value, C = decltype(cc)::value, TH = threads_of(TPR), RPB = TH / TPR;
       // as many workgroups as the chip holds at once, each with the same rows to within one
-      constexpr int most = kCus * (waves_of(C * kVec<T>) * 256 / TH);
+      constexpr int most = kCus * (waves_of(C * kVec<T>, TPR) * 256 / TH);
       static_assert(most <= kMaxParts, "the workspace's rows");
-      const int64_t groups = std::max<int64_t>(1, (int64_t(rows) + RPB - 1) / RPB), each = (groups + most - 1) / most;
+      // (few rows are one workgroup's, which spares a launch)
+      const int64_t groups = std::max<int64_t>(1, (int64_t(rows) + RPB - 1) / RPB);
+      const int64_t each = part && groups <= 4 ? groups : (groups + most - 1) / most;
       blocks = int((groups + each - 1) / each);
       auto run = [&](auto lnc) {
-        hipLaunchKernelGGL((norm_grads_kernel<T, TPR, C, decltype(lnc)::value>), dim3(unsigned(blocks)), dim3(TH), 0, st,
+        constexpr bool LN = decltype(lnc)::value;
+        const auto kernel = width % kVec<T> ? norm_grads_kernel<T, TPR, C, false, LN> : norm_grads_kernel<T, TPR, C, true, LN>;
+        hipLaunchKernelGGL(kernel, dim3(unsigned(blocks)), dim3(TH), 0, st,
                            rows, width, 1.0f / width, static_cast<T*>(in_adj), lda, static_cast<const T*>(out_adj), ldg,
-                           static_cast<const T*>(in), ldi, weight, n_node, beta_node, beta_edge, live_base, live, part);
+                           static_cast<const T*>(in), ldi, weight, n_node, beta_node, beta_edge, live_base, live, part,
+                           w_adj, b_adj, beta_w);
       };
       if (ln) run(std::true_type{});
       else run(std::false_type{});
       return hipGetLastError() == hipSuccess ? int(PET_ATTN_OK) : int(PET_ATTN_ELAUNCH);
     });
   });
-  if (e || !parts) return e;
+  if (e || !parts || blocks == 1) return e;
   hipLaunchKernelGGL(norm_parts_kernel, dim3(unsigned((width + 15) / 16), ln ? 2 : 1), dim3(1024), 0, st, blocks, width,
                      part, w_adj, b_adj, beta_w);
   return hipGetLastError() == hipSuccess ? int(PET_ATTN_OK) : int(PET_ATTN_ELAUNCH);
@@ -422,7 +421,8 @@ int pet_norm_rows_typed(int dtype, int rows, int width, void* out, int64_t ldo, 
     using T = decltype(tv);
     return with_row<T>(width, [&](auto lc, auto cc) {
       constexpr int TPR = decltype(lc)::value, C = decltype(cc)::value, TH = threads_of(TPR), RPB = TH / TPR;
-      hipLaunchKernelGGL((norm_typed_fwd_kernel<T, TPR, C>), dim3(unsigned((int64_t(rows) + RPB - 1) / RPB)), dim3(TH),
+      const auto kernel = width % kVec<T> ? norm_typed_fwd_kernel<T, TPR, C, false> : norm_typed_fwd_kernel<T, TPR, C, true>;
+      hipLaunchKernelGGL(kernel, dim3(unsigned((int64_t(rows) + RPB - 1) / RPB)), dim3(TH),
                          0, reinterpret_cast<hipStream_t>(stream), rows, width, 1.0f / width, static_cast<T*>(out), ldo,
                          static_cast<const T*>(in), ldi, weight, bias);
       return hipGetLastError() == hipSuccess ? int(PET_ATTN_OK) : int(PET_ATTN_ELAUNCH);

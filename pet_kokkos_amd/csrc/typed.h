@@ -48,17 +48,41 @@ __device__ __forceinline__ u4e pack(const float (&x)[kVec<T>]) {
   }
   return q;
 }
-// n elements at p (at least one; from the vector's on: all of it), zeros past them.
-template <class T>
-__device__ __forceinline__ void load(const T* p, int64_t n, float (&x)[kVec<T>]) {
-  if (n >= kVec<T>) {
-    unpack<T>(*reinterpret_cast<const u4e*>(p), x);
+// The 16 bytes at element d of a row of n, as they lie, with zeros past its end.
+// whole: n is a multiple of the vector. Else the row's last 16 bytes, moved down, or
+// (few: n may be less than a vector) its elements one by one.
+template <class T, bool whole = false, bool few = true>
+__device__ __forceinline__ u4e load_raw(const T* row, int64_t d, int64_t n) {
+  constexpr int V = kVec<T>, BITS = 8 * int(sizeof(T));
+  u4e q = {0u, 0u, 0u, 0u};
+  if constexpr (whole) {
+    if (d < n) q = *reinterpret_cast<const u4e*>(row + d);
+  } else if (!few || n >= V) {
+    if (d < n) {
+      q = *reinterpret_cast<const u4e*>(row + (d + V <= n ? d : n - V));
+      if (d + V > n) {
+        uint64_t lo = uint64_t(q[1]) << 32 | q[0], hi = uint64_t(q[3]) << 32 | q[2];
+        const int by = int(d + V - n) * BITS;  // 16 .. 112 bits
+        lo = by >= 64 ? hi >> (by - 64) : lo >> by | hi << (64 - by);
+        hi = by >= 64 ? 0 : hi >> by;
+        q = u4e{unsigned(lo), unsigned(lo >> 32), unsigned(hi), unsigned(hi >> 32)};
+      }
+    }
   } else {
+#pragma unroll 1
+    for (int i = 0; i < int(n - d); ++i) {
+      unsigned v;
+      if constexpr (BITS == 32) v = __float_as_uint(row[d + i]);
+      else v = unsigned(__builtin_bit_cast(unsigned short, row[d + i])) << (16 * (i & 1));
 #pragma unroll
-    for (int i = 0; i < kVec<T>; ++i) x[i] = float(p[min(int64_t(i), n - 1)]);  // (all in flight)
-#pragma unroll
-    for (int i = 0; i < kVec<T>; ++i) x[i] = i < n ? x[i] : 0.f;
+      for (int w = 0; w < 4; ++w) q[w] |= w == i * BITS / 32 ? v : 0u;
+    }
   }
+  return q;
+}
+template <class T>
+__device__ __forceinline__ void load(const T* row, int64_t d, int64_t n, float (&x)[kVec<T>]) {
+  unpack<T>(load_raw<T>(row, d, n), x);
 }
 template <class T>
 __device__ __forceinline__ void store(T* p, int64_t n, const float (&x)[kVec<T>]) {
