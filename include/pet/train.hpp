@@ -1,0 +1,116 @@
+// pet/train.hpp -- what a training step adds, for a C++ caller: the norm's and a
+// dense layer's parameter gradients, an attention layer's, and the norm and
+// clipping of them all (pet_norm_rows_grads, pet_linear_grads,
+// pet_attention_layer_grads, pet_grad_norm, pet_grad_clip). The reference
+// (peterspackman/pet-kokkos) evaluates only, so none of it has a counterpart
+// there; the views, the Workspace that holds the scratch and the exceptions are
+// those of pet/attention.hpp. A Workspace serves one stream at a time.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <string>
+#include <vector>
+
+#include "../pet_model.h"
+#include "attention.hpp"
+
+namespace pet {
+
+// Rows of activations or their adjoints in fp32, bf16 or fp16 (PET_DTYPE_*).
+struct Rows {
+  void* ptr = nullptr;
+  int rows = 0, cols = 0;
+  int64_t ld = 0;  // in elements
+  int dtype = PET_DTYPE_F32;
+  Rows() = default;
+  Rows(const View2D& v) : ptr(v.data()), rows(v.extent(0)), cols(v.extent(1)), ld(v.stride(0)) {}
+  Rows(void* p, int r, int c, int type, int64_t stride = -1) : ptr(p), rows(r), cols(c), ld(stride < 0 ? c : stride), dtype(type) {}
+};
+
+inline void check_rows(const Rows& a, const Rows& b, const char* what) {
+  if (a.dtype != b.dtype || a.rows != b.rows) throw std::runtime_error(std::string("pet: ") + what + ": rows of one type and number are needed");
+}
+
+// out = norm(in), RMSNorm or with a bias LayerNorm.
+inline void norm_rows(const Rows& out, const Rows& in, View1D weight, View1D bias, hipStream_t stream = nullptr) {
+  check_rows(out, in, "norm_rows");
+  check(pet_norm_rows_typed(in.dtype, in.rows, in.cols, out.ptr, out.ld, in.ptr, in.ld, weight.data(), bias.data(),
+                            stream),
+        "norm_rows");
+}
+
+// in_adj (may hold no pointer) = beta in_adj + the norm's adjoint, weight_adj
+// and bias_adj (may hold none) onto beta_w times themselves; live: the device's
+// count of rows that count, or null.
+inline void norm_rows_grads(Workspace& ws, const Rows& in_adj, View1D weight_adj, View1D bias_adj, const Rows& out_adj,
+                            const Rows& in, View1D weight, bool ln, Net beta = 0, Net beta_w = 0,
+                            const int* live = nullptr, hipStream_t stream = nullptr) {
+  check_rows(out_adj, in, "norm_rows_grads");
+  if (in_adj.ptr) check_rows(in_adj, in, "norm_rows_grads");
+  const bool params = weight_adj.data() || bias_adj.data();
+  const size_t need = params ? pet_norm_rows_grads_workspace(in.rows, in.cols) : 0;
+  void* scratch = params ? ws.bytes("norm_rows_grads:scratch", need) : nullptr;
+  check(pet_norm_rows_grads(in.dtype, in.rows, in.cols, in_adj.ptr, in_adj.ld, beta, out_adj.ptr, out_adj.ld, in.ptr,
+                            in.ld, weight.data(), ln ? 1 : 0, weight_adj.data(), bias_adj.data(), beta_w, live,
+                            scratch, need, stream),
+        "norm_rows_grads");
+}
+
+// w_adj [N, K] = beta w_adj + out_adj^T in, b_adj (may hold none) = beta b_adj + the sum of out_adj's rows.
+inline void linear_grads(Workspace& ws, const Rows& out_adj, const Rows& in, View2D w_adj, View1D b_adj, Net beta = 0,
+                         const int* live = nullptr, hipStream_t stream = nullptr) {
+  check_rows(out_adj, in, "linear_grads");
+  if (w_adj.extent(0) != out_adj.cols || w_adj.extent(1) != in.cols)
+    throw std::runtime_error("pet: linear_grads: w_adj is not [out_adj's columns, in's columns]");
+  const size_t need = pet_linear_grads_workspace(in.dtype, in.rows, out_adj.cols, in.cols);
+  void* scratch = ws.bytes("linear_grads:scratch", need);
+  check(pet_linear_grads(in.dtype, in.rows, out_adj.cols, in.cols, out_adj.ptr, out_adj.ld, in.ptr, in.ld, live,
+                         w_adj.data(), w_adj.stride(0), b_adj.data(), beta, scratch, need, stream),
+        "linear_grads");
+}
+
+// attention_layer_bwd with the gradients of the layer's parameters (null pointers: not made).
+inline void attention_layer_grads(Workspace& ws, const std::string& key, const pet_layer_grads& grads,
+                                  View2D tokens_adj, View2D cf_seq_adj, View2D out_adj, View2D tokens, View1D norm_w,
+                                  View1D norm_b, const WeightRef& w_in, View1D b_in, View2D cf_seq,
+                                  const WeightRef& w_out, const Tokens& tk, int S, int heads, int head_dim,
+                                  double temperature, hipStream_t stream = nullptr) {
+  const int T = tokens.extent(0);
+  const pet_attn_shape sh = make_shape(tk, T, S, heads, head_dim, temperature);
+  const View2D merged = ws.peek2(key + ":merged"), ml = ws.peek2(key + ":ml");
+  const size_t need = pet_attention_layer_grads_workspace(&sh);
+  void* scratch = ws.bytes("attention_layer_grads:scratch", need);
+  check(pet_attention_layer_grads(&sh, &grads, tokens_adj.data(), tokens_adj.stride(0), cf_seq_adj.data(),
+                                  cf_seq_adj.stride(0), out_adj.data(), out_adj.stride(0), tokens.data(),
+                                  tokens.stride(0), norm_w.data(), norm_b.data(), w_in.v.data(), b_in.data(),
+                                  cf_seq.data(), cf_seq.stride(0), w_out.v.data(), tk.off, merged.data(), ml.data(),
+                                  scratch, need, stream),
+        "attention_layer_grads");
+}
+
+// One tensor of a list of gradients: consecutive elements, or rows of a wider matrix.
+inline pet_grad_tensor gradient(void* data, int64_t numel, int dtype = PET_DTYPE_F32) {
+  return {data, 1, numel, numel, dtype};
+}
+inline pet_grad_tensor gradient(const View2D& v) {
+  return {v.data(), v.extent(0), v.extent(1), v.stride(0), PET_DTYPE_F32};
+}
+
+// *norm (device) of all gradients times scale; p 1 or 2, or 0 for the largest magnitude.
+inline void grad_norm(Workspace& ws, const std::vector<pet_grad_tensor>& grads, float* norm, int p = 2,
+                      double scale = 1.0, hipStream_t stream = nullptr) {
+  const size_t need = pet_grad_workspace(int(grads.size()));
+  check(pet_grad_norm(grads.data(), int(grads.size()), p, scale, norm, ws.bytes("grads:scratch", need), need, stream),
+        "grad_norm");
+}
+// ... and every gradient times scale min(1, max_norm / (*norm + eps)) in place.
+inline void clip_grads(Workspace& ws, const std::vector<pet_grad_tensor>& grads, double max_norm, float* norm,
+                       int p = 2, double scale = 1.0, double eps = 1e-6, hipStream_t stream = nullptr) {
+  const size_t need = pet_grad_workspace(int(grads.size()));
+  check(pet_grad_clip(grads.data(), int(grads.size()), p, scale, max_norm, eps, norm, ws.bytes("grads:scratch", need),
+                      need, stream),
+        "clip_grads");
+}
+
+}  // namespace pet

@@ -17,7 +17,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libpet_attn.so")
-SOURCES = ["attention.hip", "attention_pair.hip", "attention_stream.hip", "ops.hip", "rows.hip", "norm_grads.hip", "wgrad.hip", "grad_clip.hip", "forces.hip", "model.hip", "gemm.hip", "gemm_rows.hip", "probe.hip"]
+SOURCES = ["attention.hip", "attention_pair.hip", "attention_stream.hip", "ops.hip", "rows.hip", "norm_grads.hip",
+           "wgrad.hip", "grad_clip.hip", "forces.hip", "model.hip", "gemm.hip", "gemm_rows.hip", "probe.hip"]
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",
@@ -45,12 +46,16 @@ CPP_TEST2_SRC = os.path.join(ROOT, "tests", "cpp", "layer_forces_test.cpp")
 CPP_TEST2 = os.path.join(ROOT, "tests", "cpp", "layer_forces_test")
 CPP_TEST3_SRC = os.path.join(ROOT, "tests", "cpp", "model_test.cpp")
 CPP_TEST3 = os.path.join(ROOT, "tests", "cpp", "model_test")
+CPP_TEST4_SRC = os.path.join(ROOT, "tests", "cpp", "train_test.cpp")
+CPP_TEST4 = os.path.join(ROOT, "tests", "cpp", "train_test")
 
 
 def build_cpp_test(verbose: bool = False) -> str:
-    """The C++ callers of include/pet/attention.hpp, include/pet/forces.hpp and
-    include/pet/model.hpp that tests/test_gpu_cpp_api.py runs."""
-    for src, exe in ((CPP_TEST_SRC, CPP_TEST), (CPP_TEST2_SRC, CPP_TEST2), (CPP_TEST3_SRC, CPP_TEST3)):
+    """The C++ callers of include/pet/attention.hpp, include/pet/forces.hpp,
+    include/pet/model.hpp and include/pet/train.hpp that tests/test_gpu_cpp_api.py
+    and tests/test_gpu_cpp_train.py run."""
+    for src, exe in ((CPP_TEST_SRC, CPP_TEST), (CPP_TEST2_SRC, CPP_TEST2), (CPP_TEST3_SRC, CPP_TEST3),
+                     (CPP_TEST4_SRC, CPP_TEST4)):
         cmd = [hipcc(), "--offload-arch=gfx950", "-O2", "-std=c++17", "-I", os.path.join(ROOT, "include"),
                "-o", exe, src, "-L", HERE, "-lpet_attn", "-Wl,-rpath,$ORIGIN/../../pet_kokkos_amd"]
         if verbose:

@@ -151,3 +151,14 @@ def test_layouts_of_gradients():
             grads._layout(bad, 0)
     a, b = t[0][:, :5], t[0][:, 5:]
     assert grads._side_by_side(a, b) and not grads._side_by_side(a, t[0][:, 4:])
+
+
+def test_no_training_kernel_spills(tmp_path):
+    """The weight gradients' accumulators, and the norms' rows of a multiple of the
+    vector, stay in registers: each spill is read and written every step or row."""
+    from test_kernel_resources import kernels
+    sizes = kernels(tmp_path)
+    wgrad = {n: s for n, s in sizes.items() if "wgrad_kernel" in n}
+    norms = {n: s for n, s in sizes.items() if "norm_grads_kernel" in n and "ELb1EL" in n or "norm_typed_fwd" in n}
+    assert len(wgrad) == 9 and len(norms) > 40
+    assert {n: s for n, s in {**wgrad, **norms}.items() if s > 0} == {}
