@@ -332,7 +332,11 @@ __global__ void __launch_bounds__(64 * WN * WK, TN * TK >= 16 ? 2 : 4)
 #pragma unroll
     for (int j = 0; j < TK; ++j) acc[i][j] = f4{0.f, 0.f, 0.f, 0.f};
 
+  // (a wave past the result's edge has no products to make: 62001 x 500 x 333 156 -> 147 us)
+  auto first_column = [](int r) { return r / (16 * V) * 16 * V + r / 16 % V; };
+  const bool works = n0 + first_column(rn) < a.N && k0 + first_column(rk - C::BN) < a.K;
   auto products = [&](int s) {
+    if (!works) return;
     const u4* from = stage + (s & 1) * C::STAGE;
     if constexpr (PAIRS) {
       if (__builtin_amdgcn_ballot_w64(l < C::UNITS && changed[s & 1][l < C::UNITS ? l : 0]) != 0) {

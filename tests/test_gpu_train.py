@@ -653,3 +653,25 @@ def test_streams_and_two_graphs(device):
         torch.cuda.synchronize()
         for o, e in zip(got, eager):
             assert all(torch.equal(o[k], e[k]) for k in o)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,k", [(257, 260), (384, 131), (260, 321), (129, 388), (300, 140)])
+def test_linear_grads_past_a_tile(device, dtype, n, k):
+    """Results that end a few columns into a tile, with enough rows that the widest
+    tiles take them: the waves past the edge leave their products out."""
+    gen = torch.Generator().manual_seed(n * k)
+    M = int(4.1e9 / (n * k)) + 1
+    g = torch.randn((M, n), generator=gen).to(device).to(dtype)
+    x = torch.randn((M, k), generator=gen).to(device).to(dtype)
+    wa, ba = torch.full((n, k), math.nan, device=device), torch.full((n,), math.nan, device=device)
+    D.linear_grads(g, x, wa, ba)
+    ref = torch.zeros((n, k), dtype=torch.float64)
+    size = torch.zeros((n, k), dtype=torch.float64)
+    for r in range(0, M, 65536):
+        gd, xd = g[r:r + 65536].double().cpu(), x[r:r + 65536].double().cpu()
+        ref += gd.t() @ xd
+        size += gd.abs().t() @ xd.abs()
+    # as linear_bound: normals, so no value is far below its column's largest that matters
+    within(wa, ref, (M / 32 + 320) * U * size, "w_adj")
+    within(ba, g.double().sum(0).cpu(), (M / 32 + 340) * U * g.double().abs().sum(0).cpu(), "b_adj")
