@@ -20,14 +20,14 @@ from .attention import DTYPES, _call_on, _scratch
 class GradList:
     """The tensors of a step's gradients, checked and laid out for the library
     once: contiguous in any order of their axes, or a 2-D view of rows (or a column) in
-    a wider matrix; all on one device, no two overlapping. It keeps the tensors, and every
-    call reads what they then hold."""
+    a wider matrix; all on one device, no two overlapping. It keeps the memory that
+    they have now, and every call reads what that then holds (a gradient set anew
+    needs a new list)."""
 
     def __init__(self, tensors):
-        self.tensors = list(tensors)
-        self.device = None
+        self.tensors, self.device = [], None
         entries, spans = [], []
-        for i, t in enumerate(self.tensors):
+        for i, t in enumerate(tensors):
             if not isinstance(t, torch.Tensor):
                 raise TypeError(f"gradient {i}: a torch tensor is needed")
             if t.device.type != "cuda" or (self.device is not None and t.device != self.device):
@@ -35,15 +35,21 @@ class GradList:
             if t.dtype not in DTYPES:
                 raise ValueError(f"gradient {i}: {t.dtype}, not float32, bfloat16 or float16")
             self.device = t.device
+            t = t.detach()  # (its memory, whatever becomes of the caller's tensor)
+            self.tensors.append(t)
             if t.numel() == 0:
                 continue
             rows, cols, ld = _layout(t, i)
             entries.append((t.data_ptr(), rows, cols, ld, DTYPES[t.dtype]))
             spans.append((t.data_ptr(), t.data_ptr() + ((rows - 1) * ld + cols) * t.element_size(), i, t))
-        spans.sort(key=lambda s: s[:3])
-        for (_, end, i, a), (start, _, j, b) in zip(spans, spans[1:]):
-            if start < end and not _side_by_side(a, b):
-                raise ValueError(f"gradients {min(i, j)} and {max(i, j)} overlap")
+        spans.sort(key=lambda s: s[0])
+        live = []  # the spans that reach past the next one's start
+        for span in spans:
+            live = [s for s in live if s[1] > span[0]]
+            for _, _, i, t in live:
+                if not _side_by_side(t, span[3]):
+                    raise ValueError(f"gradients {min(i, span[2])} and {max(i, span[2])} overlap")
+            live.append(span)
         self.array = (_lib.GradTensor * max(1, len(entries)))(*[_lib.GradTensor(*e) for e in entries])
         self.count = len(entries)
         self.scratch_bytes = _lib.load().pet_grad_workspace(self.count)

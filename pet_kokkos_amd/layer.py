@@ -172,10 +172,24 @@ def attention_layer_grads(ws: Workspace, key: str, grads: dict, tokens_adj: torc
     ``grads`` holds the tensors they go to by name (norm_w, norm_b, w_in, b_in,
     w_out, b_out, each of its parameter's shape; those not there are not made, a
     bias's not without its weight's), each onto beta times itself. Dead rows
-    count for none."""
+    count for none. ``ws`` serves one stream at a time; a call that is captured
+    into a graph finds its scratch there from an eager call before it."""
     lib = _lib.load()
     D, dev = heads * head_dim, tokens.device
     T = tokens.shape[0]
+    for t, name in ((tokens, "tokens"), (tokens_adj, "tokens_adj"), (out_adj, "out_adj")):
+        _typed(t, name, T, D, torch.float32, dev)
+    for t, name in ((cf_seq, "cf_seq"), (cf_seq_adj, "cf_seq_adj")):
+        _typed(t, name, tk.N, t.shape[-1], torch.float32, dev)
+        if t.shape[1] < S:
+            raise ValueError(f"{name} narrower than S")
+    for t, name, size in ((w_in, "w_in", (3 * D, D)), (w_out, "w_out", (D, D)), (norm_w, "norm_w", (D,)),
+                          (norm_b, "norm_b", (D,)), (b_in, "b_in", (3 * D,))):
+        if t is not None and (t.device != dev or t.dtype != torch.float32 or tuple(t.shape) != size
+                              or not t.is_contiguous()):
+            raise ValueError(f"{name} must be a contiguous float32 {list(size)} on {dev}")
+    if tk.off.device != dev or tk.off.dtype != torch.int32 or tk.off.numel() != tk.N + 1:
+        raise ValueError(f"tk.off must be {tk.N + 1} int32 on {dev}")
     unknown = sorted(set(grads) - set(_LAYER_GRADS))
     if unknown:
         raise ValueError(f"grads: no parameter named {', '.join(unknown)}")
@@ -193,6 +207,8 @@ def attention_layer_grads(ws: Workspace, key: str, grads: dict, tokens_adj: torc
         setattr(pg, name, g.data_ptr())
     sh = shape(tk.N, T, S, heads, head_dim, temperature, tk.dead)
     merged, ml = ws.peek2(key + ":merged"), ws.peek2(key + ":ml")
+    if merged.shape != (T, D) or ml.shape != (tk.N * heads * S, 2):
+        raise ValueError(f"the saves under {key} are of another shape")
     scratch = ws.bytes("attention_layer_grads:scratch", lib.pet_attention_layer_grads_workspace(sh))
     _call_on(dev, "pet_attention_layer_grads", lib.pet_attention_layer_grads, sh, ctypes.byref(pg),
              tokens_adj.data_ptr(), _mat(tokens_adj, "tokens_adj", D), cf_seq_adj.data_ptr(),

@@ -427,10 +427,16 @@ def test_clip_range(device):
 def test_gradient_lists_refuse(device):
     a = torch.zeros(100, device=device)
     for bad in ([a, a], [a[:60], a[59:]], [a.view(10, 10)[:, :6], a.view(10, 10)[:, 5:]], [a.view(10, 10)[::2, ::2]],
-                [a.double()], [a, a.cpu()]):
+                [a.double()], [a, a.cpu()],
+                # a third view beside the second and over the first
+                [a.view(10, 10)[:, :5], a.view(10, 10)[:, 5:], a.view(10, 10)[5:, :2]]):
         with pytest.raises(ValueError):
             G.clip_grads(bad, 1.0)
     G.clip_grads([a.view(10, 10)[:, :6], a.view(10, 10)[:, 6:]], 1.0)
+    b = torch.ones(50, device=device)
+    lst = G.GradList([b])
+    b.data = torch.zeros(50, device=device)  # the list keeps the memory it was made of
+    assert abs(float(G.grad_norm(lst)) - math.sqrt(50)) < 1e-6
     for kw in (dict(norm_type=3.0), dict(scale=math.nan), dict(eps=-1.0), dict(out=torch.zeros(2, device=device))):
         with pytest.raises(ValueError):
             G.clip_grads([a], 1.0, **kw)
@@ -547,6 +553,9 @@ def test_attention_layer_grads(device, ln, dead):
         L.attention_layer_grads(ws, "l", {"w": some["w_out"]}, *args)
     with pytest.raises(ValueError):
         L.attention_layer_grads(ws, "l", {"b_out": a["b_out"]}, *args)
+    for i, bad in ((2, a["g"][:-1]), (3, a["tokens"][:, 1:]), (6, a["w_out"]), (8, cf[:, 1:]), (0, tadj.half())):
+        with pytest.raises(ValueError):
+            L.attention_layer_grads(ws, "l", some, *args[:i], bad, *args[i + 1:])
 
 
 @pytest.mark.parametrize("ln", [False, True])
