@@ -126,8 +126,9 @@ struct Args {
   int pieces, tiles_n, tiles_k;
   float* out;      // [pieces][N][K], or with one piece w_adj
   int64_t ldo;
-  double* bout;    // [pieces][tiles_k][N], null: no bias
-  float beta;      // with one piece
+  double* bout;    // [pieces][tiles_k][N], with one piece unused
+  float* b_adj;    // null: no bias
+  float beta;
 };
 
 template <class T, int WN, int WK, int TN, int TK, int V>
@@ -238,9 +239,11 @@ __global__ void __launch_bounds__(64 * WN * WK, TN * TK >= 16 ? 2 : 4)
   float scale[PAIRS ? V : 1];  // of each column, 2^126 until a value is too large for that
 #pragma unroll
   for (int j = 0; j < (PAIRS ? V : 1); ++j) scale[j] = 0x1p126f;
-  // (a column's tiles share out the steps whose g they sum)
-  const bool bias = a.bout && is_g && reads;
+  // A column's tiles share out the steps whose g they sum; with one piece the first
+  // takes all, and the bias is done (one launch a call).
+  const bool direct = a.pieces == 1;
   const int kt = tile % a.tiles_k;
+  const bool bias = a.b_adj && is_g && reads && (!direct || kt == 0);
   int turn = 0;
   double* mine = &bsum[oct][(is_g ? group : 0) * 16 * V + c];  // LDS rows' order, as row0
   float few[V];  // of sixteen steps, then added there (every step: a tenth of the whole time)
@@ -256,7 +259,7 @@ __global__ void __launch_bounds__(64 * WN * WK, TN * TK >= 16 ? 2 : 4)
     if (!reads) return;
     if (!whole || (s + 1) * C::STEP > last - first) mend(s);
     u4* to = stage + (s & 1) * C::STAGE;
-    const bool sums = bias && turn == kt;
+    const bool sums = bias && (direct || turn == kt);
     turn = turn + 1 == a.tiles_k ? 0 : turn + 1;
     if constexpr (PAIRS) {
       unsigned x[V][8];
@@ -427,13 +430,14 @@ __global__ void __launch_bounds__(64 * WN * WK, TN * TK >= 16 ? 2 : 4)
     if (__builtin_amdgcn_ballot_w64(inf) != 0 && l == 0) special[wave] = 1;
   }
   __syncthreads();
-  if (a.bout)
+  if (a.b_adj && (!direct || kt == 0))
     for (int r = threadIdx.x; r < C::BN; r += 64 * C::WAVES) {
       const int n = n0 + r / (16 * V) * 16 * V + r % 16 * V + r / 16 % V;
       if (n < a.N) {
         double v = 0.0;
         for (int q = 0; q < 4 * C::OQ; ++q) v += bsum[q][r];
-        a.bout[(int64_t(piece) * a.tiles_k + kt) * a.N + n] = v;
+        if (!direct) a.bout[(int64_t(piece) * a.tiles_k + kt) * a.N + n] = v;
+        else a.b_adj[n] = a.beta != 0.f ? float(double(a.beta) * a.b_adj[n] + v) : float(v);
       }
     }
 
@@ -481,7 +485,6 @@ __global__ void __launch_bounds__(64 * WN * WK, TN * TK >= 16 ? 2 : 4)
     }
   }
 
-  const bool direct = a.pieces == 1;
   float* out = a.out + (direct ? 0 : int64_t(piece) * a.N * a.K);
 #pragma unroll
   for (int i = 0; i < TN; ++i)
@@ -528,7 +531,7 @@ __global__ void __launch_bounds__(256) wgrad_sum_kernel(int N, int K, int pieces
                                                         const double* __restrict__ bpart, float* __restrict__ w_adj,
                                                         int64_t ldw, float* __restrict__ b_adj, float beta) {
   __shared__ double sums[kStrips][32][4];
-  const int64_t nk = part ? int64_t(N) * K : 0, wblocks = (nk + 127) / 128;
+  const int64_t nk = int64_t(N) * K, wblocks = (nk + 127) / 128;
   const int q = threadIdx.x & 31, strip = threadIdx.x >> 5;
   const bool bias = int64_t(blockIdx.x) >= wblocks;
   const int64_t i = (int64_t(blockIdx.x) - (bias ? wblocks : 0)) * 128 + 4 * q, n = bias ? N : nk;
@@ -605,7 +608,7 @@ Plan plan_of(int dtype, int M, int N, int K) {
   return p;
 }
 size_t bias_bytes(const Plan& p, int N) {
-  return (size_t(p.pieces) * p.tiles_k * N * sizeof(double) + 15) & ~size_t(15);
+  return p.pieces == 1 ? 16 : (size_t(p.pieces) * p.tiles_k * N * sizeof(double) + 15) & ~size_t(15);
 }
 
 }  // namespace pet_wgrad
@@ -625,7 +628,7 @@ int pet_linear_grads_run(int dtype, int M, int N, int K, const void* out_adj, in
   double* bpart = static_cast<double*>(ws);
   float* part = reinterpret_cast<float*>(static_cast<char*>(ws) + bias_bytes(p, N));
   Args a{M, N, K, ldo, ldi, live_base, live, p.chunk, p.pieces, p.tiles_n, p.tiles_k,
-         p.pieces > 1 ? part : w_adj, p.pieces > 1 ? K : ldw, b_adj ? bpart : nullptr, beta};
+         p.pieces > 1 ? part : w_adj, p.pieces > 1 ? K : ldw, bpart, b_adj, beta};
   const dim3 grid(unsigned(int64_t(p.tiles_n) * p.tiles_k * p.pieces));
   const int e = pet_typed::with_dtype(dtype, [&](auto tv) {
     using T = decltype(tv);
@@ -637,10 +640,10 @@ int pet_linear_grads_run(int dtype, int M, int N, int K, const void* out_adj, in
     return hipGetLastError() == hipSuccess ? int(PET_ATTN_OK) : int(PET_ATTN_ELAUNCH);
   });
   if (e) return e;
-  const int64_t blocks = (p.pieces > 1 ? (int64_t(N) * K + 127) / 128 : 0) + (b_adj ? (int64_t(N) + 127) / 128 : 0);
-  if (blocks == 0) return PET_ATTN_OK;
-  hipLaunchKernelGGL(wgrad_sum_kernel, dim3(unsigned(blocks)), dim3(256), 0, st, N, K, p.pieces,
-                     p.pieces * p.tiles_k, p.pieces > 1 ? part : nullptr, bpart, w_adj, ldw, b_adj, beta);
+  if (p.pieces == 1) return PET_ATTN_OK;
+  const int64_t blocks = (int64_t(N) * K + 127) / 128 + (b_adj ? (int64_t(N) + 127) / 128 : 0);
+  hipLaunchKernelGGL(wgrad_sum_kernel, dim3(unsigned(blocks)), dim3(256), 0, st, N, K, p.pieces, p.pieces * p.tiles_k,
+                     part, bpart, w_adj, ldw, b_adj, beta);
   return hipGetLastError() == hipSuccess ? int(PET_ATTN_OK) : int(PET_ATTN_ELAUNCH);
 }
 
