@@ -37,10 +37,11 @@ constexpr int threads_of(int TPR) { return TPR > 256 ? TPR : 256; }
 // that a grid of it fills the chip in one round. (1024 workgroups of which 768
 // fitted took two: 65536 x 1024 in bf16 131 us.)
 constexpr int waves_of(int E, int TPR) { return TPR == 1024 ? 4 : E <= 4 ? 8 : E <= 8 ? 5 : E <= 16 ? 3 : 2; }
-// 1 / sqrt(x): the hardware's estimate and a Newton step.
+// 1 / sqrt(x): the hardware's estimate and a Newton step (0 where the squares passed
+// fp32, as 1 / sqrtf gives).
 __device__ __forceinline__ float rsqrt_nr(float x) {
   const float y = __builtin_amdgcn_rsqf(x);
-  return y * fmaf(-0.5f * x * y, y, 1.5f);
+  return y == 0.f ? y : y * fmaf(-0.5f * x * y, y, 1.5f);
 }
 
 // A lane's value from the lane that a DPP control names.

@@ -25,11 +25,11 @@
 // (rare). A value below 2^-14 of the column's largest is held to 2^-36 of that.
 //
 // What bounds it: the matrix unit under the clock that its power leaves. For
-// 486946 x 2048 x 512 in bf16 (1.25 ms, 815 TFLOP/s; a library's product of that
-// shape 2.0 ms, of 8192 cubed 1131 TFLOP/s) the products alone take 0.73 ms, the
-// rows' way into LDS alone 0.71, the loads alone 0.60; together the clock falls from
-// 2.2 to 1.8 GHz, and the matrix unit is busy 42% of the cycles. 122688 x 768 x 256
-// in fp32 takes 198 us, of which writing and adding the pieces is 30.
+// 486946 x 2048 x 512 in bf16 (1.14 to 1.21 ms, 845 to 895 TFLOP/s; a library's
+// product of that shape 2.03 ms, of 8192 cubed 1131 TFLOP/s) the products alone take
+// 0.73 ms, the rows' way into LDS alone 0.71, the loads alone 0.60; together the clock
+// falls from 2.2 to 1.8 GHz, and the matrix unit is busy 42% of the cycles. 122688 x
+// 768 x 256 in fp32 takes 187 to 200 us, of which writing and adding the pieces is 30.
 //
 // The matrix instruction rounds toward minus infinity, an error with a mean that
 // half a million rows would add up. So a step is summed from zero, the sums of
@@ -525,7 +525,7 @@ __global__ void __launch_bounds__(64 * WN * WK, TN * TK >= 16 ? 2 : 4)
 // adj = beta adj + the pieces' sums in double: a thread sums every STRIPS-th
 // piece of four elements, eight loads at a time, the strips are joined in order.
 // (One thread an element, its loads one after the other: 24 us for 80 pieces of
-// 768 x 256 against 8.)
+// 768 x 256 against 15.)
 constexpr int kStrips = 8;
 __global__ void __launch_bounds__(256) wgrad_sum_kernel(int N, int K, int pieces, int bpieces, const float* __restrict__ part,
                                                         const double* __restrict__ bpart, float* __restrict__ w_adj,

@@ -134,7 +134,8 @@ def test_norm_rows_grads_parts(device):
     out_adj and of the input; the same bits twice; many rows."""
     gen = torch.Generator().manual_seed(5)
     for dtype, rows, width, ln in ((torch.float32, 9001, 128, True), (torch.bfloat16, 5003, 512, False),
-                                   (torch.float16, 300, 9000, True)):
+                                   (torch.float16, 300, 9000, True), (torch.bfloat16, 700, 8000, True),
+                                   (torch.float32, 2000, 3001, False), (torch.float32, 600, 16384, True)):
         x, g = rows_of(gen, rows, width, dtype, device), rows_of(gen, rows, width, dtype, device, size=1e-2)
         w = (1 + 0.1 * torch.randn(width, generator=gen)).to(device)
 
@@ -228,6 +229,50 @@ def test_norm_rows_not_finite(device):
     assert torch.equal(adj[rest], clean[rest]) and torch.isnan(adj[[3, 7]]).all()
     assert torch.isnan(wa).all()  # row 7's xhat is NaN in every column
     assert torch.isnan(ba[5]) and torch.isfinite(ba[[i for i in range(64) if i != 5]]).all()
+
+
+def test_norm_rows_squares_past_fp32(device):
+    """Rows whose squares pass fp32 come out as zeros, as fp32 arithmetic makes them, and no NaN."""
+    x = torch.full((3, 4096), 1e25, device=device)
+    w, out = torch.ones(4096, device=device), torch.full((3, 4096), 7.0, device=device)
+    L.norm_rows(out, x, w, None)
+    assert (out == 0).all()
+    small = torch.full((3, 64), 1e25, device=device, dtype=torch.bfloat16)
+    L.norm_rows(small, small, w[:64], None)
+    assert (small == 0).all()
+
+
+def test_offsets_past_32_bits(device):
+    """Rows whose offsets, and a tensor whose elements, pass 2^31: the last ones count."""
+    M, ld = (1 << 21) + 70000, 1024  # 2.2e9 elements
+    base = torch.zeros((M, ld), dtype=torch.bfloat16, device=device)
+    g, x = base[:, :4], base[:, 8:14]
+    gen = torch.Generator().manual_seed(51)
+    at = torch.tensor([0, 1, 1 << 20, (1 << 21) + 5, M - 2, M - 1])
+    g[at] = torch.randn((6, 4), generator=gen).to(device).bfloat16()
+    x[at] = torch.randn((6, 6), generator=gen).to(device).bfloat16()
+    wa, ba = torch.empty((4, 6), device=device), torch.empty(4, device=device)
+    D.linear_grads(g, x, wa, ba)
+    gd, xd = g[at].double().cpu(), x[at].double().cpu()
+    within(wa, gd.t() @ xd, 16 * U * (gd.abs().t() @ xd.abs()), "w_adj")
+    within(ba, gd.sum(0), 16 * U * gd.abs().sum(0), "b_adj")
+    w, wn, bn = torch.ones(4, device=device), torch.empty(4, device=device), torch.empty(4, device=device)
+    adj = base[:, 20:24]
+    L.norm_rows_grads(adj, wn, bn, g, base[:, 8:12], w, True)
+    r = norm_ref(base[at, 8:12], g[at], w, w, True)  # (the other rows are zeros, and so are their adjoints)
+    tol = r["in_tol"] + half(torch.bfloat16) * (r["in_adj"].abs() + r["in_tol"]) + least(torch.bfloat16)
+    within(adj[at], r["in_adj"], tol, "in_adj")
+    within(wn, r["w_adj"], 8 * r["w_tol"], "w_adj")  # (8 rows' lanes and parts, with zeros between)
+    within(bn, r["b_adj"], 8 * r["b_tol"], "b_adj")
+    out = base[:, 30:34]
+    L.norm_rows(out, base[:, 8:12], w, w)
+    ref = norm_ref(base[at, 8:12], None, w, w, True)
+    within(out[at], ref["out"], ref["out_tol"] + half(torch.bfloat16) * (ref["out"].abs() + ref["out_tol"]), "out")
+    base.zero_()
+    flat = base.view(-1)[5:]
+    flat[-1], flat[0] = 3.0, 4.0
+    assert float(G.clip_grads([flat], 1.0, eps=0.0)) == 5.0
+    assert flat[-1].item() == torch.tensor(0.6).bfloat16().item() and flat[0].item() == torch.tensor(0.8).bfloat16().item()
 
 
 # ---- linear_grads -------------------------------------------------------------------
