@@ -522,26 +522,44 @@ __global__ void __launch_bounds__(64 * WN * WK, TN * TK >= 16 ? 2 : 4)
     }
 }
 
-// adj = beta adj + the pieces' sums in double: a thread sums every STRIPS-th
-// piece of four elements, eight loads at a time, the strips are joined in order.
-// (One thread an element, its loads one after the other: 24 us for 80 pieces of
-// 768 x 256 against 15.)
-constexpr int kStrips = 8;
-__global__ void __launch_bounds__(256) wgrad_sum_kernel(int N, int K, int pieces, int bpieces, const float* __restrict__ part,
+// adj = beta adj + the pieces' sums in double: a thread sums every eighth piece of
+// four elements, or every 64th of one column's biases, eight loads at a time, and
+// the strips are joined in order. MI355X: 80 pieces of 768 x 256 15 us (24 with a
+// thread an element, its loads one after the other); 26670 x 128 x 512, whose 512
+// pieces of the bias eight strips summed as they do the rest, 66 us a call and 40 now.
+constexpr int kStrips = 8, kSumElements = 4 * 256 / kStrips;
+__global__ void __launch_bounds__(256) wgrad_sum_kernel(int N, int K, int pieces, int bpieces,
+                                                        const float* __restrict__ part,
                                                         const double* __restrict__ bpart, float* __restrict__ w_adj,
                                                         int64_t ldw, float* __restrict__ b_adj, float beta) {
-  __shared__ double sums[kStrips][32][4];
-  const int64_t nk = int64_t(N) * K, wblocks = (nk + 127) / 128;
-  const int q = threadIdx.x & 31, strip = threadIdx.x >> 5;
+  constexpr int Q = 256 / kStrips, E = kSumElements;  // threads a strip, elements a workgroup
+  __shared__ double sums[256][4];             // [strip][thread][element]; a bias's [strip][column]
+  const int64_t nk = int64_t(N) * K, wblocks = (nk + E - 1) / E;
   const bool bias = int64_t(blockIdx.x) >= wblocks;
-  const int64_t i = (int64_t(blockIdx.x) - (bias ? wblocks : 0)) * 128 + 4 * q, n = bias ? N : nk;
   double v[4] = {0.0, 0.0, 0.0, 0.0};
   if (bias) {
-    for (int s = strip; s < bpieces; s += kStrips)
+    const int64_t n = (int64_t(blockIdx.x) - wblocks) * 4 + (threadIdx.x & 3);
+    if (n < N)
+      for (int s = threadIdx.x >> 2; s < bpieces; s += 8 * 64) {
+        double x[8];
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (i + e < n) v[e] += bpart[int64_t(s) * N + i + e];
-  } else if (i + 4 <= n) {
+        for (int u = 0; u < 8; ++u) x[u] = s + 64 * u < bpieces ? bpart[int64_t(s + 64 * u) * N + n] : 0.0;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v[0] += x[u];
+      }
+    sums[threadIdx.x >> 2][threadIdx.x & 3] = v[0];
+    __syncthreads();
+    if (threadIdx.x < 4 && n < N) {
+      double r = 0.0;
+#pragma unroll
+      for (int s = 0; s < 64; ++s) r += sums[s][threadIdx.x];
+      b_adj[n] = beta != 0.f ? float(double(beta) * b_adj[n] + r) : float(r);
+    }
+    return;
+  }
+  const int strip = threadIdx.x / Q;
+  const int64_t first = int64_t(blockIdx.x) * E, i = first + 4 * (threadIdx.x % Q);
+  if (i + 4 <= nk) {
     int s = strip;
     for (; s + 7 * kStrips < pieces; s += 8 * kStrips) {
       f4u x[8];
@@ -562,18 +580,18 @@ __global__ void __launch_bounds__(256) wgrad_sum_kernel(int N, int K, int pieces
     for (int s = strip; s < pieces; s += kStrips)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (i + e < n) v[e] += part[int64_t(s) * nk + i + e];
+        if (i + e < nk) v[e] += part[int64_t(s) * nk + i + e];
   }
 #pragma unroll
-  for (int e = 0; e < 4; ++e) sums[strip][q][e] = v[e];
+  for (int e = 0; e < 4; ++e) sums[threadIdx.x][e] = v[e];
   __syncthreads();
   const int t = threadIdx.x;
-  const int64_t j = i - 4 * q + t;
-  if (t >= 128 || j >= n) return;
+  if (t >= E || first + t >= nk) return;
   double r = 0.0;
 #pragma unroll
-  for (int s = 0; s < kStrips; ++s) r += sums[s][t >> 2][t & 3];
-  float* o = bias ? b_adj + j : w_adj + j / K * ldw + j % K;
+  for (int s = 0; s < kStrips; ++s) r += sums[s * Q + (t >> 2)][t & 3];
+  const int64_t j = first + t;
+  float* o = w_adj + j / K * ldw + j % K;
   *o = beta != 0.f ? float(double(beta) * *o + r) : float(r);
 }
 
@@ -585,18 +603,20 @@ struct Plan {
 constexpr int kEdge[3] = {256, 128, 64};
 constexpr int kResident[3] = {256, 512, 1024};  // workgroups that the chip holds at once
 
-// The largest tile that the result fills and the work feeds. MI355X, us a call:
-//   256 against 128 wide: 122688 x 768 x 256 in fp32 198 and 249, 8192 x 1024 x 1024 93 and 102, 62001 x
-//     500 x 333 156 and 158, 20011 x 1000 x 330 in fp16 64 and 66;
-//   128 against 64 wide: 26670 x 1024 x 128 62 and 72, 27318 x 128 x 128 (4.5e8 products) 34 and 42, but
-//     648 x 1024 x 256 (1.7e8) 23.6 and 20.5: its few steps wait on memory, not on the tile.
-// Pieces fill the chip, in whole eights (an XCD each in turn), of at least four
-// steps (27318 x 128 x 128: 34 us, 41 with two and 46 with sixteen).
+// The largest tile that the result fills and the work feeds. MI355X, us a call in
+// fp32:
+//   256 against 128 wide: 122688 x 768 x 256 197 and 250, 8192 x 1024 x 1024 89 and 98, 62001 x 500 x 333 (1.0e10
+//     products) 139 and 151, 20011 x 1000 x 330 in fp16 (6.6e9) 57 and 64, but 27318 x 384 x 256 (2.7e9) 56 and 48;
+//   128 against 64 wide: 26670 x 1024 x 128 (3.5e9) 59 and 69, 27318 x 384 x 256 48 and 58, 5000 x 512 x 512 (1.3e9)
+//     36.5 and 36.7, but 27318 x 128 x 128 (4.5e8) 26 and 24, 8000 x 384 x 128 27 and 24, 648 x 1024 x 256 (1.7e8) 23
+//     and 20: few steps wait on memory, not on the tile.
+// Pieces fill the chip, in whole eights (an XCD each in turn), of at least four steps (27318 x 128 x 128 in 128 wide
+// tiles 26.5 us, 28 with two and 31 with eight).
 Plan plan_of(int dtype, int M, int N, int K) {
   const int step = dtype == PET_DTYPE_F32 ? 32 : 64;
   const double work = double(M) * N * K;
   Plan p{};
-  p.tile = N > 128 && K > 128 && work >= 4e9 ? 0 : N > 64 && K > 64 && work >= 3e8 ? 1 : 2;
+  p.tile = N > 128 && K > 128 && work >= 4e9 ? 0 : N > 64 && K > 64 && work >= 1e9 ? 1 : 2;
   const int64_t edge = kEdge[p.tile], tn = (int64_t(N) + edge - 1) / edge, tk = (int64_t(K) + edge - 1) / edge;
   const int64_t steps = std::max<int64_t>(1, (int64_t(M) + step - 1) / step);
   int64_t pieces = std::max<int64_t>(1, std::min<int64_t>(kResident[p.tile] / (tn * tk), (steps + 3) / 4));
@@ -641,7 +661,7 @@ int pet_linear_grads_run(int dtype, int M, int N, int K, const void* out_adj, in
   });
   if (e) return e;
   if (p.pieces == 1) return PET_ATTN_OK;
-  const int64_t blocks = (int64_t(N) * K + 127) / 128 + (b_adj ? (int64_t(N) + 127) / 128 : 0);
+  const int64_t blocks = (int64_t(N) * K + kSumElements - 1) / kSumElements + (b_adj ? (int64_t(N) + 3) / 4 : 0);
   hipLaunchKernelGGL(wgrad_sum_kernel, dim3(unsigned(blocks)), dim3(256), 0, st, N, K, p.pieces, p.pieces * p.tiles_k,
                      part, bpart, w_adj, ldw, b_adj, beta);
   return hipGetLastError() == hipSuccess ? int(PET_ATTN_OK) : int(PET_ATTN_ELAUNCH);
