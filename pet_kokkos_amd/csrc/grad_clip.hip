@@ -182,7 +182,7 @@ int check(const pet_grad_tensor* t, int n) {
   return PET_ATTN_OK;
 }
 
-int batches_of(int n) { return (n + kTensors - 1) / kTensors; }
+int batches_of(int n) { return n / kTensors + (n % kTensors != 0); }
 
 // Tensors [i, n) into b, as many as it takes; the next one's index.
 int fill(Batch& b, const pet_grad_tensor* t, int i, int n) {

@@ -359,7 +359,13 @@ int with_row(int width, F&& f) {
   return f(integral_constant<int, 512>{}, integral_constant<int, 4 * S>{});
 }
 
-constexpr int kCus = 256, kMaxParts = 2048;
+// The backward's workgroups that the chip holds at once: its grid at most.
+constexpr int kCus = 256;
+constexpr int most_of(int E, int TPR) { return kCus * (waves_of(E, TPR) * 256 / threads_of(TPR)); }
+template <class T>
+int most_for(int width) {
+  return with_row<T>(width, [](auto lc, auto cc) { return most_of(decltype(cc)::value * kVec<T>, decltype(lc)::value); });
+}
 
 }  // namespace pet_norm
 
@@ -380,8 +386,7 @@ int pet_norm_grads_sink(int dtype, int rows, int width, void* in_adj, int64_t ld
     return with_row<T>(width, [&](auto lc, auto cc) {
       constexpr int TPR = decltype(lc)::value, C = decltype(cc)::value, TH = threads_of(TPR), RPB = TH / TPR;
       // as many workgroups as the chip holds at once, each with the same rows to within one
-      constexpr int most = kCus * (waves_of(C * kVec<T>, TPR) * 256 / TH);
-      static_assert(most <= kMaxParts, "the workspace's rows");
+      constexpr int most = most_of(C * kVec<T>, TPR);
       // (few rows are one workgroup's, which spares a launch)
       const int64_t groups = std::max<int64_t>(1, (int64_t(rows) + RPB - 1) / RPB);
       const int64_t each = part && groups <= 4 ? groups : (groups + most - 1) / most;
@@ -433,7 +438,8 @@ int pet_norm_rows_typed(int dtype, int rows, int width, void* out, int64_t ldo, 
 
 size_t pet_norm_rows_grads_workspace(int rows, int width) {
   if (rows < 0 || width < 1) return 0;
-  return size_t(kMaxParts) * 2 * size_t(width) * sizeof(float);
+  const int parts = std::max(1, std::min(rows, std::max(most_for<float>(width), most_for<_Float16>(width))));
+  return size_t(parts) * 2 * size_t(width) * sizeof(float);
 }
 
 int pet_norm_rows_grads(int dtype, int rows, int width, void* in_adj, int64_t lda, float beta, const void* out_adj,

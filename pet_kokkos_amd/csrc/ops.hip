@@ -305,7 +305,7 @@ int layer_bwd(const pet_attn_shape* sh, const pet_layer_grads* pg, float* tokens
   if (!sh || !tokens_adj || !tokens || !norm_w || !w_in || !off) return PET_ATTN_EINVAL;
   const int D = sh->heads * sh->head_dim, T = sh->n_rows;
   if (ldt < D || lda < D) return PET_ATTN_EINVAL;
-  if (pg && (!out_adj || !merged || ldo < D)) return PET_ATTN_EINVAL;
+  if (pg && (!out_adj || !merged || ldo < D || D > PET_NORM_MAX_WIDTH)) return PET_ATTN_EINVAL;
   const size_t need = pet_attention_layer_workspace(sh);
   if (!workspace || workspace_bytes < need + (pg ? layer_grads_bytes(sh) : 0)) return PET_ATTN_EWORKSPACE;
   if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0) return PET_ATTN_EALIGN;

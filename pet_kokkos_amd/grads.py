@@ -79,6 +79,8 @@ def _side_by_side(a: torch.Tensor, b: torch.Tensor) -> bool:
     if a.dim() != 2 or b.dim() != 2 or a.dtype != b.dtype or a.stride() != b.stride() or a.stride(1) != 1:
         return False
     ld = a.stride(0)
+    if ld < 1:
+        return False
     gap = (b.data_ptr() - a.data_ptr()) // a.element_size() % ld
     return gap >= a.shape[1] and gap + b.shape[1] <= ld
 

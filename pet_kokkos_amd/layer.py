@@ -207,8 +207,8 @@ def attention_layer_grads(ws: Workspace, key: str, grads: dict, tokens_adj: torc
         setattr(pg, name, g.data_ptr())
     sh = shape(tk.N, T, S, heads, head_dim, temperature, tk.dead)
     merged, ml = ws.peek2(key + ":merged"), ws.peek2(key + ":ml")
-    if merged.shape != (T, D) or ml.shape != (tk.N * heads * S, 2):
-        raise ValueError(f"the saves under {key} are of another shape")
+    if merged.shape != (T, D) or ml.shape != (tk.N * heads * S, 2) or merged.device != dev:
+        raise ValueError(f"the saves under {key} are of another shape or on another device")
     scratch = ws.bytes("attention_layer_grads:scratch", lib.pet_attention_layer_grads_workspace(sh))
     _call_on(dev, "pet_attention_layer_grads", lib.pet_attention_layer_grads, sh, ctypes.byref(pg),
              tokens_adj.data_ptr(), _mat(tokens_adj, "tokens_adj", D), cf_seq_adj.data_ptr(),

@@ -729,3 +729,41 @@ def test_linear_grads_past_a_tile(device, dtype, n, k):
     # as linear_bound: normals, so no value is far below its column's largest that matters
     within(wa, ref, (M / 32 + 320) * U * size, "w_adj")
     within(ba, g.double().sum(0).cpu(), (M / 32 + 340) * U * g.double().abs().sum(0).cpu(), "b_adj")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_workspaces_are_enough(device, dtype):
+    """Nothing is written past the bytes that the workspace functions name."""
+    lib, guard = A._lib.load(), 1 << 20
+    for rows, width in ((1, 300), (5, 16384), (9, 4096), (70, 64), (700, 8192), (3000, 513), (40000, 200), (40000, 7)):
+        need = lib.pet_norm_rows_grads_workspace(rows, width)
+        room = torch.full((need + guard,), 171, dtype=torch.uint8, device=device)
+        x, w = torch.ones((rows, width), dtype=dtype, device=device), torch.ones(width, device=device)
+        L.norm_rows_grads(None, torch.empty_like(w), torch.empty_like(w), x, x, w, True, scratch=room[:need])
+        assert (room[need:] == 171).all(), (rows, width)
+    for M, N, K in ((3, 40, 50), (3000, 130, 70), (50000, 300, 300), (2000, 65, 65)):
+        need = lib.pet_linear_grads_workspace(A.DTYPES[dtype], M, N, K)
+        room = torch.full((need + guard,), 171, dtype=torch.uint8, device=device)
+        g, x = torch.ones((M, N), dtype=dtype, device=device), torch.ones((M, K), dtype=dtype, device=device)
+        w, b = torch.empty((N, K), device=device), torch.empty(N, device=device)
+        D.linear_grads(g, x, w, b, scratch=room[:need])
+        assert (room[need:] == 171).all() and (w == M).all() and (b == M).all(), (M, N, K)
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:])
+def test_linear_grads_subnormal(device, dtype):
+    """16-bit values below the type's smallest normal one count like any other."""
+    gen = torch.Generator().manual_seed(31)
+    step = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    top = int(1 / torch.finfo(dtype).eps) - 1
+    for M, N, K in ((3000, 300, 260), (648, 64, 64)):
+        g = (torch.randint(-top, top + 1, (M, N), generator=gen).double() * step).to(dtype)
+        x = (torch.randn((M, K), generator=gen) * (2.0 ** 20 if dtype == torch.bfloat16 else 1.0)).to(dtype)
+        gd, xd, ref = g.to(device), x.to(device), g.double().t() @ x.double()
+        wa, ba, turned = (torch.empty(s, device=device) for s in ((N, K), (N,), (K, N)))
+        D.linear_grads(gd, xd, wa, ba)
+        D.linear_grads(xd, gd, turned)
+        tol = linear_bound(g, x, dtype) + 400 * least(torch.float32)
+        within(wa, ref, tol, "w_adj")
+        within(turned.t(), ref, tol, "the other way round")
+        within(ba, g.double().sum(0), (M / 32 + 340) * U * g.double().abs().sum(0) + least(torch.float32), "b_adj")

@@ -153,6 +153,26 @@ def test_layouts_of_gradients():
     assert grads._side_by_side(a, b) and not grads._side_by_side(a, t[0][:, 4:])
 
 
+def test_views_of_one_row():
+    """A row expanded to a matrix of one has a leading dimension of 0."""
+    t = torch.zeros(10)
+    a, b = t[:6].as_strided((1, 6), (0, 1)), t[4:].as_strided((1, 6), (0, 1))
+    assert not grads._side_by_side(a, b)
+
+
+def test_workspaces_follow_the_sizes():
+    """The norm gradients' workspace holds a row of sums a workgroup: no more than
+    there are rows, nor than the chip takes of that width at once."""
+    need = _lib.load().pet_norm_rows_grads_workspace
+    for width in (1, 100, 512, 513, 4096, 4097, 16384):
+        row = 2 * 4 * width
+        assert need(0, width) == need(1, width) == row and need(3, width) == 3 * row
+        most = need((1 << 31) - 1, width)
+        assert most % row == 0 and 256 * row <= most <= 2048 * row
+    assert need((1 << 31) - 1, 16384) == 256 * 2 * 4 * 16384
+    assert _lib.load().pet_grad_workspace((1 << 31) - 1) > 0
+
+
 def test_no_training_kernel_spills(tmp_path):
     """The weight gradients' accumulators, and the norms' rows of a multiple of the
     vector, stay in registers: each spill is read and written every step or row."""
