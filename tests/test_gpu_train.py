@@ -767,3 +767,21 @@ def test_linear_grads_subnormal(device, dtype):
         within(wa, ref, tol, "w_adj")
         within(turned.t(), ref, tol, "the other way round")
         within(ba, g.double().sum(0), (M / 32 + 340) * U * g.double().abs().sum(0) + least(torch.float32), "b_adj")
+
+
+def test_many_tensors_of_every_layout(device):
+    """More tensors than a launch takes, consecutive and with rows apart by turns,
+    then only the one and only the other, with chunks' edges among their sizes."""
+    gen = torch.Generator().manual_seed(37)
+    sizes = [1, 8191, 8192, 8193, 77, 16384, 5, 300]
+    flat = [torch.randn(sizes[i % 8], generator=gen).to(TYPES[i % 3]).to(device) for i in range(500)]
+    base = [torch.randn((sizes[i % 8] // 60 + 1, 70), generator=gen).to(TYPES[i % 3]).to(device) for i in range(260)]
+    apart = [b[:, 2:66] for b in base]
+    for t in (flat, apart, [x for pair in zip(flat, apart) for x in pair]):
+        before, edges = [x.double().cpu() for x in t], [b[:, [0, 1, 66, 67, 68, 69]].clone() for b in base]
+        ref = math.sqrt(sum(float((b ** 2).sum()) for b in before))
+        assert abs(float(G.grad_norm(t)) - ref) <= 1.01 * U * ref
+        assert abs(float(G.clip_grads(t, 0.75 * ref, eps=0.0)) - ref) <= 1.01 * U * ref
+        for x, b in zip(t, before):
+            within(x, 0.75 * b, (2.01 * U + half(x.dtype)) * 0.75 * b.abs() + least(x.dtype), "clipped")
+        assert all(torch.equal(b[:, [0, 1, 66, 67, 68, 69]], e) for b, e in zip(base, edges))
