@@ -29,7 +29,7 @@
 // product of that shape 2.03 ms, of 8192 cubed 1131 TFLOP/s) the products alone take
 // 0.73 ms, the rows' way into LDS alone 0.71, the loads alone 0.60; together the clock
 // falls from 2.2 to 1.8 GHz, and the matrix unit is busy 42% of the cycles. 122688 x
-// 768 x 256 in fp32 takes 187 to 200 us, of which writing and adding the pieces is 30.
+// 768 x 256 in fp32 takes 187 to 200 us, of which writing and adding the pieces is 25.
 //
 // The matrix instruction rounds toward minus infinity, an error with a mean that
 // half a million rows would add up. So a step is summed from zero, the sums of
@@ -335,7 +335,7 @@ __global__ void __launch_bounds__(64 * WN * WK, TN * TK >= 16 ? 2 : 4)
 #pragma unroll
     for (int j = 0; j < TK; ++j) acc[i][j] = f4{0.f, 0.f, 0.f, 0.f};
 
-  // (a wave past the result's edge has no products to make: 62001 x 500 x 333 156 -> 147 us)
+  // (a wave past the result's edge has no products to make: 6% of 62001 x 500 x 333)
   auto first_column = [](int r) { return r / (16 * V) * 16 * V + r / 16 % V; };
   const bool works = n0 + first_column(rn) < a.N && k0 + first_column(rk - C::BN) < a.K;
   auto products = [&](int s) {
@@ -524,7 +524,7 @@ __global__ void __launch_bounds__(64 * WN * WK, TN * TK >= 16 ? 2 : 4)
 
 // adj = beta adj + the pieces' sums in double: a thread sums every eighth piece of
 // four elements, or every 64th of one column's biases, eight loads at a time, and
-// the strips are joined in order. MI355X: 80 pieces of 768 x 256 15 us (24 with a
+// the strips are joined in order. MI355X: 80 pieces of 768 x 256 11 us (24 with a
 // thread an element, its loads one after the other); 26670 x 128 x 512, whose 512
 // pieces of the bias eight strips summed as they do the rest, 66 us a call and 40 now.
 constexpr int kStrips = 8, kSumElements = 4 * 256 / kStrips;
