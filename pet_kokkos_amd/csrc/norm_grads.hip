@@ -457,6 +457,7 @@ int pet_norm_rows_grads(int dtype, int rows, int width, void* in_adj, int64_t ld
   if (weight_adj || bias_adj) {
     if (!workspace || workspace_bytes < pet_norm_rows_grads_workspace(rows, width)) return PET_ATTN_EWORKSPACE;
     if ((reinterpret_cast<uintptr_t>(workspace) & 15u) != 0) return PET_ATTN_EALIGN;
+    if (weight_adj == bias_adj) return PET_ATTN_EINVAL;  // one tensor for both
   }
   return pet_norm_grads_sink(dtype, rows, width, in_adj, lda, out_adj, ldg, in, ldi, weight, ln, weight_adj, bias_adj,
                              beta_w, rows, beta, beta, 0, live, workspace, reinterpret_cast<hipStream_t>(stream));

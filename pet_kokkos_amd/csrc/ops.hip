@@ -569,6 +569,10 @@ int pet_attention_layer_grads(const pet_attn_shape* sh, const pet_layer_grads* g
                               void* stream) {
   if (!grads || (grads->norm_b && !norm_b) || (grads->b_in && !grads->w_in) || (grads->b_out && !grads->w_out))
     return PET_ATTN_EINVAL;
+  const float* to[] = {grads->norm_w, grads->norm_b, grads->w_in, grads->b_in, grads->w_out, grads->b_out};
+  for (int i = 0; i < 6; ++i)  // no tensor twice
+    for (int j = 0; j < i; ++j)
+      if (to[i] && to[i] == to[j]) return PET_ATTN_EINVAL;
   return layer_bwd(sh, grads, tokens_adj, lda, cf_seq_adj, ldca, out_adj, ldo, tokens, ldt, norm_w, norm_b, w_in, b_in,
                    cf_seq, ldc, w_out, off, merged, ml, workspace, workspace_bytes,
                    reinterpret_cast<hipStream_t>(stream));

@@ -153,6 +153,17 @@ def test_layouts_of_gradients():
     assert grads._side_by_side(a, b) and not grads._side_by_side(a, t[0][:, 4:])
 
 
+def test_a_gradient_twice():
+    """One tensor for two gradients would be written by both."""
+    assert norm_grads(wa=A, ba=A) == _lib.EINVAL
+    assert linear_grads(wa=C, ba=C) == _lib.EINVAL
+    sh = _lib.Shape(2, 6, 4, 1, 16, 0, 0.25)
+    need = _lib.load().pet_attention_layer_grads_workspace(ctypes.byref(sh))
+    for pg in (_lib.LayerGrads(norm_w=B, norm_b=B), _lib.LayerGrads(w_in=B, w_out=B), _lib.LayerGrads(norm_w=B, w_out=C, b_out=B)):
+        assert _lib.load().pet_attention_layer_grads(ctypes.byref(sh), ctypes.byref(pg), A, 16, A, 4, A, 16, A, 16, A, A, A,
+                                                     None, A, 4, A, A, A, A, 1 << 20, need, None) == _lib.EINVAL
+
+
 def test_views_of_one_row():
     """A row expanded to a matrix of one has a leading dimension of 0."""
     t = torch.zeros(10)
