@@ -420,7 +420,7 @@ typedef struct pet_layer_grads {
   float beta;
 } pet_layer_grads;
 
-/* Bytes of device workspace pet_attention_layer_grads needs. */
+/* Bytes of device workspace pet_attention_layer_grads needs (0 for a shape that it refuses). */
 PET_ATTN_API size_t pet_attention_layer_grads_workspace(const pet_attn_shape* shape);
 
 /* pet_attention_layer_bwd with the gradients of the layer's parameters

@@ -182,6 +182,10 @@ ChunkWs chunk_ws(const pet_attn_shape& sh, int64_t rows, void* base) {
 
 using namespace pet_attn;
 
+// attention.hip: what a shape has to be
+namespace pet_attn {
+int check_shape(const pet_attn_shape* sh);
+}
 // rows.hip: the norm's backward with the reference's sink
 int pet_rows_norm_bwd_sink(int rows, int width, float* in_adj, int64_t lda, const float* out_adj, int64_t ldg,
                            const float* in, int64_t ldi, const float* weight, int ln, int n_node, float beta_node,
@@ -288,8 +292,16 @@ int attention_bwd_xf(const pet_attn_shape* sh, float* in_adj, int64_t ldi, int d
   return gemm_nn(in_adj, ldi, qkv_adj, 3 * D, w_in, T, 3 * D, d_in, beta, st);
 }
 
+// A shape whose layer has gradients (a layer without tokens may be without slots too).
+int check_layer_shape(const pet_attn_shape* sh) {
+  if (!sh) return PET_ATTN_EINVAL;
+  pet_attn_shape s = *sh;
+  if (s.n_rows == 0 && s.slots == 0) s.slots = 1;
+  return check_shape(&s);
+}
+
 // The room of a layer's parameters' gradients past pet_attention_layer_workspace: the
-// linears' or the norm's, one after the other.
+// linears' or the norm's, one after the other (of a shape that check_layer_shape takes).
 size_t layer_grads_bytes(const pet_attn_shape* sh) {
   const int D = sh->heads * sh->head_dim, T = sh->n_rows;
   return align256(std::max({pet_linear_grads_bytes(PET_DTYPE_F32, T, D, D),
@@ -303,8 +315,11 @@ int layer_bwd(const pet_attn_shape* sh, const pet_layer_grads* pg, float* tokens
               const float* w_out, const int* off, const float* merged, const float* ml, void* workspace,
               size_t workspace_bytes, hipStream_t st) {
   if (!sh || !tokens_adj || !tokens || !norm_w || !w_in || !off) return PET_ATTN_EINVAL;
+  if (pg)
+    if (int e = check_layer_shape(sh)) return e;
   const int D = sh->heads * sh->head_dim, T = sh->n_rows;
   if (ldt < D || lda < D) return PET_ATTN_EINVAL;
+  if (T > 0 && (!out_adj || !w_out || ldo < D)) return PET_ATTN_EINVAL;  // (read before the attention's own checks)
   if (pg && (!out_adj || !merged || ldo < D || D > PET_NORM_MAX_WIDTH)) return PET_ATTN_EINVAL;
   const size_t need = pet_attention_layer_workspace(sh);
   if (!workspace || workspace_bytes < need + (pg ? layer_grads_bytes(sh) : 0)) return PET_ATTN_EWORKSPACE;
@@ -558,7 +573,7 @@ int pet_attention_layer_bwd(const pet_attn_shape* sh, float* tokens_adj, int64_t
 }
 
 size_t pet_attention_layer_grads_workspace(const pet_attn_shape* sh) {
-  return sh ? pet_attention_layer_workspace(sh) + layer_grads_bytes(sh) : 0;
+  return check_layer_shape(sh) == PET_ATTN_OK ? pet_attention_layer_workspace(sh) + layer_grads_bytes(sh) : 0;
 }
 
 int pet_attention_layer_grads(const pet_attn_shape* sh, const pet_layer_grads* grads, float* tokens_adj, int64_t lda,

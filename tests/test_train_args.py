@@ -193,3 +193,34 @@ def test_no_training_kernel_spills(tmp_path):
     norms = {n: s for n, s in sizes.items() if "norm_grads_kernel" in n and "ELb1EL" in n or "norm_typed_fwd" in n}
     assert len(wgrad) == 9 and len(norms) > 40
     assert {n: s for n, s in {**wgrad, **norms}.items() if s > 0} == {}
+
+
+def test_layer_grads_refuse_a_shape():
+    """A shape without heads, columns or rows enough comes back as an error (no size is
+    computed of it), and so do products of nothing."""
+    lib = _lib.load()
+
+    def call(sh, w_out=A, out_adj=A, pg=_lib.LayerGrads(), ldo=16):
+        return lib.pet_attention_layer_grads(ctypes.byref(sh), ctypes.byref(pg), A, 16, A, 4, out_adj, ldo, A, 16, A, A, A,
+                                             None, A, 4, w_out, A, A, A, 1 << 20, 1 << 40, None)
+    for bad, code in (((2, 6, 4, 0, 16), _lib.EINVAL), ((2, 6, 4, 1, 0), _lib.EHEADDIM), ((2, 6, 4, -1, 16), _lib.EINVAL),
+                      ((2, 6, 4, 1, -16), _lib.EHEADDIM), ((2, 6, 4, 1, 129), _lib.EHEADDIM), ((2, -6, 4, 1, 16), _lib.EINVAL),
+                      ((2, 1, 4, 1, 16), _lib.EINVAL), ((-1, 6, 4, 1, 16), _lib.EINVAL), ((2, 6, 0, 1, 16), _lib.EINVAL),
+                      ((0, 0, 0, 0, 16), _lib.EINVAL), ((2, (1 << 31) - 1, 4, 64, 128), _lib.EINDEX)):
+        sh = _lib.Shape(*bad, 0, 0.25)
+        assert lib.pet_attention_layer_grads_workspace(ctypes.byref(sh)) == 0, bad
+        assert call(sh) == code, bad
+    sh = _lib.Shape(2, 6, 4, 1, 16, 0, 0.25)
+    assert call(sh, w_out=None) == call(sh, out_adj=None) == call(sh, ldo=15) == _lib.EINVAL
+    assert lib.pet_attention_layer_grads_workspace(ctypes.byref(_lib.Shape(0, 0, 0, 1, 16, 0, 0.25))) > 0  # no tokens: no slots
+
+
+def test_layer_bwd_refuses_no_operands():
+    """The backward without parameters' gradients: a null operand of its first product."""
+    lib = _lib.load()
+    sh = _lib.Shape(2, 6, 4, 1, 16, 0, 0.25)
+
+    def call(w_out=A, out_adj=A, ldo=16):
+        return lib.pet_attention_layer_bwd(ctypes.byref(sh), A, 16, A, 4, out_adj, ldo, A, 16, A, A, A, None, A, 4, w_out, A,
+                                           A, A, 1 << 20, 1 << 40, None)
+    assert call(w_out=None) == call(out_adj=None) == call(ldo=15) == _lib.EINVAL
