@@ -20,8 +20,8 @@ from .attention import DTYPES, _call_on, _scratch
 class GradList:
     """The tensors of a step's gradients, checked and laid out for the library
     once: contiguous in any order of their axes, or a 2-D view of rows (or a column) in
-    a wider matrix; all on one device, no two overlapping. It keeps the memory that
-    they have now, and every call reads what that then holds (a gradient set anew
+    a wider matrix; all on one device, no two overlapping (different columns of one
+    matrix do not). It keeps the memory that they have now, and every call reads what that then holds (a gradient set anew
     needs a new list)."""
 
     def __init__(self, tensors):
@@ -75,14 +75,14 @@ def _layout(t: torch.Tensor, i: int):
 
 
 def _side_by_side(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether two 2-D views whose spans overlap are different columns of one matrix."""
-    if a.dim() != 2 or b.dim() != 2 or a.dtype != b.dtype or a.stride() != b.stride() or a.stride(1) != 1:
-        return False
-    ld = a.stride(0)
-    if ld < 1:
-        return False
-    gap = (b.data_ptr() - a.data_ptr()) // a.element_size() % ld
-    return gap >= a.shape[1] and gap + b.shape[1] <= ld
+    """Whether two views whose spans overlap are different columns of one matrix: their
+    rows lie whole multiples of the leading dimensions' common divisor apart, so
+    columns that are apart modulo that never meet."""
+    (rows_a, cols_a, ld_a), (rows_b, cols_b, ld_b) = _layout(a, 0), _layout(b, 1)
+    wide_a, wide_b = cols_a * a.element_size(), cols_b * b.element_size()
+    step = math.gcd(ld_a * a.element_size() if rows_a > 1 else 0, ld_b * b.element_size() if rows_b > 1 else 0)
+    gap = (b.data_ptr() - a.data_ptr()) % step if step else 0
+    return gap >= wide_a and gap + wide_b <= step
 
 
 def _arguments(grads, norm_type, scale):

@@ -785,3 +785,20 @@ def test_many_tensors_of_every_layout(device):
         for x, b in zip(t, before):
             within(x, 0.75 * b, (2.01 * U + half(x.dtype)) * 0.75 * b.abs() + least(x.dtype), "clipped")
         assert all(torch.equal(b[:, [0, 1, 66, 67, 68, 69]], e) for b, e in zip(base, edges))
+
+
+def test_gradients_between_each_other(device):
+    """Columns of one matrix as gradients of their own, transposed views among them."""
+    m = torch.arange(1.0, 2401.0, device=device).view(40, 60)
+    before = m.double().cpu()
+    for views in ([m[:, 0], m[:, 1], m[:, 2]], [m.t()[:7], m.t()[7:50]], [m[::2, :9], m[1::2, :9], m[:, 9]]):
+        took = torch.zeros(40, 60, dtype=torch.bool, device=device)
+        for v in views:
+            torch.as_strided(took, v.shape, v.stride(), v.storage_offset()).fill_(True)
+        took, m0 = took.cpu(), m.double().cpu()
+        ref = float(m0[took].pow(2).sum().sqrt())
+        assert abs(float(G.clip_grads(views, 0.5 * ref, eps=0.0)) - ref) <= 1.01 * U * ref
+        within(m, torch.where(took, 0.5 * m0, m0), torch.where(took, 2.01 * U * m0, 0.0), "clipped")
+        m.copy_(before)
+    with pytest.raises(ValueError):
+        G.GradList([m[:, :2], m[:, 1]])

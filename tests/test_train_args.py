@@ -224,3 +224,15 @@ def test_layer_bwd_refuses_no_operands():
         return lib.pet_attention_layer_bwd(ctypes.byref(sh), A, 16, A, 4, out_adj, ldo, A, 16, A, A, A, None, A, 4, w_out, A,
                                            A, A, 1 << 20, 1 << 40, None)
     assert call(w_out=None) == call(out_adj=None) == call(ldo=15) == _lib.EINVAL
+
+
+def test_columns_side_by_side():
+    """Views whose elements lie between each other's are apart where their columns are."""
+    m, h = torch.zeros(12, 10), torch.zeros(12, 20, dtype=torch.float16)
+    for a, b in ((m[:, 0], m[:, 1]), (m[:, 1], m[:, 0]), (m.t()[:3], m.t()[3:]), (m.t()[:3], m[:, 3:]), (m[:, 0], m[:, 1:]),
+                 (m[::2, :4], m[:, 4:]), (m[::3, :4], m[::2, 4:]), (m[::2], m[1::2]), (m[2, 3:5], m[:, :3]),
+                 (m[:, :3], m[2, 3:5]), (h[:, :6], h.view(torch.float32)[:, 3:])):
+        assert grads._side_by_side(a, b) and grads._side_by_side(b, a)
+    for a, b in ((m[:, 0], m[:, 0]), (m[:, :2], m[:, 1]), (m.t()[:4], m[:, 3:]), (m[::2, :5], m[:, 4:]), (m[::2], m[::3]),
+                 (m[2], m[:, :3]), (m[2, 2:5], m[:, :3]), (m, m[:, 3]), (h[:, :7], h.view(torch.float32)[:, 3:])):
+        assert not grads._side_by_side(a, b) and not grads._side_by_side(b, a)
