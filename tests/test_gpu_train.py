@@ -802,3 +802,20 @@ def test_gradients_between_each_other(device):
         m.copy_(before)
     with pytest.raises(ValueError):
         G.GradList([m[:, :2], m[:, 1]])
+
+
+def test_norm_rows_past_a_launch(device):
+    """More rows than one launch's threads: 2^28 of them at 16 lanes a row."""
+    rows = (1 << 28) + 21
+    x = torch.empty((rows, 1), dtype=torch.bfloat16, device=device)
+    for r in range(0, rows, 1 << 26):
+        n = min(1 << 26, rows - r)
+        x[r:r + n, 0] = (torch.arange(r, r + n, device=device) % 7 - 3).bfloat16()
+    out, w = torch.full_like(x, 9.0), torch.full((1,), 2.0, device=device)
+    L.norm_rows(out, x, w, None)
+    for r in range(0, rows, 1 << 26):  # x / |x|: exact in bf16
+        assert torch.equal(out[r:r + (1 << 26)], 2 * torch.sign(x[r:r + (1 << 26)]))
+    x32, out32 = x[:1000].float(), torch.empty((1000, 1), device=device)
+    A._lib.check(A._lib.load().pet_norm_rows_typed(0, 1000, 1, out32.data_ptr(), 1, x32.data_ptr(), 1, w.data_ptr(), None,
+                                                   A._stream()), "fp32")
+    assert torch.equal(out32.bfloat16(), out[:1000])
