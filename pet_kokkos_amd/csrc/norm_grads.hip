@@ -31,7 +31,9 @@ using pet_typed::u4e;
 constexpr float kRmsEps = 1.1920928955078125e-07f;  // float32 epsilon
 constexpr float kLnEps = 1e-5f;
 
-constexpr int64_t kLaunchThreads = int64_t(1) << 31;  // of a launch at most
+// A launch's threads at most: HIP takes them modulo 2^32 and reports nothing
+// (2^28 + 21 rows of 16 lanes in one: all but the first rows left as they were).
+constexpr int64_t kLaunchThreads = int64_t(1) << 31;
 
 constexpr int threads_of(int TPR) { return TPR > 256 ? TPR : 256; }
 // Waves a SIMD of the backward, by the elements a lane holds (x, g, the weight and
@@ -422,29 +424,23 @@ int pet_norm_rows_typed(int dtype, int rows, int width, void* out, int64_t ldo, 
       !pet_typed::element_aligned(weight, PET_DTYPE_F32) || !pet_typed::element_aligned(bias, PET_DTYPE_F32))
     return PET_ATTN_EALIGN;
   if (rows == 0) return PET_ATTN_OK;
-  // in launches of `most` rows: HIP takes a launch's threads modulo 2^32 and reports nothing
-  // (2^28 + 21 rows of 16 lanes in one: all but the first rows left as they were)
-  auto launches = [&](int64_t most, auto&& launch) {
-    for (int64_t r = 0; r < rows; r += most)
-      if (int e = launch(r, int(std::min(most, rows - r)))) return e;
-    return int(PET_ATTN_OK);
-  };
   if (dtype == PET_DTYPE_F32 && width <= 2048)
-    return launches(kLaunchThreads / 64, [&](int64_t r, int n) {
-      return pet_norm_rows(n, width, static_cast<float*>(out) + r * ldo, ldo, static_cast<const float*>(in) + r * ldi,
-                           ldi, weight, bias, stream);
-    });
+    return pet_norm_rows(rows, width, static_cast<float*>(out), ldo, static_cast<const float*>(in), ldi, weight, bias,
+                         stream);
   return pet_typed::with_dtype(dtype, [&](auto tv) {
     using T = decltype(tv);
     return with_row<T>(width, [&](auto lc, auto cc) {
       constexpr int TPR = decltype(lc)::value, C = decltype(cc)::value, TH = threads_of(TPR), RPB = TH / TPR;
       const auto kernel = width % kVec<T> ? norm_typed_fwd_kernel<T, TPR, C, false> : norm_typed_fwd_kernel<T, TPR, C, true>;
-      return launches(kLaunchThreads / TPR, [&](int64_t r, int n) {
+      constexpr int64_t most = kLaunchThreads / TPR;
+      for (int64_t r = 0; r < rows; r += most) {
+        const int n = int(std::min(most, rows - r));
         hipLaunchKernelGGL(kernel, dim3(unsigned((int64_t(n) + RPB - 1) / RPB)), dim3(TH), 0,
                            reinterpret_cast<hipStream_t>(stream), n, width, 1.0f / width, static_cast<T*>(out) + r * ldo,
                            ldo, static_cast<const T*>(in) + r * ldi, ldi, weight, bias);
-        return hipGetLastError() == hipSuccess ? int(PET_ATTN_OK) : int(PET_ATTN_ELAUNCH);
-      });
+        if (hipGetLastError() != hipSuccess) return int(PET_ATTN_ELAUNCH);
+      }
+      return int(PET_ATTN_OK);
     });
   });
 }

@@ -11,6 +11,7 @@
 // row is read from memory once.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
 #include <type_traits>
 
@@ -374,6 +375,15 @@ int with_vec(int width, F&& f) {
 inline bool aligned16(const void* p, int64_t ld) {
   return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 4 == 0;
 }
+// HIP takes a launch's threads modulo 2^32 and reports nothing, so more rows than
+// these (at 64 lanes each 2^31 threads) go in launches of them, or are refused.
+constexpr int64_t kLaunchRows = int64_t(1) << 25;
+template <class F>
+int launches(int rows, F&& f) {
+  for (int64_t r = 0; r < rows; r += kLaunchRows)
+    if (int e = f(r, int(std::min(kLaunchRows, rows - r)))) return e;
+  return PET_ATTN_OK;
+}
 
 }  // namespace pet_rows
 
@@ -388,9 +398,16 @@ int pet_rows_norm_bwd_sink(int rows, int width, float* in_adj, int64_t lda, cons
   if (rows < 0 || width < 1) return PET_ATTN_EINVAL;
   if (!in_adj || !out_adj || !in || !weight || lda < width || ldg < width || ldi < width) return PET_ATTN_EINVAL;
   if (rows == 0) return PET_ATTN_OK;
+  if (rows > kLaunchRows && !live_off)
+    return launches(rows, [&](int64_t r, int n) {
+      return pet_rows_norm_bwd_sink(n, width, in_adj + r * lda, lda, out_adj + r * ldg, ldg, in + r * ldi, ldi, weight,
+                                    ln, int(std::min(std::max(n_node - r, int64_t(0)), int64_t(n))), beta_node,
+                                    beta_edge, nullptr, st);
+    });
   if (aligned16(in_adj, lda) && aligned16(out_adj, ldg) && aligned16(in, ldi) && aligned16(weight, 4)) {
     const int e = with_vec(width, [&](auto lc, auto cc) {
       constexpr int LPR = decltype(lc)::value, C4 = decltype(cc)::value, RPB = 4 * (64 / LPR);
+      if (rows > kLaunchRows / LPR * 64) return int(PET_ATTN_EINDEX);
       hipLaunchKernelGGL((norm_bwd4_kernel<LPR, C4>), dim3(unsigned((rows + RPB - 1) / RPB)), dim3(256), 0, st, rows,
                          width, in_adj, lda, out_adj, ldg, in, ldi, weight, ln, n_node, beta_node, beta_edge,
                          live_off);
@@ -400,6 +417,7 @@ int pet_rows_norm_bwd_sink(int rows, int width, float* in_adj, int64_t lda, cons
   }
   return with_lanes(width, [&](auto vc) {
     constexpr int V = decltype(vc)::value;
+    if (rows > kLaunchRows) return int(PET_ATTN_EINDEX);
     hipLaunchKernelGGL(norm_bwd_kernel<V>, dim3(unsigned((rows + 3) / 4)), dim3(256), 0, st, rows, width, in_adj, lda,
                        out_adj, ldg, in, ldi, weight, ln, n_node, beta_node, beta_edge, live_off);
     return hipGetLastError() == hipSuccess ? int(PET_ATTN_OK) : int(PET_ATTN_ELAUNCH);
@@ -409,6 +427,8 @@ int pet_rows_norm_bwd_sink(int rows, int width, float* in_adj, int64_t lda, cons
 int pet_rows_rms_inv(int rows, int width, const float* in, int64_t ldi, float* inv, hipStream_t st) {
   if (rows < 0 || width < 1 || !in || !inv || ldi < width) return PET_ATTN_EINVAL;
   if (rows == 0) return PET_ATTN_OK;
+  if (rows > kLaunchRows)
+    return launches(rows, [&](int64_t r, int n) { return pet_rows_rms_inv(n, width, in + r * ldi, ldi, inv + r, st); });
   if (aligned16(in, ldi)) {
     const int e = with_vec(width, [&](auto lc, auto cc) {
       constexpr int LPR = decltype(lc)::value, C4 = decltype(cc)::value, RPB = 4 * (64 / LPR);
@@ -449,6 +469,10 @@ int pet_norm_rows(int rows, int width, float* out, int64_t ldo, const float* in,
                   const float* bias, void* stream) {
   if (rows < 0 || width < 1 || !out || !in || !weight || ldo < width || ldi < width) return PET_ATTN_EINVAL;
   if (rows == 0) return PET_ATTN_OK;
+  if (rows > kLaunchRows)
+    return launches(rows, [&](int64_t r, int n) {
+      return pet_norm_rows(n, width, out + r * ldo, ldo, in + r * ldi, ldi, weight, bias, stream);
+    });
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   if (aligned16(out, ldo) && aligned16(in, ldi) && aligned16(weight, 4) && (!bias || aligned16(bias, 4))) {
     const int e = with_vec(width, [&](auto lc, auto cc) {

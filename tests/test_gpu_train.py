@@ -819,3 +819,25 @@ def test_norm_rows_past_a_launch(device):
     A._lib.check(A._lib.load().pet_norm_rows_typed(0, 1000, 1, out32.data_ptr(), 1, x32.data_ptr(), 1, w.data_ptr(), None,
                                                    A._stream()), "fp32")
     assert torch.equal(out32.bfloat16(), out[:1000])
+
+
+def test_fp32_rows_past_a_launch(device):
+    """The same of the fp32 norms to 2048 columns, at 64 lanes a row: forward, the
+    typed entry that calls it, backward."""
+    rows = (1 << 26) + 300
+    x = (torch.arange(rows, device=device) % 5 - 2).float()[:, None]
+    w, lib = torch.full((1,), 2.0, device=device), A._lib.load()
+    for call in (lambda o: L.norm_rows(o, x, w, None),
+                 lambda o: A._lib.check(lib.pet_norm_rows_typed(0, rows, 1, o.data_ptr(), 1, x.data_ptr(), 1, w.data_ptr(), None,
+                                                                A._stream()), "typed")):
+        out = torch.full_like(x, 9.0)
+        call(out)
+        for r in range(0, 5):  # a value's rows are of the same bits, 2 sign(x) to eps and four roundings
+            part = out[r::5]
+            assert (part == part[0]).all() and abs(float(part[0]) - 2 * ((r > 2) - (r < 2))) <= 10 * U
+    adj = torch.full_like(x, 9.0)
+    L.norm_rows_bwd(adj, torch.ones_like(x), x, w, False)
+    for r in range(0, 5):  # 2 eps / (x^2 + eps)^1.5: of x = 0 2 / sqrt(eps), else eps and the roundings of 2 - 2 xhat^2
+        part = adj[r::5]
+        ref, tol = (2 * 2 ** 11.5, 8 * U * 2 ** 12.5) if r == 2 else (0.0, 32 * U)
+        assert (part == part[0]).all() and abs(float(part[0]) - ref) <= tol
