@@ -244,7 +244,8 @@ PET_ATTN_API size_t pet_linear_grads_workspace(int dtype, int M, int N, int K);
  * rows' products exact, the sums in fp32 and in a fixed order. live (device, may
  * be NULL): only rows m < *live count, the rows after are not read. w_adj and
  * b_adj overlap nothing; workspace 16-byte aligned, its contents nobody's after
- * the call. No counterpart in the reference, which has no gradients of parameters. */
+ * the call. W has at most 2^30 elements, and fewer than 2^24 tiles of 64 x 64. No
+ * counterpart in the reference, which has no gradients of parameters. */
 PET_ATTN_API int pet_linear_grads(int dtype, int M, int N, int K, const void* out_adj, int64_t ldo, const void* in,
                                   int64_t ldi, const int* live, float* w_adj, int64_t ldw, float* b_adj, float beta,
                                   void* workspace, size_t workspace_bytes, void* stream);

@@ -680,6 +680,8 @@ int pet_linear_grads(int dtype, int M, int N, int K, const void* out_adj, int64_
   if (!pet_typed::dtype_ok(dtype) || M < 0 || N < 1 || K < 1) return PET_ATTN_EINVAL;
   if (!w_adj || b_adj == w_adj || ldo < N || ldi < K || ldw < K || (M > 0 && (!out_adj || !in))) return PET_ATTN_EINVAL;
   if (int64_t(N) > (int64_t(1) << 30) / K) return PET_ATTN_EINDEX;
+  // (2^24 workgroups of 256 threads would come out as none: HIP takes them modulo 2^32)
+  if ((int64_t(N) + 63) / 64 * ((int64_t(K) + 63) / 64) >> 24) return PET_ATTN_EINDEX;
   if (!pet_typed::element_aligned(out_adj, dtype) || !pet_typed::element_aligned(in, dtype) ||
       !pet_typed::element_aligned(w_adj, PET_DTYPE_F32) || !pet_typed::element_aligned(b_adj, PET_DTYPE_F32))
     return PET_ATTN_EALIGN;

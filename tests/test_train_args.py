@@ -236,3 +236,11 @@ def test_columns_side_by_side():
     for a, b in ((m[:, 0], m[:, 0]), (m[:, :2], m[:, 1]), (m.t()[:4], m[:, 3:]), (m[::2, :5], m[:, 4:]), (m[::2], m[::3]),
                  (m[2], m[:, :3]), (m[2, 2:5], m[:, :3]), (m, m[:, 3]), (h[:, :7], h.view(torch.float32)[:, 3:])):
         assert not grads._side_by_side(a, b) and not grads._side_by_side(b, a)
+
+
+def test_linear_grads_past_a_launch():
+    """A weight of 2^24 tiles: 2^32 threads of one launch, which would come out as none."""
+    one, edge = 1 << 30, (1 << 30) - 64
+    assert linear_grads(N=one, K=1, ldg=one, ldx=1, ldw=1) == linear_grads(N=1, K=one, ldg=1, ldx=one, ldw=one) == _lib.EINDEX
+    assert linear_grads(N=edge + 1, K=1, ldg=one, ldx=1, ldw=1) == _lib.EINDEX
+    assert linear_grads(N=edge, K=1, ldg=one, ldx=1, ldw=1, ws=None) == _lib.EWORKSPACE  # fits
