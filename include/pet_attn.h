@@ -354,7 +354,8 @@ enum { PET_DTYPE_F32 = 0, PET_DTYPE_BF16 = 1, PET_DTYPE_F16 = 2 };
 /* pet_norm_rows with rows in fp32, bf16 or fp16 (dtype, in's and out's; the
  * weights fp32, the sums in fp32, one rounding to the type at the end), up to
  * PET_NORM_MAX_WIDTH wide; any alignment of an element (fp32 to 2048 columns is
- * pet_norm_rows itself). No counterpart in the reference. */
+ * pet_norm_rows itself). out may be in (with its leading dimension), and nothing
+ * else may overlap. No counterpart in the reference. */
 PET_ATTN_API int pet_norm_rows_typed(int dtype, int rows, int width, void* out, int64_t ldo, const void* in,
                                      int64_t ldi, const float* weight, const float* bias, void* stream);
 

@@ -420,6 +420,7 @@ int pet_norm_rows_typed(int dtype, int rows, int width, void* out, int64_t ldo, 
                         const float* weight, const float* bias, void* stream) {
   if (!pet_typed::dtype_ok(dtype) || rows < 0 || width < 1 || width > PET_NORM_MAX_WIDTH) return PET_ATTN_EINVAL;
   if ((rows > 0 && (!out || !in)) || !weight || ldo < width || ldi < width) return PET_ATTN_EINVAL;
+  if (rows > 1 && out == in && ldo != ldi) return PET_ATTN_EINVAL;  // in place, but of other rows
   if (!pet_typed::element_aligned(out, dtype) || !pet_typed::element_aligned(in, dtype) ||
       !pet_typed::element_aligned(weight, PET_DTYPE_F32) || !pet_typed::element_aligned(bias, PET_DTYPE_F32))
     return PET_ATTN_EALIGN;
@@ -459,6 +460,7 @@ int pet_norm_rows_grads(int dtype, int rows, int width, void* in_adj, int64_t ld
   if ((rows > 0 && (!out_adj || !in)) || !weight || ldg < width || ldi < width || (in_adj && lda < width))
     return PET_ATTN_EINVAL;
   if ((rows > 0 && !in_adj && !weight_adj && !bias_adj) || (bias_adj && !ln)) return PET_ATTN_EINVAL;
+  if (rows > 1 && ((in_adj == out_adj && lda != ldg) || (in_adj == in && lda != ldi))) return PET_ATTN_EINVAL;
   if (!pet_typed::element_aligned(in_adj, dtype) || !pet_typed::element_aligned(out_adj, dtype) ||
       !pet_typed::element_aligned(in, dtype) || !pet_typed::element_aligned(weight, PET_DTYPE_F32) ||
       !pet_typed::element_aligned(weight_adj, PET_DTYPE_F32) || !pet_typed::element_aligned(bias_adj, PET_DTYPE_F32))

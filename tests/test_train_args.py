@@ -244,3 +244,12 @@ def test_linear_grads_past_a_launch():
     assert linear_grads(N=one, K=1, ldg=one, ldx=1, ldw=1) == linear_grads(N=1, K=one, ldg=1, ldx=one, ldw=one) == _lib.EINDEX
     assert linear_grads(N=edge + 1, K=1, ldg=one, ldx=1, ldw=1) == _lib.EINDEX
     assert linear_grads(N=edge, K=1, ldg=one, ldx=1, ldw=1, ws=None) == _lib.EWORKSPACE  # fits
+
+
+def test_in_place_needs_the_same_rows():
+    """In place with another leading dimension a row would be written over one not yet read."""
+    assert norm(out=A, inp=A, ldo=8, ldi=9) == norm(dtype=F32, out=A, inp=A, ldo=9, ldi=8) == _lib.EINVAL
+    assert norm_grads(in_adj=A, lda=9, g=A, ldg=8) == norm_grads(in_adj=A, lda=8, x=A, ldx=9) == _lib.EINVAL
+    # one row has no next one: past that check, to the workspace's
+    assert norm_grads(rows=1, in_adj=A, lda=9, g=A, ldg=8, ws=None) == _lib.EWORKSPACE
+    assert norm_grads(in_adj=A, lda=9, g=A, ldg=9, ws=None) == norm_grads(in_adj=None, lda=0, g=A, ws=None) == _lib.EWORKSPACE
