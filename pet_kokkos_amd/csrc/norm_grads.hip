@@ -130,10 +130,11 @@ __device__ __forceinline__ void center(float (&x)[n], float mu, int left) {
   }
 }
 
+// (out may be in: neither is __restrict__, here or in the backward, where in_adj may be either)
 template <class T, int TPR, int C, bool WHOLE>
-__global__ void __launch_bounds__(threads_of(TPR)) norm_typed_fwd_kernel(int rows, int width, float per, T* __restrict__ out,
-                                                                         int64_t ldo, const T* __restrict__ in,
-                                                                         int64_t ldi, const float* __restrict__ weight,
+__global__ void __launch_bounds__(threads_of(TPR)) norm_typed_fwd_kernel(int rows, int width, float per, T* out,
+                                                                         int64_t ldo, const T* in, int64_t ldi,
+                                                                         const float* __restrict__ weight,
                                                                          const float* __restrict__ bias) {
   constexpr int V = kVec<T>, RPB = threads_of(TPR) / TPR;
   __shared__ float red[TPR > 64 ? TPR / 64 : 1][2][3];
@@ -185,10 +186,10 @@ __global__ void __launch_bounds__(threads_of(TPR)) norm_typed_fwd_kernel(int row
 // gradients, and go onto beta_w times w_adj and b_adj themselves.
 template <class T, int TPR, int C, bool WHOLE, bool LN>
 __global__ void __launch_bounds__(threads_of(TPR), waves_of(C * kVec<T>, TPR))
-    norm_grads_kernel(int rows, int width, float per, T* __restrict__ in_adj, int64_t lda,
-                      const T* __restrict__ out_adj, int64_t ldg, const T* __restrict__ in, int64_t ldi, const float* __restrict__ weight, int n_node,
-                      float beta_node, float beta_edge, int live_base, const int* __restrict__ live,
-                      float* __restrict__ part, float* __restrict__ w_adj, float* __restrict__ b_adj, float beta_w) {
+    norm_grads_kernel(int rows, int width, float per, T* in_adj, int64_t lda, const T* out_adj, int64_t ldg,
+                      const T* in, int64_t ldi, const float* __restrict__ weight, int n_node, float beta_node,
+                      float beta_edge, int live_base, const int* __restrict__ live, float* __restrict__ part,
+                      float* __restrict__ w_adj, float* __restrict__ b_adj, float beta_w) {
   constexpr int V = kVec<T>, RPB = threads_of(TPR) / TPR;
   __shared__ float red[TPR > 64 ? TPR / 64 : 1][2][3];
   const int t = threadIdx.x % TPR, g0 = threadIdx.x / TPR;

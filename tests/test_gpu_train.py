@@ -841,3 +841,29 @@ def test_fp32_rows_past_a_launch(device):
         part = adj[r::5]
         ref, tol = (2 * 2 ** 11.5, 8 * U * 2 ** 12.5) if r == 2 else (0.0, 32 * U)
         assert (part == part[0]).all() and abs(float(part[0]) - ref) <= tol
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("ln", [False, True])
+def test_norms_in_place(device, dtype, ln):
+    """The forward over its input, the adjoint over out_adj and over the input (beta
+    0 and not): the bits of the calls that write elsewhere."""
+    gen = torch.Generator().manual_seed(41)
+    for width, pad in ((5, 0), (63, 3), (200, 0), (777, 1), (1024, 0), (3001, 1), (5000, 0), (9001, 1)):
+        x, g = rows_of(gen, 41, width, dtype, device, pad), rows_of(gen, 41, width, dtype, device, pad, size=1e-2)
+        w = (1 + 0.1 * torch.randn(width, generator=gen)).to(device)
+        b = (0.1 * torch.randn(width, generator=gen)).to(device) if ln else None
+
+        def copy(t):
+            return torch.empty_strided(t.shape, t.stride(), dtype=dtype, device=device).copy_(t)
+        out, into = copy(x), copy(x)
+        L.norm_rows(out, x, w, b)
+        L.norm_rows(into, into, w, b)
+        assert torch.equal(out, into), width
+        for beta in (0.0, 0.5):
+            for at in (0, 1):
+                args = [copy(g), copy(x)]
+                adj = copy(args[at])
+                L.norm_rows_grads(adj, None, None, *args, w, ln, beta)
+                L.norm_rows_grads(args[at], None, None, *args, w, ln, beta)
+                assert torch.equal(adj, args[at]), (width, beta, at)
