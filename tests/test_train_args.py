@@ -253,3 +253,11 @@ def test_in_place_needs_the_same_rows():
     # one row has no next one: past that check, to the workspace's
     assert norm_grads(rows=1, in_adj=A, lda=9, g=A, ldg=8, ws=None) == _lib.EWORKSPACE
     assert norm_grads(in_adj=A, lda=9, g=A, ldg=9, ws=None) == norm_grads(in_adj=None, lda=0, g=A, ws=None) == _lib.EWORKSPACE
+
+
+def test_a_launch_takes_what_its_arguments_hold():
+    """4096 bytes of arguments: 56 of a launch's own, then 16 a slot, two a tensor whose
+    rows are apart; the workspace is of that many tensors a launch."""
+    need = _lib.load().pet_grad_workspace
+    most = (4096 - 56) // 16 // 2
+    assert need(most) == need(1) and need(most + 1) == 2 * need(1) and need(10 * most) == 10 * need(1)
