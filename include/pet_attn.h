@@ -425,8 +425,8 @@ typedef struct pet_layer_grads {
 PET_ATTN_API size_t pet_attention_layer_grads_workspace(const pet_attn_shape* shape);
 
 /* pet_attention_layer_bwd with the gradients of the layer's parameters
- * (pet_linear_grads of the two linears, pet_norm_rows_grads of the norm) over
- * the live rows: the layer's training backward. tokens_adj and cf_seq_adj as
+ * (pet_linear_grads of the two linears, at its accuracy for fp32 rows,
+ * pet_norm_rows_grads of the norm) over the live rows: the layer's training backward. tokens_adj and cf_seq_adj as
  * pet_attention_layer_bwd's (to fp32 roundings: qkv's adjoint is kept in fp32
  * for w_in's gradient). No counterpart in the reference. */
 PET_ATTN_API int pet_attention_layer_grads(const pet_attn_shape* shape, const pet_layer_grads* grads,

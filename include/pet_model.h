@@ -240,8 +240,14 @@ PET_ATTN_API size_t pet_linear_grads_workspace(int dtype, int M, int N, int K);
  * ldo), both of one dtype (PET_DTYPE_*), at any alignment of an element:
  *   w_adj[n][k] = beta w_adj[n][k] + sum over m of out_adj[m][n] in[m][k],
  *   b_adj[n]    = beta b_adj[n]    + sum over m of out_adj[m][n]  (b_adj may be NULL),
- * fp32 (w_adj ld ldw); beta 0 overwrites. fp32 rows at fp32 accuracy, 16-bit
- * rows' products exact, the sums in fp32 and in a fixed order. live (device, may
+ * fp32 (w_adj ld ldw); beta 0 overwrites. The sums run in fp32 and in a fixed
+ * order; 16-bit rows' products are exact. fp32 rows go as pairs of fp16 values under
+ * a power of two a column: a factor is held to 2^-23 of itself or 2^-36 of its
+ * column's largest magnitude, whichever is more, and a product to a further 2^-22. So
+ * a column whose largest value passes the rest 2^13 times holds the rest to fewer
+ * digits, which shows where that value's other factor is zero: 1e6 times the rest
+ * in 1024 rows 2e-7 of sum |out_adj| |in|, 1e8 times 3e-5 (plain fp32 6e-8). An
+ * infinity anywhere is multiplied in fp32. live (device, may
  * be NULL): only rows m < *live count, the rows after are not read. w_adj and
  * b_adj overlap nothing; workspace 16-byte aligned, its contents nobody's after
  * the call. W has at most 2^30 elements, and fewer than 2^24 tiles of 64 x 64. No

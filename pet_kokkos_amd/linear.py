@@ -293,7 +293,9 @@ def linear_grads(out_adj, inp, w_adj, b_adj=None, beta=0.0, live=None, scratch=N
     """The parameters' gradients of out = inp W^T + b: w_adj [N, K] = beta *
     w_adj + out_adj^T inp and b_adj [N] (None: not made) = beta * b_adj + the
     sum of out_adj's rows, from inp [M, K] and out_adj [M, N] of one type
-    (float32, bfloat16 or float16); the gradients are float32. ``live`` (one
+    (float32, bfloat16 or float16); the gradients are float32. A value of float32
+    rows is held to 2^-23 of itself or 2^-36 of its column's largest, whichever is
+    more (pet_linear_grads says what an outlier costs). ``live`` (one
     int32 on the device): only rows before it count, the rows after are not read.
     ``scratch``: pet_linear_grads_workspace(dtype, M, N, K) bytes, else
     allocated."""

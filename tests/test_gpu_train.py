@@ -867,3 +867,35 @@ def test_norms_in_place(device, dtype, ln):
                 L.norm_rows_grads(adj, None, None, *args, w, ln, beta)
                 L.norm_rows_grads(args[at], None, None, *args, w, ln, beta)
                 assert torch.equal(adj, args[at]), (width, beta, at)
+
+
+def fp32_rows_bound(g, x):
+    """What include/pet_model.h states of fp32 rows: a factor is held to 2^-23 of itself or
+    2^-36 of its column's largest, a product to a further 2^-22; then the sum's roundings
+    (linear_bound)."""
+    g, x = g.double().cpu().abs(), x.double().cpu().abs()
+    off_g = torch.maximum(2.0 ** -23 * g, 2.0 ** -36 * g.amax(0, keepdim=True))
+    off_x = torch.maximum(2.0 ** -23 * x, 2.0 ** -36 * x.amax(0, keepdim=True))
+    products = off_g.t() @ (x + off_x) + g.t() @ off_x + 2.0 ** -22 * (g.t() @ x)
+    return products + (len(g) / 32 + 308) * U * (g.t() @ x + products)
+
+
+@pytest.mark.parametrize("times", [1e4, 1e6, 1e8, 1e12])
+def test_linear_grads_outliers(device, times):
+    """One value `times` the rest of its column, where the other factor is zero: the
+    column's other products are held to 2^-36 of it, and no other column is touched."""
+    gen = torch.Generator().manual_seed(61)
+    for M, N, K in ((1024, 80, 70), (40000, 300, 400)):
+        g, x = torch.randn((M, N), generator=gen), torch.randn((M, K), generator=gen)
+        g[M // 3, 7], x[M // 3] = times, 0.0
+        x[M // 2, 11], g[M // 2] = -times, 0.0
+        wa, ba = torch.empty((N, K), device=device), torch.empty(N, device=device)
+        D.linear_grads(g.to(device), x.to(device), wa, ba)
+        ref, size = g.double().t() @ x.double(), g.double().abs().t() @ x.double().abs()
+        within(wa, ref, fp32_rows_bound(g, x), "w_adj")
+        rest = torch.ones((N, K), dtype=torch.bool)
+        rest[7], rest[:, 11] = False, False
+        off = (wa.double().cpu() - ref).abs() / size
+        print(f"{M} x {N} x {K}, {times:g}: {float(off[rest].max()):.1e} of the sum's magnitude, with outliers {float(off[~rest].max()):.1e}")
+        assert float(off[rest].max()) <= (M / 32 + 308 + 8) * U
+        within(ba, g.double().sum(0), (M / 32 + 340) * U * g.double().abs().sum(0), "b_adj")
