@@ -869,15 +869,15 @@ def test_norms_in_place(device, dtype, ln):
                 assert torch.equal(adj, args[at]), (width, beta, at)
 
 
-def fp32_rows_bound(g, x):
+def fp32_rows_bound(g, x, roundings=None):
     """What include/pet_model.h states of fp32 rows: a factor is held to 2^-23 of itself or
     2^-36 of its column's largest, a product to a further 2^-22; then the sum's roundings
-    (linear_bound)."""
+    (linear_bound's where none are given)."""
     g, x = g.double().cpu().abs(), x.double().cpu().abs()
     off_g = torch.maximum(2.0 ** -23 * g, 2.0 ** -36 * g.amax(0, keepdim=True))
     off_x = torch.maximum(2.0 ** -23 * x, 2.0 ** -36 * x.amax(0, keepdim=True))
     products = off_g.t() @ (x + off_x) + g.t() @ off_x + 2.0 ** -22 * (g.t() @ x)
-    return products + (len(g) / 32 + 308) * U * (g.t() @ x + products)
+    return products + (roundings or len(g) / 32 + 308) * U * (g.t() @ x + products)
 
 
 @pytest.mark.parametrize("times", [1e4, 1e6, 1e8, 1e12])
@@ -899,3 +899,101 @@ def test_linear_grads_outliers(device, times):
         print(f"{M} x {N} x {K}, {times:g}: {float(off[rest].max()):.1e} of the sum's magnitude, with outliers {float(off[~rest].max()):.1e}")
         assert float(off[rest].max()) <= (M / 32 + 308 + 8) * U
         within(ba, g.double().sum(0), (M / 32 + 340) * U * g.double().abs().sum(0), "b_adj")
+
+
+# ---- every tile of the weight gradients: 256, 128 and 64 columns wide, many pieces and one ----
+
+
+def tile_of(dtype, M, N, K):
+    """The tile that a size takes, told from its workspace (the pieces' sums and their
+    biases'), or None of one piece, which needs none."""
+    step = 32 if dtype == torch.float32 else 64
+    need = A._lib.load().pet_linear_grads_workspace(A.DTYPES[dtype], M, N, K)
+    if need <= 16:
+        return None
+    found = []
+    for tile, (edge, resident) in enumerate(((256, 256), (128, 512), (64, 1024))):
+        tn, tk, steps = -(-N // edge), -(-K // edge), -(-M // step)
+        pieces = max(1, min(resident // (tn * tk), (steps + 3) // 4))
+        pieces = pieces & ~7 if pieces > 8 else pieces
+        pieces = -(-M // (-(-steps // pieces) * step))
+        pieces = (pieces + 7) & ~7 if pieces > 8 else pieces
+        if need == (pieces * tk * N * 8 + 15) // 16 * 16 + pieces * N * K * 4:
+            found.append(tile)
+    assert len(found) == 1, (dtype, M, N, K, need)
+    return found[0]
+
+
+TILES = [(0, 30011, 401, 355), (0, 8001, 257, 2000), (1, 5003, 390, 517), (1, 18001, 330, 200), (2, 26671, 128, 130),
+         (2, 5003, 77, 129), (None, 400, 4097, 4099), (None, 70, 4097, 4099), (None, 5, 2050, 2049)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tile,M,N,K", TILES)
+def test_tiles_of_integers(device, dtype, tile, M, N, K):
+    """Small integers, whose sums fp32 holds: every tile's result is exact, onto beta times
+    what was there, from rows at any address, and of the live rows alone."""
+    assert tile_of(dtype, M, N, K) == tile
+    gen = torch.Generator(device=device).manual_seed(M)
+    ints = lambda *s: torch.randint(-8, 9, s, generator=gen, device=device)
+    for pad, off, beta, live in ((0, 0, 0.0, None), (3, 1, 0.5, None), (8, 0, 1.0, M - M // 3), (1, 2, 0.0, 1), (0, 0, 0.5, 0)):
+        n = M if live is None else live
+        g, x = (torch.full((off + M * (c + pad),), math.nan, dtype=dtype, device=device)[off:].view(M, c + pad)[:, :c]
+                for c in (N, K))
+        g[:n], x[:n] = ints(n, N).to(dtype), ints(n, K).to(dtype)
+        w0, b0 = 2.0 * ints(N, K), 2.0 * ints(N)
+        wa = torch.full((N, K + pad), 77.0, device=device)
+        wa[:, :K] = w0
+        ba = b0.clone()
+        D.linear_grads(g, x, wa[:, :K], ba, beta, live=None if live is None else torch.tensor([live], dtype=torch.int32, device=device))
+        gd = g[:n].double()
+        ref = gd.t().contiguous() @ x[:n].double()
+        assert float(ref.abs().max()) < 2 ** 22 and torch.equal(wa[:, :K].double(), ref + beta * w0)
+        assert torch.equal(ba.double(), gd.sum(0) + beta * b0) and (wa[:, K:] == 77).all()
+
+
+@pytest.mark.parametrize("tile,M,N,K", TILES)
+@pytest.mark.parametrize("way", ["even", "grow", "shrink", "columns"])
+def test_tiles_of_few_rows(device, tile, M, N, K, way):
+    """fp32 rows that are zero but for a few, so that a bound of a few roundings holds:
+    the pairs' low parts count, and scales that change from row to row are handed on
+    to every wave. One factor grows or shrinks by 10^20 along the rows."""
+    gen = torch.Generator(device=device).manual_seed(N)
+    at = torch.unique(torch.tensor([0, 1, 31, 32, 33, 64, 95, 127, M // 3, M // 2, M - 40, M - 2, M - 1], device=device).clamp(0, M - 1))
+    g, x = torch.zeros((M, N), device=device), torch.zeros((M, K), device=device)
+    ramp = torch.linspace(-10, 10, len(at), device=device)[:, None]
+    size_g, size_x = {"even": (0 * ramp, 0 * ramp), "grow": (ramp, 0 * ramp), "shrink": (0 * ramp, -ramp),
+                      "columns": (torch.linspace(-15, 15, N, device=device)[None], torch.linspace(15, -15, K, device=device)[None])}[way]
+    g[at] = torch.randn((len(at), N), generator=gen, device=device) * 10 ** size_g
+    x[at] = torch.randn((len(at), K), generator=gen, device=device) * 10 ** size_x
+    wa, ba = torch.full((N, K), math.nan, device=device), torch.full((N,), math.nan, device=device)
+    D.linear_grads(g, x, wa, ba)
+    gd, xd = g[at].double().cpu(), x[at].double().cpu()
+    ref = gd.t() @ xd
+    # a step's own products 8 roundings (linear_bound), its sum's addition one more, and the joining of the pieces
+    within(wa, ref, fp32_rows_bound(gd, xd, 9 * len(at) + 4), "w_adj")
+    within(ba, gd.sum(0), (len(at) + 4) * U * gd.abs().sum(0), "b_adj")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tile,M,N,K", [t for t in TILES if t[0] in (0, 1)] + [(None, 400, 4097, 4099)])
+def test_tiles_not_finite(device, dtype, tile, M, N, K):
+    """Infinities and NaN in every tile: where the formula takes them and nowhere else."""
+    gen = torch.Generator(device=device).manual_seed(K)
+    g, x = (torch.randint(-8, 9, (M, c), generator=gen, device=device).to(dtype) for c in (N, K))
+    g[g == 0], x[x == 0] = 1.0, 1.0
+    g[7, 3], g[M - 2, 80], x[9, 11], x[M // 2, K - 1] = math.inf, math.nan, -math.inf, math.nan
+    x[7, 100] = 0.0  # inf * 0
+    wa, ba = torch.empty((N, K), device=device), torch.empty(N, device=device)
+    D.linear_grads(g, x, wa, ba)
+    clean = g.double().nan_to_num(0, 0, 0).t().contiguous() @ x.double().nan_to_num(0, 0, 0)
+    ref = clean.clone()
+    ref[3] = torch.copysign(torch.full((K,), math.inf, dtype=torch.float64, device=device), x[7].double())
+    up = torch.copysign(torch.full((N,), math.inf, dtype=torch.float64, device=device), -g[9].double())
+    ref[:, 11] = torch.where(torch.isinf(ref[:, 11]) & (ref[:, 11] != up), math.nan, up)
+    ref[3, 100], ref[80], ref[:, K - 1] = math.nan, math.nan, math.nan
+    got = wa.double()
+    assert torch.equal(torch.isnan(got), torch.isnan(ref))
+    ok = ~torch.isnan(ref)
+    assert torch.equal(got[ok], ref[ok])  # the rest are integers that fp32 holds
+    assert torch.isinf(ba[3]) and torch.isnan(ba[80]) and int(torch.isfinite(ba).sum()) == N - 2
