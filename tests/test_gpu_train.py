@@ -997,3 +997,65 @@ def test_tiles_not_finite(device, dtype, tile, M, N, K):
     ok = ~torch.isnan(ref)
     assert torch.equal(got[ok], ref[ok])  # the rest are integers that fp32 holds
     assert torch.isinf(ba[3]) and torch.isnan(ba[80]) and int(torch.isfinite(ba).sum()) == N - 2
+
+
+# ---- the attention layer's gradients at the sizes of its other products --------------------
+
+
+def large_layer(device, H, hd, atoms, ln, extra, seed=71):
+    rng = np.random.default_rng(seed)
+    Dm = H * hd
+    tk = systems.tokens_from_counts(list(rng.integers(1, 150, atoms)), seed=seed)
+    T = tk.n_rows + extra
+    a = {"tokens": rng.standard_normal((T, Dm)), "nw": 1 + 0.1 * rng.standard_normal(Dm), "nb": 0.1 * rng.standard_normal(Dm),
+         "w_in": rng.standard_normal((3 * Dm, Dm)) / Dm ** 0.5, "b_in": 0.1 * rng.standard_normal(3 * Dm),
+         "w_out": rng.standard_normal((Dm, Dm)) / Dm ** 0.5, "b_out": 0.1 * rng.standard_normal(Dm),
+         "g": rng.standard_normal((T, Dm))}
+    a = {k: torch.from_numpy(v.astype(np.float32)).to(device) for k, v in a.items()}
+    if not ln:
+        a["nb"] = None
+    return a, tk, T
+
+
+@pytest.mark.parametrize("ln", [False, True])
+@pytest.mark.parametrize("H,hd,atoms", [(4, 32, 120), (8, 32, 300), (4, 64, 300), (2, 32, 8)])
+def test_attention_layer_grads_large(device, H, hd, atoms, ln):
+    """Every parameter's gradient where the layer's products take the three-part kernels
+    (2^27 products and more) and the split ones (2^32, where the plain backward keeps
+    no fp32 adjoint of qkv), against float64 and the plain backward. The rows of a
+    capacity hold NaN, in out_adj, the tokens and the saved rows: none is read."""
+    Dm, temp = H * hd, 1.1
+    a, tk, T = large_layer(device, H, hd, atoms, ln, 77)
+    live, S = tk.n_rows, tk.slots
+    for k in ("g", "tokens"):
+        a[k][live:] = math.nan
+    off, cf = torch.from_numpy(tk.off).to(device), torch.from_numpy(tk.cf_seq).to(device)
+    t, ws = A.Tokens(off, tk.n_atoms, True), A.Workspace(device)
+    out = torch.empty((T, Dm), device=device)
+    L.attention_layer(ws, "l", out, a["tokens"], a["nw"], a["nb"], a["w_in"], a["b_in"], cf, a["w_out"], a["b_out"], t, S, H, hd, temp)
+    ws.peek2("l:merged")[live:] = math.nan
+    grads = {n: torch.full_like(a[k], math.nan) for n, k in NAMES.items() if a[k] is not None}
+    got = []
+    for with_grads in (True, False):
+        tadj, csa = torch.full((T, Dm), 0.5, device=device), torch.zeros((tk.n_atoms, S), device=device)
+        args = (tadj, csa, a["g"], a["tokens"], a["nw"], a["nb"], a["w_in"], a["b_in"], cf, a["w_out"], t, S, H, hd, temp)
+        if with_grads:
+            L.attention_layer_grads(ws, "l", grads, *args)
+        else:
+            L.attention_layer_bwd(ws, "l", *args)
+        assert (tadj[live:] == 0.5).all() and torch.isfinite(tadj).all() and torch.isfinite(csa).all(), with_grads
+        got.append((tadj, csa))
+    for x, y in zip(*got):
+        assert float((x - y).abs().max()) <= 1e-5 * float(y.abs().max())
+    leaves = {n: a[k].double().cpu().requires_grad_() for n, k in NAMES.items() if a[k] is not None}
+    tokens = a["tokens"][:live].double().cpu().requires_grad_()
+    ref = attention_f64(tokens, leaves["norm_w"], leaves.get("norm_b"), leaves["w_in"], leaves["b_in"],
+                        leaves["w_out"], leaves["b_out"], tk, torch.from_numpy(tk.cf_seq).double(), H, hd, temp)
+    (ref * a["g"][:live].double().cpu()).sum().backward()
+    for n, g in grads.items():
+        want = leaves[n].grad
+        off_by = float((g.double().cpu() - want).abs().max()) / float(want.abs().max())
+        print(f"{H} x {hd}, {live} rows, {n}: {off_by:.1e}", flush=True)
+        assert off_by <= 1e-5, n
+    sink = tokens.grad + 0.5 * (torch.arange(live) >= tk.n_atoms)[:, None]
+    assert float((got[0][0][:live].double().cpu() - sink).abs().max()) <= 1e-5 * float(sink.abs().max())
