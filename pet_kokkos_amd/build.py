@@ -48,14 +48,16 @@ CPP_TEST3_SRC = os.path.join(ROOT, "tests", "cpp", "model_test.cpp")
 CPP_TEST3 = os.path.join(ROOT, "tests", "cpp", "model_test")
 CPP_TEST4_SRC = os.path.join(ROOT, "tests", "cpp", "train_test.cpp")
 CPP_TEST4 = os.path.join(ROOT, "tests", "cpp", "train_test")
+CPP_TEST5_SRC = os.path.join(ROOT, "tests", "cpp", "train_shapes_test.cpp")
+CPP_TEST5 = os.path.join(ROOT, "tests", "cpp", "train_shapes_test")
 
 
 def build_cpp_test(verbose: bool = False) -> str:
     """The C++ callers of include/pet/attention.hpp, include/pet/forces.hpp,
-    include/pet/model.hpp and include/pet/train.hpp that tests/test_gpu_cpp_api.py
-    and tests/test_gpu_cpp_train.py run."""
+    include/pet/model.hpp and include/pet/train.hpp that tests/test_gpu_cpp_api.py,
+    tests/test_gpu_cpp_train.py and tests/test_train_args.py run."""
     for src, exe in ((CPP_TEST_SRC, CPP_TEST), (CPP_TEST2_SRC, CPP_TEST2), (CPP_TEST3_SRC, CPP_TEST3),
-                     (CPP_TEST4_SRC, CPP_TEST4)):
+                     (CPP_TEST4_SRC, CPP_TEST4), (CPP_TEST5_SRC, CPP_TEST5)):
         cmd = [hipcc(), "--offload-arch=gfx950", "-O2", "-std=c++17", "-I", os.path.join(ROOT, "include"),
                "-o", exe, src, "-L", HERE, "-lpet_attn", "-Wl,-rpath,$ORIGIN/../../pet_kokkos_amd"]
         if verbose:

@@ -4,6 +4,8 @@ from __future__ import annotations
 
 import ctypes
 import math
+import os
+import subprocess
 
 import pytest
 import torch
@@ -261,3 +263,12 @@ def test_a_launch_takes_what_its_arguments_hold():
     need = _lib.load().pet_grad_workspace
     most = (4096 - 56) // 16 // 2
     assert need(most) == need(1) and need(most + 1) == 2 * need(1) and need(10 * most) == 10 * need(1)
+
+
+def test_cpp_calls_refuse_shapes():
+    """The C++ training calls throw for views that do not fit together."""
+    from pet_kokkos_amd import build
+    if not os.path.exists(build.CPP_TEST5):
+        pytest.fail(f"{build.CPP_TEST5} is not built (python -m pet_kokkos_amd.build)")
+    res = subprocess.run([build.CPP_TEST5], capture_output=True, text=True, timeout=60)
+    assert res.returncode == 0 and res.stdout == "", res.stdout + res.stderr
