@@ -66,7 +66,12 @@ class Workspace:
         return self._named[key]
 
 
+MOST = (1 << 31) - 1  # rows or columns: the library counts them in int, and ctypes wraps what passes it
+
+
 def _mat(t: torch.Tensor, name: str, width: int | None = None) -> int:
+    if t.dim() == 2 and max(t.shape) > MOST:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}: at most {MOST} rows and columns")
     if t.device.type != "cuda":
         raise ValueError(f"{name} must be a device tensor")
     if t.dtype != torch.float32:
@@ -101,6 +106,8 @@ def _typed(t: torch.Tensor, name: str, rows: int, width: int, dtype: torch.dtype
     """The leading dimension of a row-major [rows, width] view of the dtype on the device."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name}: a torch tensor is needed")
+    if rows > MOST or width > MOST:
+        raise ValueError(f"{name}: {rows} x {width}, at most {MOST} rows and columns")
     if t.dtype is dtype and t.shape == (rows, width) and t.device == device and rows > 1 and width > 1:
         ld, step = t.stride()  # (what a small call's host side waits for: the checks below again, in one go)
         if step == 1 and ld >= width and device.type == "cuda" and dtype in DTYPES:

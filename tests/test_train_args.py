@@ -272,3 +272,15 @@ def test_cpp_calls_refuse_shapes():
         pytest.fail(f"{build.CPP_TEST5} is not built (python -m pet_kokkos_amd.build)")
     res = subprocess.run([build.CPP_TEST5], capture_output=True, text=True, timeout=60)
     assert res.returncode == 0 and res.stdout == "", res.stdout + res.stderr
+
+
+def test_rows_past_an_int():
+    """2^32 rows and more would come to the library as what is left of them modulo 2^32."""
+    w = torch.ones(1)
+    for dtype in (torch.bfloat16, torch.float32):
+        x = torch.zeros(1, dtype=dtype).expand((1 << 32) + 5, 1)
+        for call in (lambda: layer.norm_rows(x, x, w, None), lambda: layer.norm_rows_bwd(x, x, x, w, False),
+                     lambda: layer.norm_rows_grads(x, w, None, x, x, w, False), lambda: linear.linear_grads(x, x, w[:, None]),
+                     lambda: linear.linear_grads(x.t(), x.t(), w[:, None])):
+            with pytest.raises(ValueError, match=str((1 << 31) - 1)):
+                call()
