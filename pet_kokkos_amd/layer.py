@@ -188,8 +188,9 @@ def attention_layer_grads(ws: Workspace, key: str, grads: dict, tokens_adj: torc
         if t is not None and (t.device != dev or t.dtype != torch.float32 or tuple(t.shape) != size
                               or not t.is_contiguous()):
             raise ValueError(f"{name} must be a contiguous float32 {list(size)} on {dev}")
-    if tk.off.device != dev or tk.off.dtype != torch.int32 or tk.off.numel() != tk.N + 1:
-        raise ValueError(f"tk.off must be {tk.N + 1} int32 on {dev}")
+    if tk.off.device != dev or tk.off.dtype != torch.int32 or tk.off.numel() != tk.N + 1 \
+            or not tk.off.is_contiguous():
+        raise ValueError(f"tk.off must be {tk.N + 1} contiguous int32 on {dev}")
     unknown = sorted(set(grads) - set(_LAYER_GRADS))
     if unknown:
         raise ValueError(f"grads: no parameter named {', '.join(unknown)}")

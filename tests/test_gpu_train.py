@@ -1059,3 +1059,35 @@ def test_attention_layer_grads_large(device, H, hd, atoms, ln):
         assert off_by <= 1e-5, n
     sink = tokens.grad + 0.5 * (torch.arange(live) >= tk.n_atoms)[:, None]
     assert float((got[0][0][:live].double().cpu() - sink).abs().max()) <= 1e-5 * float(sink.abs().max())
+
+
+def test_attention_layer_grads_views(device):
+    """Rows in wider buffers: the results of contiguous ones, to the products' other
+    kernels, and nothing beside the rows is touched. Offsets that are not consecutive
+    are refused."""
+    a, tk, T, H, hd = layer_case(device, True, False)
+    Dm, S = H * hd, tk.slots
+    off, cf = torch.from_numpy(tk.off).to(device), torch.from_numpy(tk.cf_seq).to(device)
+    t, ws = A.Tokens(off, tk.n_atoms, False), A.Workspace(device)
+    out = torch.empty((T, Dm), device=device)
+    L.attention_layer(ws, "l", out, a["tokens"], a["nw"], a["nb"], a["w_in"], a["b_in"], cf, a["w_out"], a["b_out"], t, S, H, hd, 1.0)
+    results = []
+    for pad in (0, 4, 3):
+        def wide(x):
+            buf = torch.full((x.shape[0], x.shape[1] + pad), 9.0, device=device)
+            buf[:, :x.shape[1]] = x
+            return buf[:, :x.shape[1]], buf[:, x.shape[1]:]
+        (tadj, e0), (csa, e1) = wide(torch.full((T, Dm), 0.5, device=device)), wide(torch.zeros((tk.n_atoms, S), device=device))
+        (g, _), (tokens, _), (c, _) = wide(a["g"]), wide(a["tokens"]), wide(cf)
+        grads = {n: torch.full_like(a[k], math.nan) for n, k in NAMES.items()}
+        args = (grads, tadj, csa, g, tokens, a["nw"], a["nb"], a["w_in"], a["b_in"], c, a["w_out"])
+        L.attention_layer_grads(ws, "l", *args, t, S, H, hd, 1.0)
+        assert (e0 == 9).all() and (e1 == 9).all()
+        results.append([tadj, csa, *grads.values()])
+    for got in results[1:]:
+        for x, y in zip(got, results[0]):
+            assert float((x - y).abs().max()) <= 1e-6 * float(y.abs().max())
+    apart = torch.zeros(2 * (tk.n_atoms + 1), dtype=torch.int32, device=device)[::2]
+    apart.copy_(off)
+    with pytest.raises(ValueError):
+        L.attention_layer_grads(ws, "l", *args, A.Tokens(apart, tk.n_atoms, False), S, H, hd, 1.0)
