@@ -396,7 +396,8 @@ int pet_rows_norm_bwd_sink(int rows, int width, float* in_adj, int64_t lda, cons
                            const float* in, int64_t ldi, const float* weight, int ln, int n_node, float beta_node,
                            float beta_edge, const int* live_off, hipStream_t st) {
   if (rows < 0 || width < 1) return PET_ATTN_EINVAL;
-  if (!in_adj || !out_adj || !in || !weight || lda < width || ldg < width || ldi < width) return PET_ATTN_EINVAL;
+  if ((rows > 0 && (!in_adj || !out_adj || !in)) || !weight || lda < width || ldg < width || ldi < width)
+    return PET_ATTN_EINVAL;
   if (rows == 0) return PET_ATTN_OK;
   if (rows > kLaunchRows && !live_off)
     return launches(rows, [&](int64_t r, int n) {
@@ -467,7 +468,8 @@ int pet_attn_cf_seq(const pet_attn_shape* sh, const int* off, const float* cut, 
 
 int pet_norm_rows(int rows, int width, float* out, int64_t ldo, const float* in, int64_t ldi, const float* weight,
                   const float* bias, void* stream) {
-  if (rows < 0 || width < 1 || !out || !in || !weight || ldo < width || ldi < width) return PET_ATTN_EINVAL;
+  if (rows < 0 || width < 1 || (rows > 0 && (!out || !in)) || !weight || ldo < width || ldi < width)
+    return PET_ATTN_EINVAL;
   if (rows == 0) return PET_ATTN_OK;
   if (rows > kLaunchRows)
     return launches(rows, [&](int64_t r, int n) {

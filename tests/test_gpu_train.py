@@ -1091,3 +1091,10 @@ def test_attention_layer_grads_views(device):
     apart.copy_(off)
     with pytest.raises(ValueError):
         L.attention_layer_grads(ws, "l", *args, A.Tokens(apart, tk.n_atoms, False), S, H, hd, 1.0)
+
+
+def test_no_fp32_rows(device):
+    x, w = torch.zeros((0, 40), device=device), torch.ones(40, device=device)
+    L.norm_rows(x, x, w, None)
+    L.norm_rows(x, x, w, w)
+    L.norm_rows_bwd(x, x, x, w, True)

@@ -284,3 +284,12 @@ def test_rows_past_an_int():
                      lambda: linear.linear_grads(x.t(), x.t(), w[:, None])):
             with pytest.raises(ValueError, match=str((1 << 31) - 1)):
                 call()
+
+
+def test_no_fp32_rows():
+    """No rows have no addresses: the fp32 norms take them as the typed ones do."""
+    lib = _lib.load()
+    assert lib.pet_norm_rows(0, 8, None, 8, None, 8, W, None, None) == _lib.OK == norm(rows=0, out=None, inp=None)
+    assert lib.pet_norm_rows_bwd(0, 8, None, 8, 0.0, None, 8, None, 8, W, 0, None) == _lib.OK
+    assert lib.pet_norm_rows(0, 8, None, 8, None, 8, None, None, None) == lib.pet_norm_rows(1, 8, None, 8, A, 8, W, None, None) == _lib.EINVAL
+    assert lib.pet_norm_rows_bwd(1, 8, A, 8, 0.0, None, 8, B, 8, W, 0, None) == _lib.EINVAL
