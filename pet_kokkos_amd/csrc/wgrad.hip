@@ -33,7 +33,10 @@
 // product of that shape 2.03 ms, of 8192 cubed 1131 TFLOP/s) the products alone take
 // 0.73 ms, the rows' way into LDS alone 0.71, the loads alone 0.60; together the clock
 // falls from 2.2 to 1.8 GHz, and the matrix unit is busy 42% of the cycles. 122688 x
-// 768 x 256 in fp32 takes 187 to 200 us, of which writing and adding the pieces is 25.
+// 768 x 256 in fp32 takes 187 to 200 us, of which writing and adding the pieces is 25:
+// the matrix unit is busy 41% of the cycles, the vector unit 58% (the splits), the
+// waves wait 33%. Small results are bound by the pieces: 27318 x 128 x 128 takes 21.5
+// to 24 us (5.8 at the copy's rate), and their sums move 82% of the operands' bytes.
 //
 // The matrix instruction rounds toward minus infinity, an error with a mean that
 // half a million rows would add up. So a step is summed from zero, the sums of

@@ -172,8 +172,10 @@ def attention_layer_grads(ws: Workspace, key: str, grads: dict, tokens_adj: torc
     ``grads`` holds the tensors they go to by name (norm_w, norm_b, w_in, b_in,
     w_out, b_out, each of its parameter's shape; those not there are not made, a
     bias's not without its weight's), each onto beta times itself. Dead rows
-    count for none. ``ws`` serves one stream at a time; a call that is captured
-    into a graph finds its scratch there from an eager call before it."""
+    count for none, whatever they hold. ``ws`` serves one stream at a time; a call
+    that is captured into a graph finds its scratch there from an eager call before
+    it, and a call of a larger shape replaces that scratch: a graph has a ``ws`` of its
+    own."""
     lib = _lib.load()
     D, dev = heads * head_dim, tokens.device
     T = tokens.shape[0]
