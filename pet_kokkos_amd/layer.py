@@ -45,6 +45,12 @@ def _width(D: int) -> None:
         raise ValueError(f"rows of {D} columns: the norms take 1 to {MAX_WIDTH}")
 
 
+def _reach(t: torch.Tensor | None, name: str, n: int, what: str) -> None:
+    """Rows and vectors beside inp are as long as it needs them."""
+    if t is not None and (t.shape[0] if what == "rows" else t.numel()) < n:
+        raise ValueError(f"{name} has {tuple(t.shape)} {what}, expected {n}")
+
+
 def norm_rows(out: torch.Tensor, inp: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None) -> None:
     """out = norm(inp) row by row (out may be inp): RMSNorm, or LayerNorm with a
     bias. Rows in float32, bfloat16 or float16, up to 16384 columns; the
@@ -59,6 +65,9 @@ def norm_rows(out: torch.Tensor, inp: torch.Tensor, weight: torch.Tensor, bias: 
                  inp.data_ptr(), ldi, _vector(weight, "weight", D, dev),
                  None if bias is None else _vector(bias, "bias", D, dev))
         return
+    _reach(out, "out", rows, "rows")
+    _reach(weight, "weight", D, "elements")
+    _reach(bias, "bias", D, "elements")
     _lib.check(lib.pet_norm_rows(rows, D, out.data_ptr(), _mat(out, "out", D), inp.data_ptr(), _mat(inp, "in", D),
                                  _weight(weight, "weight"), None if bias is None else _weight(bias, "bias"),
                                  _stream()), "pet_norm_rows")
@@ -73,6 +82,9 @@ def norm_rows_bwd(in_adj: torch.Tensor, out_adj: torch.Tensor, inp: torch.Tensor
     if inp.dtype != torch.float32 or D > 2048:
         norm_rows_grads(in_adj, None, None, out_adj, inp, weight, ln, beta)
         return
+    _reach(in_adj, "in_adj", rows, "rows")
+    _reach(out_adj, "out_adj", rows, "rows")
+    _reach(weight, "weight", D, "elements")
     _lib.check(lib.pet_norm_rows_bwd(rows, D, in_adj.data_ptr(), _mat(in_adj, "in_adj", D), float(beta),
                                      out_adj.data_ptr(), _mat(out_adj, "out_adj", D), inp.data_ptr(),
                                      _mat(inp, "in", D), _weight(weight, "weight"), int(bool(ln)), _stream()),

@@ -1098,3 +1098,21 @@ def test_no_fp32_rows(device):
     L.norm_rows(x, x, w, None)
     L.norm_rows(x, x, w, w)
     L.norm_rows_bwd(x, x, x, w, True)
+
+
+@pytest.mark.parametrize("ln", [False, True])
+def test_attention_layer_grads_whatever_is_dead(device, ln):
+    """What a capacity's rows of out_adj hold changes no bit of any result."""
+    results = []
+    for dead in ("nan", True):
+        a, tk, T, H, hd = layer_case(device, ln, dead)
+        Dm, S = H * hd, tk.slots
+        off, cf = torch.from_numpy(tk.off).to(device), torch.from_numpy(tk.cf_seq).to(device)
+        t, ws = A.Tokens(off, tk.n_atoms, True), A.Workspace(device)
+        out, tadj, csa = torch.empty((T, Dm), device=device), torch.zeros((T, Dm), device=device), torch.zeros((tk.n_atoms, S), device=device)
+        args = (a["tokens"], a["nw"], a["nb"], a["w_in"], a["b_in"], cf, a["w_out"])
+        L.attention_layer(ws, "l", out, *args, a["b_out"], t, S, H, hd, 1.0)
+        grads = {n: torch.full_like(a[k], math.nan) for n, k in NAMES.items() if a[k] is not None}
+        L.attention_layer_grads(ws, "l", grads, tadj, csa, a["g"], *args, t, S, H, hd, 1.0)
+        results.append([tadj, csa, *grads.values()])
+    assert all(torch.equal(x, y) and torch.isfinite(x).all() for x, y in zip(*results))

@@ -293,3 +293,13 @@ def test_no_fp32_rows():
     assert lib.pet_norm_rows_bwd(0, 8, None, 8, 0.0, None, 8, None, 8, W, 0, None) == _lib.OK
     assert lib.pet_norm_rows(0, 8, None, 8, None, 8, None, None, None) == lib.pet_norm_rows(1, 8, None, 8, A, 8, W, None, None) == _lib.EINVAL
     assert lib.pet_norm_rows_bwd(1, 8, A, 8, 0.0, None, 8, B, 8, W, 0, None) == _lib.EINVAL
+
+
+def test_fp32_norms_reach_no_further():
+    """Fewer rows or a shorter vector than the input's would be read or written past their end."""
+    x, w = torch.zeros(4, 8), torch.zeros(8)
+    for call in (lambda: layer.norm_rows(x[:3], x, w, None), lambda: layer.norm_rows(x, x, w[:7], None),
+                 lambda: layer.norm_rows(x, x, w, w[:7]), lambda: layer.norm_rows_bwd(x[:3], x, x, w, True),
+                 lambda: layer.norm_rows_bwd(x, x[:3], x, w, True), lambda: layer.norm_rows_bwd(x, x, x, w[:7], False)):
+        with pytest.raises(ValueError, match="(rows|elements), expected"):
+            call()
