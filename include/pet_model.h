@@ -280,7 +280,9 @@ PET_ATTN_API int pet_grad_norm(const pet_grad_tensor* grads, int n, int p, doubl
  * the factor made on the device in double and rounded to fp32, the product
  * rounded once to g's type: scale undoes a loss's scale or averages over
  * micro-batches. An infinite norm scales by 0 (0 for a finite g, NaN for an
- * infinite one), a NaN by NaN; max_norm infinity does not clip. No two tensors
+ * infinite one), a NaN by NaN; a finite one past fp32 reads infinite in *norm and
+ * scales by what it is, a factor below 2^-126 to fewer digits; max_norm infinity does
+ * not clip. No two tensors
  * may overlap. max_norm and eps at least 0, scale finite. */
 PET_ATTN_API int pet_grad_clip(const pet_grad_tensor* grads, int n, int p, double scale, double max_norm, double eps,
                                float* norm, void* workspace, size_t workspace_bytes, void* stream);

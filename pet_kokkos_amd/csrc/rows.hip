@@ -376,8 +376,9 @@ inline bool aligned16(const void* p, int64_t ld) {
   return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 4 == 0;
 }
 // HIP takes a launch's threads modulo 2^32 and reports nothing, so more rows than
-// these (at 64 lanes each 2^31 threads) go in launches of them, or are refused.
-constexpr int64_t kLaunchRows = int64_t(1) << 25;
+// kLaunchRows (at 64 lanes each 2^31 threads) go in launches of them; where that is
+// not done, more than kMostBlocks workgroups of 256 are refused.
+constexpr int64_t kLaunchRows = int64_t(1) << 25, kMostBlocks = (int64_t(1) << 24) - 1;
 template <class F>
 int launches(int rows, F&& f) {
   for (int64_t r = 0; r < rows; r += kLaunchRows)
@@ -408,7 +409,7 @@ int pet_rows_norm_bwd_sink(int rows, int width, float* in_adj, int64_t lda, cons
   if (aligned16(in_adj, lda) && aligned16(out_adj, ldg) && aligned16(in, ldi) && aligned16(weight, 4)) {
     const int e = with_vec(width, [&](auto lc, auto cc) {
       constexpr int LPR = decltype(lc)::value, C4 = decltype(cc)::value, RPB = 4 * (64 / LPR);
-      if (rows > kLaunchRows / LPR * 64) return int(PET_ATTN_EINDEX);
+      if (rows > kMostBlocks * RPB) return int(PET_ATTN_EINDEX);
       hipLaunchKernelGGL((norm_bwd4_kernel<LPR, C4>), dim3(unsigned((rows + RPB - 1) / RPB)), dim3(256), 0, st, rows,
                          width, in_adj, lda, out_adj, ldg, in, ldi, weight, ln, n_node, beta_node, beta_edge,
                          live_off);
@@ -418,7 +419,7 @@ int pet_rows_norm_bwd_sink(int rows, int width, float* in_adj, int64_t lda, cons
   }
   return with_lanes(width, [&](auto vc) {
     constexpr int V = decltype(vc)::value;
-    if (rows > kLaunchRows) return int(PET_ATTN_EINDEX);
+    if (rows > kMostBlocks * 4) return int(PET_ATTN_EINDEX);
     hipLaunchKernelGGL(norm_bwd_kernel<V>, dim3(unsigned((rows + 3) / 4)), dim3(256), 0, st, rows, width, in_adj, lda,
                        out_adj, ldg, in, ldi, weight, ln, n_node, beta_node, beta_edge, live_off);
     return hipGetLastError() == hipSuccess ? int(PET_ATTN_OK) : int(PET_ATTN_ELAUNCH);
