@@ -1116,3 +1116,61 @@ def test_attention_layer_grads_whatever_is_dead(device, ln):
         L.attention_layer_grads(ws, "l", grads, tadj, csa, a["g"], *args, t, S, H, hd, 1.0)
         results.append([tadj, csa, *grads.values()])
     assert all(torch.equal(x, y) and torch.isfinite(x).all() for x, y in zip(*results))
+
+
+def attention_of_normed(normed, w_in, b_in, w_out, b_out, tk, cf, H, hd):
+    """attention_f64 (temperature 1) from the normed tokens on."""
+    q, k, v = ((normed @ w_in.t() + b_in)[:, i * H * hd:(i + 1) * H * hd] for i in range(3))
+    merged = torch.zeros_like(normed)
+    for n in range(tk.n_atoms):
+        rows = [n] + list(range(tk.n_atoms + int(tk.off[n]), tk.n_atoms + int(tk.off[n + 1])))
+        c = cf[n, :len(rows)]
+        on = [r for r, x in zip(rows, c) if x > 0]
+        cols = [slice(h * hd, (h + 1) * hd) for h in range(H)]
+        o = [torch.softmax(q[on, s] @ k[on, s].t() / math.sqrt(hd) + torch.log(c[c > 0]), -1) @ v[on, s] for s in cols]
+        merged[on] = torch.cat(o, 1)
+    return merged @ w_out.t() + b_out
+
+
+@pytest.mark.parametrize("ln", [False, True])
+@pytest.mark.parametrize("H,hd,counts,kind", [(3, 5, [4, 0, 9], "random"), (1, 24, [1, 30], "zeros"), (2, 40, [0], "ones"),
+                                              (4, 16, [300, 5, 0, 700], "zeros"), (1, 128, [17, 3], "zeros"), (2, 1, [6, 2], "random")])
+def test_attention_layer_grads_of_any_shape(device, H, hd, counts, kind, ln):
+    """Head widths of no vector's multiple, atoms without edges, edges at their cutoff
+    (whose rows are masked), more slots than the LDS-staged kernels hold."""
+    Dm = H * hd
+    rng = np.random.default_rng(91)
+    tk = systems.tokens_from_counts(counts, seed=5, cf_kind=kind)
+    T, S, N = tk.n_rows, tk.slots, tk.n_atoms
+    r = lambda *s: torch.from_numpy(rng.standard_normal(s).astype(np.float32)).to(device)
+    tokens, g, nw, nb = r(T, Dm), r(T, Dm), 1 + 0.1 * r(Dm), 0.1 * r(Dm) if ln else None
+    w_in, b_in, w_out, b_out = r(3 * Dm, Dm) / Dm ** 0.5, 0.1 * r(3 * Dm), r(Dm, Dm) / Dm ** 0.5, r(Dm)
+    off, cf = torch.from_numpy(tk.off).to(device), torch.from_numpy(tk.cf_seq).to(device)
+    t, ws = A.Tokens(off, N), A.Workspace(device)
+    out, tadj, csa = torch.empty((T, Dm), device=device), torch.zeros((T, Dm), device=device), torch.zeros((N, S), device=device)
+    L.attention_layer(ws, "l", out, tokens, nw, nb, w_in, b_in, cf, w_out, b_out, t, S, H, hd, 1.0)
+    given = {"norm_w": nw, "norm_b": nb, "w_in": w_in, "b_in": b_in, "w_out": w_out, "b_out": b_out}
+    grads = {n: torch.full_like(v, math.nan) for n, v in given.items() if v is not None}
+    L.attention_layer_grads(ws, "l", grads, tadj, csa, g, tokens, nw, nb, w_in, b_in, cf, w_out, t, S, H, hd, 1.0)
+    leaves = {n: v.double().cpu().requires_grad_() for n, v in given.items() if v is not None}
+    x, gd, w = tokens.double().cpu().requires_grad_(), g.double().cpu(), leaves["norm_w"]
+    c = x - x.mean(1, keepdim=True) if ln else x
+    inv = 1 / torch.sqrt((c ** 2).mean(1, keepdim=True) + (1e-5 if ln else 2.0 ** -23))
+    normed = c * inv * w + leaves["norm_b"] if ln else c * inv * w
+    normed.retain_grad()
+    ref = attention_of_normed(normed, leaves["w_in"], leaves["b_in"], leaves["w_out"], leaves["b_out"], tk,
+                              torch.from_numpy(tk.cf_seq).double(), H, hd)
+    (ref * gd).sum().backward()
+    for name, got, want in [("out", out, ref.detach())] + [(n, v, leaves[n].grad) for n, v in grads.items()]:
+        # the attention's bar, of a tensor's largest value; where that is a cancellation of larger terms, of those
+        scale = max(float(want.abs().max()), 1e-2)
+        assert float((got.double().cpu() - want).abs().max()) <= 1e-5 * scale, name
+    # The normed tokens' adjoint h is within that bar, and the norm's adjoint is linear in it:
+    # inv (h w - [mean(h w)] - xhat mean(h w xhat)) is within 1e-5 of the largest sum of its
+    # terms' magnitudes. (Of two columns LayerNorm's terms cancel to 1e-5 of themselves: xhat is
+    # +-1 to eps, and what is left of terms of 15 is 0.2.)
+    with torch.no_grad():
+        hw, xhat = (normed.grad * w).abs(), (c * inv).abs()
+        terms = inv * (hw + (hw.mean(1, keepdim=True) if ln else 0.0) + xhat * (hw * xhat).mean(1, keepdim=True))
+        print(f"{H} x {hd}, ln {ln}: terms to {float(terms.max()):.2g}, adjoint to {float(x.grad.abs().max()):.2g}")
+        assert float((tadj.double().cpu() - x.grad).abs().max()) <= 1e-5 * float(terms.max())
