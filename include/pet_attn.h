@@ -379,6 +379,79 @@ PET_ATTN_API int pet_norm_rows_grads(int dtype, int rows, int width, void* in_ad
                                      const float* weight, int ln, float* weight_adj, float* bias_adj, float beta_w,
                                      const int* live, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- attention of 16-bit rows for training: dropout, shared heads, a learned bias -- */
+
+/* A dropout: elements are left out with probability p (counted in steps of 2^-16, at
+ * most 65534 / 65536) and the rest scaled by 1 / (1 - p) (p as counted). Nothing of the
+ * mask is stored: an element stays where its 16-bit number of a counter generator is at
+ * least 65536 p. state (device): a seed and a step, read when the kernels run, so a
+ * program that raises the step on the device draws anew in each replay of a graph; the
+ * step counts by its low 32 bits. call: tells the calls of one step apart. The same
+ * (seed, step, call) and place give the same decision in a forward and its backward.
+ * The numbers: Threefry-2x32 of 13 rounds keyed with the block of (step, call) under the
+ * seed; block (row, column / 4) of pet_dropout_rows, (the query's row, key slot / 4 *
+ * heads + head) of the attention; the first word's low and high half, then the second's. */
+typedef struct pet_dropout {
+  const int64_t* state; /* device: seed, step */
+  double p;
+  uint32_t call;
+} pet_dropout;
+
+/* out = residual + M in row by row, M the dropout's mask with its scale (residual may be
+ * NULL: out = M in, which is also the backward, of the adjoint): rows of any width in
+ * fp32, bf16 or fp16, any alignment of an element, one rounding at the end. A left-out
+ * element is 0 whatever in holds. out may be in or residual (with its leading
+ * dimension), and nothing else may overlap. live (device, may be NULL): only rows <
+ * *live count, the rows after are neither read nor written. No counterpart in the
+ * reference, which does not train. */
+PET_ATTN_API int pet_dropout_rows(int dtype, int rows, int width, void* out, int64_t ldo, const void* in, int64_t ldi,
+                                  const void* residual, int64_t ldr, const pet_dropout* dropout, const int* live,
+                                  void* stream);
+
+#define PET_BIAS_MAX_BUCKETS 64
+#define PET_BIAS_MAX_REACH 1024
+
+/* A learned bias of the logits by the tokens' relative positions: query i and key j of
+ * head h add table[buckets[clamp(positions[row j] - positions[row i], -reach, reach) +
+ * reach]][h] (device: table fp32 [n_buckets, heads], buckets int32 [2 reach + 1], values
+ * outside 0 .. n_buckets - 1 taken to the nearer end, positions int32 [n_rows]). */
+typedef struct pet_attn_bias {
+  const float* table;
+  const int* buckets;
+  const int* positions;
+  int n_buckets, reach;
+} pet_attn_bias;
+
+/* pet_attn_fwd of rows in bf16 or fp16 (dtype; qkv's and merged's): qkv [T, (heads + 2
+ * kv_heads) head_dim] = [Q | K | V], heads / kv_heads query heads to a key and value
+ * head, the logits with a bias and the probabilities with a dropout (each may be NULL),
+ * sums and statistics in fp32, the probabilities rounded to the type for their product
+ * with V. ml (may be NULL) as pet_attn_fwd's, but (0, 0) where no token or no key is, and
+ * 8-byte aligned. A key counts where cf > 0 (a NaN does not); what masked rows hold
+ * reaches no result. Any alignment of an element otherwise; head_dim 1..128, any number
+ * of slots. Nothing may overlap. No counterpart in the reference. */
+PET_ATTN_API int pet_attn_fwd_typed(int dtype, const pet_attn_shape* shape, int kv_heads, const void* qkv, int64_t ldq,
+                                    const int* off, const float* cf_seq, int64_t ldc, const pet_attn_bias* bias,
+                                    const pet_dropout* dropout, void* merged, int64_t ldm, float* ml, void* stream);
+
+/* Bytes of device workspace pet_attn_bwd_typed needs (n_buckets 0 without a bias; 0 for
+ * what it refuses). */
+PET_ATTN_API size_t pet_attn_bwd_typed_workspace(int dtype, const pet_attn_shape* shape, int kv_heads, int n_buckets);
+
+/* Its backward from dmerged (the adjoint of merged), merged and ml as the forward left
+ * them, the probabilities and the mask made again: qkv_adj [T, (heads + 2 kv_heads)
+ * head_dim] (dead rows zeroed when shape->dead), and onto beta times itself cf_seq_adj
+ * [N, S] (may be NULL; the whole of it is written) and table_adj [n_buckets, heads]
+ * (contiguous; may be NULL). dO.O is formed from merged as it was rounded. workspace
+ * 16-byte aligned, its contents nobody's after the call: calls that may run at once have
+ * one each. */
+PET_ATTN_API int pet_attn_bwd_typed(int dtype, const pet_attn_shape* shape, int kv_heads, const void* qkv, int64_t ldq,
+                                    const int* off, const void* dmerged, int64_t ldg, const void* merged, int64_t ldm,
+                                    const float* ml, const float* cf_seq, int64_t ldc, const pet_attn_bias* bias,
+                                    const pet_dropout* dropout, void* qkv_adj, int64_t lda, float* cf_seq_adj,
+                                    int64_t ldca, float* table_adj, float beta, void* workspace, size_t workspace_bytes,
+                                    void* stream);
+
 /* Bytes of device workspace pet_attention_layer / _layer_bwd need: the
  * normed tokens [T, D] and qkv [T, 3D], with pet_attention_bwd_workspace's,
  * each 256-byte aligned. */

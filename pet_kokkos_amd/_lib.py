@@ -73,6 +73,10 @@ EXPORTS = (
     "pet_grad_clip",
     "pet_attention_layer_grads_workspace",
     "pet_attention_layer_grads",
+    "pet_dropout_rows",
+    "pet_attn_fwd_typed",
+    "pet_attn_bwd_typed_workspace",
+    "pet_attn_bwd_typed",
 )
 
 OK, EINVAL, EHEADDIM, ESLOTS, EALIGN, ELAUNCH, EBLAS, EWORKSPACE, EINDEX, ESCRATCH = range(10)
@@ -136,6 +140,17 @@ class LayerGrads(ctypes.Structure):
     """pet_layer_grads (include/pet_attn.h)."""
     _fields_ = [(n, ctypes.c_void_p) for n in ("norm_w", "norm_b", "w_in", "b_in", "w_out", "b_out")] + \
                [("beta", ctypes.c_float)]
+
+
+class DropoutArgs(ctypes.Structure):
+    """pet_dropout (include/pet_attn.h)."""
+    _fields_ = [("state", ctypes.c_void_p), ("p", ctypes.c_double), ("call", ctypes.c_uint32)]
+
+
+class BiasArgs(ctypes.Structure):
+    """pet_attn_bias (include/pet_attn.h)."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("table", "buckets", "positions")] + \
+               [("n_buckets", ctypes.c_int), ("reach", ctypes.c_int)]
 
 
 class PetAttnError(RuntimeError):
@@ -300,6 +315,16 @@ def load() -> ctypes.CDLL:
     lib.pet_attention_layer_grads.restype = ctypes.c_int
     lib.pet_attention_layer_grads.argtypes = [sp, ctypes.POINTER(LayerGrads), _P, _I64, _P, _I64, _P, _I64, _P, _I64,
                                               _P, _P, _P, _P, _P, _I64, _P, _P, _P, _P, _P, _Z, _P]
+    dp, bp = ctypes.POINTER(DropoutArgs), ctypes.POINTER(BiasArgs)
+    lib.pet_dropout_rows.restype = ctypes.c_int
+    lib.pet_dropout_rows.argtypes = [_I, _I, _I, _P, _I64, _P, _I64, _P, _I64, dp, _P, _P]
+    lib.pet_attn_fwd_typed.restype = ctypes.c_int
+    lib.pet_attn_fwd_typed.argtypes = [_I, sp, _I, _P, _I64, _P, _P, _I64, bp, dp, _P, _I64, _P, _P]
+    lib.pet_attn_bwd_typed_workspace.restype = _Z
+    lib.pet_attn_bwd_typed_workspace.argtypes = [_I, sp, _I, _I]
+    lib.pet_attn_bwd_typed.restype = ctypes.c_int
+    lib.pet_attn_bwd_typed.argtypes = [_I, sp, _I, _P, _I64, _P, _P, _I64, _P, _I64, _P, _P, _I64, bp, dp, _P, _I64,
+                                       _P, _I64, _P, _F, _P, _Z, _P]
     _lib = lib
     return lib
 

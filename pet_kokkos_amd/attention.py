@@ -13,7 +13,13 @@ chunked forms (src/ops.hpp:133-146): runs of atoms of about ``chunk`` tokens,
 qkv made per run by a ``make_qkv(qkv_rows, r0, r1)`` callable.
 
 ``attn_fwd`` / ``attn_bwd`` expose the core kernels alone (no linears),
-``attn_fwd_run`` / ``attn_bwd_run`` their per-run forms. All
+``attn_fwd_run`` / ``attn_bwd_run`` their per-run forms.
+
+For training, which the reference does not do: ``attn_fwd_typed`` /
+``attn_bwd_typed`` are the core of bfloat16 and float16 rows, with key and value
+heads shared by groups of query heads, a learned bias by relative position
+(``RelativeBias``, ``relative_buckets``) and dropout of the probabilities
+(``Dropout``), whose mask the backward makes again. All
 work runs in libpet_attn.so on the current torch stream; torch only provides
 device memory and the stream.
 """
@@ -227,6 +233,194 @@ def attn_bwd(qkv: torch.Tensor, off: torch.Tensor, dmerged: torch.Tensor, merged
                                 _mat(qkv_adj, "qkv_adj", 3 * D), cfh.data_ptr(), cf_seq_adj.data_ptr(),
                                 _mat(cf_seq_adj, "cf_seq_adj"), _stream()), "pet_attn_bwd")
     return qkv_adj, cf_seq_adj, cfh
+
+
+@dataclasses.dataclass
+class Dropout:
+    """Elements left out with probability ``p`` (in steps of 2^-16, at most 65534 /
+    65536), the rest scaled by 1 / (1 - p). ``state``: two int64 on the device, a seed
+    and a step (its low 32 bits count), read as the kernels run: a program that adds to
+    the step there draws anew in each replay of a graph. ``call`` (0 .. 2^32 - 1) tells
+    the calls of one step apart; a backward is given its forward's."""
+    p: float
+    state: torch.Tensor
+    call: int = 0
+
+
+def _dropout(d, device):
+    """The library's argument of a Dropout, None for none."""
+    if d is None:
+        return None
+    if not isinstance(d, Dropout):
+        raise TypeError("dropout: a Dropout is needed")
+    t = d.state
+    if not isinstance(t, torch.Tensor):
+        raise TypeError("dropout: state: a torch tensor is needed")
+    if t.device != device or t.dtype != torch.int64 or tuple(t.shape) != (2,) or not t.is_contiguous():
+        raise ValueError(f"dropout: state must be two contiguous int64 on {device}")
+    if not 0.0 <= d.p <= 65534 / 65536:
+        raise ValueError(f"dropout: p {d.p}: 0 to 65534/65536")
+    if not 0 <= d.call < 1 << 32:
+        raise ValueError(f"dropout: call {d.call}: 0 to 2^32 - 1")
+    return _lib.DropoutArgs(t.data_ptr(), float(d.p), int(d.call))
+
+
+MAX_BUCKETS, MAX_REACH = 64, 1024  # PET_BIAS_MAX_BUCKETS, PET_BIAS_MAX_REACH
+
+
+@dataclasses.dataclass
+class RelativeBias:
+    """A learned bias of the logits: key j adds table[buckets[clamp(positions[j] -
+    positions[i], -reach, reach) + reach]][h] for query i of head h, the positions of
+    their rows. ``table`` float32 [n_buckets, heads] (at most 64 buckets), ``buckets``
+    int32 [2 reach + 1] (``relative_buckets`` makes one; values past the table's ends count
+    as its ends), ``positions`` int32, one a row of qkv: any whole numbers, an order's
+    or an edge's radial shell's."""
+    table: torch.Tensor
+    buckets: torch.Tensor
+    positions: torch.Tensor
+
+
+def relative_buckets(n_buckets: int, reach: int, two_sided: bool = True, device=None) -> torch.Tensor:
+    """The bucket of each offset -reach .. reach (key's position less the query's) as
+    int32 [2 reach + 1]: half of the buckets to each sign (an odd one is left over), of a
+    half the first half one to an offset, the rest at equal ratios up to ``reach``, the
+    last taking what lies past it. Not ``two_sided``: all of them to keys at or before
+    the query, a key after it in bucket 0. Borders are found in whole numbers."""
+    if not 1 <= n_buckets <= MAX_BUCKETS or not 0 <= reach <= MAX_REACH:
+        raise ValueError(f"{n_buckets} buckets, reach {reach}: 1 to {MAX_BUCKETS} buckets, reach 0 to {MAX_REACH}")
+    half = max(1, n_buckets // 2 if two_sided else n_buckets)
+    single = max(1, half // 2)
+    wide = half - single
+    side = []
+    for d in range(reach + 1):
+        # b is the last bucket with d >= single (reach / single)^((b - single) / wide)
+        b = min(d, half - 1)
+        if d >= single:
+            b = min(single, half - 1)
+            while b < half - 1 and d ** wide * single ** (b + 1 - single) >= reach ** (b + 1 - single) * single ** wide:
+                b += 1
+        side.append(b)
+    after = [b + (half if n_buckets > 1 else 0) for b in side[1:]] if two_sided else [0] * reach
+    return torch.tensor(side[:0:-1] + side[:1] + after, dtype=torch.int32, device=device)
+
+
+def _bias(b, heads: int, rows: int, device):
+    """The library's argument of a RelativeBias, None for none."""
+    if b is None:
+        return None
+    if not isinstance(b, RelativeBias):
+        raise TypeError("bias: a RelativeBias is needed")
+    for t, name in ((b.table, "table"), (b.buckets, "buckets"), (b.positions, "positions")):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"bias: {name}: a torch tensor is needed")
+        kind = torch.float32 if name == "table" else torch.int32
+        if t.device != device or t.dtype != kind or not t.is_contiguous():
+            raise ValueError(f"bias: {name} must be contiguous {kind} on {device}")
+    if b.table.dim() != 2 or b.table.shape[1] != heads or not 1 <= b.table.shape[0] <= MAX_BUCKETS:
+        raise ValueError(f"bias: table has shape {tuple(b.table.shape)}, expected 1 to {MAX_BUCKETS} rows of {heads}")
+    if b.buckets.dim() != 1 or b.buckets.numel() % 2 != 1 or b.buckets.numel() > 2 * MAX_REACH + 1:
+        raise ValueError(f"bias: buckets has shape {tuple(b.buckets.shape)}: 2 reach + 1, reach at most {MAX_REACH}")
+    if tuple(b.positions.shape) != (rows,):
+        raise ValueError(f"bias: positions has shape {tuple(b.positions.shape)}, expected {(rows,)}")
+    return _lib.BiasArgs(b.table.data_ptr(), b.buckets.data_ptr(), b.positions.data_ptr(), b.table.shape[0],
+                         b.buckets.numel() // 2)
+
+
+def _typed_call(qkv, off, cf_seq, heads, head_dim, kv_heads, temperature, dead, N):
+    """What attn_fwd_typed and attn_bwd_typed check alike: (shape, kv_heads, ldq, ldc)."""
+    if not isinstance(qkv, torch.Tensor) or not isinstance(off, torch.Tensor) or not isinstance(cf_seq, torch.Tensor):
+        raise TypeError("qkv, off and cf_seq: torch tensors are needed")
+    dev = qkv.device
+    kv_heads = heads if kv_heads is None else kv_heads
+    if heads < 1 or kv_heads < 1 or heads % kv_heads or not 1 <= head_dim <= 128:
+        raise ValueError(f"{heads} heads, {kv_heads} key heads of {head_dim}: whole groups of heads of 1 to 128")
+    if qkv.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"qkv: {qkv.dtype}, not bfloat16 or float16 (float32 rows: attn_fwd, attn_bwd)")
+    if qkv.dim() != 2:
+        raise ValueError("qkv must be a row-major 2-D view")
+    T = qkv.shape[0]
+    ldq = _typed(qkv, "qkv", T, (heads + 2 * kv_heads) * head_dim, qkv.dtype, dev)
+    if off.device != dev or off.dtype != torch.int32 or off.dim() != 1 or not off.is_contiguous() or off.numel() < 1:
+        raise ValueError(f"off must be contiguous int32 [N + 1] on {dev}")
+    N = off.numel() - 1 if N is None else N
+    if not 0 <= N < off.numel() or T < N:
+        raise ValueError(f"{N} atoms: off has {off.numel()} entries, qkv {T} rows")
+    if cf_seq.dim() != 2 or cf_seq.shape[1] < 1:
+        raise ValueError("cf_seq must be a row-major 2-D view")
+    ldc = _typed(cf_seq, "cf_seq", N, cf_seq.shape[1], torch.float32, dev)
+    if not temperature > 0.0:
+        raise ValueError(f"temperature {temperature}: more than 0 is needed")
+    return shape(N, T, cf_seq.shape[1], heads, head_dim, temperature, dead), kv_heads, ldq, ldc
+
+
+def _saves(ml, count: int, device) -> int:
+    if not isinstance(ml, torch.Tensor):
+        raise TypeError("ml: a torch tensor is needed")
+    if ml.device != device or ml.dtype != torch.float32 or tuple(ml.shape) != (count, 2) or not ml.is_contiguous():
+        raise ValueError(f"ml must be a contiguous float32 {[count, 2]} on {device}")
+    return ml.data_ptr()
+
+
+def attn_fwd_typed(qkv: torch.Tensor, off: torch.Tensor, cf_seq: torch.Tensor, heads: int, head_dim: int,
+                   temperature: float = 1.0, kv_heads: int | None = None, bias: RelativeBias | None = None,
+                   dropout: Dropout | None = None, N: int | None = None, dead: bool = False,
+                   merged: torch.Tensor | None = None, ml: torch.Tensor | None = None, save: bool = True):
+    """attn_fwd of bfloat16 or float16 rows: (merged [T, heads * head_dim], ml
+    [N*heads*S, 2] or None). qkv [T, (heads + 2 kv_heads) * head_dim] = [Q | K | V];
+    key head k serves the query heads k G .. k G + G - 1, G = heads / kv_heads. ml holds
+    (max, 1/sum), (0, 0) where no token or no key is."""
+    sh, kv_heads, ldq, ldc = _typed_call(qkv, off, cf_seq, heads, head_dim, kv_heads, temperature, dead, N)
+    dev, T, D, S = qkv.device, qkv.shape[0], heads * head_dim, cf_seq.shape[1]
+    b, d = _bias(bias, heads, T, dev), _dropout(dropout, dev)
+    if merged is None:
+        merged = torch.empty((T, D), dtype=qkv.dtype, device=dev)
+    ldm = _typed(merged, "merged", T, D, qkv.dtype, dev)
+    if ml is None and save:
+        ml = torch.empty((sh.n_atoms * heads * S, 2), dtype=torch.float32, device=dev)
+    _call_on(dev, "pet_attn_fwd_typed", _lib.load().pet_attn_fwd_typed, DTYPES[qkv.dtype], sh, kv_heads, qkv.data_ptr(),
+             ldq, off.data_ptr(), cf_seq.data_ptr(), ldc, b, d, merged.data_ptr(), ldm,
+             None if ml is None else _saves(ml, sh.n_atoms * heads * S, dev))
+    return merged, ml
+
+
+def attn_bwd_typed(qkv: torch.Tensor, off: torch.Tensor, dmerged: torch.Tensor, merged: torch.Tensor, ml: torch.Tensor,
+                   cf_seq: torch.Tensor, heads: int, head_dim: int, temperature: float = 1.0,
+                   kv_heads: int | None = None, bias: RelativeBias | None = None, dropout: Dropout | None = None,
+                   qkv_adj: torch.Tensor | None = None, cf_seq_adj: torch.Tensor | None = None,
+                   bias_adj: torch.Tensor | None = None, beta: float = 0.0, N: int | None = None, dead: bool = False,
+                   scratch: torch.Tensor | None = None):
+    """attn_fwd_typed's backward from the adjoint of merged, merged and ml as it left
+    them and its bias and dropout: qkv_adj [T, (heads + 2 kv_heads) * head_dim], and
+    where given, each onto beta times itself, cf_seq_adj [N, S] and bias_adj (the bias
+    table's shape, float32). ``scratch``: pet_attn_bwd_typed_workspace bytes, else
+    allocated. Returns (qkv_adj, cf_seq_adj, bias_adj)."""
+    sh, kv_heads, ldq, ldc = _typed_call(qkv, off, cf_seq, heads, head_dim, kv_heads, temperature, dead, N)
+    dev, dt, T, D, S = qkv.device, qkv.dtype, qkv.shape[0], heads * head_dim, cf_seq.shape[1]
+    W = D + 2 * kv_heads * head_dim
+    b, d = _bias(bias, heads, T, dev), _dropout(dropout, dev)
+    ldg, ldm = _typed(dmerged, "dmerged", T, D, dt, dev), _typed(merged, "merged", T, D, dt, dev)
+    if qkv_adj is None:
+        qkv_adj = torch.empty((T, W), dtype=dt, device=dev)
+    lda = _typed(qkv_adj, "qkv_adj", T, W, dt, dev)
+    ldca = 0 if cf_seq_adj is None else _typed(cf_seq_adj, "cf_seq_adj", sh.n_atoms, S, torch.float32, dev)
+    if bias_adj is not None:
+        if bias is None:
+            raise ValueError("bias_adj without a bias")
+        if not isinstance(bias_adj, torch.Tensor):
+            raise TypeError("bias_adj: a torch tensor is needed")
+        if bias_adj.device != dev or bias_adj.dtype != torch.float32 or bias_adj.shape != bias.table.shape \
+                or not bias_adj.is_contiguous():
+            raise ValueError(f"bias_adj must be a contiguous float32 {list(bias.table.shape)} on {dev}")
+    lib = _lib.load()
+    scratch = _scratch(scratch, lib.pet_attn_bwd_typed_workspace(DTYPES[dt], sh, kv_heads, 0 if b is None else b.n_buckets),
+                       dev)
+    _call_on(dev, "pet_attn_bwd_typed", lib.pet_attn_bwd_typed, DTYPES[dt], sh, kv_heads, qkv.data_ptr(), ldq,
+             off.data_ptr(), dmerged.data_ptr(), ldg, merged.data_ptr(), ldm,
+             _saves(ml, sh.n_atoms * heads * S, dev), cf_seq.data_ptr(), ldc, b, d, qkv_adj.data_ptr(), lda,
+             _ptr(cf_seq_adj), ldca, _ptr(bias_adj), float(beta), scratch.data_ptr(),
+             scratch.numel() * scratch.element_size())
+    return qkv_adj, cf_seq_adj, bias_adj
 
 
 def attention(ws: Workspace, key: str, out: torch.Tensor, qkv: torch.Tensor, cf_seq: torch.Tensor,

@@ -17,8 +17,9 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libpet_attn.so")
-SOURCES = ["attention.hip", "attention_pair.hip", "attention_stream.hip", "ops.hip", "rows.hip", "norm_grads.hip",
-           "wgrad.hip", "grad_clip.hip", "forces.hip", "model.hip", "gemm.hip", "gemm_rows.hip", "probe.hip"]
+SOURCES = ["attention.hip", "attention_pair.hip", "attention_stream.hip", "attention_typed.hip",
+           "attention_typed_bwd.hip", "ops.hip", "rows.hip", "norm_grads.hip", "dropout.hip", "wgrad.hip",
+           "grad_clip.hip", "forces.hip", "model.hip", "gemm.hip", "gemm_rows.hip", "probe.hip"]
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",

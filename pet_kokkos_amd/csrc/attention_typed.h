@@ -1,0 +1,220 @@
+// Attention of 16-bit rows for training (attention_typed.hip, the forward;
+// attention_typed_bwd.hip): what the kernels share.
+//
+// For query i and key j of atom n (slots of its CSR segment) and head h,
+//   s_ij = scale q_i.k_j + log cf_j + b_ij,   b_ij = table[bucket(pos_j - pos_i)][h],
+//   P_ij = exp(s_ij - max_j s_ij) / sum_j,    O_i = sum_j P_ij M_ij v_j,
+// M the dropout mask (0 or 1 / (1 - p)), keys with cf <= 0 left out, queries on
+// edges with cf <= 0 zero. All in base 2 inside: exp(s) = 2^(s log2 e).
+//
+// The 16x16x32 matrix instruction of the row type: lane l = (c, g) = (l % 16, l / 16)
+// holds row (A) or column (B) c at k = 8g .. 8g + 7, and of the result column c at
+// rows 4g .. 4g + 3. Products that contract over tokens take the result of one
+// product as the B operand of the next without an exchange: of 32 tokens,
+// instruction t (0, 1) computes those 8a + 4t + r (a, r = 0 .. 3) as its rows 4a + r,
+// so a lane ends with tokens 8g .. 8g + 7, which is what B wants of it. LDS rows lie
+// in that order (lds_row). The same map over pairs of 16-dim tiles gives a lane
+// eight consecutive dims of its token's output: one 16-byte store.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+#include <cstdint>
+#include <type_traits>
+
+#include "../../include/pet_attn.h"
+#include "attn_common.h"
+#include "counter_rng.h"
+#include "typed.h"
+
+namespace pet_tattn {
+
+using pet_attn::f4;
+using pet_rng::Drop;
+using pet_rng::Words;
+using pet_typed::u4e;
+
+typedef unsigned u4 __attribute__((ext_vector_type(4)));
+typedef unsigned u2 __attribute__((ext_vector_type(2)));
+typedef int i4 __attribute__((ext_vector_type(4)));
+
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+constexpr float kInf = __builtin_huge_valf();
+
+template <class T>
+__device__ __forceinline__ f4 mfma(const u4& a, const u4& b, const f4& c) {
+  typedef T t8 __attribute__((ext_vector_type(8)));
+  if constexpr (std::is_same<T, __bf16>::value)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(t8, a), __builtin_bit_cast(t8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(t8, a), __builtin_bit_cast(t8, b), c, 0, 0, 0);
+}
+
+// The transposing LDS read (ds_read_b64_tr_b16) on the 16 lanes of a row: lane j's
+// element m is element j % 4 of what lane 4m + j / 4 addressed.
+template <class T>
+__device__ __forceinline__ u2 lds_tr(const T* p) {
+  typedef short s4 __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) s4 lds_s4;
+  return __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(p)));
+}
+
+// An LDS row's elements: HD dims and 16 bytes of padding, so that the 16 rows that a
+// wave reads at once start in different banks.
+template <int HD>
+constexpr int kPitch = HD + 8;
+
+// Where token k of a stage lies: of each 32, tokens 8a + 4t + r at row 16t + 4a + r.
+__device__ __forceinline__ int lds_row(int k) {
+  return (k & ~31) | (k & 4) << 2 | (k & 24) >> 1 | (k & 3);
+}
+
+// The A operand of a product over 32 staged tokens (rows base .. base + 31): row m of
+// it is dim 32 jp + 8 (m / 4) + 4 t + m % 4.
+template <class T, int HD>
+__device__ __forceinline__ u4 transposed(const T* rows, int base, int jp, int t, int lane) {
+  const int i = lane & 15, g = lane >> 4;
+  const T* p = rows + (base + 4 * g + (i >> 2)) * kPitch<HD> + 32 * jp + 8 * (i & 3) + 4 * t;
+  const u2 lo = lds_tr(p), hi = lds_tr(p + 16 * kPitch<HD>);
+  return u4{lo[0], lo[1], hi[0], hi[1]};
+}
+// Its plain A operand: rows 16t .. 16t + 15 of the 32 at base, dims 32 step .. + 31.
+template <class T, int HD>
+__device__ __forceinline__ u4 straight(const T* rows, int base, int t, int step, int lane) {
+  return *reinterpret_cast<const u4*>(rows + (base + 16 * t + (lane & 15)) * kPitch<HD> + 32 * step + 8 * (lane >> 4));
+}
+
+template <class T>
+__device__ __forceinline__ u4 pack8(const float (&x)[8]) {
+  return __builtin_bit_cast(u4, pet_typed::pack<T>(x));
+}
+
+__host__ __device__ inline int round_up(int64_t x, int to) { return int((x + to - 1) / to * to); }
+
+// What every kernel of a call is given.
+struct Args {
+  const void* qkv;
+  int64_t ldq;
+  const int* off;
+  const float* cf;
+  int64_t ldc;
+  int N, T, S, H, Hk, hd;
+  float scale, scale2, inv2;  // scale, scale log2 e, and its reciprocal
+  const float* table;         // [nb, H], or null
+  const int* buckets;         // [2 reach + 1]
+  const int* pos;             // [T]
+  int nb, reach;
+  Drop drop;
+};
+
+// Atom n's tokens. Counts past S or past the rows would be the caller's error; they
+// are cut, so that no row outside 0 .. T - 1 is touched whatever off holds.
+struct Segment {
+  int n, count;
+  int64_t edge;  // slot s >= 1 is row edge + s
+  __device__ __forceinline__ Segment(const Args& a, int n_) : n(n_) {
+    const int64_t o0 = a.off[n], o1 = a.off[n + 1];
+    int64_t c = o1 - o0, room = int64_t(a.T) - a.N - o0;
+    c = c < a.S - 1 ? c : a.S - 1;
+    c = c < room ? c : room;
+    count = o0 < 0 || c < 0 ? 1 : int(c) + 1;
+    edge = int64_t(a.N) + o0 - 1;
+  }
+  __device__ __forceinline__ int64_t row(int s) const { return s == 0 ? int64_t(n) : edge + s; }
+  __device__ __forceinline__ float cf(const Args& a, int s) const { return a.cf[int64_t(n) * a.ldc + s]; }
+  __device__ __forceinline__ bool key(const Args& a, int s) const { return s < count && cf(a, s) > 0.f; }
+  __device__ __forceinline__ bool query(const Args& a, int s) const {
+    return s < count && (s == 0 || cf(a, s) > 0.f);
+  }
+};
+
+// Dims d .. d + 7 of a row of hd, zeros past its end.
+template <class T>
+__device__ __forceinline__ u4 row_chunk(const T* row, int d, int hd) {
+  return __builtin_bit_cast(u4, (hd & 7) == 0 ? pet_typed::load_raw<T, true>(row, d, hd) : pet_typed::load_raw<T>(row, d, hd));
+}
+
+// Slots s0 .. s0 + n - 1 (n a multiple of 32) of the columns at src into LDS rows,
+// zeros where `live` says no: nothing that a masked row holds is ever multiplied.
+template <class T, int HD, class Live>
+__device__ __forceinline__ void stage(T* rows, const T* src, int64_t ld, const Segment& seg, int s0, int n, int hd,
+                                      const Live& live) {
+  constexpr int CH = HD / 8;
+  for (int i = threadIdx.x; i < n * CH; i += blockDim.x) {
+    const int k = i / CH, ch = i % CH, s = s0 + k;
+    u4 x = {0u, 0u, 0u, 0u};
+    if (live(s)) x = row_chunk(src + seg.row(s) * ld, 8 * ch, hd);
+    *reinterpret_cast<u4*>(rows + lds_row(k) * kPitch<HD> + 8 * ch) = x;
+  }
+}
+
+// A lane's B operand of a token's own columns: dims 32 step + 8g .. + 7.
+template <class T>
+__device__ __forceinline__ u4 own_chunk(const T* src, int64_t ld, int64_t row, bool live, int step, int lane, int hd) {
+  u4 x = {0u, 0u, 0u, 0u};
+  if (live) x = row_chunk(src + row * ld, 32 * step + 8 * (lane >> 4), hd);
+  return x;
+}
+
+// A row's eight dims 32 jp + 8g of a result's tile pair, times f.
+template <class T>
+__device__ __forceinline__ void put8(T* row, const f4& lo, const f4& hi, float f, int d, int hd) {
+  if (d >= hd) return;
+  float x[8];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) x[r] = lo[r] * f, x[4 + r] = hi[r] * f;
+  pet_typed::store<T>(row + d, hd - d, x);
+}
+
+// The offset of a pair in positions as an index 0 .. 2 reach (the difference does not wrap).
+__device__ __forceinline__ int pair_index(int pos_key, int pos_query, int reach) {
+  const int d = __builtin_elementwise_sub_sat(pos_key, pos_query);
+  return (d < -reach ? -reach : d > reach ? reach : d) + reach;
+}
+__device__ __forceinline__ int bucket_of(const Args& a, int i) {
+  const int b = a.buckets[i];
+  return b < 0 ? 0 : b >= a.nb ? a.nb - 1 : b;
+}
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// log2 of cutoff factors, in units of the scores before their scale
+__device__ __forceinline__ float log_weight(float cf) { return log2f(cf); }
+
+// Workgroups go round the XCDs, and so do the items of a head: block b has head
+// (b / 8) % heads and items slot, slot + step, ... of it, so the heads of an atom
+// run on one XCD close in time and its rows' lines meet in one L2.
+struct Share {
+  int head, slot, step;
+  __device__ __forceinline__ explicit Share(int heads) {
+    const int b = blockIdx.x;
+    head = (b >> 3) % heads;
+    slot = (b >> 3) / heads * 8 + (b & 7);
+    step = int(gridDim.x) / heads;
+  }
+};
+
+// ---- the host's half --------------------------------------------------------------
+
+
+
+// Arguments that forward and backward share; fills `a`.
+int check_args(int dtype, const pet_attn_shape* sh, int kv_heads, const void* qkv, int64_t ldq, const int* off,
+               const float* cf_seq, int64_t ldc, const pet_attn_bias* bias, const pet_dropout* dropout, Args& a);
+
+// Rows N + off[N] .. T - 1 of x set to zero.
+int zero_dead(const Args& a, void* x, int64_t ld, int width, hipStream_t st);
+
+template <class F>
+int with_head_dim(int hd, F&& f) {
+  if (hd <= 32) return f(std::integral_constant<int, 32>{});
+  if (hd <= 64) return f(std::integral_constant<int, 64>{});
+  return f(std::integral_constant<int, 128>{});
+}
+template <class F>
+int with_row_type(int dtype, F&& f) {
+  return dtype == PET_DTYPE_BF16 ? f(__bf16{}) : f(_Float16{});
+}
+
+}  // namespace pet_tattn

@@ -1,0 +1,284 @@
+// The forward of attention_typed.h: one pass over an atom's keys with each query's
+// running maximum and sum.
+//
+// A workgroup has a head and goes through its items, (atom, block of queries): its
+// waves hold QT tiles of 16 queries each as B operands in registers; keys and values
+// are staged in LDS, masked ones as zeros with a weight of -inf, and S^T = K Q^T
+// comes with a lane's query in its column, so maxima and sums are the lane's own but
+// for two lane swaps, and P^T is the B operand of O^T += V^T P^T as it lies. log cf
+// is the product's first summand, the bias a gather from LDS by the pair's offset.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+
+#include "../../include/pet_attn.h"
+#include "attention_typed.h"
+
+namespace pet_tattn {
+namespace {
+
+template <int HD>
+constexpr int fwd_stage_bytes(int keys) { return keys * (2 * kPitch<HD> * 2 + 8); }
+
+template <class T, int HD, int QT, bool BIAS, bool DROP>
+__global__ __launch_bounds__(512) void typed_fwd_kernel(Args a, int keys, int qblocks, T* merged, int64_t ldm,
+                                                        float* ml) {
+  extern __shared__ __align__(16) char lds[];
+  constexpr int DS = HD / 32, DT = HD / 16;
+  T* const ks = reinterpret_cast<T*>(lds);
+  T* const vs = ks + keys * kPitch<HD>;
+  float* const weight = reinterpret_cast<float*>(vs + keys * kPitch<HD>);
+  int* const kpos = reinterpret_cast<int*>(weight + keys);
+  float* const lut = reinterpret_cast<float*>(kpos + keys);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
+  const int per = int(blockDim.x >> 6) * QT * 16;
+  const Share share(a.H);
+  const int h = share.head, hk = h / (a.H / a.Hk);
+  const T* const qkv = static_cast<const T*>(a.qkv);
+  const T* const qcols = qkv + h * a.hd;
+  const T* const kcols = qkv + (a.H + hk) * a.hd;
+  const T* const vcols = qkv + (a.H + a.Hk + hk) * a.hd;
+  Words key{};
+  if constexpr (DROP) key = a.drop.key();
+  if constexpr (BIAS)
+    for (int i = threadIdx.x; i <= 2 * a.reach; i += blockDim.x)
+      lut[i] = a.table[int64_t(bucket_of(a, i)) * a.H + h] * kLog2e;
+
+  const int items = a.N * qblocks;
+  for (int item = share.slot; item < items; item += share.step) {
+    const int n = item / qblocks, qb = item - n * qblocks;
+    const Segment seg(a, n);
+    const int q0 = qb * per + wave * QT * 16;
+    // the wave's queries
+    u4 qf[QT][DS];
+    int64_t qrow[QT];
+    int qpos[QT];
+    bool qlive[QT];
+    f4 o[QT][DT];
+    float top[QT], sum[QT];
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      const int s = q0 + 16 * qt + c;
+      qlive[qt] = seg.query(a, s);
+      qrow[qt] = qlive[qt] ? seg.row(s) : 0;
+#pragma unroll
+      for (int d = 0; d < DS; ++d) qf[qt][d] = own_chunk(qcols, a.ldq, qrow[qt], qlive[qt], d, lane, a.hd);
+      if constexpr (BIAS) qpos[qt] = a.pos[qrow[qt]];
+#pragma unroll
+      for (int j = 0; j < DT; ++j) o[qt][j] = f4{0.f, 0.f, 0.f, 0.f};
+      top[qt] = -kInf, sum[qt] = 0.f;
+    }
+    if (qb * per < seg.count)  // (the same for the whole workgroup)
+      for (int k0 = 0; k0 < seg.count; k0 += keys) {
+        const int n_keys = min(keys, round_up(seg.count - k0, 32));
+        __syncthreads();
+        const auto live = [&](int s) { return seg.key(a, s); };
+        stage<T, HD>(ks, kcols, a.ldq, seg, k0, n_keys, a.hd, live);
+        stage<T, HD>(vs, vcols, a.ldq, seg, k0, n_keys, a.hd, live);
+        for (int k = threadIdx.x; k < n_keys; k += blockDim.x) {
+          const bool on = live(k0 + k);
+          weight[k] = on ? log_weight(seg.cf(a, k0 + k)) * a.inv2 : -kInf;
+          if constexpr (BIAS) kpos[k] = on ? a.pos[seg.row(k0 + k)] : 0;
+        }
+        __syncthreads();
+        if (q0 >= seg.count) continue;
+        for (int kb = 0; kb < n_keys; kb += 64) {
+          f4 s[QT][2][2];
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            if (kb + 32 * u >= n_keys) {
+#pragma unroll
+              for (int qt = 0; qt < QT; ++qt) s[qt][u][0] = s[qt][u][1] = f4{-kInf, -kInf, -kInf, -kInf};
+              continue;
+            }
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              const int at = kb + 32 * u + 8 * g + 4 * t;
+              const f4 w = *reinterpret_cast<const f4*>(weight + at);
+#pragma unroll
+              for (int qt = 0; qt < QT; ++qt) s[qt][u][t] = w;
+#pragma unroll
+              for (int d = 0; d < DS; ++d) {
+                const u4 kf = straight<T, HD>(ks, kb + 32 * u, t, d, lane);
+#pragma unroll
+                for (int qt = 0; qt < QT; ++qt) s[qt][u][t] = mfma<T>(kf, qf[qt][d], s[qt][u][t]);
+              }
+              if constexpr (BIAS) {
+                const i4 kp = *reinterpret_cast<const i4*>(kpos + at);
+#pragma unroll
+                for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+                  for (int r = 0; r < 4; ++r)
+                    s[qt][u][t][r] = fmaf(s[qt][u][t][r], a.scale2, lut[pair_index(kp[r], qpos[qt], a.reach)]);
+              }
+            }
+          }
+          const float f = BIAS ? 1.f : a.scale2;
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt) {
+            float m = -kInf;
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+              for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) m = fmaxf(m, s[qt][u][t][r]);
+            const float now = fmaxf(top[qt], pet_attn::max_g(m) * f);
+            const float base = now == -kInf ? 0.f : now;
+            const float fade = exp2_fast(top[qt] - base);
+            top[qt] = now;
+            sum[qt] *= fade;
+#pragma unroll
+            for (int j = 0; j < DT; ++j) o[qt][j] *= fade;
+            u4 pf[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              float p[8];
+#pragma unroll
+              for (int t = 0; t < 2; ++t) {
+                Words w{};
+                if constexpr (DROP)
+                  w = a.drop.block(key, uint32_t(qrow[qt]),
+                                   uint32_t((k0 + kb + 32 * u + 8 * g + 4 * t) >> 2) * uint32_t(a.H) + uint32_t(h));
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                  const float x = s[qt][u][t][r];
+                  float e = exp2_fast(BIAS ? x - base : fmaf(x, f, -base));
+                  sum[qt] += e;
+                  if constexpr (DROP) e = Drop::number(w, r) >= a.drop.least ? e : 0.f;
+                  p[4 * t + r] = e;
+                }
+              }
+              pf[u] = pack8<T>(p);
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              if (kb + 32 * u >= n_keys) continue;
+#pragma unroll
+              for (int j = 0; j < DT; ++j)
+                o[qt][j] = mfma<T>(transposed<T, HD>(vs, kb + 32 * u, j >> 1, j & 1, lane), pf[u], o[qt][j]);
+            }
+          }
+        }
+      }
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      const int s = q0 + 16 * qt + c;
+      const float l = pet_attn::sum_g(sum[qt]);
+      const bool some = qlive[qt] && l != 0.f;
+      const float inv = some ? 1.f / l : 0.f;
+      if (ml && g == 0 && s < a.S)
+        *reinterpret_cast<float2*>(ml + ((int64_t(n) * a.H + h) * a.S + s) * 2) =
+            make_float2(some ? top[qt] * kLn2 : 0.f, inv);
+      if (s < seg.count) {
+        T* const row = merged + seg.row(s) * ldm + h * a.hd;
+        const float f = DROP ? inv * a.drop.scale : inv;
+#pragma unroll
+        for (int jp = 0; jp < DS; ++jp) {
+          f4 lo = o[qt][2 * jp], hi = o[qt][2 * jp + 1];
+          if (!some) lo = hi = f4{0.f, 0.f, 0.f, 0.f};
+          put8(row, lo, hi, f, 32 * jp + 8 * g, a.hd);
+        }
+      }
+    }
+  }
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void zero_dead_kernel(const int* off, int N, int rows, int width, T* x, int64_t ld) {
+  int64_t first = int64_t(N) + off[N];
+  first = first < 0 ? 0 : first;
+  for (int64_t r = first + blockIdx.x; r < rows; r += gridDim.x)
+    for (int c = threadIdx.x; c < width; c += 256) x[r * ld + c] = T(0.f);
+}
+
+}  // namespace
+
+int zero_dead(const Args& a, void* x, int64_t ld, int width, hipStream_t st) {
+  typedef unsigned short u16;
+  hipLaunchKernelGGL(zero_dead_kernel<u16>, dim3(unsigned(std::min(a.T, 2048))), dim3(256), 0, st, a.off, a.N, a.T,
+                     width, static_cast<u16*>(x), ld);
+  return hipGetLastError() == hipSuccess ? PET_ATTN_OK : PET_ATTN_ELAUNCH;
+}
+
+int check_args(int dtype, const pet_attn_shape* sh, int kv_heads, const void* qkv, int64_t ldq, const int* off,
+               const float* cf_seq, int64_t ldc, const pet_attn_bias* bias, const pet_dropout* dropout, Args& a) {
+  if (!sh || (dtype != PET_DTYPE_BF16 && dtype != PET_DTYPE_F16)) return PET_ATTN_EINVAL;
+  if (sh->n_atoms < 0 || sh->n_rows < sh->n_atoms || sh->slots < 1 || sh->heads < 1) return PET_ATTN_EINVAL;
+  if (sh->head_dim < 1 || sh->head_dim > 128) return PET_ATTN_EHEADDIM;
+  if (kv_heads < 1 || sh->heads % kv_heads != 0) return PET_ATTN_EINVAL;
+  const int64_t width = (int64_t(sh->heads) + 2 * int64_t(kv_heads)) * sh->head_dim;
+  if (width > INT32_MAX) return PET_ATTN_EINDEX;
+  if (!off || ldq < width || ldc < sh->slots) return PET_ATTN_EINVAL;
+  if ((sh->n_rows > 0 && !qkv) || (sh->n_atoms > 0 && !cf_seq)) return PET_ATTN_EINVAL;
+  const float scale2 = sh->scale * kLog2e;
+  if (!(sh->scale > 0.f) || !std::isfinite(scale2) || !std::isfinite(1.f / scale2)) return PET_ATTN_EINVAL;
+  // a query's dropout counter, key / 4 by head, is 32 bits; an item's number is an int
+  if ((int64_t(sh->slots) + 3) / 4 * sh->heads > int64_t(UINT32_MAX)) return PET_ATTN_EINDEX;
+  if (int64_t(sh->n_atoms) * ((int64_t(sh->slots) + 15) / 16) > (1 << 30)) return PET_ATTN_EINDEX;
+  a = Args{};
+  if (bias) {
+    if (!bias->table || !bias->buckets || (sh->n_rows > 0 && !bias->positions)) return PET_ATTN_EINVAL;
+    if (bias->n_buckets < 1 || bias->n_buckets > PET_BIAS_MAX_BUCKETS || bias->reach < 0 || bias->reach > PET_BIAS_MAX_REACH)
+      return PET_ATTN_EINVAL;
+    for (const void* p : {static_cast<const void*>(bias->table), static_cast<const void*>(bias->buckets),
+                          static_cast<const void*>(bias->positions)})
+      if (!pet_typed::element_aligned(p, PET_DTYPE_F32)) return PET_ATTN_EALIGN;
+    a.table = bias->table, a.buckets = bias->buckets, a.pos = bias->positions;
+    a.nb = bias->n_buckets, a.reach = bias->reach;
+  }
+  if (dropout)
+    if (const int e = pet_rng::make_drop(dropout, a.drop)) return e;
+  if (!pet_typed::element_aligned(qkv, dtype) || !pet_typed::element_aligned(off, PET_DTYPE_F32) ||
+      !pet_typed::element_aligned(cf_seq, PET_DTYPE_F32))
+    return PET_ATTN_EALIGN;
+  a.qkv = qkv, a.ldq = ldq, a.off = off, a.cf = cf_seq, a.ldc = ldc;
+  a.N = sh->n_atoms, a.T = sh->n_rows, a.S = sh->slots, a.H = sh->heads, a.Hk = kv_heads, a.hd = sh->head_dim;
+  a.scale = sh->scale, a.scale2 = scale2, a.inv2 = 1.f / scale2;
+  return PET_ATTN_OK;
+}
+
+}  // namespace pet_tattn
+
+using namespace pet_tattn;
+
+extern "C" int pet_attn_fwd_typed(int dtype, const pet_attn_shape* shape, int kv_heads, const void* qkv, int64_t ldq,
+                                  const int* off, const float* cf_seq, int64_t ldc, const pet_attn_bias* bias,
+                                  const pet_dropout* dropout, void* merged, int64_t ldm, float* ml, void* stream) {
+  Args a;
+  if (const int e = check_args(dtype, shape, kv_heads, qkv, ldq, off, cf_seq, ldc, bias, dropout, a)) return e;
+  const int D = a.H * a.hd;
+  if ((a.T > 0 && !merged) || ldm < D) return PET_ATTN_EINVAL;
+  if (!pet_typed::element_aligned(merged, dtype) || (reinterpret_cast<uintptr_t>(ml) & 7u) != 0) return PET_ATTN_EALIGN;
+  if (a.T == 0) return PET_ATTN_OK;
+  const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  if (shape->dead)
+    if (const int e = zero_dead(a, merged, ldm, D, st)) return e;
+  if (a.N == 0) return PET_ATTN_OK;
+  return with_row_type(dtype, [&](auto tv) {
+    using T = decltype(tv);
+    return with_head_dim(a.hd, [&](auto hc) {
+      constexpr int HD = decltype(hc)::value;
+      const auto run = [&](auto qc, auto bc, auto dc) {
+        constexpr int QT = decltype(qc)::value;
+        const auto kernel = typed_fwd_kernel<T, HD, QT, decltype(bc)::value, decltype(dc)::value>;
+        const int waves = QT == 1 ? std::min(8, round_up(a.S, 16) / 16) : 4;
+        const int qblocks = (a.S + waves * QT * 16 - 1) / (waves * QT * 16);
+        const int keys = a.S <= 64 ? round_up(a.S, 32) : QT == 1 ? 128 : 64;
+        const size_t bytes = size_t(fwd_stage_bytes<HD>(keys)) + (a.table ? size_t(2 * a.reach + 1) * 4 : 0);
+        if (const int e = pet_attn::raise_lds(reinterpret_cast<const void*>(kernel), bytes)) return e;
+        const int64_t slots = std::min<int64_t>((int64_t(a.N) * qblocks + 7) / 8 * 8, 2048);
+        if (slots * a.H * waves * 64 > INT32_MAX) return int(PET_ATTN_EINDEX);
+        hipLaunchKernelGGL(kernel, dim3(unsigned(slots * a.H)), dim3(unsigned(waves * 64)), bytes, st, a, keys, qblocks,
+                           static_cast<T*>(merged), ldm, ml);
+        return hipGetLastError() == hipSuccess ? int(PET_ATTN_OK) : int(PET_ATTN_ELAUNCH);
+      };
+      const auto pick = [&](auto qc) {
+        if (a.table) return dropout ? run(qc, std::true_type{}, std::true_type{}) : run(qc, std::true_type{}, std::false_type{});
+        return dropout ? run(qc, std::false_type{}, std::true_type{}) : run(qc, std::false_type{}, std::false_type{});
+      };
+      return a.S <= 128 ? pick(std::integral_constant<int, 1>{}) : pick(std::integral_constant<int, 2>{});
+    });
+  });
+}

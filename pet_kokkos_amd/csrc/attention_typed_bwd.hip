@@ -1,0 +1,626 @@
+// The backward of attention_typed.h, the probabilities recomputed from the saved
+// (max, 1/sum): with D_i = dO_i.O_i,
+//   dP_ij = M_ij dO_i.v_j,   dS_ij = P_ij (dP_ij - D_i),
+//   dQ_i = scale sum_j dS_ij k_j,   dK_j = scale sum_i dS_ij q_i,   dV_j = sum_i P_ij M_ij dO_i,
+//   dcf_j = sum over heads and i of dS_ij / cf_j,   dtable[b][h] = sum over pairs in bucket b of dS_ij.
+// Keys and values shared by a group of heads sum over it.
+//
+// Nothing is atomic across lanes and every sum has one owner and a fixed order, so
+// results repeat bit for bit: the bias table's gradient goes through a column of LDS
+// of each lane's own (a bucket a row: the lanes' additions never meet, nor do their
+// banks), the columns are summed in order, and so are the workgroups' sums.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+
+#include "../../include/pet_attn.h"
+#include "attention_typed.h"
+
+namespace pet_tattn {
+namespace {
+
+constexpr int kQueries = 64;     // queries a stage
+constexpr int kMaxSlots = 1024;  // workgroups a head at most (a partial sum of the table each)
+
+// What the backward's kernels are given beside Args.
+struct Grads {
+  const void *out_adj, *out;
+  int64_t ldg, ldm;
+  const float* ml;
+  void* adj;
+  int64_t lda;
+  float* delta;  // [T, H]: dO.O
+  float* norms;  // fp16: [T, H] |dO|, then [T, Hk] |v|
+  float* cfh;    // [N, H, S], or null
+  float* part;   // [slots, H, nb], with a table's gradient
+};
+
+// dO.O of each row and head, and for fp16 rows |dO| and |v|: a group of lanes takes
+// a head's slice, eight elements each.
+template <class T, int LG>
+__global__ __launch_bounds__(256) void delta_kernel(Args a, Grads b) {
+  const bool half = std::is_same<T, _Float16>::value;
+  const int64_t heads = int64_t(a.T) * a.H, all = heads + (half ? int64_t(a.T) * a.Hk : 0);
+  const int l = threadIdx.x % LG;
+  for (int64_t i = (int64_t(blockIdx.x) * 256 + threadIdx.x) / LG; i < all; i += int64_t(gridDim.x) * (256 / LG)) {
+    const bool q = i < heads;
+    const int64_t j = q ? i : i - heads, per = q ? a.H : a.Hk, row = j / per;
+    const int h = int(j - row * per);
+    float x[8], y[8], dot = 0.f, sq = 0.f;
+    const T* p = q ? static_cast<const T*>(b.out_adj) + row * b.ldg + h * a.hd
+                   : static_cast<const T*>(a.qkv) + row * a.ldq + (a.H + a.Hk + h) * a.hd;
+    pet_typed::unpack<T>(__builtin_bit_cast(u4e, row_chunk(p, 8 * l, a.hd)), x);
+    if (q)
+      pet_typed::unpack<T>(__builtin_bit_cast(u4e, row_chunk(static_cast<const T*>(b.out) + row * b.ldm + h * a.hd, 8 * l, a.hd)), y);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (q) dot = fmaf(x[e], y[e], dot);
+      if (half) sq = fmaf(x[e], x[e], sq);
+    }
+#pragma unroll
+    for (int m = 1; m < LG; m <<= 1) {
+      dot += __shfl_xor(dot, m, LG);
+      if (half) sq += __shfl_xor(sq, m, LG);
+    }
+    if (l == 0) {
+      if (q) b.delta[i] = dot;
+      if (half) b.norms[i] = sqrtf(sq);
+    }
+  }
+}
+
+// fp16 holds down to 2^-14 at full precision, and a long row's dS lie far under the
+// adjoints that they come from: the power of two that brings a bound of them,
+// max |dO| max |v| scale + max |D| over the atom and the group of heads, to 2^14 .. 2^15.
+// bf16 has fp32's range, and takes 1. Every wave of the workgroup calls it; room: 3
+// floats a wave.
+template <class T>
+__device__ __forceinline__ float adjoint_scale(const Args& a, const Grads& b, const Segment& seg, int hk, float* room) {
+  if constexpr (!std::is_same<T, _Float16>::value) return 1.f;
+  const int G = a.H / a.Hk;
+  float m[3] = {0.f, 0.f, 0.f};
+  for (int s = threadIdx.x; s < seg.count; s += blockDim.x) {
+    if (!seg.query(a, s)) continue;
+    const int64_t row = seg.row(s);
+    for (int i = 0; i < G; ++i) {
+      m[0] = fmaxf(m[0], b.norms[row * a.H + hk * G + i]);
+      m[1] = fmaxf(m[1], fabsf(b.delta[row * a.H + hk * G + i]));
+    }
+    if (seg.key(a, s)) m[2] = fmaxf(m[2], b.norms[int64_t(a.T) * a.H + row * a.Hk + hk]);
+  }
+#pragma unroll
+  for (int i = 0; i < 3; ++i)
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) m[i] = fmaxf(m[i], __shfl_xor(m[i], d));
+  const int waves = int(blockDim.x >> 6), wave = threadIdx.x >> 6;
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0)
+#pragma unroll
+    for (int i = 0; i < 3; ++i) room[3 * wave + i] = m[i];
+  __syncthreads();
+  for (int w = 0; w < waves; ++w)
+#pragma unroll
+    for (int i = 0; i < 3; ++i) m[i] = fmaxf(m[i], room[3 * w + i]);
+  const float bound = m[0] * m[2] * a.drop.scale + m[1];
+  if (!(bound > 0.f) || !(bound < kInf)) return 1.f;
+  const int e = 14 - ilogbf(bound);
+  return ldexpf(1.f, e < -60 ? -60 : e > 60 ? 60 : e);
+}
+
+// A query's exponent: P = 2^(s - this), +inf (P = 0) for one that attends to nothing.
+__device__ __forceinline__ float exponent(const Args& a, const Grads& b, int n, int h, int s, bool live) {
+  if (!live) return kInf;
+  const float2 v = *reinterpret_cast<const float2*>(b.ml + ((int64_t(n) * a.H + h) * a.S + s) * 2);
+  return v.y == 0.f ? kInf : v.x * kLog2e - log2f(v.y);
+}
+
+// The mask of 16 keys (slots key0 ..) by 32 queries (query_row: that of query l % 32), as
+// lane (c, g)'s eight queries 8g .. 8g + 7 of its key c: bit 8 r of word t is query 8g +
+// 4t + r's. A block of numbers is a query's four keys, so a lane makes two of its query
+// (keys 8j + 4 (l / 32) + r), eight bits, and the bytes of eight lanes are what a lane
+// of the key reads. exchange: 64 bytes of LDS of the wave's own.
+__device__ __forceinline__ u2 keys_mask(const Args& a, const Words& key, uint32_t query_row, int key0, int h, int lane,
+                                        unsigned char* exchange) {
+  unsigned byte = 0;
+  Words w[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+    w[j] = a.drop.block(key, query_row, uint32_t((key0 >> 2) + 2 * j + (lane >> 5)) * uint32_t(a.H) + uint32_t(h));
+#pragma unroll
+  for (int i = 7; i >= 0; --i) byte = byte + byte + unsigned(Drop::number(w[i >> 2], i & 3) >= a.drop.least);
+  const int c = lane & 15, g = lane >> 4;
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+  exchange[lane] = static_cast<unsigned char>(byte);
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+  __builtin_amdgcn_wave_barrier();
+  const u2 got = *reinterpret_cast<const u2*>(exchange + 8 * (c & 4) + 8 * g);
+  __builtin_amdgcn_wave_barrier();
+  return got >> unsigned((c >> 3) * 4 + (c & 3));
+}
+__device__ __forceinline__ float masked(float x, const u2& bits, int t, int r) {
+  return __uint_as_float(__float_as_uint(x) & unsigned(int(bits[t] << (31 - 8 * r)) >> 31));
+}
+
+struct BiasEntry {
+  float value;    // table[bucket][h] log2 e
+  int hist;       // the bucket's row in a wave's columns, in floats
+};
+
+template <int HD>
+struct KvLds {
+  static constexpr size_t rows = size_t(2) * kQueries * kPitch<HD> * 2, queries = rows + size_t(kQueries) * 12;
+  // + a wave's masks and maxima
+  // + the bias's entries, the lanes' columns
+  static size_t bytes(const Args& a, int waves, bool hist) {
+    return queries + size_t(waves) * (64 + 12) + 8 + (a.table ? size_t(2 * a.reach + 1) * 8 : 0) +
+           (hist ? size_t(waves) * a.nb * 256 : 0);
+  }
+};
+
+// dK, dV, the cutoff factors' and the table's adjoints: a wave has KT tiles of 16 keys
+// as B operands, dK^T and dV^T in registers, and goes over all queries of the group's
+// heads, staged in LDS: S = Q K^T and dP = dO V^T with a lane's key in its column, so P
+// and dS are the B operands of dV^T += dO^T P and dK^T += Q^T dS as they lie.
+template <class T, int HD, int KT, bool BIAS, bool DROP>
+__global__ __launch_bounds__(256) void typed_bwd_kv_kernel(Args a, Grads b, int kblocks) {
+  extern __shared__ __align__(16) char lds[];
+  constexpr int DS = HD / 32, DT = HD / 16;
+  constexpr bool HALF = std::is_same<T, _Float16>::value;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = int(blockDim.x >> 6), c = lane & 15, g = lane >> 4;
+  T* const qs = reinterpret_cast<T*>(lds);
+  T* const gs = qs + kQueries * kPitch<HD>;
+  float* const expo = reinterpret_cast<float*>(gs + kQueries * kPitch<HD>);
+  float* const delta = expo + kQueries;
+  int* const qpos = reinterpret_cast<int*>(delta + kQueries);
+  unsigned char* const exchange = reinterpret_cast<unsigned char*>(qpos + kQueries) + 64 * wave;
+  float* const room = reinterpret_cast<float*>(qpos + kQueries + 16 * waves);
+  BiasEntry* const lut = reinterpret_cast<BiasEntry*>(room + (3 * waves + 1) / 2 * 2);
+  float* const columns = reinterpret_cast<float*>(lut + (BIAS ? 2 * a.reach + 1 : 0));
+  const int G = a.H / a.Hk, per = waves * KT * 16;
+  const Share share(a.Hk);
+  const int hk = share.head;
+  const bool hist = BIAS && b.part;
+  const T* const qkv = static_cast<const T*>(a.qkv);
+  const T* const kcols = qkv + (a.H + hk) * a.hd;
+  const T* const vcols = qkv + (a.H + a.Hk + hk) * a.hd;
+  Words key{};
+  if constexpr (DROP) key = a.drop.key();
+  float* const mine = columns + wave * a.nb * 64 + lane;
+  float* const sums = b.part + (int64_t(share.slot) * a.H + hk * G) * a.nb;  // the workgroup's own, a head's by one thread a bucket
+  if (hist) {
+    for (int i = 0; i < a.nb; ++i) mine[64 * i] = 0.f;
+    for (int k = threadIdx.x; k < a.nb; k += blockDim.x)
+      for (int i = 0; i < G; ++i) sums[i * a.nb + k] = 0.f;
+  }
+  // the lanes' columns onto a head's sums, and cleared
+  const auto flush = [&](int i) {
+    __syncthreads();
+    for (int k = threadIdx.x; k < a.nb; k += blockDim.x) {
+      float sum = 0.f;
+      for (int w = 0; w < waves; ++w)
+        for (int l = 0; l < 64; ++l) sum += columns[(w * a.nb + k) * 64 + ((l + k) & 63)];
+      sums[i * a.nb + k] += sum;
+    }
+    __syncthreads();
+    for (int k = 0; k < a.nb; ++k) mine[64 * k] = 0.f;
+  };
+  const auto entries = [&](int h) {
+    for (int i = threadIdx.x; i <= 2 * a.reach; i += blockDim.x) {
+      const int bucket = bucket_of(a, i);
+      lut[i] = BiasEntry{a.table[int64_t(bucket) * a.H + h] * kLog2e, bucket * 64};
+    }
+  };
+  if (BIAS && G == 1) entries(hk);
+
+  const int items = a.N * kblocks;
+  for (int item = share.slot; item < items; item += share.step) {
+    const int n = item / kblocks, kb = item - n * kblocks;
+    const Segment seg(a, n);
+    if (kb * per >= seg.count) continue;
+    const float sc = adjoint_scale<T>(a, b, seg, hk, room), back = 1.f / sc;
+    const int k0 = kb * per + wave * KT * 16;
+    u4 kf[KT][DS], vf[KT][DS];
+    f4 dk[KT][DT], dv[KT][DT];
+    float weight[KT];
+    int kpos[KT];
+    bool klive[KT];
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+      const int s = k0 + 16 * kt + c;
+      klive[kt] = seg.key(a, s);
+      const int64_t row = klive[kt] ? seg.row(s) : 0;
+#pragma unroll
+      for (int d = 0; d < DS; ++d) {
+        kf[kt][d] = own_chunk(kcols, a.ldq, row, klive[kt], d, lane, a.hd);
+        vf[kt][d] = own_chunk(vcols, a.ldq, row, klive[kt], d, lane, a.hd);
+      }
+      weight[kt] = klive[kt] ? log_weight(seg.cf(a, s)) : -kInf;
+      if constexpr (BIAS) kpos[kt] = a.pos[row];
+#pragma unroll
+      for (int j = 0; j < DT; ++j) dk[kt][j] = dv[kt][j] = f4{0.f, 0.f, 0.f, 0.f};
+    }
+    for (int i = 0; i < G; ++i) {
+      const int h = hk * G + i;
+      float cf_sum[KT] = {};
+      if (BIAS && G > 1) {
+        __syncthreads();
+        entries(h);
+      }
+      const T* const qcols = qkv + h * a.hd;
+      const T* const gcols = static_cast<const T*>(b.out_adj) + h * a.hd;
+      for (int q0 = 0; q0 < seg.count; q0 += kQueries) {
+        const int n_queries = min(kQueries, round_up(seg.count - q0, 32));
+        __syncthreads();
+        const auto live = [&](int s) { return seg.query(a, s); };
+        stage<T, HD>(qs, qcols, a.ldq, seg, q0, n_queries, a.hd, live);
+        stage<T, HD>(gs, gcols, b.ldg, seg, q0, n_queries, a.hd, live);
+        for (int q = threadIdx.x; q < n_queries; q += blockDim.x) {
+          const bool on = live(q0 + q);
+          const int64_t row = on ? seg.row(q0 + q) : 0;
+          float e = exponent(a, b, n, h, q0 + q, on);
+          if constexpr (DROP) e -= log2f(a.drop.scale);
+          expo[q] = -e * a.inv2;
+          delta[q] = on ? b.delta[row * a.H + h] / a.drop.scale : 0.f;
+          if constexpr (BIAS) qpos[q] = a.pos[row];
+        }
+        __syncthreads();
+        if (k0 >= seg.count) continue;
+        for (int qb = 0; qb < n_queries; qb += 32) {
+          u2 bits[KT];
+          if constexpr (DROP) {
+            const int s = q0 + qb + (lane & 31);
+            const uint32_t row = uint32_t(s < seg.count ? seg.row(s) : 0);
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) bits[kt] = keys_mask(a, key, row, k0 + 16 * kt, h, lane, exchange);
+          }
+          float p[KT][8], ds[KT][8];
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const int at = qb + 8 * g + 4 * t;
+            f4 s[KT], dp[KT];
+            const f4 e4 = *reinterpret_cast<const f4*>(expo + at), d4 = *reinterpret_cast<const f4*>(delta + at);
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) s[kt] = e4, dp[kt] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int d = 0; d < DS; ++d) {
+              const u4 qf = straight<T, HD>(qs, qb, t, d, lane), gf = straight<T, HD>(gs, qb, t, d, lane);
+#pragma unroll
+              for (int kt = 0; kt < KT; ++kt) {
+                s[kt] = mfma<T>(qf, kf[kt][d], s[kt]);
+                dp[kt] = mfma<T>(gf, vf[kt][d], dp[kt]);
+              }
+            }
+            i4 qp{};
+            if constexpr (BIAS) qp = *reinterpret_cast<const i4*>(qpos + at);
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                float w = weight[kt];
+                BiasEntry be{};
+                if constexpr (BIAS) {
+                  be = lut[pair_index(kpos[kt], qp[r], a.reach)];
+                  w += be.value;
+                }
+                const float e = exp2_fast(fmaf(s[kt][r], a.scale2, w));
+                float kept = e;
+                if constexpr (DROP) kept = masked(e, bits[kt], t, r);
+                p[kt][4 * t + r] = kept;
+                const float es = HALF ? e * sc : e;
+                const float x = fmaf(HALF ? kept * sc : kept, dp[kt][r], -es * d4[r]);
+                ds[kt][4 * t + r] = x;
+                cf_sum[kt] += x;
+                if (hist) __hip_atomic_fetch_add(mine + be.hist, x * back, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
+              }
+          }
+#pragma unroll
+          for (int kt = 0; kt < KT; ++kt) {
+            const u4 pf = pack8<T>(p[kt]), df = pack8<T>(ds[kt]);
+#pragma unroll
+            for (int j = 0; j < DT; ++j) {
+              dv[kt][j] = mfma<T>(transposed<T, HD>(gs, qb, j >> 1, j & 1, lane), pf, dv[kt][j]);
+              dk[kt][j] = mfma<T>(transposed<T, HD>(qs, qb, j >> 1, j & 1, lane), df, dk[kt][j]);
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt) {
+        const float sum = pet_attn::sum_g(cf_sum[kt]) * back;
+        const int s = k0 + 16 * kt + c;
+        if (b.cfh && g == 0 && s < seg.count) b.cfh[(int64_t(n) * a.H + h) * a.S + s] = sum;
+      }
+      if (hist && G > 1) flush(i);
+    }
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+      const int s = k0 + 16 * kt + c;
+      if (s >= seg.count) continue;
+      T* const row = static_cast<T*>(b.adj) + seg.row(s) * b.lda;
+#pragma unroll
+      for (int jp = 0; jp < DS; ++jp) {
+        if (!klive[kt]) dk[kt][2 * jp] = dk[kt][2 * jp + 1] = dv[kt][2 * jp] = dv[kt][2 * jp + 1] = f4{0.f, 0.f, 0.f, 0.f};
+        put8(row + (a.H + hk) * a.hd, dk[kt][2 * jp], dk[kt][2 * jp + 1], a.scale * back, 32 * jp + 8 * g, a.hd);
+        put8(row + (a.H + a.Hk + hk) * a.hd, dv[kt][2 * jp], dv[kt][2 * jp + 1], 1.f, 32 * jp + 8 * g, a.hd);
+      }
+    }
+  }
+  if (hist && G == 1) flush(0);
+}
+
+// dQ: a wave has QT tiles of 16 queries as B operands and goes over the keys: S^T and
+// dP^T with a lane's query in its column, dS^T the B operand of dQ^T += K^T dS^T.
+template <class T, int HD, int QT, bool BIAS, bool DROP>
+__global__ __launch_bounds__(256) void typed_bwd_q_kernel(Args a, Grads b, int qblocks) {
+  extern __shared__ __align__(16) char lds[];
+  constexpr int DS = HD / 32, DT = HD / 16, kKeys = kQueries;
+  constexpr bool HALF = std::is_same<T, _Float16>::value;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = int(blockDim.x >> 6), c = lane & 15, g = lane >> 4;
+  T* const ks = reinterpret_cast<T*>(lds);
+  T* const vs = ks + kKeys * kPitch<HD>;
+  float* const weight = reinterpret_cast<float*>(vs + kKeys * kPitch<HD>);
+  int* const kpos = reinterpret_cast<int*>(weight + kKeys);
+  float* const room = reinterpret_cast<float*>(kpos + kKeys);
+  float* const lut = room + 3 * waves;
+  const int per = waves * QT * 16;
+  const Share share(a.H);
+  const int h = share.head, hk = h / (a.H / a.Hk);
+  const T* const qkv = static_cast<const T*>(a.qkv);
+  const T* const qcols = qkv + h * a.hd;
+  const T* const gcols = static_cast<const T*>(b.out_adj) + h * a.hd;
+  const T* const kcols = qkv + (a.H + hk) * a.hd;
+  const T* const vcols = qkv + (a.H + a.Hk + hk) * a.hd;
+  Words key{};
+  if constexpr (DROP) key = a.drop.key();
+  if constexpr (BIAS)
+    for (int i = threadIdx.x; i <= 2 * a.reach; i += blockDim.x)
+      lut[i] = a.table[int64_t(bucket_of(a, i)) * a.H + h] * kLog2e;
+
+  const int items = a.N * qblocks;
+  for (int item = share.slot; item < items; item += share.step) {
+    const int n = item / qblocks, qb = item - n * qblocks;
+    const Segment seg(a, n);
+    if (qb * per >= seg.count) continue;
+    const float sc = adjoint_scale<T>(a, b, seg, hk, room), back = 1.f / sc;
+    const int q0 = qb * per + wave * QT * 16;
+    u4 qf[QT][DS], gf[QT][DS];
+    f4 dq[QT][DT];
+    float expo[QT], delta[QT];
+    int qpos[QT];
+    int64_t qrow[QT];
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      const int s = q0 + 16 * qt + c;
+      const bool on = seg.query(a, s);
+      qrow[qt] = on ? seg.row(s) : 0;
+#pragma unroll
+      for (int d = 0; d < DS; ++d) {
+        qf[qt][d] = own_chunk(qcols, a.ldq, qrow[qt], on, d, lane, a.hd);
+        gf[qt][d] = own_chunk(gcols, b.ldg, qrow[qt], on, d, lane, a.hd);
+      }
+      expo[qt] = exponent(a, b, n, h, s, on);
+      if constexpr (DROP) expo[qt] -= log2f(a.drop.scale);
+      delta[qt] = on ? b.delta[qrow[qt] * a.H + h] / a.drop.scale : 0.f;
+      if constexpr (BIAS) qpos[qt] = a.pos[qrow[qt]];
+#pragma unroll
+      for (int j = 0; j < DT; ++j) dq[qt][j] = f4{0.f, 0.f, 0.f, 0.f};
+    }
+    for (int k0 = 0; k0 < seg.count; k0 += kKeys) {
+      const int n_keys = min(kKeys, round_up(seg.count - k0, 32));
+      __syncthreads();
+      const auto live = [&](int s) { return seg.key(a, s); };
+      stage<T, HD>(ks, kcols, a.ldq, seg, k0, n_keys, a.hd, live);
+      stage<T, HD>(vs, vcols, a.ldq, seg, k0, n_keys, a.hd, live);
+      for (int k = threadIdx.x; k < n_keys; k += blockDim.x) {
+        const bool on = live(k0 + k);
+        weight[k] = on ? log_weight(seg.cf(a, k0 + k)) * a.inv2 : -kInf;
+        if constexpr (BIAS) kpos[k] = on ? a.pos[seg.row(k0 + k)] : 0;
+      }
+      __syncthreads();
+      if (q0 >= seg.count) continue;
+      for (int kb = 0; kb < n_keys; kb += 32) {
+        float ds[QT][8];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const int at = kb + 8 * g + 4 * t;
+          f4 s[QT], dp[QT];
+          const f4 w4 = *reinterpret_cast<const f4*>(weight + at);
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt) s[qt] = w4, dp[qt] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int d = 0; d < DS; ++d) {
+            const u4 kf = straight<T, HD>(ks, kb, t, d, lane), vf = straight<T, HD>(vs, kb, t, d, lane);
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt) {
+              s[qt] = mfma<T>(kf, qf[qt][d], s[qt]);
+              dp[qt] = mfma<T>(vf, gf[qt][d], dp[qt]);
+            }
+          }
+          i4 kp{};
+          if constexpr (BIAS) kp = *reinterpret_cast<const i4*>(kpos + at);
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt) {
+            Words w{};
+            if constexpr (DROP)
+              w = a.drop.block(key, uint32_t(qrow[qt]), uint32_t((k0 + at) >> 2) * uint32_t(a.H) + uint32_t(h));
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              float x = -expo[qt];
+              if constexpr (BIAS) x += lut[pair_index(kp[r], qpos[qt], a.reach)];
+              float e = exp2_fast(fmaf(s[qt][r], a.scale2, x));
+              if constexpr (HALF) e *= sc;
+              float kept = e;
+              if constexpr (DROP) kept = Drop::number(w, r) >= a.drop.least ? e : 0.f;
+              ds[qt][4 * t + r] = fmaf(kept, dp[qt][r], -e * delta[qt]);
+            }
+          }
+        }
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) {
+          const u4 df = pack8<T>(ds[qt]);
+#pragma unroll
+          for (int j = 0; j < DT; ++j)
+            dq[qt][j] = mfma<T>(transposed<T, HD>(ks, kb, j >> 1, j & 1, lane), df, dq[qt][j]);
+        }
+      }
+    }
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      const int s = q0 + 16 * qt + c;
+      if (s >= seg.count) continue;
+      T* const row = static_cast<T*>(b.adj) + seg.row(s) * b.lda + h * a.hd;
+#pragma unroll
+      for (int jp = 0; jp < DS; ++jp)
+        put8(row, dq[qt][2 * jp], dq[qt][2 * jp + 1], a.scale * back, 32 * jp + 8 * g, a.hd);
+    }
+  }
+}
+
+// cf_adj[n][k] = beta cf_adj[n][k] + (sum over heads in order of cfh[n][h][k]) / cf (keys that count)
+__global__ __launch_bounds__(256) void typed_cf_kernel(Args a, const float* cfh, float* adj, int64_t lda, float beta) {
+  const int64_t all = int64_t(a.N) * a.S;
+  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < all; i += int64_t(gridDim.x) * 256) {
+    const int64_t n = i / a.S;
+    const int s = int(i - n * a.S);
+    const Segment seg(a, int(n));
+    float sum = 0.f;
+    if (seg.key(a, s)) {
+      for (int h = 0; h < a.H; ++h) sum += cfh[(n * a.H + h) * a.S + s];
+      sum /= seg.cf(a, s);
+    }
+    float* const to = adj + n * lda + s;
+    *to = beta == 0.f ? sum : fmaf(beta, *to, sum);
+  }
+}
+
+// table_adj[b][h] = beta table_adj[b][h] + the workgroups' sums in order: workgroup h, 16 strips of them in double.
+__global__ __launch_bounds__(1024) void typed_table_kernel(const float* part, int slots, int H, int nb, float* adj,
+                                                           float beta) {
+  __shared__ double strips[16][64];
+  const int h = blockIdx.x, b = threadIdx.x & 63, strip = threadIdx.x >> 6;
+  double sum = 0.0;
+  if (b < nb)
+    for (int s = strip; s < slots; s += 16) sum += double(part[(int64_t(s) * H + h) * nb + b]);
+  strips[strip][b] = sum;
+  __syncthreads();
+  if (strip || b >= nb) return;
+  sum = 0.0;
+  for (int i = 0; i < 16; ++i) sum += strips[i][b];
+  float* const to = adj + int64_t(b) * H + h;
+  *to = float(beta == 0.f ? sum : double(beta) * *to + sum);
+}
+
+constexpr size_t aligned(size_t n) { return (n + 255) & ~size_t(255); }
+
+struct Workspace {
+  size_t delta, norms, cfh, part, bytes;
+  Workspace(int dtype, const pet_attn_shape& s, int kv_heads, int nb) {
+    const size_t T = size_t(s.n_rows), H = size_t(s.heads);
+    delta = 0;
+    norms = delta + aligned(T * H * 4);
+    cfh = norms + (dtype == PET_DTYPE_F16 ? aligned(T * (H + size_t(kv_heads)) * 4) : 0);
+    part = cfh + aligned(size_t(s.n_atoms) * H * size_t(s.slots) * 4);
+    bytes = part + aligned(size_t(kMaxSlots) * H * size_t(nb) * 4);
+  }
+};
+
+}  // namespace
+}  // namespace pet_tattn
+
+using namespace pet_tattn;
+
+extern "C" size_t pet_attn_bwd_typed_workspace(int dtype, const pet_attn_shape* shape, int kv_heads, int n_buckets) {
+  if (!shape || (dtype != PET_DTYPE_BF16 && dtype != PET_DTYPE_F16) || kv_heads < 1 || shape->heads < 1 ||
+      shape->heads % kv_heads != 0 || shape->n_atoms < 0 || shape->n_rows < 0 || shape->slots < 1 || n_buckets < 0 ||
+      n_buckets > PET_BIAS_MAX_BUCKETS)
+    return 0;
+  return Workspace(dtype, *shape, kv_heads, n_buckets).bytes;
+}
+
+extern "C" int pet_attn_bwd_typed(int dtype, const pet_attn_shape* shape, int kv_heads, const void* qkv, int64_t ldq,
+                                  const int* off, const void* dmerged, int64_t ldg, const void* merged, int64_t ldm,
+                                  const float* ml, const float* cf_seq, int64_t ldc, const pet_attn_bias* bias,
+                                  const pet_dropout* dropout, void* qkv_adj, int64_t lda, float* cf_seq_adj,
+                                  int64_t ldca, float* table_adj, float beta, void* workspace, size_t workspace_bytes,
+                                  void* stream) {
+  Args a;
+  if (const int e = check_args(dtype, shape, kv_heads, qkv, ldq, off, cf_seq, ldc, bias, dropout, a)) return e;
+  const int D = a.H * a.hd, W = (a.H + 2 * a.Hk) * a.hd;
+  if ((a.T > 0 && (!dmerged || !merged || !qkv_adj)) || (a.N > 0 && !ml) || ldg < D || ldm < D || lda < W) return PET_ATTN_EINVAL;
+  if ((cf_seq_adj && ldca < a.S) || (table_adj && !bias)) return PET_ATTN_EINVAL;
+  for (const void* p : {dmerged, merged, static_cast<const void*>(qkv_adj)})
+    if (!pet_typed::element_aligned(p, dtype)) return PET_ATTN_EALIGN;
+  if ((reinterpret_cast<uintptr_t>(ml) & 7u) != 0 || !pet_typed::element_aligned(cf_seq_adj, PET_DTYPE_F32) ||
+      !pet_typed::element_aligned(table_adj, PET_DTYPE_F32))
+    return PET_ATTN_EALIGN;
+  const Workspace ws(dtype, *shape, kv_heads, a.nb);
+  if (!workspace || workspace_bytes < ws.bytes) return PET_ATTN_EWORKSPACE;
+  if ((reinterpret_cast<uintptr_t>(workspace) & 15u) != 0) return PET_ATTN_EALIGN;
+  const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  char* const base = static_cast<char*>(workspace);
+  Grads b{dmerged, merged, ldg, ldm, ml, qkv_adj, lda, reinterpret_cast<float*>(base + ws.delta),
+          reinterpret_cast<float*>(base + ws.norms), cf_seq_adj ? reinterpret_cast<float*>(base + ws.cfh) : nullptr,
+          table_adj ? reinterpret_cast<float*>(base + ws.part) : nullptr};
+  if (shape->dead && a.T > 0)
+    if (const int e = zero_dead(a, qkv_adj, lda, W, st)) return e;
+  int slots = 0;
+  const int err = a.N == 0 ? int(PET_ATTN_OK) : with_row_type(dtype, [&](auto tv) {
+    using T = decltype(tv);
+    {
+      const int64_t rows = int64_t(a.T) * (a.H + (dtype == PET_DTYPE_F16 ? a.Hk : 0));
+      const auto run = [&](auto lc) {
+        constexpr int LG = decltype(lc)::value;
+        const int64_t blocks = std::min<int64_t>((rows * LG + 255) / 256, 16384);
+        hipLaunchKernelGGL((delta_kernel<T, LG>), dim3(unsigned(blocks)), dim3(256), 0, st, a, b);
+        return hipGetLastError() == hipSuccess ? int(PET_ATTN_OK) : int(PET_ATTN_ELAUNCH);
+      };
+      const int e = a.hd <= 8 ? run(std::integral_constant<int, 1>{}) : a.hd <= 16 ? run(std::integral_constant<int, 2>{})
+                    : a.hd <= 32 ? run(std::integral_constant<int, 4>{}) : a.hd <= 64 ? run(std::integral_constant<int, 8>{})
+                    : run(std::integral_constant<int, 16>{});
+      if (e) return e;
+    }
+    return with_head_dim(a.hd, [&](auto hc) {
+      constexpr int HD = decltype(hc)::value;
+      const auto run = [&](auto bc, auto dc) {
+        constexpr bool BIAS = decltype(bc)::value, DROP = decltype(dc)::value;
+        const int waves = std::min(4, round_up(a.S, 16) / 16), blocks = (a.S + waves * 16 - 1) / (waves * 16);
+        const int64_t items = (int64_t(a.N) * blocks + 7) / 8 * 8;
+        {
+          const auto kernel = typed_bwd_kv_kernel<T, HD, 1, BIAS, DROP>;
+          const size_t bytes = KvLds<HD>::bytes(a, waves, b.part != nullptr);
+          if (const int e = pet_attn::raise_lds(reinterpret_cast<const void*>(kernel), bytes)) return e;
+          slots = int(std::min<int64_t>(items, b.part ? std::clamp(2048 / a.Hk / 8 * 8, 8, kMaxSlots) : kMaxSlots));
+          if (int64_t(slots) * a.Hk * waves * 64 > INT32_MAX) return int(PET_ATTN_EINDEX);
+          hipLaunchKernelGGL(kernel, dim3(unsigned(slots * a.Hk)), dim3(unsigned(waves * 64)), bytes, st, a, b, blocks);
+          if (hipGetLastError() != hipSuccess) return int(PET_ATTN_ELAUNCH);
+        }
+        {
+          const auto kernel = typed_bwd_q_kernel<T, HD, 1, BIAS, DROP>;
+          const size_t bytes = size_t(kQueries) * (2 * kPitch<HD> * 2 + 8) + size_t(waves) * 12 +
+                               (a.table ? size_t(2 * a.reach + 1) * 4 : 0);
+          if (const int e = pet_attn::raise_lds(reinterpret_cast<const void*>(kernel), bytes)) return e;
+          const int64_t q_slots = std::min<int64_t>(items, 2048);
+          if (q_slots * a.H * waves * 64 > INT32_MAX) return int(PET_ATTN_EINDEX);
+          hipLaunchKernelGGL(kernel, dim3(unsigned(q_slots * a.H)), dim3(unsigned(waves * 64)), bytes, st, a, b, blocks);
+          if (hipGetLastError() != hipSuccess) return int(PET_ATTN_ELAUNCH);
+        }
+        return int(PET_ATTN_OK);
+      };
+      if (a.table) return dropout ? run(std::true_type{}, std::true_type{}) : run(std::true_type{}, std::false_type{});
+      return dropout ? run(std::false_type{}, std::true_type{}) : run(std::false_type{}, std::false_type{});
+    });
+  });
+  if (err) return err;
+  if (cf_seq_adj && a.N > 0) {
+    const int64_t blocks = std::min<int64_t>((int64_t(a.N) * a.S + 255) / 256, 16384);
+    hipLaunchKernelGGL(typed_cf_kernel, dim3(unsigned(blocks)), dim3(256), 0, st, a, b.cfh, cf_seq_adj, ldca, beta);
+    if (hipGetLastError() != hipSuccess) return PET_ATTN_ELAUNCH;
+  }
+  if (table_adj) {
+    hipLaunchKernelGGL(typed_table_kernel, dim3(unsigned(a.H)), dim3(1024), 0, st, b.part, slots, a.H, a.nb, table_adj,
+                       beta);
+    if (hipGetLastError() != hipSuccess) return PET_ATTN_ELAUNCH;
+  }
+  return PET_ATTN_OK;
+}

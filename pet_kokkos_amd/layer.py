@@ -11,7 +11,8 @@ tokens' adjoint (atom rows set, live edge rows accumulated).
 
 For training, which the reference does not do: the norms take rows in bfloat16
 and float16 and up to 16384 columns, ``norm_rows_grads`` makes the norm's
-parameters' gradients with its input's adjoint, and ``attention_layer_grads``
+parameters' gradients with its input's adjoint, ``dropout_rows`` drops elements
+onto a residual, and ``attention_layer_grads``
 the gradients of every parameter of an attention block with its backward. All
 work runs in libpet_attn.so on the current torch stream.
 """
@@ -22,8 +23,8 @@ import ctypes
 import torch
 
 from . import _lib
-from .attention import (DTYPES, Tokens, Workspace, _call_on, _live, _mat, _ptr, _scratch, _stream, _typed, _vector,
-                        _weight, shape)
+from .attention import (DTYPES, Dropout, Tokens, Workspace, _call_on, _dropout, _live, _mat, _ptr, _scratch, _stream,
+                        _typed, _vector, _weight, shape)
 
 MAX_WIDTH = 16384  # PET_NORM_MAX_WIDTH
 
@@ -123,6 +124,25 @@ def norm_rows_grads(in_adj: torch.Tensor | None, weight_adj: torch.Tensor | None
     _call_on(dev, "pet_norm_rows_grads", lib.pet_norm_rows_grads, DTYPES[dt], rows, D, _ptr(in_adj), lda, float(beta),
              out_adj.data_ptr(), ldg, inp.data_ptr(), ldi, _vector(weight, "weight", D, dev), int(bool(ln)), w_adj,
              b_adj, float(beta_w), _live(live, dev), ws, nbytes)
+
+
+def dropout_rows(out: torch.Tensor, inp: torch.Tensor, dropout: Dropout, residual: torch.Tensor | None = None,
+                 live: torch.Tensor | None = None) -> None:
+    """out = residual + inp where the dropout keeps an element (times 1 / (1 - p)), out =
+    residual where not; without a residual 0, which makes it its own backward: in_adj
+    from out_adj with the same dropout (the residual's adjoint is out_adj). Rows of any
+    width in float32, bfloat16 or float16; out may be inp or residual. ``live`` (one int32
+    on the device): only rows before it count, the rows after are neither read nor
+    written."""
+    if not isinstance(inp, torch.Tensor) or inp.dim() != 2 or inp.shape[1] < 1:
+        raise ValueError("in must be a row-major 2-D view")
+    if dropout is None:
+        raise TypeError("dropout: a Dropout is needed")
+    (rows, D), dev, dt = inp.shape, inp.device, inp.dtype
+    ldi, ldo = _typed(inp, "in", rows, D, dt, dev), _typed(out, "out", rows, D, dt, dev)
+    ldr = 0 if residual is None else _typed(residual, "residual", rows, D, dt, dev)
+    _call_on(dev, "pet_dropout_rows", _lib.load().pet_dropout_rows, DTYPES[dt], rows, D, out.data_ptr(), ldo,
+             inp.data_ptr(), ldi, _ptr(residual), ldr, _dropout(dropout, dev), _live(live, dev))
 
 
 def attention_layer(ws: Workspace, key: str, out: torch.Tensor, tokens: torch.Tensor, norm_w: torch.Tensor,
