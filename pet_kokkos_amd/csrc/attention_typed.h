@@ -61,9 +61,21 @@ __device__ __forceinline__ u2 lds_tr(const T* p) {
 }
 
 // An LDS row's elements: HD dims and 16 bytes of padding, so that the 16 rows that a
-// wave reads at once start in different banks.
+// wave reads at once start in different banks. Of each 32 dims, the pieces of four go
+// 0 2 4 6 1 3 5 7: those that `transposed` reads for one tile lie side by side (apart, its
+// reads took half of the banks twice), and a product over dims has them in any order
+// that both its operands have.
 template <int HD>
 constexpr int kPitch = HD + 8;
+
+// The most slots whose atoms a workgroup holds whole.
+constexpr int kShort = 128;
+
+// Tokens a stage past that: the registers that hold the next one while the present
+// one is used leave room for the rest at 32 of 128 dims (at 64, 200 to 400 bytes a lane
+// of the kernels' were spilled).
+template <int HD>
+constexpr int kStage = HD == 128 ? 32 : 64;
 
 // Where token k of a stage lies: of each 32, tokens 8a + 4t + r at row 16t + 4a + r.
 __device__ __forceinline__ int lds_row(int k) {
@@ -75,7 +87,7 @@ __device__ __forceinline__ int lds_row(int k) {
 template <class T, int HD>
 __device__ __forceinline__ u4 transposed(const T* rows, int base, int jp, int t, int lane) {
   const int i = lane & 15, g = lane >> 4;
-  const T* p = rows + (base + 4 * g + (i >> 2)) * kPitch<HD> + 32 * jp + 8 * (i & 3) + 4 * t;
+  const T* p = rows + (base + 4 * g + (i >> 2)) * kPitch<HD> + 32 * jp + 16 * t + 4 * (i & 3);
   const u2 lo = lds_tr(p), hi = lds_tr(p + 16 * kPitch<HD>);
   return u4{lo[0], lo[1], hi[0], hi[1]};
 }
@@ -83,6 +95,13 @@ __device__ __forceinline__ u4 transposed(const T* rows, int base, int jp, int t,
 template <class T, int HD>
 __device__ __forceinline__ u4 straight(const T* rows, int base, int t, int step, int lane) {
   return *reinterpret_cast<const u4*>(rows + (base + 16 * t + (lane & 15)) * kPitch<HD> + 32 * step + 8 * (lane >> 4));
+}
+// Dims 8 ch .. + 7 of a row into its place.
+template <class T>
+__device__ __forceinline__ void put_piece(T* row, int ch, const u4& x) {
+  T* const at = row + 32 * (ch >> 2) + 4 * (ch & 3);
+  *reinterpret_cast<u2*>(at) = u2{x[0], x[1]};
+  *reinterpret_cast<u2*>(at + 16) = u2{x[2], x[3]};
 }
 
 template <class T>
@@ -106,6 +125,7 @@ struct Args {
   const int* pos;             // [T]
   int nb, reach;
   Drop drop;
+  bool whole;  // head_dim in pieces of 8, and a segment's offsets in 32 bits
 };
 
 // Atom n's tokens. Counts past S or past the rows would be the caller's error; they
@@ -132,29 +152,157 @@ struct Segment {
 // Dims d .. d + 7 of a row of hd, zeros past its end.
 template <class T>
 __device__ __forceinline__ u4 row_chunk(const T* row, int d, int hd) {
-  return __builtin_bit_cast(u4, (hd & 7) == 0 ? pet_typed::load_raw<T, true>(row, d, hd) : pet_typed::load_raw<T>(row, d, hd));
+  return __builtin_bit_cast(u4, pet_typed::load_raw<T>(row, d, hd));
 }
 
-// Slots s0 .. s0 + n - 1 (n a multiple of 32) of the columns at src into LDS rows,
-// zeros where `live` says no: nothing that a masked row holds is ever multiplied.
-template <class T, int HD, class Live>
-__device__ __forceinline__ void stage(T* rows, const T* src, int64_t ld, const Segment& seg, int s0, int n, int hd,
-                                      const Live& live) {
+// A column of a matrix over an atom's tokens: the row of slot 0, that of slot 1 (less a
+// row), and the rows' distance in bytes.
+struct Column {
+  const char *own, *edges;
+  uint32_t ld;
+  template <class T>
+  __device__ __forceinline__ Column(const T* src, int64_t ld_, const Segment& seg)
+      : own(reinterpret_cast<const char*>(src + int64_t(seg.n) * ld_)),
+        edges(reinterpret_cast<const char*>(src + seg.edge * ld_)), ld(uint32_t(ld_ * sizeof(T))) {}
+  // dims d .. of slot s (both there), where Args::whole
+  __device__ __forceinline__ const char* at(int s, int d) const {
+    const char* const p = s == 0 ? own : edges;
+    return p + uint32_t(__umul24(uint32_t(s), ld) + 2u * uint32_t(d));
+  }
+};
+typedef unsigned u2e __attribute__((ext_vector_type(2), aligned(2)));
+
+__device__ __forceinline__ u4 where(bool on, const u4& x) {
+  return u4{on ? x[0] : 0u, on ? x[1] : 0u, on ? x[2] : 0u, on ? x[3] : 0u};
+}
+
+// Two columns of slots s0 .. s0 + n - 1 (n a multiple of 32), keys and values or queries
+// and adjoints, into LDS rows, zeros where the slot's weight says that it is left out:
+// nothing that a masked row holds is ever multiplied. EACH pieces of both a thread are
+// loaded at once, without a branch (one that is not wanted is of a place that is there).
+// more(slot, dim): what else is loaded with a piece; take(row k, chunk, x, y, on, that).
+template <class T, int HD, int EACH, bool QUERY, class More, class Take>
+__device__ __forceinline__ void stage_pair(const Args& a, T* xs, const T* xsrc, int64_t ldx, T* ys, const T* ysrc,
+                                           int64_t ldy, const Segment& seg, int s0, int n, const More& more,
+                                           const Take& take) {
   constexpr int CH = HD / 8;
-  for (int i = threadIdx.x; i < n * CH; i += blockDim.x) {
-    const int k = i / CH, ch = i % CH, s = s0 + k;
-    u4 x = {0u, 0u, 0u, 0u};
-    if (live(s)) x = row_chunk(src + seg.row(s) * ld, 8 * ch, hd);
-    *reinterpret_cast<u4*>(rows + lds_row(k) * kPitch<HD> + 8 * ch) = x;
+  const int nt = blockDim.x, total = n * CH, last = seg.count - 1;
+  const Column xc(xsrc, ldx, seg), yc(ysrc, ldy, seg);
+  for (int i0 = threadIdx.x; i0 < total; i0 += EACH * nt) {
+    u4 x[EACH], y[EACH];
+    bool on[EACH];
+    decltype(more(0, 0)) m[EACH];
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+      const int i = i0 + j * nt, s = s0 + i / CH, ch = 8 * (i % CH), at = s < last ? s : last;
+      if (a.whole) {
+        const float w = seg.cf(a, at);
+        const int d = ch < a.hd ? ch : 0;
+        x[j] = __builtin_bit_cast(u4, *reinterpret_cast<const u4e*>(xc.at(at, d)));
+        y[j] = __builtin_bit_cast(u4, *reinterpret_cast<const u4e*>(yc.at(at, d)));
+        m[j] = more(at, d);
+        on[j] = s <= last && ch < a.hd && (w > 0.f || (QUERY && s == 0));
+      } else {
+        on[j] = QUERY ? seg.query(a, s) : seg.key(a, s);
+        x[j] = y[j] = u4{0u, 0u, 0u, 0u};
+        if (on[j]) {
+          x[j] = row_chunk(xsrc + seg.row(s) * ldx, ch, a.hd), y[j] = row_chunk(ysrc + seg.row(s) * ldy, ch, a.hd);
+          m[j] = more(s, ch);
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+      const int i = i0 + j * nt, k = i / CH;
+      if (i < total) {
+        x[j] = where(on[j], x[j]), y[j] = where(on[j], y[j]);
+        const int row = lds_row(k) * kPitch<HD>;
+        put_piece(xs + row, i % CH, x[j]);
+        put_piece(ys + row, i % CH, y[j]);
+        take(k, i % CH, x[j], y[j], on[j], m[j]);
+      }
+    }
   }
 }
 
-// A lane's B operand of a token's own columns: dims 32 step + 8g .. + 7.
-template <class T>
-__device__ __forceinline__ u4 own_chunk(const T* src, int64_t ld, int64_t row, bool live, int step, int lane, int hd) {
-  u4 x = {0u, 0u, 0u, 0u};
-  if (live) x = row_chunk(src + row * ld, 32 * step + 8 * (lane >> 4), hd);
-  return x;
+// The same for kernels of 256 threads that go over stages of KS slots: the loads of the
+// next stage go out before the present one is used (where Args::whole; else they are
+// loaded as they are stored, and the registers of the main path stay few).
+template <class T, int HD, int KS, bool QUERY>
+struct Ahead {
+  static constexpr int CH = HD / 8, EACH = KS * CH / 256;
+  u4 x[EACH], y[EACH];
+  bool on[EACH];
+  __device__ __forceinline__ void load(const Args& a, const T* xsrc, int64_t ldx, const T* ysrc, int64_t ldy,
+                                       const Segment& seg, int s0) {
+    if (!a.whole) return;
+    const int last = seg.count - 1;
+    const Column xc(xsrc, ldx, seg), yc(ysrc, ldy, seg);
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+      const int i = threadIdx.x + 256 * j, s = s0 + i / CH, ch = 8 * (i % CH), at = s < last ? s : last;
+      const int d = ch < a.hd ? ch : 0;
+      const float w = seg.cf(a, at);
+      x[j] = __builtin_bit_cast(u4, *reinterpret_cast<const u4e*>(xc.at(at, d)));
+      y[j] = __builtin_bit_cast(u4, *reinterpret_cast<const u4e*>(yc.at(at, d)));
+      on[j] = s <= last && ch < a.hd && (w > 0.f || (QUERY && s == 0));
+    }
+  }
+  __device__ __forceinline__ void store(const Args& a, T* xs, const T* xsrc, int64_t ldx, T* ys, const T* ysrc,
+                                        int64_t ldy, const Segment& seg, int s0) const {
+    if (!a.whole) {
+#pragma unroll 1
+      for (int i = threadIdx.x; i < KS * CH; i += 256) {
+        const int s = s0 + i / CH, d = 8 * (i % CH), row = lds_row(i / CH) * kPitch<HD>;
+        u4 u = {0u, 0u, 0u, 0u}, v = u;
+        if (QUERY ? seg.query(a, s) : seg.key(a, s)) {
+          u = row_chunk(xsrc + seg.row(s) * ldx, d, a.hd);
+          v = row_chunk(ysrc + seg.row(s) * ldy, d, a.hd);
+        }
+        put_piece(xs + row, i % CH, u);
+        put_piece(ys + row, i % CH, v);
+      }
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+      const int i = threadIdx.x + 256 * j, row = lds_row(i / CH) * kPitch<HD>;
+      put_piece(xs + row, i % CH, where(on[j], x[j]));
+      put_piece(ys + row, i % CH, where(on[j], y[j]));
+    }
+  }
+};
+
+// A lane's B operands of a token's own columns (slot s, zeros unless live): of dims 32
+// step .. + 31 the pieces that lie at 8g of an LDS row.
+template <class T, int DS>
+__device__ __forceinline__ void own_pieces(const Args& a, const T* src, int64_t ld, const Segment& seg, int s, bool live,
+                                           int lane, u4 (&out)[DS]) {
+  const int g = lane >> 4, d0 = 16 * (g & 1) + 4 * (g >> 1);
+  if (a.whole) {
+    const Column col(src, ld, seg);
+    const int at = s < seg.count ? s : 0;
+#pragma unroll
+    for (int step = 0; step < DS; ++step) {
+      const int d = 32 * step + d0;
+      const u2 lo = __builtin_bit_cast(u2, *reinterpret_cast<const u2e*>(col.at(at, d < a.hd ? d : 0)));
+      const u2 hi = __builtin_bit_cast(u2, *reinterpret_cast<const u2e*>(col.at(at, d + 8 < a.hd ? d + 8 : 0)));
+      const bool l = live && d < a.hd, h = live && d + 8 < a.hd;
+      out[step] = u4{l ? lo[0] : 0u, l ? lo[1] : 0u, h ? hi[0] : 0u, h ? hi[1] : 0u};
+    }
+  } else {
+#pragma unroll
+    for (int step = 0; step < DS; ++step) {
+      out[step] = u4{0u, 0u, 0u, 0u};
+      if (live)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int d = 32 * step + d0 + 8 * (e >> 2) + (e & 3);
+          if (d < a.hd)
+            out[step][e >> 1] |= unsigned(__builtin_bit_cast(unsigned short, src[seg.row(s) * ld + d])) << (16 * (e & 1));
+        }
+    }
+  }
 }
 
 // A row's eight dims 32 jp + 8g of a result's tile pair, times f.
@@ -202,6 +350,8 @@ struct Share {
 // Arguments that forward and backward share; fills `a`.
 int check_args(int dtype, const pet_attn_shape* sh, int kv_heads, const void* qkv, int64_t ldq, const int* off,
                const float* cf_seq, int64_t ldc, const pet_attn_bias* bias, const pet_dropout* dropout, Args& a);
+
+bool narrow(const Args& a, int64_t ld);
 
 // Rows N + off[N] .. T - 1 of x set to zero.
 int zero_dead(const Args& a, void* x, int64_t ld, int width, hipStream_t st);

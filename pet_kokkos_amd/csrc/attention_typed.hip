@@ -21,18 +21,163 @@ namespace {
 template <int HD>
 constexpr int fwd_stage_bytes(int keys) { return keys * (2 * kPitch<HD> * 2 + 8); }
 
-template <class T, int HD, int QT, bool BIAS, bool DROP>
-__global__ __launch_bounds__(512) void typed_fwd_kernel(Args a, int keys, int qblocks, T* merged, int64_t ldm,
-                                                        float* ml) {
+// The tiles of 16 queries at q[], QT of them, against staged keys kb .. kb + 32 U - 1
+// (slots k0 + kb ..; those past n_keys do not count): scores, the running maximum and sum,
+// and the products with the values onto o.
+template <class T, int HD, int QT, int U, bool BIAS, bool DROP>
+struct Tiles {
+  static constexpr int DS = HD / 32, DT = HD / 16;
+  u4 qf[QT][DS];
+  f4 o[QT][DT];
+  float top[QT], sum[QT];
+  int64_t row[QT];
+  int pos[QT];
+  bool live[QT];
+
+  __device__ __forceinline__ void start(const Args& a, const T* qcols, const Segment& seg, int q0, int lane) {
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      const int s = q0 + 16 * qt + (lane & 15);
+      live[qt] = seg.query(a, s);
+      row[qt] = live[qt] ? seg.row(s) : 0;
+      own_pieces(a, qcols, a.ldq, seg, s, live[qt], lane, qf[qt]);
+      if constexpr (BIAS) pos[qt] = a.pos[row[qt]];
+#pragma unroll
+      for (int j = 0; j < DT; ++j) o[qt][j] = f4{0.f, 0.f, 0.f, 0.f};
+      top[qt] = -kInf, sum[qt] = 0.f;
+    }
+  }
+
+  __device__ __forceinline__ void keys(const Args& a, const Words& key, int h, const T* ks, const T* vs,
+                                       const float* weight, const int* kpos, const float* lut, int k0, int kb, int n_keys,
+                                       int lane) {
+    const int g = lane >> 4;
+    f4 s[QT][U][2];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (kb + 32 * u >= n_keys) {
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) s[qt][u][0] = s[qt][u][1] = f4{-kInf, -kInf, -kInf, -kInf};
+        continue;
+      }
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int at = kb + 32 * u + 8 * g + 4 * t;
+        const f4 w = *reinterpret_cast<const f4*>(weight + at);
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) s[qt][u][t] = w;
+#pragma unroll
+        for (int d = 0; d < DS; ++d) {
+          const u4 kf = straight<T, HD>(ks, kb + 32 * u, t, d, lane);
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt) s[qt][u][t] = mfma<T>(kf, qf[qt][d], s[qt][u][t]);
+        }
+        if constexpr (BIAS) {
+          const i4 kp = *reinterpret_cast<const i4*>(kpos + at);
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              s[qt][u][t][r] = fmaf(s[qt][u][t][r], a.scale2, lut[pair_index(kp[r], pos[qt], a.reach)]);
+        }
+      }
+    }
+    const float f = BIAS ? 1.f : a.scale2;
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      float m = -kInf;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) m = fmaxf(m, s[qt][u][t][r]);
+      const float now = fmaxf(top[qt], pet_attn::max_g(m) * f);
+      const float base = now == -kInf ? 0.f : now;
+      if (k0 + kb > 0) {
+        const float fade = exp2_fast(top[qt] - base);
+        sum[qt] *= fade;
+#pragma unroll
+        for (int j = 0; j < DT; ++j) o[qt][j] *= fade;
+      }
+      top[qt] = now;
+      u4 pf[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (u > 0 && kb + 32 * u >= n_keys) continue;
+        float p[8];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          Words w{};
+          if constexpr (DROP)
+            w = a.drop.block(key, uint32_t(row[qt]),
+                             uint32_t((k0 + kb + 32 * u + 8 * g + 4 * t) >> 2) * uint32_t(a.H) + uint32_t(h));
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float x = s[qt][u][t][r];
+            float e = exp2_fast(BIAS ? x - base : fmaf(x, f, -base));
+            sum[qt] += e;
+            if constexpr (DROP) e = Drop::number(w, r) >= a.drop.least ? e : 0.f;
+            p[4 * t + r] = e;
+          }
+        }
+        pf[u] = pack8<T>(p);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (u > 0 && kb + 32 * u >= n_keys) continue;
+#pragma unroll
+        for (int j = 0; j < DT; ++j)
+          o[qt][j] = mfma<T>(transposed<T, HD>(vs, kb + 32 * u, j >> 1, j & 1, lane), pf[u], o[qt][j]);
+      }
+    }
+  }
+
+  __device__ __forceinline__ void finish(const Args& a, const Segment& seg, int h, int q0, int lane, T* merged,
+                                         int64_t ldm, float* ml) {
+    const int c = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      const int s = q0 + 16 * qt + c;
+      const float l = pet_attn::sum_g(sum[qt]);
+      const bool some = live[qt] && l != 0.f;
+      const float inv = some ? 1.f / l : 0.f;
+      if (ml && g == 0 && s < a.S)
+        *reinterpret_cast<float2*>(ml + ((int64_t(seg.n) * a.H + h) * a.S + s) * 2) =
+            make_float2(some ? top[qt] * kLn2 : 0.f, inv);
+      if (s < seg.count) {
+        T* const to = merged + seg.row(s) * ldm + h * a.hd;
+        const float f = DROP ? inv * a.drop.scale : inv;
+#pragma unroll
+        for (int jp = 0; jp < DS; ++jp) {
+          f4 lo = o[qt][2 * jp], hi = o[qt][2 * jp + 1];
+          if (!some) lo = hi = f4{0.f, 0.f, 0.f, 0.f};
+          put8(to, lo, hi, f, 32 * jp + 8 * g, a.hd);
+        }
+      }
+    }
+  }
+};
+
+__device__ __forceinline__ void fill_lut(const Args& a, float* lut, int h) {
+  for (int i = threadIdx.x; i <= 2 * a.reach; i += blockDim.x)
+    lut[i] = a.table[int64_t(bucket_of(a, i)) * a.H + h] * kLog2e;
+}
+
+// Up to 128 slots: an item is an atom, all of its keys staged at once, its tiles of
+// queries dealt to the workgroup's waves (4 from 33 slots on: a workgroup's waves start
+// at one SIMD, and 5 of them, one a tile of 71 slots, left room for no third workgroup
+// on the CU; which wave has the odd tile goes round by the atom).
+template <class T, int HD, bool BIAS, bool DROP>
+__global__ __launch_bounds__(256, HD == 128 ? 2 : 4) void typed_fwd_short_kernel(Args a, int keys, T* merged, int64_t ldm,
+                                                                                float* ml) {
   extern __shared__ __align__(16) char lds[];
-  constexpr int DS = HD / 32, DT = HD / 16;
   T* const ks = reinterpret_cast<T*>(lds);
   T* const vs = ks + keys * kPitch<HD>;
   float* const weight = reinterpret_cast<float*>(vs + keys * kPitch<HD>);
   int* const kpos = reinterpret_cast<int*>(weight + keys);
   float* const lut = reinterpret_cast<float*>(kpos + keys);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
-  const int per = int(blockDim.x >> 6) * QT * 16;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = int(blockDim.x >> 6);
   const Share share(a.H);
   const int h = share.head, hk = h / (a.H / a.Hk);
   const T* const qkv = static_cast<const T*>(a.qkv);
@@ -41,147 +186,86 @@ __global__ __launch_bounds__(512) void typed_fwd_kernel(Args a, int keys, int qb
   const T* const vcols = qkv + (a.H + a.Hk + hk) * a.hd;
   Words key{};
   if constexpr (DROP) key = a.drop.key();
-  if constexpr (BIAS)
-    for (int i = threadIdx.x; i <= 2 * a.reach; i += blockDim.x)
-      lut[i] = a.table[int64_t(bucket_of(a, i)) * a.H + h] * kLog2e;
+  if constexpr (BIAS) fill_lut(a, lut, h);
+  for (int n = share.slot; n < a.N; n += share.step) {
+    const Segment seg(a, n);
+    const int n_keys = round_up(seg.count, 32);
+    __syncthreads();
+    for (int k = threadIdx.x; k < n_keys; k += blockDim.x) {
+      const bool there = k < seg.count;
+      const float w = there ? seg.cf(a, k) : 0.f;
+      weight[k] = w > 0.f ? log_weight(w) * a.inv2 : -kInf;
+      if constexpr (BIAS) kpos[k] = there ? a.pos[seg.row(k)] : 0;
+    }
+    stage_pair<T, HD, 2, false>(a, ks, kcols, a.ldq, vs, vcols, a.ldq, seg, 0, n_keys, [](int, int) { return 0; },
+                                [](int, int, const u4&, const u4&, bool, int) {});
+    __syncthreads();
+    const int tiles = (seg.count + 15) >> 4, slots = (a.S + 15) >> 4;
+    for (int tile = (wave + n) & (waves - 1); tile < slots; tile += waves) {
+      Tiles<T, HD, 1, 2, BIAS, DROP> q;
+      q.start(a, qcols, seg, 16 * tile, lane);
+      if (tile < tiles)
+        for (int kb = 0; kb < n_keys; kb += 64) q.keys(a, key, h, ks, vs, weight, kpos, lut, 0, kb, n_keys, lane);
+      q.finish(a, seg, h, 16 * tile, lane, merged, ldm, ml);
+    }
+  }
+}
 
+// Past 128 slots: an item is an atom's 128 queries, two tiles a wave, and the keys come in
+// stages, the next one's loads on their way while the present one is used.
+template <class T, int HD, bool BIAS, bool DROP>
+__global__ __launch_bounds__(256, 2) void typed_fwd_long_kernel(Args a, int qblocks, T* merged, int64_t ldm, float* ml) {
+  extern __shared__ __align__(16) char lds[];
+  constexpr int KS = kStage<HD>, QT = 2, per = 4 * QT * 16;
+  T* const ks = reinterpret_cast<T*>(lds);
+  T* const vs = ks + KS * kPitch<HD>;
+  float* const weight = reinterpret_cast<float*>(vs + KS * kPitch<HD>);
+  int* const kpos = reinterpret_cast<int*>(weight + KS);
+  float* const lut = reinterpret_cast<float*>(kpos + KS);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const Share share(a.H);
+  const int h = share.head, hk = h / (a.H / a.Hk);
+  const T* const qkv = static_cast<const T*>(a.qkv);
+  const T* const qcols = qkv + h * a.hd;
+  const T* const kcols = qkv + (a.H + hk) * a.hd;
+  const T* const vcols = qkv + (a.H + a.Hk + hk) * a.hd;
+  Words key{};
+  if constexpr (DROP) key = a.drop.key();
+  if constexpr (BIAS) fill_lut(a, lut, h);
   const int items = a.N * qblocks;
   for (int item = share.slot; item < items; item += share.step) {
     const int n = item / qblocks, qb = item - n * qblocks;
     const Segment seg(a, n);
     const int q0 = qb * per + wave * QT * 16;
-    // the wave's queries
-    u4 qf[QT][DS];
-    int64_t qrow[QT];
-    int qpos[QT];
-    bool qlive[QT];
-    f4 o[QT][DT];
-    float top[QT], sum[QT];
-#pragma unroll
-    for (int qt = 0; qt < QT; ++qt) {
-      const int s = q0 + 16 * qt + c;
-      qlive[qt] = seg.query(a, s);
-      qrow[qt] = qlive[qt] ? seg.row(s) : 0;
-#pragma unroll
-      for (int d = 0; d < DS; ++d) qf[qt][d] = own_chunk(qcols, a.ldq, qrow[qt], qlive[qt], d, lane, a.hd);
-      if constexpr (BIAS) qpos[qt] = a.pos[qrow[qt]];
-#pragma unroll
-      for (int j = 0; j < DT; ++j) o[qt][j] = f4{0.f, 0.f, 0.f, 0.f};
-      top[qt] = -kInf, sum[qt] = 0.f;
-    }
-    if (qb * per < seg.count)  // (the same for the whole workgroup)
-      for (int k0 = 0; k0 < seg.count; k0 += keys) {
-        const int n_keys = min(keys, round_up(seg.count - k0, 32));
+    Tiles<T, HD, QT, KS / 32, BIAS, DROP> q;
+    q.start(a, qcols, seg, q0, lane);
+    Ahead<T, HD, KS, false> ahead;
+    float next_weight = 0.f;
+    int next_pos = 0;
+    const auto load = [&](int k0) {
+      ahead.load(a, kcols, a.ldq, vcols, a.ldq, seg, k0);
+      if (threadIdx.x < KS) {
+        const int k = k0 + int(threadIdx.x);
+        next_weight = k < seg.count ? seg.cf(a, k) : 0.f;
+        if constexpr (BIAS) next_pos = k < seg.count ? a.pos[seg.row(k)] : 0;
+      }
+    };
+    if (qb * per < seg.count) {  // (the same for the whole workgroup)
+      load(0);
+      for (int k0 = 0; k0 < seg.count; k0 += KS) {
         __syncthreads();
-        const auto live = [&](int s) { return seg.key(a, s); };
-        stage<T, HD>(ks, kcols, a.ldq, seg, k0, n_keys, a.hd, live);
-        stage<T, HD>(vs, vcols, a.ldq, seg, k0, n_keys, a.hd, live);
-        for (int k = threadIdx.x; k < n_keys; k += blockDim.x) {
-          const bool on = live(k0 + k);
-          weight[k] = on ? log_weight(seg.cf(a, k0 + k)) * a.inv2 : -kInf;
-          if constexpr (BIAS) kpos[k] = on ? a.pos[seg.row(k0 + k)] : 0;
+        ahead.store(a, ks, kcols, a.ldq, vs, vcols, a.ldq, seg, k0);
+        if (threadIdx.x < KS) {
+          weight[threadIdx.x] = next_weight > 0.f ? log_weight(next_weight) * a.inv2 : -kInf;
+          if constexpr (BIAS) kpos[threadIdx.x] = next_pos;
         }
         __syncthreads();
-        if (q0 >= seg.count) continue;
-        for (int kb = 0; kb < n_keys; kb += 64) {
-          f4 s[QT][2][2];
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            if (kb + 32 * u >= n_keys) {
-#pragma unroll
-              for (int qt = 0; qt < QT; ++qt) s[qt][u][0] = s[qt][u][1] = f4{-kInf, -kInf, -kInf, -kInf};
-              continue;
-            }
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-              const int at = kb + 32 * u + 8 * g + 4 * t;
-              const f4 w = *reinterpret_cast<const f4*>(weight + at);
-#pragma unroll
-              for (int qt = 0; qt < QT; ++qt) s[qt][u][t] = w;
-#pragma unroll
-              for (int d = 0; d < DS; ++d) {
-                const u4 kf = straight<T, HD>(ks, kb + 32 * u, t, d, lane);
-#pragma unroll
-                for (int qt = 0; qt < QT; ++qt) s[qt][u][t] = mfma<T>(kf, qf[qt][d], s[qt][u][t]);
-              }
-              if constexpr (BIAS) {
-                const i4 kp = *reinterpret_cast<const i4*>(kpos + at);
-#pragma unroll
-                for (int qt = 0; qt < QT; ++qt)
-#pragma unroll
-                  for (int r = 0; r < 4; ++r)
-                    s[qt][u][t][r] = fmaf(s[qt][u][t][r], a.scale2, lut[pair_index(kp[r], qpos[qt], a.reach)]);
-              }
-            }
-          }
-          const float f = BIAS ? 1.f : a.scale2;
-#pragma unroll
-          for (int qt = 0; qt < QT; ++qt) {
-            float m = -kInf;
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-              for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) m = fmaxf(m, s[qt][u][t][r]);
-            const float now = fmaxf(top[qt], pet_attn::max_g(m) * f);
-            const float base = now == -kInf ? 0.f : now;
-            const float fade = exp2_fast(top[qt] - base);
-            top[qt] = now;
-            sum[qt] *= fade;
-#pragma unroll
-            for (int j = 0; j < DT; ++j) o[qt][j] *= fade;
-            u4 pf[2];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              float p[8];
-#pragma unroll
-              for (int t = 0; t < 2; ++t) {
-                Words w{};
-                if constexpr (DROP)
-                  w = a.drop.block(key, uint32_t(qrow[qt]),
-                                   uint32_t((k0 + kb + 32 * u + 8 * g + 4 * t) >> 2) * uint32_t(a.H) + uint32_t(h));
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                  const float x = s[qt][u][t][r];
-                  float e = exp2_fast(BIAS ? x - base : fmaf(x, f, -base));
-                  sum[qt] += e;
-                  if constexpr (DROP) e = Drop::number(w, r) >= a.drop.least ? e : 0.f;
-                  p[4 * t + r] = e;
-                }
-              }
-              pf[u] = pack8<T>(p);
-            }
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              if (kb + 32 * u >= n_keys) continue;
-#pragma unroll
-              for (int j = 0; j < DT; ++j)
-                o[qt][j] = mfma<T>(transposed<T, HD>(vs, kb + 32 * u, j >> 1, j & 1, lane), pf[u], o[qt][j]);
-            }
-          }
-        }
-      }
-#pragma unroll
-    for (int qt = 0; qt < QT; ++qt) {
-      const int s = q0 + 16 * qt + c;
-      const float l = pet_attn::sum_g(sum[qt]);
-      const bool some = qlive[qt] && l != 0.f;
-      const float inv = some ? 1.f / l : 0.f;
-      if (ml && g == 0 && s < a.S)
-        *reinterpret_cast<float2*>(ml + ((int64_t(n) * a.H + h) * a.S + s) * 2) =
-            make_float2(some ? top[qt] * kLn2 : 0.f, inv);
-      if (s < seg.count) {
-        T* const row = merged + seg.row(s) * ldm + h * a.hd;
-        const float f = DROP ? inv * a.drop.scale : inv;
-#pragma unroll
-        for (int jp = 0; jp < DS; ++jp) {
-          f4 lo = o[qt][2 * jp], hi = o[qt][2 * jp + 1];
-          if (!some) lo = hi = f4{0.f, 0.f, 0.f, 0.f};
-          put8(row, lo, hi, f, 32 * jp + 8 * g, a.hd);
-        }
+        if (k0 + KS < seg.count) load(k0 + KS);
+        if (q0 < seg.count)
+          q.keys(a, key, h, ks, vs, weight, kpos, lut, k0, 0, min(KS, round_up(seg.count - k0, 32)), lane);
       }
     }
+    q.finish(a, seg, h, q0, lane, merged, ldm, ml);
   }
 }
 
@@ -201,6 +285,9 @@ int zero_dead(const Args& a, void* x, int64_t ld, int width, hipStream_t st) {
                      width, static_cast<u16*>(x), ld);
   return hipGetLastError() == hipSuccess ? PET_ATTN_OK : PET_ATTN_ELAUNCH;
 }
+
+// Whether a segment's offsets of a matrix are the product of 24-bit numbers under 2^32.
+bool narrow(const Args& a, int64_t ld) { return ld < (1 << 23) && a.S < (1 << 24) && int64_t(a.S) * ld * 2 < INT64_C(1) << 32; }
 
 int check_args(int dtype, const pet_attn_shape* sh, int kv_heads, const void* qkv, int64_t ldq, const int* off,
                const float* cf_seq, int64_t ldc, const pet_attn_bias* bias, const pet_dropout* dropout, Args& a) {
@@ -236,6 +323,7 @@ int check_args(int dtype, const pet_attn_shape* sh, int kv_heads, const void* qk
   a.qkv = qkv, a.ldq = ldq, a.off = off, a.cf = cf_seq, a.ldc = ldc;
   a.N = sh->n_atoms, a.T = sh->n_rows, a.S = sh->slots, a.H = sh->heads, a.Hk = kv_heads, a.hd = sh->head_dim;
   a.scale = sh->scale, a.scale2 = scale2, a.inv2 = 1.f / scale2;
+  a.whole = a.hd % 8 == 0 && narrow(a, ldq);
   return PET_ATTN_OK;
 }
 
@@ -260,25 +348,30 @@ extern "C" int pet_attn_fwd_typed(int dtype, const pet_attn_shape* shape, int kv
     using T = decltype(tv);
     return with_head_dim(a.hd, [&](auto hc) {
       constexpr int HD = decltype(hc)::value;
-      const auto run = [&](auto qc, auto bc, auto dc) {
-        constexpr int QT = decltype(qc)::value;
-        const auto kernel = typed_fwd_kernel<T, HD, QT, decltype(bc)::value, decltype(dc)::value>;
-        const int waves = QT == 1 ? std::min(8, round_up(a.S, 16) / 16) : 4;
-        const int qblocks = (a.S + waves * QT * 16 - 1) / (waves * QT * 16);
-        const int keys = a.S <= 64 ? round_up(a.S, 32) : QT == 1 ? 128 : 64;
-        const size_t bytes = size_t(fwd_stage_bytes<HD>(keys)) + (a.table ? size_t(2 * a.reach + 1) * 4 : 0);
-        if (const int e = pet_attn::raise_lds(reinterpret_cast<const void*>(kernel), bytes)) return e;
-        const int64_t slots = std::min<int64_t>((int64_t(a.N) * qblocks + 7) / 8 * 8, 2048);
-        if (slots * a.H * waves * 64 > INT32_MAX) return int(PET_ATTN_EINDEX);
-        hipLaunchKernelGGL(kernel, dim3(unsigned(slots * a.H)), dim3(unsigned(waves * 64)), bytes, st, a, keys, qblocks,
-                           static_cast<T*>(merged), ldm, ml);
+      const auto run = [&](auto bc, auto dc) {
+        constexpr bool BIAS = decltype(bc)::value, DROP = decltype(dc)::value;
+        const size_t lut = a.table ? size_t(2 * a.reach + 1) * 4 : 0;
+        const int64_t qblocks = a.S <= kShort ? 1 : (int64_t(a.S) + 127) / 128;
+        const int64_t slots = std::min<int64_t>((a.N * qblocks + 7) / 8 * 8, 2048);
+        if (slots * a.H * 256 > INT32_MAX) return int(PET_ATTN_EINDEX);
+        if (a.S <= kShort) {
+          const auto kernel = typed_fwd_short_kernel<T, HD, BIAS, DROP>;
+          const int keys = round_up(a.S, 32);
+          const size_t bytes = size_t(fwd_stage_bytes<HD>(keys)) + lut;
+          if (const int e = pet_attn::raise_lds(reinterpret_cast<const void*>(kernel), bytes)) return e;
+          hipLaunchKernelGGL(kernel, dim3(unsigned(slots * a.H)), dim3(a.S <= 16 ? 64 : a.S <= 32 ? 128 : 256), bytes, st, a,
+                             keys, static_cast<T*>(merged), ldm, ml);
+        } else {
+          const auto kernel = typed_fwd_long_kernel<T, HD, BIAS, DROP>;
+          const size_t bytes = size_t(fwd_stage_bytes<HD>(kStage<HD>)) + lut;
+          if (const int e = pet_attn::raise_lds(reinterpret_cast<const void*>(kernel), bytes)) return e;
+          hipLaunchKernelGGL(kernel, dim3(unsigned(slots * a.H)), dim3(256), bytes, st, a, int(qblocks),
+                             static_cast<T*>(merged), ldm, ml);
+        }
         return hipGetLastError() == hipSuccess ? int(PET_ATTN_OK) : int(PET_ATTN_ELAUNCH);
       };
-      const auto pick = [&](auto qc) {
-        if (a.table) return dropout ? run(qc, std::true_type{}, std::true_type{}) : run(qc, std::true_type{}, std::false_type{});
-        return dropout ? run(qc, std::false_type{}, std::true_type{}) : run(qc, std::false_type{}, std::false_type{});
-      };
-      return a.S <= 128 ? pick(std::integral_constant<int, 1>{}) : pick(std::integral_constant<int, 2>{});
+      if (a.table) return dropout ? run(std::true_type{}, std::true_type{}) : run(std::true_type{}, std::false_type{});
+      return dropout ? run(std::false_type{}, std::true_type{}) : run(std::false_type{}, std::false_type{});
     });
   });
 }

@@ -20,8 +20,9 @@
 namespace pet_tattn {
 namespace {
 
-constexpr int kQueries = 64;     // queries a stage
-constexpr int kMaxSlots = 1024;  // workgroups a head at most (a partial sum of the table each)
+constexpr int kMaxSlots = 1024;    // workgroups a head at most (a partial sum of the table each)
+constexpr int kMaxima = 256;
+constexpr int kColumns = 32;       // columns of a bucket's sum
 
 // What the backward's kernels are given beside Args.
 struct Grads {
@@ -30,18 +31,43 @@ struct Grads {
   const float* ml;
   void* adj;
   int64_t lda;
-  float* delta;  // [T, H]: dO.O
-  float* norms;  // fp16: [T, H] |dO|, then [T, Hk] |v|
-  float* cfh;    // [N, H, S], or null
-  float* part;   // [slots, H, nb], with a table's gradient
+  float* delta;   // [T, H]: dO.O
+  float* norms;   // [T, H] |dO|, then [T, Hk] |v|: fp16, or a table's gradient
+  float* maxima;  // [kMaxima, 3], with a table's gradient: of |dO|, |v| and |dO.O|
+  float* cfh;     // [N, H, S], or null
+  double* part;   // [slots, H, nb], with a table's gradient
 };
 
-// dO.O of each row and head, and for fp16 rows |dO| and |v|: a group of lanes takes
-// a head's slice, eight elements each.
+__device__ __forceinline__ float power_of_two(int e) { return ldexpf(1.f, e); }
+
+// Over groups of `n` lanes (4, 8, 16) within a row of 16.
+template <int n>
+__device__ __forceinline__ float row_sum(float x) {
+  const auto swap = [](float v, auto ctrl) {
+    return __uint_as_float(__builtin_amdgcn_update_dpp(0u, __float_as_uint(v), decltype(ctrl)::value, 0xf, 0xf, true));
+  };
+  x += swap(x, std::integral_constant<int, 0xB1>{});                        // lane ^ 1
+  x += swap(x, std::integral_constant<int, 0x4E>{});                        // lane ^ 2
+  if constexpr (n >= 8) x += swap(x, std::integral_constant<int, 0x141>{});  // 7 - lane of eight
+  if constexpr (n >= 16) x += swap(x, std::integral_constant<int, 0x140>{});  // 15 - lane
+  return x;
+}
+__device__ __forceinline__ float wave_max(float x) {
+  const auto swap = [](float v, auto ctrl) {
+    return __uint_as_float(__builtin_amdgcn_update_dpp(0u, __float_as_uint(v), decltype(ctrl)::value, 0xf, 0xf, true));
+  };
+  x = fmaxf(x, swap(x, std::integral_constant<int, 0xB1>{}));
+  x = fmaxf(x, swap(x, std::integral_constant<int, 0x4E>{}));
+  x = fmaxf(x, swap(x, std::integral_constant<int, 0x141>{}));
+  x = fmaxf(x, swap(x, std::integral_constant<int, 0x140>{}));
+  return pet_attn::max_g(x);
+}
+
+// dO.O of each row and head (and |dO| and |v| where b.norms is there): a group of lanes
+// takes a head's slice, eight elements each.
 template <class T, int LG>
 __global__ __launch_bounds__(256) void delta_kernel(Args a, Grads b) {
-  const bool half = std::is_same<T, _Float16>::value;
-  const int64_t heads = int64_t(a.T) * a.H, all = heads + (half ? int64_t(a.T) * a.Hk : 0);
+  const int64_t heads = int64_t(a.T) * a.H, all = heads + (b.norms ? int64_t(a.T) * a.Hk : 0);
   const int l = threadIdx.x % LG;
   for (int64_t i = (int64_t(blockIdx.x) * 256 + threadIdx.x) / LG; i < all; i += int64_t(gridDim.x) * (256 / LG)) {
     const bool q = i < heads;
@@ -56,44 +82,22 @@ __global__ __launch_bounds__(256) void delta_kernel(Args a, Grads b) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       if (q) dot = fmaf(x[e], y[e], dot);
-      if (half) sq = fmaf(x[e], x[e], sq);
+      sq = fmaf(x[e], x[e], sq);
     }
-#pragma unroll
-    for (int m = 1; m < LG; m <<= 1) {
-      dot += __shfl_xor(dot, m, LG);
-      if (half) sq += __shfl_xor(sq, m, LG);
-    }
+    dot = row_sum<LG>(dot);
+    if (b.norms) sq = sqrtf(row_sum<LG>(sq));
     if (l == 0) {
       if (q) b.delta[i] = dot;
-      if (half) b.norms[i] = sqrtf(sq);
+      if (b.norms) b.norms[i] = sq;
     }
   }
 }
 
-// fp16 holds down to 2^-14 at full precision, and a long row's dS lie far under the
-// adjoints that they come from: the power of two that brings a bound of them,
-// max |dO| max |v| scale + max |D| over the atom and the group of heads, to 2^14 .. 2^15.
-// bf16 has fp32's range, and takes 1. Every wave of the workgroup calls it; room: 3
-// floats a wave.
-template <class T>
-__device__ __forceinline__ float adjoint_scale(const Args& a, const Grads& b, const Segment& seg, int hk, float* room) {
-  if constexpr (!std::is_same<T, _Float16>::value) return 1.f;
-  const int G = a.H / a.Hk;
-  float m[3] = {0.f, 0.f, 0.f};
-  for (int s = threadIdx.x; s < seg.count; s += blockDim.x) {
-    if (!seg.query(a, s)) continue;
-    const int64_t row = seg.row(s);
-    for (int i = 0; i < G; ++i) {
-      m[0] = fmaxf(m[0], b.norms[row * a.H + hk * G + i]);
-      m[1] = fmaxf(m[1], fabsf(b.delta[row * a.H + hk * G + i]));
-    }
-    if (seg.key(a, s)) m[2] = fmaxf(m[2], b.norms[int64_t(a.T) * a.H + row * a.Hk + hk]);
-  }
-#pragma unroll
-  for (int i = 0; i < 3; ++i)
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) m[i] = fmaxf(m[i], __shfl_xor(m[i], d));
+// Three maxima over the workgroup: m of every thread of every wave. room: 3 floats a wave.
+__device__ __forceinline__ void block_max(float (&m)[3], float* room) {
   const int waves = int(blockDim.x >> 6), wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int i = 0; i < 3; ++i) m[i] = wave_max(m[i]);
   __syncthreads();
   if ((threadIdx.x & 63) == 0)
 #pragma unroll
@@ -102,10 +106,56 @@ __device__ __forceinline__ float adjoint_scale(const Args& a, const Grads& b, co
   for (int w = 0; w < waves; ++w)
 #pragma unroll
     for (int i = 0; i < 3; ++i) m[i] = fmaxf(m[i], room[3 * w + i]);
-  const float bound = m[0] * m[2] * a.drop.scale + m[1];
+}
+
+// The power of two that brings a bound to 2^to .. 2^(to + 1); 1 for 0 and for what is not finite.
+__device__ __forceinline__ float scale_to(float bound, int to) {
   if (!(bound > 0.f) || !(bound < kInf)) return 1.f;
-  const int e = 14 - ilogbf(bound);
-  return ldexpf(1.f, e < -60 ? -60 : e > 60 ? 60 : e);
+  const int e = to - ilogbf(bound);
+  return power_of_two(e < -110 ? -110 : e > 80 ? 80 : e);
+}
+
+// The largest |dO|, |v| and |dO.O| of slot s and the heads of hk onto m, for a token that
+// counts; a NaN is infinite.
+__device__ __forceinline__ void live_maxima(const Args& a, const Grads& b, const Segment& seg, int s, int hk, float (&m)[3]) {
+  if (!seg.query(a, s)) return;
+  const int G = a.H / a.Hk;
+  const int64_t row = seg.row(s);
+  const auto onto = [](float& at, float x) { at = fmaxf(at, x == x ? fabsf(x) : kInf); };
+  for (int i = 0; i < G; ++i) {
+    onto(m[0], b.norms[row * a.H + hk * G + i]);
+    onto(m[2], b.delta[row * a.H + hk * G + i]);
+  }
+  if (seg.key(a, s)) onto(m[1], b.norms[int64_t(a.T) * a.H + row * a.Hk + hk]);
+}
+
+// fp16 holds down to 2^-14 at full precision, and a long row's dS lie far under the
+// adjoints that they come from: they are scaled by the power of two that brings a bound
+// of them, max |dO| max |v| / (1 - p) + max |dO.O| over the atom and the group of heads,
+// to 2^14 .. 2^15. bf16 has fp32's range, and takes 1.
+template <class T>
+__device__ __forceinline__ float adjoint_scale(const Args& a, const Grads& b, const Segment& seg, int hk, float* room) {
+  if constexpr (!std::is_same<T, _Float16>::value) return 1.f;
+  float m[3] = {0.f, 0.f, 0.f};
+  for (int s = threadIdx.x; s < seg.count; s += blockDim.x) live_maxima(a, b, seg, s, hk, m);
+  block_max(m, room);
+  return scale_to(m[0] * m[1] * a.drop.scale + m[2], 14);
+}
+
+// The same maxima over the whole call, a workgroup's at b.maxima[3 block].
+__global__ __launch_bounds__(256) void maxima_kernel(Args a, Grads b) {
+  __shared__ float room[12];
+  float m[3] = {0.f, 0.f, 0.f};
+  const int strips = (a.S + 255) / 256;
+  const int64_t items = int64_t(a.N) * strips;
+  for (int64_t i = blockIdx.x; i < items; i += gridDim.x) {
+    const int64_t n = i / strips;
+    const Segment seg(a, int(n));
+    const int s = int(i - n * strips) * 256 + threadIdx.x;
+    for (int hk = 0; hk < a.Hk && s < seg.count; ++hk) live_maxima(a, b, seg, s, hk, m);
+  }
+  block_max(m, room);
+  if (threadIdx.x < 3) b.maxima[3 * blockIdx.x + threadIdx.x] = m[threadIdx.x];
 }
 
 // A query's exponent: P = 2^(s - this), +inf (P = 0) for one that attends to nothing.
@@ -143,18 +193,51 @@ __device__ __forceinline__ float masked(float x, const u2& bits, int t, int r) {
 }
 
 struct BiasEntry {
-  float value;    // table[bucket][h] log2 e
-  int hist;       // the bucket's row in a wave's columns, in floats
+  float value;  // table[bucket][h] log2 e
+  int column;   // the bucket's first column, in bytes
 };
+
+// The bias table's gradient, sums of dS by bucket, in whole numbers of a power of two
+// that brings the bound of a dS to 2^28 .. 2^30: additions in any order give one result,
+// so a bucket's 32 columns are shared by the workgroup's waves, and the LDS adds 64-bit
+// integers to them at 8 cycles a wave where its fp32 addition takes 194 (a CU, measured:
+// a lane at a time). A dS is rounded by 2^-31 of the bound.
+__device__ __forceinline__ void count_in(char* columns, const BiasEntry& at, float x) {
+  int q;
+  asm("v_cvt_rpi_i32_f32 %0, %1" : "=v"(q) : "v"(x));  // floor(x + 1/2)
+  __hip_atomic_fetch_add(reinterpret_cast<unsigned long long*>(columns + at.column), static_cast<unsigned long long>(int64_t(q)),
+                         __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+}
+// A head's columns summed in units of `unit` onto the workgroup's own row of sums, and cleared.
+__device__ __forceinline__ void flush_columns(int64_t* columns, int nb, double unit, double* sums) {
+  __syncthreads();
+  for (int k = threadIdx.x; k < nb; k += blockDim.x) {
+    int64_t sum = 0;
+    for (int l = 0; l < kColumns; ++l) {
+      int64_t* const at = columns + k * kColumns + ((l + k) & (kColumns - 1));
+      sum += *at;
+      *at = 0;
+    }
+    sums[k] += double(sum) * unit;
+  }
+  __syncthreads();
+}
+__device__ __forceinline__ void bias_entries(const Args& a, BiasEntry* lut, int h) {
+  for (int i = threadIdx.x; i <= 2 * a.reach; i += blockDim.x) {
+    const int bucket = bucket_of(a, i);
+    lut[i] = BiasEntry{a.table[int64_t(bucket) * a.H + h] * kLog2e, bucket * kColumns * 8};
+  }
+}
+
+// ---- past 128 slots: a pass over the keys and one over the queries --------------------
 
 template <int HD>
 struct KvLds {
-  static constexpr size_t rows = size_t(2) * kQueries * kPitch<HD> * 2, queries = rows + size_t(kQueries) * 12;
-  // + a wave's masks and maxima
-  // + the bias's entries, the lanes' columns
-  static size_t bytes(const Args& a, int waves, bool hist) {
-    return queries + size_t(waves) * (64 + 12) + 8 + (a.table ? size_t(2 * a.reach + 1) * 8 : 0) +
-           (hist ? size_t(waves) * a.nb * 256 : 0);
+  static constexpr size_t rows = size_t(2) * kStage<HD> * kPitch<HD> * 2, queries = rows + size_t(kStage<HD>) * 12,
+                          waves = queries + 4 * (64 + 16);  // masks and maxima
+  // + the bias's entries, the buckets' columns
+  static size_t bytes(const Args& a, bool hist) {
+    return waves + (a.table ? size_t(2 * a.reach + 1) * 8 : 0) + (hist ? size_t(a.nb) * kColumns * 8 : 0);
   }
 };
 
@@ -163,21 +246,22 @@ struct KvLds {
 // heads, staged in LDS: S = Q K^T and dP = dO V^T with a lane's key in its column, so P
 // and dS are the B operands of dV^T += dO^T P and dK^T += Q^T dS as they lie.
 template <class T, int HD, int KT, bool BIAS, bool DROP>
-__global__ __launch_bounds__(256) void typed_bwd_kv_kernel(Args a, Grads b, int kblocks) {
+__global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, int kblocks) {
   extern __shared__ __align__(16) char lds[];
-  constexpr int DS = HD / 32, DT = HD / 16;
+  constexpr int DS = HD / 32, DT = HD / 16, per = 4 * KT * 16;
   constexpr bool HALF = std::is_same<T, _Float16>::value;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = int(blockDim.x >> 6), c = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
   T* const qs = reinterpret_cast<T*>(lds);
-  T* const gs = qs + kQueries * kPitch<HD>;
-  float* const expo = reinterpret_cast<float*>(gs + kQueries * kPitch<HD>);
-  float* const delta = expo + kQueries;
-  int* const qpos = reinterpret_cast<int*>(delta + kQueries);
-  unsigned char* const exchange = reinterpret_cast<unsigned char*>(qpos + kQueries) + 64 * wave;
-  float* const room = reinterpret_cast<float*>(qpos + kQueries + 16 * waves);
-  BiasEntry* const lut = reinterpret_cast<BiasEntry*>(room + (3 * waves + 1) / 2 * 2);
-  float* const columns = reinterpret_cast<float*>(lut + (BIAS ? 2 * a.reach + 1 : 0));
-  const int G = a.H / a.Hk, per = waves * KT * 16;
+  T* const gs = qs + kStage<HD> * kPitch<HD>;
+  float* const expo = reinterpret_cast<float*>(gs + kStage<HD> * kPitch<HD>);
+  float* const delta = expo + kStage<HD>;
+  int* const qpos = reinterpret_cast<int*>(delta + kStage<HD>);
+  unsigned char* const exchange = reinterpret_cast<unsigned char*>(qpos + kStage<HD>) + 64 * wave;
+  float* const room = reinterpret_cast<float*>(qpos + kStage<HD> + 64);
+  BiasEntry* const lut = reinterpret_cast<BiasEntry*>(room + 16);
+  int64_t* const columns = reinterpret_cast<int64_t*>(lut + (BIAS ? 2 * a.reach + 1 : 0));
+  char* const mine = reinterpret_cast<char*>(columns + (lane & (kColumns - 1)));
+  const int G = a.H / a.Hk;
   const Share share(a.Hk);
   const int hk = share.head;
   const bool hist = BIAS && b.part;
@@ -186,39 +270,30 @@ __global__ __launch_bounds__(256) void typed_bwd_kv_kernel(Args a, Grads b, int 
   const T* const vcols = qkv + (a.H + a.Hk + hk) * a.hd;
   Words key{};
   if constexpr (DROP) key = a.drop.key();
-  float* const mine = columns + wave * a.nb * 64 + lane;
-  float* const sums = b.part + (int64_t(share.slot) * a.H + hk * G) * a.nb;  // the workgroup's own, a head's by one thread a bucket
+  // the unit of the table's sums is one for the whole call
+  float units = 1.f;
+  double unit = 1.0;
+  double* const sums = hist ? b.part + (int64_t(share.slot) * a.H + hk * G) * a.nb : nullptr;
   if (hist) {
-    for (int i = 0; i < a.nb; ++i) mine[64 * i] = 0.f;
-    for (int k = threadIdx.x; k < a.nb; k += blockDim.x)
-      for (int i = 0; i < G; ++i) sums[i * a.nb + k] = 0.f;
+    float m[3] = {0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < 3; ++k) m[k] = b.maxima[3 * threadIdx.x + k];
+    block_max(m, room);
+    const float bound = m[0] * m[1] * a.drop.scale + m[2];
+    units = scale_to(bound, 28);
+    unit = bound < kInf ? 1.0 / double(units) : double(__builtin_nanf(""));  // (no unit holds an infinite dS)
+    for (int i = threadIdx.x; i < a.nb * kColumns; i += 256) columns[i] = 0;
+    for (int k = threadIdx.x; k < a.nb; k += 256)
+      for (int i = 0; i < G; ++i) sums[i * a.nb + k] = 0.0;
   }
-  // the lanes' columns onto a head's sums, and cleared
-  const auto flush = [&](int i) {
-    __syncthreads();
-    for (int k = threadIdx.x; k < a.nb; k += blockDim.x) {
-      float sum = 0.f;
-      for (int w = 0; w < waves; ++w)
-        for (int l = 0; l < 64; ++l) sum += columns[(w * a.nb + k) * 64 + ((l + k) & 63)];
-      sums[i * a.nb + k] += sum;
-    }
-    __syncthreads();
-    for (int k = 0; k < a.nb; ++k) mine[64 * k] = 0.f;
-  };
-  const auto entries = [&](int h) {
-    for (int i = threadIdx.x; i <= 2 * a.reach; i += blockDim.x) {
-      const int bucket = bucket_of(a, i);
-      lut[i] = BiasEntry{a.table[int64_t(bucket) * a.H + h] * kLog2e, bucket * 64};
-    }
-  };
-  if (BIAS && G == 1) entries(hk);
+  if (BIAS && G == 1) bias_entries(a, lut, hk);
 
   const int items = a.N * kblocks;
   for (int item = share.slot; item < items; item += share.step) {
     const int n = item / kblocks, kb = item - n * kblocks;
     const Segment seg(a, n);
     if (kb * per >= seg.count) continue;
-    const float sc = adjoint_scale<T>(a, b, seg, hk, room), back = 1.f / sc;
+    const float sc = adjoint_scale<T>(a, b, seg, hk, room), back = 1.f / sc, counts = hist ? units * back : 0.f;
     const int k0 = kb * per + wave * KT * 16;
     u4 kf[KT][DS], vf[KT][DS];
     f4 dk[KT][DT], dv[KT][DT];
@@ -230,11 +305,8 @@ __global__ __launch_bounds__(256) void typed_bwd_kv_kernel(Args a, Grads b, int 
       const int s = k0 + 16 * kt + c;
       klive[kt] = seg.key(a, s);
       const int64_t row = klive[kt] ? seg.row(s) : 0;
-#pragma unroll
-      for (int d = 0; d < DS; ++d) {
-        kf[kt][d] = own_chunk(kcols, a.ldq, row, klive[kt], d, lane, a.hd);
-        vf[kt][d] = own_chunk(vcols, a.ldq, row, klive[kt], d, lane, a.hd);
-      }
+      own_pieces(a, kcols, a.ldq, seg, s, klive[kt], lane, kf[kt]);
+      own_pieces(a, vcols, a.ldq, seg, s, klive[kt], lane, vf[kt]);
       weight[kt] = klive[kt] ? log_weight(seg.cf(a, s)) : -kInf;
       if constexpr (BIAS) kpos[kt] = a.pos[row];
 #pragma unroll
@@ -245,27 +317,39 @@ __global__ __launch_bounds__(256) void typed_bwd_kv_kernel(Args a, Grads b, int 
       float cf_sum[KT] = {};
       if (BIAS && G > 1) {
         __syncthreads();
-        entries(h);
+        bias_entries(a, lut, h);
       }
       const T* const qcols = qkv + h * a.hd;
       const T* const gcols = static_cast<const T*>(b.out_adj) + h * a.hd;
-      for (int q0 = 0; q0 < seg.count; q0 += kQueries) {
-        const int n_queries = min(kQueries, round_up(seg.count - q0, 32));
+      Ahead<T, HD, kStage<HD>, true> ahead;
+      float next_expo = 0.f, next_delta = 0.f;
+      int next_pos = 0;
+      const auto load = [&](int q0) {
+        ahead.load(a, qcols, a.ldq, gcols, b.ldg, seg, q0);
+        if (threadIdx.x < kStage<HD>) {
+          const int s = q0 + int(threadIdx.x);
+          const bool on = seg.query(a, s);
+          const int64_t row = on ? seg.row(s) : 0;
+          next_expo = exponent(a, b, n, h, s, on);
+          next_delta = on ? b.delta[row * a.H + h] : 0.f;
+          if constexpr (BIAS) next_pos = a.pos[row];
+        }
+      };
+      load(0);
+      for (int q0 = 0; q0 < seg.count; q0 += kStage<HD>) {
+        const int n_queries = min(kStage<HD>, round_up(seg.count - q0, 32));
         __syncthreads();
-        const auto live = [&](int s) { return seg.query(a, s); };
-        stage<T, HD>(qs, qcols, a.ldq, seg, q0, n_queries, a.hd, live);
-        stage<T, HD>(gs, gcols, b.ldg, seg, q0, n_queries, a.hd, live);
-        for (int q = threadIdx.x; q < n_queries; q += blockDim.x) {
-          const bool on = live(q0 + q);
-          const int64_t row = on ? seg.row(q0 + q) : 0;
-          float e = exponent(a, b, n, h, q0 + q, on);
-          if constexpr (DROP) e -= log2f(a.drop.scale);
-          expo[q] = -e * a.inv2;
-          delta[q] = on ? b.delta[row * a.H + h] / a.drop.scale : 0.f;
-          if constexpr (BIAS) qpos[q] = a.pos[row];
+        ahead.store(a, qs, qcols, a.ldq, gs, gcols, b.ldg, seg, q0);
+        if (threadIdx.x < kStage<HD>) {
+          // P is scaled by 1 / (1 - p) with its exponent
+          expo[threadIdx.x] = (DROP ? log2f(a.drop.scale) - next_expo : -next_expo) * a.inv2;
+          delta[threadIdx.x] = DROP ? next_delta / a.drop.scale : next_delta;
+          if constexpr (BIAS) qpos[threadIdx.x] = next_pos;
         }
         __syncthreads();
+        if (q0 + kStage<HD> < seg.count) load(q0 + kStage<HD>);
         if (k0 >= seg.count) continue;
+        float part_sum[KT] = {};
         for (int qb = 0; qb < n_queries; qb += 32) {
           u2 bits[KT];
           if constexpr (DROP) {
@@ -274,6 +358,7 @@ __global__ __launch_bounds__(256) void typed_bwd_kv_kernel(Args a, Grads b, int 
 #pragma unroll
             for (int kt = 0; kt < KT; ++kt) bits[kt] = keys_mask(a, key, row, k0 + 16 * kt, h, lane, exchange);
           }
+          u4 pf[KT], df[KT];
           float p[KT][8], ds[KT][8];
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
@@ -310,20 +395,24 @@ __global__ __launch_bounds__(256) void typed_bwd_kv_kernel(Args a, Grads b, int 
                 const float es = HALF ? e * sc : e;
                 const float x = fmaf(HALF ? kept * sc : kept, dp[kt][r], -es * d4[r]);
                 ds[kt][4 * t + r] = x;
-                cf_sum[kt] += x;
-                if (hist) __hip_atomic_fetch_add(mine + be.hist, x * back, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
+                part_sum[kt] += x;
+                if (hist) count_in(mine, be, x * counts);
               }
           }
 #pragma unroll
-          for (int kt = 0; kt < KT; ++kt) {
-            const u4 pf = pack8<T>(p[kt]), df = pack8<T>(ds[kt]);
+          for (int kt = 0; kt < KT; ++kt) pf[kt] = pack8<T>(p[kt]), df[kt] = pack8<T>(ds[kt]);
 #pragma unroll
-            for (int j = 0; j < DT; ++j) {
-              dv[kt][j] = mfma<T>(transposed<T, HD>(gs, qb, j >> 1, j & 1, lane), pf, dv[kt][j]);
-              dk[kt][j] = mfma<T>(transposed<T, HD>(qs, qb, j >> 1, j & 1, lane), df, dk[kt][j]);
+          for (int j = 0; j < DT; ++j) {
+            const u4 gt = transposed<T, HD>(gs, qb, j >> 1, j & 1, lane), qt = transposed<T, HD>(qs, qb, j >> 1, j & 1, lane);
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) {
+              dv[kt][j] = mfma<T>(gt, pf[kt], dv[kt][j]);
+              dk[kt][j] = mfma<T>(qt, df[kt], dk[kt][j]);
             }
           }
         }
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) cf_sum[kt] += part_sum[kt];  // (a stage's sum at a time: its error grows by the stages)
       }
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt) {
@@ -331,7 +420,7 @@ __global__ __launch_bounds__(256) void typed_bwd_kv_kernel(Args a, Grads b, int 
         const int s = k0 + 16 * kt + c;
         if (b.cfh && g == 0 && s < seg.count) b.cfh[(int64_t(n) * a.H + h) * a.S + s] = sum;
       }
-      if (hist && G > 1) flush(i);
+      if (hist && G > 1) flush_columns(columns, a.nb, unit, sums + i * a.nb);
     }
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) {
@@ -346,24 +435,23 @@ __global__ __launch_bounds__(256) void typed_bwd_kv_kernel(Args a, Grads b, int 
       }
     }
   }
-  if (hist && G == 1) flush(0);
+  if (hist && G == 1) flush_columns(columns, a.nb, unit, sums);
 }
 
 // dQ: a wave has QT tiles of 16 queries as B operands and goes over the keys: S^T and
 // dP^T with a lane's query in its column, dS^T the B operand of dQ^T += K^T dS^T.
 template <class T, int HD, int QT, bool BIAS, bool DROP>
-__global__ __launch_bounds__(256) void typed_bwd_q_kernel(Args a, Grads b, int qblocks) {
+__global__ __launch_bounds__(256, 2) void typed_bwd_q_kernel(Args a, Grads b, int qblocks) {
   extern __shared__ __align__(16) char lds[];
-  constexpr int DS = HD / 32, DT = HD / 16, kKeys = kQueries;
+  constexpr int DS = HD / 32, DT = HD / 16, per = 4 * QT * 16;
   constexpr bool HALF = std::is_same<T, _Float16>::value;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = int(blockDim.x >> 6), c = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
   T* const ks = reinterpret_cast<T*>(lds);
-  T* const vs = ks + kKeys * kPitch<HD>;
-  float* const weight = reinterpret_cast<float*>(vs + kKeys * kPitch<HD>);
-  int* const kpos = reinterpret_cast<int*>(weight + kKeys);
-  float* const room = reinterpret_cast<float*>(kpos + kKeys);
-  float* const lut = room + 3 * waves;
-  const int per = waves * QT * 16;
+  T* const vs = ks + kStage<HD> * kPitch<HD>;
+  float* const weight = reinterpret_cast<float*>(vs + kStage<HD> * kPitch<HD>);
+  int* const kpos = reinterpret_cast<int*>(weight + kStage<HD>);
+  float* const room = reinterpret_cast<float*>(kpos + kStage<HD>);
+  float* const lut = room + 16;
   const Share share(a.H);
   const int h = share.head, hk = h / (a.H / a.Hk);
   const T* const qkv = static_cast<const T*>(a.qkv);
@@ -374,7 +462,7 @@ __global__ __launch_bounds__(256) void typed_bwd_q_kernel(Args a, Grads b, int q
   Words key{};
   if constexpr (DROP) key = a.drop.key();
   if constexpr (BIAS)
-    for (int i = threadIdx.x; i <= 2 * a.reach; i += blockDim.x)
+    for (int i = threadIdx.x; i <= 2 * a.reach; i += 256)
       lut[i] = a.table[int64_t(bucket_of(a, i)) * a.H + h] * kLog2e;
 
   const int items = a.N * qblocks;
@@ -394,11 +482,8 @@ __global__ __launch_bounds__(256) void typed_bwd_q_kernel(Args a, Grads b, int q
       const int s = q0 + 16 * qt + c;
       const bool on = seg.query(a, s);
       qrow[qt] = on ? seg.row(s) : 0;
-#pragma unroll
-      for (int d = 0; d < DS; ++d) {
-        qf[qt][d] = own_chunk(qcols, a.ldq, qrow[qt], on, d, lane, a.hd);
-        gf[qt][d] = own_chunk(gcols, b.ldg, qrow[qt], on, d, lane, a.hd);
-      }
+      own_pieces(a, qcols, a.ldq, seg, s, on, lane, qf[qt]);
+      own_pieces(a, gcols, b.ldg, seg, s, on, lane, gf[qt]);
       expo[qt] = exponent(a, b, n, h, s, on);
       if constexpr (DROP) expo[qt] -= log2f(a.drop.scale);
       delta[qt] = on ? b.delta[qrow[qt] * a.H + h] / a.drop.scale : 0.f;
@@ -406,18 +491,28 @@ __global__ __launch_bounds__(256) void typed_bwd_q_kernel(Args a, Grads b, int q
 #pragma unroll
       for (int j = 0; j < DT; ++j) dq[qt][j] = f4{0.f, 0.f, 0.f, 0.f};
     }
-    for (int k0 = 0; k0 < seg.count; k0 += kKeys) {
-      const int n_keys = min(kKeys, round_up(seg.count - k0, 32));
+    Ahead<T, HD, kStage<HD>, false> ahead;
+    float next_weight = 0.f;
+    int next_pos = 0;
+    const auto load = [&](int k0) {
+      ahead.load(a, kcols, a.ldq, vcols, a.ldq, seg, k0);
+      if (threadIdx.x < kStage<HD>) {
+        const int s = k0 + int(threadIdx.x);
+        next_weight = s < seg.count ? seg.cf(a, s) : 0.f;
+        if constexpr (BIAS) next_pos = s < seg.count ? a.pos[seg.row(s)] : 0;
+      }
+    };
+    load(0);
+    for (int k0 = 0; k0 < seg.count; k0 += kStage<HD>) {
+      const int n_keys = min(kStage<HD>, round_up(seg.count - k0, 32));
       __syncthreads();
-      const auto live = [&](int s) { return seg.key(a, s); };
-      stage<T, HD>(ks, kcols, a.ldq, seg, k0, n_keys, a.hd, live);
-      stage<T, HD>(vs, vcols, a.ldq, seg, k0, n_keys, a.hd, live);
-      for (int k = threadIdx.x; k < n_keys; k += blockDim.x) {
-        const bool on = live(k0 + k);
-        weight[k] = on ? log_weight(seg.cf(a, k0 + k)) * a.inv2 : -kInf;
-        if constexpr (BIAS) kpos[k] = on ? a.pos[seg.row(k0 + k)] : 0;
+      ahead.store(a, ks, kcols, a.ldq, vs, vcols, a.ldq, seg, k0);
+      if (threadIdx.x < kStage<HD>) {
+        weight[threadIdx.x] = next_weight > 0.f ? log_weight(next_weight) * a.inv2 : -kInf;
+        if constexpr (BIAS) kpos[threadIdx.x] = next_pos;
       }
       __syncthreads();
+      if (k0 + kStage<HD> < seg.count) load(k0 + kStage<HD>);
       if (q0 >= seg.count) continue;
       for (int kb = 0; kb < n_keys; kb += 32) {
         float ds[QT][8];
@@ -495,13 +590,13 @@ __global__ __launch_bounds__(256) void typed_cf_kernel(Args a, const float* cfh,
 }
 
 // table_adj[b][h] = beta table_adj[b][h] + the workgroups' sums in order: workgroup h, 16 strips of them in double.
-__global__ __launch_bounds__(1024) void typed_table_kernel(const float* part, int slots, int H, int nb, float* adj,
+__global__ __launch_bounds__(1024) void typed_table_kernel(const double* part, int slots, int H, int nb, float* adj,
                                                            float beta) {
   __shared__ double strips[16][64];
   const int h = blockIdx.x, b = threadIdx.x & 63, strip = threadIdx.x >> 6;
   double sum = 0.0;
   if (b < nb)
-    for (int s = strip; s < slots; s += 16) sum += double(part[(int64_t(s) * H + h) * nb + b]);
+    for (int s = strip; s < slots; s += 16) sum += part[(int64_t(s) * H + h) * nb + b];
   strips[strip][b] = sum;
   __syncthreads();
   if (strip || b >= nb) return;
@@ -514,14 +609,15 @@ __global__ __launch_bounds__(1024) void typed_table_kernel(const float* part, in
 constexpr size_t aligned(size_t n) { return (n + 255) & ~size_t(255); }
 
 struct Workspace {
-  size_t delta, norms, cfh, part, bytes;
+  size_t delta, norms, maxima, cfh, part, bytes;
   Workspace(int dtype, const pet_attn_shape& s, int kv_heads, int nb) {
     const size_t T = size_t(s.n_rows), H = size_t(s.heads);
     delta = 0;
     norms = delta + aligned(T * H * 4);
-    cfh = norms + (dtype == PET_DTYPE_F16 ? aligned(T * (H + size_t(kv_heads)) * 4) : 0);
+    maxima = norms + (dtype == PET_DTYPE_F16 || nb ? aligned(T * (H + size_t(kv_heads)) * 4) : 0);
+    cfh = maxima + aligned(nb ? size_t(kMaxima) * 12 : 0);
     part = cfh + aligned(size_t(s.n_atoms) * H * size_t(s.slots) * 4);
-    bytes = part + aligned(size_t(kMaxSlots) * H * size_t(nb) * 4);
+    bytes = part + aligned(size_t(kMaxSlots) * H * size_t(nb) * 8);
   }
 };
 
@@ -559,53 +655,55 @@ extern "C" int pet_attn_bwd_typed(int dtype, const pet_attn_shape* shape, int kv
   if ((reinterpret_cast<uintptr_t>(workspace) & 15u) != 0) return PET_ATTN_EALIGN;
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   char* const base = static_cast<char*>(workspace);
-  Grads b{dmerged, merged, ldg, ldm, ml, qkv_adj, lda, reinterpret_cast<float*>(base + ws.delta),
-          reinterpret_cast<float*>(base + ws.norms), cf_seq_adj ? reinterpret_cast<float*>(base + ws.cfh) : nullptr,
-          table_adj ? reinterpret_cast<float*>(base + ws.part) : nullptr};
+  a.whole = a.whole && narrow(a, ldg) && narrow(a, ldm);
+  const bool half = dtype == PET_DTYPE_F16;
+  const auto at = [&](size_t offset) { return reinterpret_cast<float*>(base + offset); };
+  const Grads b{dmerged, merged, ldg, ldm, ml, qkv_adj, lda, at(ws.delta), half || table_adj ? at(ws.norms) : nullptr,
+                table_adj ? at(ws.maxima) : nullptr, cf_seq_adj ? at(ws.cfh) : nullptr,
+                table_adj ? reinterpret_cast<double*>(base + ws.part) : nullptr};
   if (shape->dead && a.T > 0)
     if (const int e = zero_dead(a, qkv_adj, lda, W, st)) return e;
   int slots = 0;
+  const auto launched = [] { return hipGetLastError() == hipSuccess ? int(PET_ATTN_OK) : int(PET_ATTN_ELAUNCH); };
   const int err = a.N == 0 ? int(PET_ATTN_OK) : with_row_type(dtype, [&](auto tv) {
     using T = decltype(tv);
-    {
-      const int64_t rows = int64_t(a.T) * (a.H + (dtype == PET_DTYPE_F16 ? a.Hk : 0));
-      const auto run = [&](auto lc) {
-        constexpr int LG = decltype(lc)::value;
-        const int64_t blocks = std::min<int64_t>((rows * LG + 255) / 256, 16384);
-        hipLaunchKernelGGL((delta_kernel<T, LG>), dim3(unsigned(blocks)), dim3(256), 0, st, a, b);
-        return hipGetLastError() == hipSuccess ? int(PET_ATTN_OK) : int(PET_ATTN_ELAUNCH);
-      };
-      const int e = a.hd <= 8 ? run(std::integral_constant<int, 1>{}) : a.hd <= 16 ? run(std::integral_constant<int, 2>{})
-                    : a.hd <= 32 ? run(std::integral_constant<int, 4>{}) : a.hd <= 64 ? run(std::integral_constant<int, 8>{})
-                    : run(std::integral_constant<int, 16>{});
-      if (e) return e;
-    }
     return with_head_dim(a.hd, [&](auto hc) {
       constexpr int HD = decltype(hc)::value;
       const auto run = [&](auto bc, auto dc) {
         constexpr bool BIAS = decltype(bc)::value, DROP = decltype(dc)::value;
-        const int waves = std::min(4, round_up(a.S, 16) / 16), blocks = (a.S + waves * 16 - 1) / (waves * 16);
-        const int64_t items = (int64_t(a.N) * blocks + 7) / 8 * 8;
         {
-          const auto kernel = typed_bwd_kv_kernel<T, HD, 1, BIAS, DROP>;
-          const size_t bytes = KvLds<HD>::bytes(a, waves, b.part != nullptr);
+          const int64_t groups = int64_t(a.T) * (a.H + (b.norms ? a.Hk : 0));
+          const unsigned blocks = unsigned(std::min<int64_t>((groups * (HD / 8) + 255) / 256, 16384));
+          hipLaunchKernelGGL((delta_kernel<T, HD / 8>), dim3(blocks), dim3(256), 0, st, a, b);
+          if (const int e = launched()) return e;
+          if (table_adj) {
+            hipLaunchKernelGGL(maxima_kernel, dim3(kMaxima), dim3(256), 0, st, a, b);
+            if (const int e = launched()) return e;
+          }
+        }
+        {
+          constexpr int KT = HD == 128 ? 1 : 2;
+          const auto kernel = typed_bwd_kv_kernel<T, HD, KT, BIAS, DROP>;
+          const int blocks = (a.S + KT * 64 - 1) / (KT * 64);
+          const int64_t items = (int64_t(a.N) * blocks + 7) / 8 * 8;
+          const size_t bytes = KvLds<HD>::bytes(a, b.part != nullptr);
           if (const int e = pet_attn::raise_lds(reinterpret_cast<const void*>(kernel), bytes)) return e;
           slots = int(std::min<int64_t>(items, b.part ? std::clamp(2048 / a.Hk / 8 * 8, 8, kMaxSlots) : kMaxSlots));
-          if (int64_t(slots) * a.Hk * waves * 64 > INT32_MAX) return int(PET_ATTN_EINDEX);
-          hipLaunchKernelGGL(kernel, dim3(unsigned(slots * a.Hk)), dim3(unsigned(waves * 64)), bytes, st, a, b, blocks);
-          if (hipGetLastError() != hipSuccess) return int(PET_ATTN_ELAUNCH);
+          if (int64_t(slots) * a.Hk * 256 > INT32_MAX) return int(PET_ATTN_EINDEX);
+          hipLaunchKernelGGL(kernel, dim3(unsigned(slots * a.Hk)), dim3(256), bytes, st, a, b, blocks);
+          if (const int e = launched()) return e;
         }
         {
-          const auto kernel = typed_bwd_q_kernel<T, HD, 1, BIAS, DROP>;
-          const size_t bytes = size_t(kQueries) * (2 * kPitch<HD> * 2 + 8) + size_t(waves) * 12 +
-                               (a.table ? size_t(2 * a.reach + 1) * 4 : 0);
+          constexpr int QT = 2;
+          const auto kernel = typed_bwd_q_kernel<T, HD, QT, BIAS, DROP>;
+          const int blocks = (a.S + QT * 64 - 1) / (QT * 64);
+          const size_t bytes = size_t(kStage<HD>) * (2 * kPitch<HD> * 2 + 8) + 64 + (a.table ? size_t(2 * a.reach + 1) * 4 : 0);
           if (const int e = pet_attn::raise_lds(reinterpret_cast<const void*>(kernel), bytes)) return e;
-          const int64_t q_slots = std::min<int64_t>(items, 2048);
-          if (q_slots * a.H * waves * 64 > INT32_MAX) return int(PET_ATTN_EINDEX);
-          hipLaunchKernelGGL(kernel, dim3(unsigned(q_slots * a.H)), dim3(unsigned(waves * 64)), bytes, st, a, b, blocks);
-          if (hipGetLastError() != hipSuccess) return int(PET_ATTN_ELAUNCH);
+          const int64_t q_slots = std::min<int64_t>((int64_t(a.N) * blocks + 7) / 8 * 8, 2048);
+          if (q_slots * a.H * 256 > INT32_MAX) return int(PET_ATTN_EINDEX);
+          hipLaunchKernelGGL(kernel, dim3(unsigned(q_slots * a.H)), dim3(256), bytes, st, a, b, blocks);
+          return launched();
         }
-        return int(PET_ATTN_OK);
       };
       if (a.table) return dropout ? run(std::true_type{}, std::true_type{}) : run(std::true_type{}, std::false_type{});
       return dropout ? run(std::false_type{}, std::true_type{}) : run(std::false_type{}, std::false_type{});
