@@ -128,6 +128,7 @@ struct Args {
   bool whole;  // head_dim in pieces of 8, and a segment's offsets in 32 bits
 };
 
+
 // Atom n's tokens. Counts past S or past the rows would be the caller's error; they
 // are cut, so that no row outside 0 .. T - 1 is touched whatever off holds.
 struct Segment {
@@ -181,61 +182,65 @@ __device__ __forceinline__ u4 where(bool on, const u4& x) {
 // nothing that a masked row holds is ever multiplied. EACH pieces of both a thread are
 // loaded at once, without a branch (one that is not wanted is of a place that is there).
 // more(slot, dim): what else is loaded with a piece; take(row k, chunk, x, y, on, that).
-template <class T, int HD, int EACH, bool QUERY, class More, class Take>
+template <class T, int HD, int EACH, bool WHOLE, bool QUERY, class More, class Take>
 __device__ __forceinline__ void stage_pair(const Args& a, T* xs, const T* xsrc, int64_t ldx, T* ys, const T* ysrc,
                                            int64_t ldy, const Segment& seg, int s0, int n, const More& more,
                                            const Take& take) {
   constexpr int CH = HD / 8;
   const int nt = blockDim.x, total = n * CH, last = seg.count - 1;
   const Column xc(xsrc, ldx, seg), yc(ysrc, ldy, seg);
+  const auto put = [&](int i, const u4& x, const u4& y, bool on, const auto& m) {
+    const int k = i / CH, row = lds_row(k) * kPitch<HD>;
+    put_piece(xs + row, i % CH, x);
+    put_piece(ys + row, i % CH, y);
+    take(k, i % CH, x, y, on, m);
+  };
+  if constexpr (!WHOLE) {
+#pragma unroll 1
+    for (int i = threadIdx.x; i < total; i += nt) {
+      const int s = s0 + i / CH, ch = 8 * (i % CH);
+      const bool on = QUERY ? seg.query(a, s) : seg.key(a, s);
+      u4 x = {0u, 0u, 0u, 0u}, y = x;
+      decltype(more(0, 0)) m = {};
+      if (on) {
+        const int64_t row = seg.row(s);
+        x = row_chunk(xsrc + row * ldx, ch, a.hd), y = row_chunk(ysrc + row * ldy, ch, a.hd);
+        m = more(s, ch);
+      }
+      put(i, x, y, on, m);
+    }
+    return;
+  }
   for (int i0 = threadIdx.x; i0 < total; i0 += EACH * nt) {
     u4 x[EACH], y[EACH];
     bool on[EACH];
     decltype(more(0, 0)) m[EACH];
 #pragma unroll
     for (int j = 0; j < EACH; ++j) {
-      const int i = i0 + j * nt, s = s0 + i / CH, ch = 8 * (i % CH), at = s < last ? s : last;
-      if (a.whole) {
-        const float w = seg.cf(a, at);
-        const int d = ch < a.hd ? ch : 0;
-        x[j] = __builtin_bit_cast(u4, *reinterpret_cast<const u4e*>(xc.at(at, d)));
-        y[j] = __builtin_bit_cast(u4, *reinterpret_cast<const u4e*>(yc.at(at, d)));
-        m[j] = more(at, d);
-        on[j] = s <= last && ch < a.hd && (w > 0.f || (QUERY && s == 0));
-      } else {
-        on[j] = QUERY ? seg.query(a, s) : seg.key(a, s);
-        x[j] = y[j] = u4{0u, 0u, 0u, 0u};
-        if (on[j]) {
-          x[j] = row_chunk(xsrc + seg.row(s) * ldx, ch, a.hd), y[j] = row_chunk(ysrc + seg.row(s) * ldy, ch, a.hd);
-          m[j] = more(s, ch);
-        }
-      }
+      const int i = i0 + j * nt, s = s0 + i / CH, ch = 8 * (i % CH), at = s < last ? s : last, d = ch < a.hd ? ch : 0;
+      const float w = seg.cf(a, at);
+      x[j] = __builtin_bit_cast(u4, *reinterpret_cast<const u4e*>(xc.at(at, d)));
+      y[j] = __builtin_bit_cast(u4, *reinterpret_cast<const u4e*>(yc.at(at, d)));
+      m[j] = more(at, d);
+      on[j] = s <= last && ch < a.hd && (w > 0.f || (QUERY && s == 0));
     }
 #pragma unroll
-    for (int j = 0; j < EACH; ++j) {
-      const int i = i0 + j * nt, k = i / CH;
-      if (i < total) {
-        x[j] = where(on[j], x[j]), y[j] = where(on[j], y[j]);
-        const int row = lds_row(k) * kPitch<HD>;
-        put_piece(xs + row, i % CH, x[j]);
-        put_piece(ys + row, i % CH, y[j]);
-        take(k, i % CH, x[j], y[j], on[j], m[j]);
-      }
-    }
+    for (int j = 0; j < EACH; ++j)
+      if (i0 + j * nt < total) put(i0 + j * nt, where(on[j], x[j]), where(on[j], y[j]), on[j], m[j]);
   }
 }
 
 // The same for kernels of 256 threads that go over stages of KS slots: the loads of the
-// next stage go out before the present one is used (where Args::whole; else they are
-// loaded as they are stored, and the registers of the main path stay few).
-template <class T, int HD, int KS, bool QUERY>
+// next stage go out before the present one is used (not WHOLE: they are loaded as they are
+// stored).
+template <class T, int HD, int KS, bool WHOLE, bool QUERY>
 struct Ahead {
   static constexpr int CH = HD / 8, EACH = KS * CH / 256;
   u4 x[EACH], y[EACH];
   bool on[EACH];
   __device__ __forceinline__ void load(const Args& a, const T* xsrc, int64_t ldx, const T* ysrc, int64_t ldy,
                                        const Segment& seg, int s0) {
-    if (!a.whole) return;
+    if constexpr (!WHOLE) return;
     const int last = seg.count - 1;
     const Column xc(xsrc, ldx, seg), yc(ysrc, ldy, seg);
 #pragma unroll
@@ -250,7 +255,7 @@ struct Ahead {
   }
   __device__ __forceinline__ void store(const Args& a, T* xs, const T* xsrc, int64_t ldx, T* ys, const T* ysrc,
                                         int64_t ldy, const Segment& seg, int s0) const {
-    if (!a.whole) {
+    if constexpr (!WHOLE) {
 #pragma unroll 1
       for (int i = threadIdx.x; i < KS * CH; i += 256) {
         const int s = s0 + i / CH, d = 8 * (i % CH), row = lds_row(i / CH) * kPitch<HD>;
@@ -275,11 +280,11 @@ struct Ahead {
 
 // A lane's B operands of a token's own columns (slot s, zeros unless live): of dims 32
 // step .. + 31 the pieces that lie at 8g of an LDS row.
-template <class T, int DS>
+template <class T, bool WHOLE, int DS>
 __device__ __forceinline__ void own_pieces(const Args& a, const T* src, int64_t ld, const Segment& seg, int s, bool live,
                                            int lane, u4 (&out)[DS]) {
   const int g = lane >> 4, d0 = 16 * (g & 1) + 4 * (g >> 1);
-  if (a.whole) {
+  if constexpr (WHOLE) {
     const Column col(src, ld, seg);
     const int at = s < seg.count ? s : 0;
 #pragma unroll
@@ -291,16 +296,14 @@ __device__ __forceinline__ void own_pieces(const Args& a, const T* src, int64_t 
       out[step] = u4{l ? lo[0] : 0u, l ? lo[1] : 0u, h ? hi[0] : 0u, h ? hi[1] : 0u};
     }
   } else {
+    const T* const row = src + (live ? seg.row(s) : 0) * ld;
 #pragma unroll
     for (int step = 0; step < DS; ++step) {
       out[step] = u4{0u, 0u, 0u, 0u};
-      if (live)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int d = 32 * step + d0 + 8 * (e >> 2) + (e & 3);
-          if (d < a.hd)
-            out[step][e >> 1] |= unsigned(__builtin_bit_cast(unsigned short, src[seg.row(s) * ld + d])) << (16 * (e & 1));
-        }
+      if (live) {
+        const u4 lo = row_chunk(row, 32 * step + d0, a.hd), hi = row_chunk(row, 32 * step + d0 + 8, a.hd);
+        out[step] = u4{lo[0], lo[1], hi[0], hi[1]};
+      }
     }
   }
 }
@@ -356,11 +359,16 @@ bool narrow(const Args& a, int64_t ld);
 // Rows N + off[N] .. T - 1 of x set to zero.
 int zero_dead(const Args& a, void* x, int64_t ld, int width, hipStream_t st);
 
+// f(HD, WHOLE): heads of whole pieces at the next of 32, 64 and 128 dims; the rest (a
+// head_dim that is no multiple of 8, strides past 2^23) at 128, by loads of any address
+// that keep few pieces on their way: with both in one kernel their registers cost the
+// main path a third of its waves.
 template <class F>
-int with_head_dim(int hd, F&& f) {
-  if (hd <= 32) return f(std::integral_constant<int, 32>{});
-  if (hd <= 64) return f(std::integral_constant<int, 64>{});
-  return f(std::integral_constant<int, 128>{});
+int with_head_dim(const Args& a, F&& f) {
+  if (!a.whole) return f(std::integral_constant<int, 128>{}, std::false_type{});
+  if (a.hd <= 32) return f(std::integral_constant<int, 32>{}, std::true_type{});
+  if (a.hd <= 64) return f(std::integral_constant<int, 64>{}, std::true_type{});
+  return f(std::integral_constant<int, 128>{}, std::true_type{});
 }
 template <class F>
 int with_row_type(int dtype, F&& f) {

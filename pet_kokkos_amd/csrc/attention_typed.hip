@@ -24,7 +24,7 @@ constexpr int fwd_stage_bytes(int keys) { return keys * (2 * kPitch<HD> * 2 + 8)
 // The tiles of 16 queries at q[], QT of them, against staged keys kb .. kb + 32 U - 1
 // (slots k0 + kb ..; those past n_keys do not count): scores, the running maximum and sum,
 // and the products with the values onto o.
-template <class T, int HD, int QT, int U, bool BIAS, bool DROP>
+template <class T, int HD, int QT, int U, bool WHOLE, bool BIAS, bool DROP>
 struct Tiles {
   static constexpr int DS = HD / 32, DT = HD / 16;
   u4 qf[QT][DS];
@@ -40,7 +40,7 @@ struct Tiles {
       const int s = q0 + 16 * qt + (lane & 15);
       live[qt] = seg.query(a, s);
       row[qt] = live[qt] ? seg.row(s) : 0;
-      own_pieces(a, qcols, a.ldq, seg, s, live[qt], lane, qf[qt]);
+      own_pieces<T, WHOLE>(a, qcols, a.ldq, seg, s, live[qt], lane, qf[qt]);
       if constexpr (BIAS) pos[qt] = a.pos[row[qt]];
 #pragma unroll
       for (int j = 0; j < DT; ++j) o[qt][j] = f4{0.f, 0.f, 0.f, 0.f};
@@ -168,7 +168,7 @@ __device__ __forceinline__ void fill_lut(const Args& a, float* lut, int h) {
 // queries dealt to the workgroup's waves (4 from 33 slots on: a workgroup's waves start
 // at one SIMD, and 5 of them, one a tile of 71 slots, left room for no third workgroup
 // on the CU; which wave has the odd tile goes round by the atom).
-template <class T, int HD, bool BIAS, bool DROP>
+template <class T, int HD, bool WHOLE, bool BIAS, bool DROP>
 __global__ __launch_bounds__(256, HD == 128 ? 2 : 4) void typed_fwd_short_kernel(Args a, int keys, T* merged, int64_t ldm,
                                                                                 float* ml) {
   extern __shared__ __align__(16) char lds[];
@@ -197,12 +197,12 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 4) void typed_fwd_short_kernel
       weight[k] = w > 0.f ? log_weight(w) * a.inv2 : -kInf;
       if constexpr (BIAS) kpos[k] = there ? a.pos[seg.row(k)] : 0;
     }
-    stage_pair<T, HD, 2, false>(a, ks, kcols, a.ldq, vs, vcols, a.ldq, seg, 0, n_keys, [](int, int) { return 0; },
+    stage_pair<T, HD, 2, WHOLE, false>(a, ks, kcols, a.ldq, vs, vcols, a.ldq, seg, 0, n_keys, [](int, int) { return 0; },
                                 [](int, int, const u4&, const u4&, bool, int) {});
     __syncthreads();
     const int tiles = (seg.count + 15) >> 4, slots = (a.S + 15) >> 4;
     for (int tile = (wave + n) & (waves - 1); tile < slots; tile += waves) {
-      Tiles<T, HD, 1, 2, BIAS, DROP> q;
+      Tiles<T, HD, 1, 2, WHOLE, BIAS, DROP> q;
       q.start(a, qcols, seg, 16 * tile, lane);
       if (tile < tiles)
         for (int kb = 0; kb < n_keys; kb += 64) q.keys(a, key, h, ks, vs, weight, kpos, lut, 0, kb, n_keys, lane);
@@ -213,7 +213,7 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 4) void typed_fwd_short_kernel
 
 // Past 128 slots: an item is an atom's 128 queries, two tiles a wave, and the keys come in
 // stages, the next one's loads on their way while the present one is used.
-template <class T, int HD, bool BIAS, bool DROP>
+template <class T, int HD, bool WHOLE, bool BIAS, bool DROP>
 __global__ __launch_bounds__(256, 2) void typed_fwd_long_kernel(Args a, int qblocks, T* merged, int64_t ldm, float* ml) {
   extern __shared__ __align__(16) char lds[];
   constexpr int KS = kStage<HD>, QT = 2, per = 4 * QT * 16;
@@ -237,9 +237,9 @@ __global__ __launch_bounds__(256, 2) void typed_fwd_long_kernel(Args a, int qblo
     const int n = item / qblocks, qb = item - n * qblocks;
     const Segment seg(a, n);
     const int q0 = qb * per + wave * QT * 16;
-    Tiles<T, HD, QT, KS / 32, BIAS, DROP> q;
+    Tiles<T, HD, QT, KS / 32, WHOLE, BIAS, DROP> q;
     q.start(a, qcols, seg, q0, lane);
-    Ahead<T, HD, KS, false> ahead;
+    Ahead<T, HD, KS, WHOLE, false> ahead;
     float next_weight = 0.f;
     int next_pos = 0;
     const auto load = [&](int k0) {
@@ -346,8 +346,9 @@ extern "C" int pet_attn_fwd_typed(int dtype, const pet_attn_shape* shape, int kv
   if (a.N == 0) return PET_ATTN_OK;
   return with_row_type(dtype, [&](auto tv) {
     using T = decltype(tv);
-    return with_head_dim(a.hd, [&](auto hc) {
+    return with_head_dim(a, [&](auto hc, auto wc) {
       constexpr int HD = decltype(hc)::value;
+      constexpr bool WHOLE = decltype(wc)::value;
       const auto run = [&](auto bc, auto dc) {
         constexpr bool BIAS = decltype(bc)::value, DROP = decltype(dc)::value;
         const size_t lut = a.table ? size_t(2 * a.reach + 1) * 4 : 0;
@@ -355,14 +356,14 @@ extern "C" int pet_attn_fwd_typed(int dtype, const pet_attn_shape* shape, int kv
         const int64_t slots = std::min<int64_t>((a.N * qblocks + 7) / 8 * 8, 2048);
         if (slots * a.H * 256 > INT32_MAX) return int(PET_ATTN_EINDEX);
         if (a.S <= kShort) {
-          const auto kernel = typed_fwd_short_kernel<T, HD, BIAS, DROP>;
+          const auto kernel = typed_fwd_short_kernel<T, HD, WHOLE, BIAS, DROP>;
           const int keys = round_up(a.S, 32);
           const size_t bytes = size_t(fwd_stage_bytes<HD>(keys)) + lut;
           if (const int e = pet_attn::raise_lds(reinterpret_cast<const void*>(kernel), bytes)) return e;
           hipLaunchKernelGGL(kernel, dim3(unsigned(slots * a.H)), dim3(a.S <= 16 ? 64 : a.S <= 32 ? 128 : 256), bytes, st, a,
                              keys, static_cast<T*>(merged), ldm, ml);
         } else {
-          const auto kernel = typed_fwd_long_kernel<T, HD, BIAS, DROP>;
+          const auto kernel = typed_fwd_long_kernel<T, HD, WHOLE, BIAS, DROP>;
           const size_t bytes = size_t(fwd_stage_bytes<HD>(kStage<HD>)) + lut;
           if (const int e = pet_attn::raise_lds(reinterpret_cast<const void*>(kernel), bytes)) return e;
           hipLaunchKernelGGL(kernel, dim3(unsigned(slots * a.H)), dim3(256), bytes, st, a, int(qblocks),

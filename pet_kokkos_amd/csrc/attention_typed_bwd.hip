@@ -198,15 +198,34 @@ struct BiasEntry {
 };
 
 // The bias table's gradient, sums of dS by bucket, in whole numbers of a power of two
-// that brings the bound of a dS to 2^28 .. 2^30: additions in any order give one result,
-// so a bucket's 32 columns are shared by the workgroup's waves, and the LDS adds 64-bit
-// integers to them at 8 cycles a wave where its fp32 addition takes 194 (a CU, measured:
-// a lane at a time). A dS is rounded by 2^-31 of the bound.
-__device__ __forceinline__ void count_in(char* columns, const BiasEntry& at, float x) {
+// that brings a bound of the dS to 2^33 .. 2^35 (past 128 slots, where probabilities are
+// small, to 2^37): additions in any order give one result, so a bucket's 32 columns are
+// shared by the workgroup's waves, and the LDS adds 64-bit integers to them at 8 cycles a
+// wave where its fp32 addition takes 194 (a CU, measured: a lane at a time). A query's
+// |dS| sum to at most about the bound, so a column holds 2^25 queries and more. Four of a
+// lane's dS at a time: under 2^30, as nearly all are, one conversion to 32 bits each.
+__device__ __forceinline__ int nearest(float x) {
   int q;
   asm("v_cvt_rpi_i32_f32 %0, %1" : "=v"(q) : "v"(x));  // floor(x + 1/2)
-  __hip_atomic_fetch_add(reinterpret_cast<unsigned long long*>(columns + at.column), static_cast<unsigned long long>(int64_t(q)),
-                         __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+  return q;
+}
+__device__ __forceinline__ void count_in(char* columns, const int (&column)[4], const float (&x)[4]) {
+  const auto add = [&](int i, int64_t q) {
+    __hip_atomic_fetch_add(reinterpret_cast<unsigned long long*>(columns + column[i]), static_cast<unsigned long long>(q),
+                           __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+  };
+  const float m = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+  if (__builtin_expect(__any(m >= 0x1p30f), 0)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int high = nearest(x[i] * 0x1p-16f);
+      add(i, int64_t(high) << 16);
+      add(i, nearest(fmaf(float(high), -0x1p16f, x[i])));
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) add(i, nearest(x[i]));
 }
 // A head's columns summed in units of `unit` onto the workgroup's own row of sums, and cleared.
 __device__ __forceinline__ void flush_columns(int64_t* columns, int nb, double unit, double* sums) {
@@ -229,6 +248,298 @@ __device__ __forceinline__ void bias_entries(const Args& a, BiasEntry* lut, int 
   }
 }
 
+// ---- up to 128 slots: an atom's whole backward in one workgroup ------------------------
+
+template <int HD>
+struct ShortLds {
+  int rows;       // R: slots to a whole 32
+  size_t stats, more, bytes;
+  ShortLds(const Args& a, bool hist) : rows(round_up(a.S, 32)) {
+    stats = size_t(2) * rows * kPitch<HD> * 2 + size_t(rows) * size_t(rows + 8) * 2;
+    more = stats + size_t(rows) * 12;
+    bytes = more + 4 * (64 + 16) + (a.table ? size_t(2 * a.reach + 1) * 8 : 0) + (hist ? size_t(a.nb) * kColumns * 8 : 0);
+  }
+};
+
+// The larger of m and the magnitudes of a piece's elements, as 16-bit patterns (a NaN's is past infinity's).
+__device__ __forceinline__ void onto_magnitude(unsigned& m, const u4& x) {
+  typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+  us2 v = __builtin_bit_cast(us2, m);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const unsigned bits = x[i] & 0x7fff7fffu;
+    v = __builtin_elementwise_max(v, __builtin_bit_cast(us2, bits));
+  }
+  m = __builtin_bit_cast(unsigned, v);
+}
+template <class T>
+__device__ __forceinline__ float magnitude(unsigned m) {
+  const unsigned short bits = static_cast<unsigned short>(std::max(m & 0xffffu, m >> 16));
+  const float x = float(__builtin_bit_cast(T, bits));
+  return x == x ? x : kInf;
+}
+
+// A wave has KT tiles of 16 keys as B operands and dK^T, dV^T in registers; a head's
+// queries and adjoints are staged in LDS whole (dO.O made of the pieces as they pass),
+// S = Q K^T and dP = dO V^T come with a lane's key in its column, and P and dS are the B
+// operands of dV^T += dO^T P and dK^T += Q^T dS as they lie. dS goes to LDS, a key's
+// queries a row, and once every wave is done with Q's rows and K's lie there, it is read
+// transposed for dQ^T += K^T dS^T, a tile of queries a wave: every product is formed once,
+// where the two passes past 128 slots form S, dP and their exponentials twice.
+template <class T, int HD, int KT, bool WHOLE, bool BIAS, bool DROP>
+__global__ __launch_bounds__(256, HD == 128 || (HD == 64 && KT == 2) ? 2 : 3) void typed_bwd_short_kernel(Args a, Grads b, int R,
+                                                                                           unsigned stats, unsigned more) {
+  extern __shared__ __align__(16) char lds[];
+  constexpr int DS = HD / 32, DT = HD / 16, CH = HD / 8, P = kPitch<HD>;
+  constexpr bool HALF = std::is_same<T, _Float16>::value;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = int(blockDim.x >> 6), c = lane & 15, g = lane >> 4;
+  T* const qs = reinterpret_cast<T*>(lds);  // Q's rows, then K's
+  T* const gs = qs + R * P;                 // dO's rows
+  T* const dss = gs + R * P;                // dS, a key's queries a row
+  const int pitch = R + 8;
+  float* const expo = reinterpret_cast<float*>(lds + stats);
+  float* const delta = expo + R;
+  int* const qpos = reinterpret_cast<int*>(delta + R);
+  unsigned char* const exchange = reinterpret_cast<unsigned char*>(lds + more) + 64 * wave;
+  float* const room = reinterpret_cast<float*>(lds + more + 256);
+  BiasEntry* const lut = reinterpret_cast<BiasEntry*>(room + 16);
+  int64_t* const columns = reinterpret_cast<int64_t*>(lut + (BIAS ? 2 * a.reach + 1 : 0));
+  char* const mine = reinterpret_cast<char*>(columns + (lane & (kColumns - 1)));
+  const int G = a.H / a.Hk;
+  const Share share(a.Hk);
+  const int hk = share.head;
+  const bool hist = BIAS && b.part;
+  const T* const qkv = static_cast<const T*>(a.qkv);
+  const T* const kcols = qkv + (a.H + hk) * a.hd;
+  const T* const vcols = qkv + (a.H + a.Hk + hk) * a.hd;
+  Words key{};
+  if constexpr (DROP) key = a.drop.key();
+  float units = 0.f;   // of the table's sums: a power of two, made smaller as larger bounds come (0: none yet)
+  bool beyond = false;  // a dS that no unit holds
+  double* const sums = hist ? b.part + (int64_t(share.slot) * a.H + hk * G) * a.nb : nullptr;
+  if (hist) {
+    for (int i = threadIdx.x; i < a.nb * kColumns; i += blockDim.x) columns[i] = 0;
+    for (int k = threadIdx.x; k < a.nb; k += blockDim.x)
+      for (int i = 0; i < G; ++i) sums[i * a.nb + k] = 0.0;
+  }
+  if (BIAS && G == 1) bias_entries(a, lut, hk);
+  const auto flush = [&](int i) {
+    flush_columns(columns, a.nb, beyond ? double(__builtin_nanf("")) : units > 0.f ? 1.0 / double(units) : 0.0, sums + i * a.nb);
+  };
+
+  for (int n = share.slot; n < a.N; n += share.step) {
+    const Segment seg(a, n);
+    const int rows = round_up(seg.count, 32), first = (wave + n) & (waves - 1);
+    u4 kf[KT][DS], vf[KT][DS];
+    f4 dk[KT][DT], dv[KT][DT];
+    float weight[KT];
+    int kpos[KT];
+    bool klive[KT];
+    unsigned vmax = 0;
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+      const int s = 16 * (first + waves * kt) + c;
+      klive[kt] = seg.key(a, s);
+      own_pieces<T, WHOLE>(a, kcols, a.ldq, seg, s, klive[kt], lane, kf[kt]);
+      own_pieces<T, WHOLE>(a, vcols, a.ldq, seg, s, klive[kt], lane, vf[kt]);
+      weight[kt] = klive[kt] ? log_weight(seg.cf(a, s)) : -kInf;
+      if constexpr (BIAS) kpos[kt] = a.pos[klive[kt] ? seg.row(s) : 0];
+      if (HALF || hist)
+#pragma unroll
+        for (int d = 0; d < DS; ++d) onto_magnitude(vmax, vf[kt][d]);
+#pragma unroll
+      for (int j = 0; j < DT; ++j) dk[kt][j] = dv[kt][j] = f4{0.f, 0.f, 0.f, 0.f};
+    }
+    float sc = 1.f;
+    for (int i = 0; i < G; ++i) {
+      const int h = hk * G + i;
+      const T* const qcols = qkv + h * a.hd;
+      const T* const gcols = static_cast<const T*>(b.out_adj) + h * a.hd;
+      const T* const ocols = static_cast<const T*>(b.out) + h * a.hd;
+      __syncthreads();  // (the last head's or atom's rows are done with)
+      if (BIAS && G > 1) bias_entries(a, lut, h);
+      for (int q = threadIdx.x; q < rows; q += blockDim.x) {
+        const bool on = seg.query(a, q);
+        const float e = exponent(a, b, n, h, q, on);
+        expo[q] = (DROP ? log2f(a.drop.scale) - e : -e) * a.inv2;  // P is scaled by 1 / (1 - p) with its exponent
+        if constexpr (BIAS) qpos[q] = a.pos[on ? seg.row(q) : 0];
+      }
+      unsigned gmax = 0;
+      float dmax = 0.f;
+      const Column ocol(ocols, b.ldm, seg);
+      stage_pair<T, HD, 2, WHOLE, true>(
+          a, qs, qcols, a.ldq, gs, gcols, b.ldg, seg, 0, rows,
+          [&](int s, int d) {
+            return WHOLE ? __builtin_bit_cast(u4, *reinterpret_cast<const u4e*>(ocol.at(s, d)))
+                           : row_chunk(ocols + seg.row(s) * b.ldm, d, a.hd);
+          },
+          [&](int k, int ch, const u4&, const u4& y, bool on, const u4& o) {
+            float u[8], v[8], dot = 0.f;
+            pet_typed::unpack<T>(__builtin_bit_cast(u4e, y), u);
+            pet_typed::unpack<T>(__builtin_bit_cast(u4e, where(on, o)), v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) dot = fmaf(u[e], v[e], dot);
+            dot = row_sum<CH>(dot);
+            if (ch == 0) delta[k] = DROP ? dot / a.drop.scale : dot;
+            if (HALF || hist) onto_magnitude(gmax, y), dmax = fmaxf(dmax, dot == dot ? fabsf(dot) : kInf);
+          });
+      if (HALF || hist) {
+        const float m[3] = {wave_max(magnitude<T>(gmax)), wave_max(magnitude<T>(vmax)), wave_max(dmax)};
+        if (lane == 0)
+#pragma unroll
+          for (int k = 0; k < 3; ++k) room[3 * wave + k] = m[k];
+      }
+      __syncthreads();
+      // what brings dS into the range of fp16, and into whole numbers (adjoint_scale, count_in)
+      float counts = 0.f;
+      if (HALF || hist) {
+        float m[3] = {0.f, 0.f, 0.f};
+        for (int w = 0; w < waves; ++w)
+#pragma unroll
+          for (int k = 0; k < 3; ++k) m[k] = fmaxf(m[k], room[3 * w + k]);
+        const float bound = float(a.hd) * m[0] * m[1] * a.drop.scale + m[2];
+        if (hist) {
+          if (!(bound < kInf)) {
+            beyond = true;
+          } else if (bound > 0.f && (units == 0.f || bound * units > 0x1p35f)) {
+            const float fit = scale_to(bound, 33);
+            if (units > 0.f) {
+              const int by = ilogbf(units) - ilogbf(fit);
+              __syncthreads();
+              for (int k = threadIdx.x; k < a.nb * kColumns; k += blockDim.x) columns[k] = by < 63 ? columns[k] >> by : 0;
+              __syncthreads();
+            }
+            units = fit;
+          }
+        }
+        if constexpr (HALF) {
+          const float was = sc;
+          sc = scale_to(bound, 14);
+          if (i > 0 && sc != was)
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+              for (int j = 0; j < DT; ++j) dk[kt][j] *= sc / was;
+        }
+        counts = units / sc;
+      }
+      const float back = 1.f / sc;
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt) {
+        const int tile = first + waves * kt;
+        if (16 * tile >= seg.count) continue;
+        float cf_sum = 0.f;
+#pragma unroll 1
+        for (int qb = 0; qb < rows; qb += 32) {
+          u2 bits{};
+          if constexpr (DROP) {
+            const int s = qb + (lane & 31);
+            bits = keys_mask(a, key, uint32_t(s < seg.count ? seg.row(s) : 0), 16 * tile, h, lane, exchange);
+          }
+          float p[8], ds[8];
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const int at = qb + 8 * g + 4 * t;
+            f4 s = *reinterpret_cast<const f4*>(expo + at), dp = {0.f, 0.f, 0.f, 0.f};
+            const f4 d4 = *reinterpret_cast<const f4*>(delta + at);
+#pragma unroll
+            for (int d = 0; d < DS; ++d) {
+              s = mfma<T>(straight<T, HD>(qs, qb, t, d, lane), kf[kt][d], s);
+              dp = mfma<T>(straight<T, HD>(gs, qb, t, d, lane), vf[kt][d], dp);
+            }
+            i4 qp{};
+            int column[4] = {};
+            float counted[4];
+            if constexpr (BIAS) qp = *reinterpret_cast<const i4*>(qpos + at);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              float w = weight[kt];
+              if constexpr (BIAS) {
+                const BiasEntry be = lut[pair_index(kpos[kt], qp[r], a.reach)];
+                w += be.value;
+                column[r] = be.column;
+              }
+              const float e = exp2_fast(fmaf(s[r], a.scale2, w));
+              float kept = e;
+              if constexpr (DROP) kept = masked(e, bits, t, r);
+              p[4 * t + r] = kept;
+              const float es = HALF ? e * sc : e;
+              const float x = fmaf(HALF ? kept * sc : kept, dp[r], -es * d4[r]);
+              ds[4 * t + r] = x;
+              cf_sum += x;
+              counted[r] = x * counts;
+            }
+            if (hist) count_in(mine, column, counted);
+          }
+          const u4 pf = pack8<T>(p), df = pack8<T>(ds);
+          *reinterpret_cast<u4*>(dss + (16 * tile + c) * pitch + qb + 8 * g) = df;
+#pragma unroll
+          for (int j = 0; j < DT; ++j) {
+            dv[kt][j] = mfma<T>(transposed<T, HD>(gs, qb, j >> 1, j & 1, lane), pf, dv[kt][j]);
+            dk[kt][j] = mfma<T>(transposed<T, HD>(qs, qb, j >> 1, j & 1, lane), df, dk[kt][j]);
+          }
+        }
+        if (b.cfh) {
+          const float sum = pet_attn::sum_g(cf_sum) * back;
+          const int s = 16 * tile + c;
+          if (g == 0 && s < seg.count) b.cfh[(int64_t(n) * a.H + h) * a.S + s] = sum;
+        }
+      }
+      __syncthreads();
+      // K's rows in the place of Q's; zeros for the tiles behind the last token's
+      const u4 none = {0u, 0u, 0u, 0u};
+      const auto put_keys = [&](int tile, const u4 (&k)[DS]) {
+        T* const row = qs + lds_row(16 * tile + c) * P + 8 * g;
+#pragma unroll
+        for (int d = 0; d < DS; ++d) *reinterpret_cast<u4*>(row + 32 * d) = k[d];
+        if (16 * tile >= seg.count)
+          for (int qb = 0; qb < rows; qb += 32) *reinterpret_cast<u4*>(dss + (16 * tile + c) * pitch + qb + 8 * g) = none;
+      };
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt)
+        if (16 * (first + waves * kt) < rows) put_keys(first + waves * kt, kf[kt]);
+      if (waves == 1) {  // (one tile of two)
+        const u4 zeros[DS] = {};
+        put_keys(1, zeros);
+      }
+      __syncthreads();
+      for (int tile = first; 16 * tile < seg.count; tile += waves) {
+        f4 dq[DT];
+#pragma unroll
+        for (int j = 0; j < DT; ++j) dq[j] = f4{0.f, 0.f, 0.f, 0.f};
+        for (int kb = 0; kb < rows; kb += 32) {
+          const T* const at = dss + (kb + 8 * g + (c >> 2)) * pitch + 16 * tile + 4 * (c & 3);
+          const u2 lo = lds_tr(at), hi = lds_tr(at + 4 * pitch);
+          const u4 df = {lo[0], lo[1], hi[0], hi[1]};
+#pragma unroll
+          for (int j = 0; j < DT; ++j) dq[j] = mfma<T>(transposed<T, HD>(qs, kb, j >> 1, j & 1, lane), df, dq[j]);
+        }
+        const int s = 16 * tile + c;
+        if (s < seg.count) {
+          T* const row = static_cast<T*>(b.adj) + seg.row(s) * b.lda + h * a.hd;
+#pragma unroll
+          for (int jp = 0; jp < DS; ++jp) put8(row, dq[2 * jp], dq[2 * jp + 1], a.scale * back, 32 * jp + 8 * g, a.hd);
+        }
+      }
+      if (hist && G > 1) flush(i);
+    }
+    const float back = 1.f / sc;
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+      const int s = 16 * (first + waves * kt) + c;
+      if (s >= seg.count) continue;
+      T* const row = static_cast<T*>(b.adj) + seg.row(s) * b.lda;
+#pragma unroll
+      for (int jp = 0; jp < DS; ++jp) {
+        if (!klive[kt]) dk[kt][2 * jp] = dk[kt][2 * jp + 1] = dv[kt][2 * jp] = dv[kt][2 * jp + 1] = f4{0.f, 0.f, 0.f, 0.f};
+        put8(row + (a.H + hk) * a.hd, dk[kt][2 * jp], dk[kt][2 * jp + 1], a.scale * back, 32 * jp + 8 * g, a.hd);
+        put8(row + (a.H + a.Hk + hk) * a.hd, dv[kt][2 * jp], dv[kt][2 * jp + 1], 1.f, 32 * jp + 8 * g, a.hd);
+      }
+    }
+  }
+  if (hist && G == 1) flush(0);
+}
+
 // ---- past 128 slots: a pass over the keys and one over the queries --------------------
 
 template <int HD>
@@ -245,7 +556,7 @@ struct KvLds {
 // as B operands, dK^T and dV^T in registers, and goes over all queries of the group's
 // heads, staged in LDS: S = Q K^T and dP = dO V^T with a lane's key in its column, so P
 // and dS are the B operands of dV^T += dO^T P and dK^T += Q^T dS as they lie.
-template <class T, int HD, int KT, bool BIAS, bool DROP>
+template <class T, int HD, int KT, bool WHOLE, bool BIAS, bool DROP>
 __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, int kblocks) {
   extern __shared__ __align__(16) char lds[];
   constexpr int DS = HD / 32, DT = HD / 16, per = 4 * KT * 16;
@@ -280,7 +591,7 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, i
     for (int k = 0; k < 3; ++k) m[k] = b.maxima[3 * threadIdx.x + k];
     block_max(m, room);
     const float bound = m[0] * m[1] * a.drop.scale + m[2];
-    units = scale_to(bound, 28);
+    units = scale_to(bound, 36);
     unit = bound < kInf ? 1.0 / double(units) : double(__builtin_nanf(""));  // (no unit holds an infinite dS)
     for (int i = threadIdx.x; i < a.nb * kColumns; i += 256) columns[i] = 0;
     for (int k = threadIdx.x; k < a.nb; k += 256)
@@ -305,8 +616,8 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, i
       const int s = k0 + 16 * kt + c;
       klive[kt] = seg.key(a, s);
       const int64_t row = klive[kt] ? seg.row(s) : 0;
-      own_pieces(a, kcols, a.ldq, seg, s, klive[kt], lane, kf[kt]);
-      own_pieces(a, vcols, a.ldq, seg, s, klive[kt], lane, vf[kt]);
+      own_pieces<T, WHOLE>(a, kcols, a.ldq, seg, s, klive[kt], lane, kf[kt]);
+      own_pieces<T, WHOLE>(a, vcols, a.ldq, seg, s, klive[kt], lane, vf[kt]);
       weight[kt] = klive[kt] ? log_weight(seg.cf(a, s)) : -kInf;
       if constexpr (BIAS) kpos[kt] = a.pos[row];
 #pragma unroll
@@ -321,7 +632,7 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, i
       }
       const T* const qcols = qkv + h * a.hd;
       const T* const gcols = static_cast<const T*>(b.out_adj) + h * a.hd;
-      Ahead<T, HD, kStage<HD>, true> ahead;
+      Ahead<T, HD, kStage<HD>, WHOLE, true> ahead;
       float next_expo = 0.f, next_delta = 0.f;
       int next_pos = 0;
       const auto load = [&](int q0) {
@@ -379,7 +690,9 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, i
             i4 qp{};
             if constexpr (BIAS) qp = *reinterpret_cast<const i4*>(qpos + at);
 #pragma unroll
-            for (int kt = 0; kt < KT; ++kt)
+            for (int kt = 0; kt < KT; ++kt) {
+              int column[4] = {};
+              float counted[4];
 #pragma unroll
               for (int r = 0; r < 4; ++r) {
                 float w = weight[kt];
@@ -387,6 +700,7 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, i
                 if constexpr (BIAS) {
                   be = lut[pair_index(kpos[kt], qp[r], a.reach)];
                   w += be.value;
+                  column[r] = be.column;
                 }
                 const float e = exp2_fast(fmaf(s[kt][r], a.scale2, w));
                 float kept = e;
@@ -396,8 +710,10 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, i
                 const float x = fmaf(HALF ? kept * sc : kept, dp[kt][r], -es * d4[r]);
                 ds[kt][4 * t + r] = x;
                 part_sum[kt] += x;
-                if (hist) count_in(mine, be, x * counts);
+                counted[r] = x * counts;
               }
+              if (hist) count_in(mine, column, counted);
+            }
           }
 #pragma unroll
           for (int kt = 0; kt < KT; ++kt) pf[kt] = pack8<T>(p[kt]), df[kt] = pack8<T>(ds[kt]);
@@ -440,7 +756,7 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, i
 
 // dQ: a wave has QT tiles of 16 queries as B operands and goes over the keys: S^T and
 // dP^T with a lane's query in its column, dS^T the B operand of dQ^T += K^T dS^T.
-template <class T, int HD, int QT, bool BIAS, bool DROP>
+template <class T, int HD, int QT, bool WHOLE, bool BIAS, bool DROP>
 __global__ __launch_bounds__(256, 2) void typed_bwd_q_kernel(Args a, Grads b, int qblocks) {
   extern __shared__ __align__(16) char lds[];
   constexpr int DS = HD / 32, DT = HD / 16, per = 4 * QT * 16;
@@ -482,8 +798,8 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_q_kernel(Args a, Grads b, in
       const int s = q0 + 16 * qt + c;
       const bool on = seg.query(a, s);
       qrow[qt] = on ? seg.row(s) : 0;
-      own_pieces(a, qcols, a.ldq, seg, s, on, lane, qf[qt]);
-      own_pieces(a, gcols, b.ldg, seg, s, on, lane, gf[qt]);
+      own_pieces<T, WHOLE>(a, qcols, a.ldq, seg, s, on, lane, qf[qt]);
+      own_pieces<T, WHOLE>(a, gcols, b.ldg, seg, s, on, lane, gf[qt]);
       expo[qt] = exponent(a, b, n, h, s, on);
       if constexpr (DROP) expo[qt] -= log2f(a.drop.scale);
       delta[qt] = on ? b.delta[qrow[qt] * a.H + h] / a.drop.scale : 0.f;
@@ -491,7 +807,7 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_q_kernel(Args a, Grads b, in
 #pragma unroll
       for (int j = 0; j < DT; ++j) dq[qt][j] = f4{0.f, 0.f, 0.f, 0.f};
     }
-    Ahead<T, HD, kStage<HD>, false> ahead;
+    Ahead<T, HD, kStage<HD>, WHOLE, false> ahead;
     float next_weight = 0.f;
     int next_pos = 0;
     const auto load = [&](int k0) {
@@ -667,10 +983,22 @@ extern "C" int pet_attn_bwd_typed(int dtype, const pet_attn_shape* shape, int kv
   const auto launched = [] { return hipGetLastError() == hipSuccess ? int(PET_ATTN_OK) : int(PET_ATTN_ELAUNCH); };
   const int err = a.N == 0 ? int(PET_ATTN_OK) : with_row_type(dtype, [&](auto tv) {
     using T = decltype(tv);
-    return with_head_dim(a.hd, [&](auto hc) {
+    return with_head_dim(a, [&](auto hc, auto wc) {
       constexpr int HD = decltype(hc)::value;
+      constexpr bool WHOLE = decltype(wc)::value;
       const auto run = [&](auto bc, auto dc) {
         constexpr bool BIAS = decltype(bc)::value, DROP = decltype(dc)::value;
+        if (a.S <= kShort) {
+          const ShortLds<HD> l(a, b.part != nullptr);
+          const auto kernel = a.S <= 64 ? typed_bwd_short_kernel<T, HD, 1, WHOLE, BIAS, DROP> : typed_bwd_short_kernel<T, HD, 2, WHOLE, BIAS, DROP>;
+          if (const int e = pet_attn::raise_lds(reinterpret_cast<const void*>(kernel), l.bytes)) return e;
+          const int64_t items = (int64_t(a.N) + 7) / 8 * 8;
+          slots = int(std::min<int64_t>(items, b.part ? std::clamp(4096 / a.Hk / 8 * 8, 8, kMaxSlots) : 4096));
+          if (int64_t(slots) * a.Hk * 256 > INT32_MAX) return int(PET_ATTN_EINDEX);
+          hipLaunchKernelGGL(kernel, dim3(unsigned(slots * a.Hk)), dim3(a.S <= 16 ? 64 : a.S <= 32 ? 128 : 256), l.bytes, st, a, b,
+                             l.rows, unsigned(l.stats), unsigned(l.more));
+          return launched();
+        }
         {
           const int64_t groups = int64_t(a.T) * (a.H + (b.norms ? a.Hk : 0));
           const unsigned blocks = unsigned(std::min<int64_t>((groups * (HD / 8) + 255) / 256, 16384));
@@ -683,7 +1011,7 @@ extern "C" int pet_attn_bwd_typed(int dtype, const pet_attn_shape* shape, int kv
         }
         {
           constexpr int KT = HD == 128 ? 1 : 2;
-          const auto kernel = typed_bwd_kv_kernel<T, HD, KT, BIAS, DROP>;
+          const auto kernel = typed_bwd_kv_kernel<T, HD, KT, WHOLE, BIAS, DROP>;
           const int blocks = (a.S + KT * 64 - 1) / (KT * 64);
           const int64_t items = (int64_t(a.N) * blocks + 7) / 8 * 8;
           const size_t bytes = KvLds<HD>::bytes(a, b.part != nullptr);
@@ -695,7 +1023,7 @@ extern "C" int pet_attn_bwd_typed(int dtype, const pet_attn_shape* shape, int kv
         }
         {
           constexpr int QT = 2;
-          const auto kernel = typed_bwd_q_kernel<T, HD, QT, BIAS, DROP>;
+          const auto kernel = typed_bwd_q_kernel<T, HD, QT, WHOLE, BIAS, DROP>;
           const int blocks = (a.S + QT * 64 - 1) / (QT * 64);
           const size_t bytes = size_t(kStage<HD>) * (2 * kPitch<HD> * 2 + 8) + 64 + (a.table ? size_t(2 * a.reach + 1) * 4 : 0);
           if (const int e = pet_attn::raise_lds(reinterpret_cast<const void*>(kernel), bytes)) return e;
