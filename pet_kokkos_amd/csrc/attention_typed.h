@@ -150,6 +150,9 @@ struct Segment {
   }
 };
 
+// The wave's number, known to be one for all of its lanes.
+__device__ __forceinline__ int wave_of() { return __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6); }
+
 // Dims d .. d + 7 of a row of hd, zeros past its end.
 template <class T>
 __device__ __forceinline__ u4 row_chunk(const T* row, int d, int hd) {

@@ -177,7 +177,7 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 4) void typed_fwd_short_kernel
   float* const weight = reinterpret_cast<float*>(vs + keys * kPitch<HD>);
   int* const kpos = reinterpret_cast<int*>(weight + keys);
   float* const lut = reinterpret_cast<float*>(kpos + keys);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = int(blockDim.x >> 6);
+  const int lane = threadIdx.x & 63, wave = wave_of(), waves = int(blockDim.x >> 6);
   const Share share(a.H);
   const int h = share.head, hk = h / (a.H / a.Hk);
   const T* const qkv = static_cast<const T*>(a.qkv);
@@ -222,7 +222,7 @@ __global__ __launch_bounds__(256, 2) void typed_fwd_long_kernel(Args a, int qblo
   float* const weight = reinterpret_cast<float*>(vs + KS * kPitch<HD>);
   int* const kpos = reinterpret_cast<int*>(weight + KS);
   float* const lut = reinterpret_cast<float*>(kpos + KS);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = wave_of();
   const Share share(a.H);
   const int h = share.head, hk = h / (a.H / a.Hk);
   const T* const qkv = static_cast<const T*>(a.qkv);

@@ -95,7 +95,7 @@ __global__ __launch_bounds__(256) void delta_kernel(Args a, Grads b) {
 
 // Three maxima over the workgroup: m of every thread of every wave. room: 3 floats a wave.
 __device__ __forceinline__ void block_max(float (&m)[3], float* room) {
-  const int waves = int(blockDim.x >> 6), wave = threadIdx.x >> 6;
+  const int waves = int(blockDim.x >> 6), wave = wave_of();
 #pragma unroll
   for (int i = 0; i < 3; ++i) m[i] = wave_max(m[i]);
   __syncthreads();
@@ -286,13 +286,14 @@ __device__ __forceinline__ float magnitude(unsigned m) {
 // queries a row, and once every wave is done with Q's rows and K's lie there, it is read
 // transposed for dQ^T += K^T dS^T, a tile of queries a wave: every product is formed once,
 // where the two passes past 128 slots form S, dP and their exponentials twice.
-template <class T, int HD, int KT, bool WHOLE, bool BIAS, bool DROP>
-__global__ __launch_bounds__(256, HD == 128 || (HD == 64 && KT == 2) ? 2 : 3) void typed_bwd_short_kernel(Args a, Grads b, int R,
+template <class T, int HD, int KT, bool GROUP, bool WHOLE, bool BIAS, bool DROP>
+__global__ __launch_bounds__(256, HD == 128 || (HD == 64 && KT == 2 && GROUP) ? 2 : 3) void typed_bwd_short_kernel(Args a, Grads b, int R,
                                                                                            unsigned stats, unsigned more) {
   extern __shared__ __align__(16) char lds[];
   constexpr int DS = HD / 32, DT = HD / 16, CH = HD / 8, P = kPitch<HD>;
+  constexpr int AT = GROUP ? KT : 1;  // tiles whose sums are kept: over a group's heads, or one at a time
   constexpr bool HALF = std::is_same<T, _Float16>::value;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = int(blockDim.x >> 6), c = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = wave_of(), waves = int(blockDim.x >> 6), c = lane & 15, g = lane >> 4;
   T* const qs = reinterpret_cast<T*>(lds);  // Q's rows, then K's
   T* const gs = qs + R * P;                 // dO's rows
   T* const dss = gs + R * P;                // dS, a key's queries a row
@@ -305,7 +306,7 @@ __global__ __launch_bounds__(256, HD == 128 || (HD == 64 && KT == 2) ? 2 : 3) vo
   BiasEntry* const lut = reinterpret_cast<BiasEntry*>(room + 16);
   int64_t* const columns = reinterpret_cast<int64_t*>(lut + (BIAS ? 2 * a.reach + 1 : 0));
   char* const mine = reinterpret_cast<char*>(columns + (lane & (kColumns - 1)));
-  const int G = a.H / a.Hk;
+  const int G = GROUP ? a.H / a.Hk : 1;
   const Share share(a.Hk);
   const int hk = share.head;
   const bool hist = BIAS && b.part;
@@ -331,7 +332,7 @@ __global__ __launch_bounds__(256, HD == 128 || (HD == 64 && KT == 2) ? 2 : 3) vo
     const Segment seg(a, n);
     const int rows = round_up(seg.count, 32), first = (wave + n) & (waves - 1);
     u4 kf[KT][DS], vf[KT][DS];
-    f4 dk[KT][DT], dv[KT][DT];
+    f4 dk[AT][DT], dv[AT][DT];
     float weight[KT];
     int kpos[KT];
     bool klive[KT];
@@ -347,10 +348,27 @@ __global__ __launch_bounds__(256, HD == 128 || (HD == 64 && KT == 2) ? 2 : 3) vo
       if (HALF || hist)
 #pragma unroll
         for (int d = 0; d < DS; ++d) onto_magnitude(vmax, vf[kt][d]);
-#pragma unroll
-      for (int j = 0; j < DT; ++j) dk[kt][j] = dv[kt][j] = f4{0.f, 0.f, 0.f, 0.f};
     }
+    const auto clear = [&](int at) {
+#pragma unroll
+      for (int j = 0; j < DT; ++j) dk[at][j] = dv[at][j] = f4{0.f, 0.f, 0.f, 0.f};
+    };
     float sc = 1.f;
+    // a tile's dK and dV to their rows
+    const auto store = [&](int kt, int at) {
+      const int s = 16 * (first + waves * kt) + c;
+      if (s >= seg.count) return;
+      T* const row = static_cast<T*>(b.adj) + seg.row(s) * b.lda;
+#pragma unroll
+      for (int jp = 0; jp < DS; ++jp) {
+        if (!klive[kt]) dk[at][2 * jp] = dk[at][2 * jp + 1] = dv[at][2 * jp] = dv[at][2 * jp + 1] = f4{0.f, 0.f, 0.f, 0.f};
+        put8(row + (a.H + hk) * a.hd, dk[at][2 * jp], dk[at][2 * jp + 1], a.scale / sc, 32 * jp + 8 * g, a.hd);
+        put8(row + (a.H + a.Hk + hk) * a.hd, dv[at][2 * jp], dv[at][2 * jp + 1], 1.f, 32 * jp + 8 * g, a.hd);
+      }
+    };
+    if constexpr (GROUP)
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt) clear(kt);
     for (int i = 0; i < G; ++i) {
       const int h = hk * G + i;
       const T* const qcols = qkv + h * a.hd;
@@ -415,11 +433,11 @@ __global__ __launch_bounds__(256, HD == 128 || (HD == 64 && KT == 2) ? 2 : 3) vo
         if constexpr (HALF) {
           const float was = sc;
           sc = scale_to(bound, 14);
-          if (i > 0 && sc != was)
+          if (GROUP && i > 0 && sc != was)
 #pragma unroll
-            for (int kt = 0; kt < KT; ++kt)
+            for (int at = 0; at < AT; ++at)
 #pragma unroll
-              for (int j = 0; j < DT; ++j) dk[kt][j] *= sc / was;
+              for (int j = 0; j < DT; ++j) dk[at][j] *= sc / was;
         }
         counts = units / sc;
       }
@@ -428,6 +446,8 @@ __global__ __launch_bounds__(256, HD == 128 || (HD == 64 && KT == 2) ? 2 : 3) vo
       for (int kt = 0; kt < KT; ++kt) {
         const int tile = first + waves * kt;
         if (16 * tile >= seg.count) continue;
+        const int at_tile = GROUP ? kt : 0;
+        if constexpr (!GROUP) clear(0);
         float cf_sum = 0.f;
 #pragma unroll 1
         for (int qb = 0; qb < rows; qb += 32) {
@@ -475,8 +495,8 @@ __global__ __launch_bounds__(256, HD == 128 || (HD == 64 && KT == 2) ? 2 : 3) vo
           *reinterpret_cast<u4*>(dss + (16 * tile + c) * pitch + qb + 8 * g) = df;
 #pragma unroll
           for (int j = 0; j < DT; ++j) {
-            dv[kt][j] = mfma<T>(transposed<T, HD>(gs, qb, j >> 1, j & 1, lane), pf, dv[kt][j]);
-            dk[kt][j] = mfma<T>(transposed<T, HD>(qs, qb, j >> 1, j & 1, lane), df, dk[kt][j]);
+            dv[at_tile][j] = mfma<T>(transposed<T, HD>(gs, qb, j >> 1, j & 1, lane), pf, dv[at_tile][j]);
+            dk[at_tile][j] = mfma<T>(transposed<T, HD>(qs, qb, j >> 1, j & 1, lane), df, dk[at_tile][j]);
           }
         }
         if (b.cfh) {
@@ -484,6 +504,7 @@ __global__ __launch_bounds__(256, HD == 128 || (HD == 64 && KT == 2) ? 2 : 3) vo
           const int s = 16 * tile + c;
           if (g == 0 && s < seg.count) b.cfh[(int64_t(n) * a.H + h) * a.S + s] = sum;
         }
+        if constexpr (!GROUP) store(kt, 0);
       }
       __syncthreads();
       // K's rows in the place of Q's; zeros for the tiles behind the last token's
@@ -523,19 +544,9 @@ __global__ __launch_bounds__(256, HD == 128 || (HD == 64 && KT == 2) ? 2 : 3) vo
       }
       if (hist && G > 1) flush(i);
     }
-    const float back = 1.f / sc;
+    if constexpr (GROUP)
 #pragma unroll
-    for (int kt = 0; kt < KT; ++kt) {
-      const int s = 16 * (first + waves * kt) + c;
-      if (s >= seg.count) continue;
-      T* const row = static_cast<T*>(b.adj) + seg.row(s) * b.lda;
-#pragma unroll
-      for (int jp = 0; jp < DS; ++jp) {
-        if (!klive[kt]) dk[kt][2 * jp] = dk[kt][2 * jp + 1] = dv[kt][2 * jp] = dv[kt][2 * jp + 1] = f4{0.f, 0.f, 0.f, 0.f};
-        put8(row + (a.H + hk) * a.hd, dk[kt][2 * jp], dk[kt][2 * jp + 1], a.scale * back, 32 * jp + 8 * g, a.hd);
-        put8(row + (a.H + a.Hk + hk) * a.hd, dv[kt][2 * jp], dv[kt][2 * jp + 1], 1.f, 32 * jp + 8 * g, a.hd);
-      }
-    }
+      for (int kt = 0; kt < KT; ++kt) store(kt, kt);
   }
   if (hist && G == 1) flush(0);
 }
@@ -561,7 +572,7 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, i
   extern __shared__ __align__(16) char lds[];
   constexpr int DS = HD / 32, DT = HD / 16, per = 4 * KT * 16;
   constexpr bool HALF = std::is_same<T, _Float16>::value;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = wave_of(), c = lane & 15, g = lane >> 4;
   T* const qs = reinterpret_cast<T*>(lds);
   T* const gs = qs + kStage<HD> * kPitch<HD>;
   float* const expo = reinterpret_cast<float*>(gs + kStage<HD> * kPitch<HD>);
@@ -761,7 +772,7 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_q_kernel(Args a, Grads b, in
   extern __shared__ __align__(16) char lds[];
   constexpr int DS = HD / 32, DT = HD / 16, per = 4 * QT * 16;
   constexpr bool HALF = std::is_same<T, _Float16>::value;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = wave_of(), c = lane & 15, g = lane >> 4;
   T* const ks = reinterpret_cast<T*>(lds);
   T* const vs = ks + kStage<HD> * kPitch<HD>;
   float* const weight = reinterpret_cast<float*>(vs + kStage<HD> * kPitch<HD>);
@@ -990,7 +1001,9 @@ extern "C" int pet_attn_bwd_typed(int dtype, const pet_attn_shape* shape, int kv
         constexpr bool BIAS = decltype(bc)::value, DROP = decltype(dc)::value;
         if (a.S <= kShort) {
           const ShortLds<HD> l(a, b.part != nullptr);
-          const auto kernel = a.S <= 64 ? typed_bwd_short_kernel<T, HD, 1, WHOLE, BIAS, DROP> : typed_bwd_short_kernel<T, HD, 2, WHOLE, BIAS, DROP>;
+          const auto kernel = a.S <= 64     ? typed_bwd_short_kernel<T, HD, 1, true, WHOLE, BIAS, DROP>
+                              : a.H > a.Hk ? typed_bwd_short_kernel<T, HD, 2, true, WHOLE, BIAS, DROP>
+                                           : typed_bwd_short_kernel<T, HD, 2, false, WHOLE, BIAS, DROP>;
           if (const int e = pet_attn::raise_lds(reinterpret_cast<const void*>(kernel), l.bytes)) return e;
           const int64_t items = (int64_t(a.N) + 7) / 8 * 8;
           slots = int(std::min<int64_t>(items, b.part ? std::clamp(4096 / a.Hk / 8 * 8, 8, kMaxSlots) : 4096));
