@@ -318,7 +318,13 @@ __device__ __forceinline__ void put8(T* row, const f4& lo, const f4& hi, float f
   float x[8];
 #pragma unroll
   for (int r = 0; r < 4; ++r) x[r] = lo[r] * f, x[4 + r] = hi[r] * f;
-  pet_typed::store<T>(row + d, hd - d, x);
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < hd - d) row[d + e] = x[e];
+  } else {
+    pet_typed::store<T>(row + d, hd - d, x);
+  }
 }
 
 // The offset of a pair in positions as an index 0 .. 2 reach (the difference does not wrap).

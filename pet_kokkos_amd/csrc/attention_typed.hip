@@ -29,7 +29,7 @@ struct Tiles {
   static constexpr int DS = HD / 32, DT = HD / 16;
   u4 qf[QT][DS];
   f4 o[QT][DT];
-  float top[QT], sum[QT];
+  float top[QT], base[QT], sum[QT];  // the largest logit, what exponents are taken from, their sum (log2 units)
   int64_t row[QT];
   int pos[QT];
   bool live[QT];
@@ -44,7 +44,7 @@ struct Tiles {
       if constexpr (BIAS) pos[qt] = a.pos[row[qt]];
 #pragma unroll
       for (int j = 0; j < DT; ++j) o[qt][j] = f4{0.f, 0.f, 0.f, 0.f};
-      top[qt] = -kInf, sum[qt] = 0.f;
+      top[qt] = base[qt] = -kInf, sum[qt] = 0.f;
     }
   }
 
@@ -92,15 +92,20 @@ struct Tiles {
         for (int t = 0; t < 2; ++t)
 #pragma unroll
           for (int r = 0; r < 4; ++r) m = fmaxf(m, s[qt][u][t][r]);
-      const float now = fmaxf(top[qt], pet_attn::max_g(m) * f);
-      const float base = now == -kInf ? 0.f : now;
-      if (k0 + kb > 0) {
-        const float fade = exp2_fast(top[qt] - base);
-        sum[qt] *= fade;
+      top[qt] = fmaxf(top[qt], pet_attn::max_g(m) * f);
+      // The sums move to a larger base only where the maximum has passed it by 2^8 (or is
+      // the first): their 4 HD / 16 products a tile were a fifth of a step's instructions.
+      if (__any(top[qt] > base[qt] + 8.f)) {
+        const float now = top[qt] == -kInf ? 0.f : top[qt];
+        if (k0 + kb > 0) {
+          const float fade = exp2_fast(base[qt] - now);
+          sum[qt] *= fade;
 #pragma unroll
-        for (int j = 0; j < DT; ++j) o[qt][j] *= fade;
+          for (int j = 0; j < DT; ++j) o[qt][j] *= fade;
+        }
+        base[qt] = top[qt];
       }
-      top[qt] = now;
+      const float from = base[qt] == -kInf ? 0.f : base[qt];
       u4 pf[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -115,7 +120,7 @@ struct Tiles {
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const float x = s[qt][u][t][r];
-            float e = exp2_fast(BIAS ? x - base : fmaf(x, f, -base));
+            float e = exp2_fast(BIAS ? x - from : fmaf(x, f, -from));
             sum[qt] += e;
             if constexpr (DROP) e = Drop::number(w, r) >= a.drop.least ? e : 0.f;
             p[4 * t + r] = e;
@@ -144,7 +149,7 @@ struct Tiles {
       const float inv = some ? 1.f / l : 0.f;
       if (ml && g == 0 && s < a.S)
         *reinterpret_cast<float2*>(ml + ((int64_t(seg.n) * a.H + h) * a.S + s) * 2) =
-            make_float2(some ? top[qt] * kLn2 : 0.f, inv);
+            make_float2(some ? top[qt] * kLn2 : 0.f, inv * exp2_fast(some ? top[qt] - base[qt] : 0.f));
       if (s < seg.count) {
         T* const to = merged + seg.row(s) * ldm + h * a.hd;
         const float f = DROP ? inv * a.drop.scale : inv;

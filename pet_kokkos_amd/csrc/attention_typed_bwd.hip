@@ -34,8 +34,11 @@ struct Grads {
   float* delta;   // [T, H]: dO.O
   float* norms;   // [T, H] |dO|, then [T, Hk] |v|: fp16, or a table's gradient
   float* maxima;  // [kMaxima, 3], with a table's gradient: of |dO|, |v| and |dO.O|
-  float* cfh;     // [N, H, S], or null
+  float* cfh;     // [queries_in, N, H, S], or null
   double* part;   // [slots, H, nb], with a table's gradient
+  // the pass over the keys in parts, of a group's heads by `heads_in`, of the queries by `queries_in`
+  int heads_in, queries_in;
+  float* kv;      // [parts, T, 2 Hk hd]: dK and dV of a part, where there is more than one
 };
 
 __device__ __forceinline__ float power_of_two(int e) { return ldexpf(1.f, e); }
@@ -610,11 +613,15 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, i
   }
   if (BIAS && G == 1) bias_entries(a, lut, hk);
 
-  const int items = a.N * kblocks;
+  const int parts = b.heads_in * b.queries_in, items = a.N * kblocks * parts;
   for (int item = share.slot; item < items; item += share.step) {
-    const int n = item / kblocks, kb = item - n * kblocks;
+    const int n = item / (kblocks * parts), kb = item / parts - n * kblocks, part = item % parts;
     const Segment seg(a, n);
     if (kb * per >= seg.count) continue;
+    const int hi = part % b.heads_in, qi = part / b.heads_in;
+    const int first_head = hi * (G / b.heads_in), last_head = first_head + G / b.heads_in;
+    const int q_each = round_up((seg.count + b.queries_in - 1) / b.queries_in, kStage<HD>);
+    const int q_first = min(qi * q_each, seg.count), q_last = min(q_first + q_each, seg.count);
     const float sc = adjoint_scale<T>(a, b, seg, hk, room), back = 1.f / sc, counts = hist ? units * back : 0.f;
     const int k0 = kb * per + wave * KT * 16;
     u4 kf[KT][DS], vf[KT][DS];
@@ -634,7 +641,7 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, i
 #pragma unroll
       for (int j = 0; j < DT; ++j) dk[kt][j] = dv[kt][j] = f4{0.f, 0.f, 0.f, 0.f};
     }
-    for (int i = 0; i < G; ++i) {
+    for (int i = first_head; i < last_head; ++i) {
       const int h = hk * G + i;
       float cf_sum[KT] = {};
       if (BIAS && G > 1) {
@@ -657,8 +664,8 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, i
           if constexpr (BIAS) next_pos = a.pos[row];
         }
       };
-      load(0);
-      for (int q0 = 0; q0 < seg.count; q0 += kStage<HD>) {
+      if (q_first < q_last) load(q_first);
+      for (int q0 = q_first; q0 < q_last; q0 += kStage<HD>) {
         const int n_queries = min(kStage<HD>, round_up(seg.count - q0, 32));
         __syncthreads();
         ahead.store(a, qs, qcols, a.ldq, gs, gcols, b.ldg, seg, q0);
@@ -669,7 +676,7 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, i
           if constexpr (BIAS) qpos[threadIdx.x] = next_pos;
         }
         __syncthreads();
-        if (q0 + kStage<HD> < seg.count) load(q0 + kStage<HD>);
+        if (q0 + kStage<HD> < q_last) load(q0 + kStage<HD>);
         if (k0 >= seg.count) continue;
         float part_sum[KT] = {};
         for (int qb = 0; qb < n_queries; qb += 32) {
@@ -745,7 +752,7 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, i
       for (int kt = 0; kt < KT; ++kt) {
         const float sum = pet_attn::sum_g(cf_sum[kt]) * back;
         const int s = k0 + 16 * kt + c;
-        if (b.cfh && g == 0 && s < seg.count) b.cfh[(int64_t(n) * a.H + h) * a.S + s] = sum;
+        if (b.cfh && g == 0 && s < seg.count) b.cfh[((int64_t(qi) * a.N + n) * a.H + h) * a.S + s] = sum;
       }
       if (hist && G > 1) flush_columns(columns, a.nb, unit, sums + i * a.nb);
     }
@@ -754,11 +761,18 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, i
       const int s = k0 + 16 * kt + c;
       if (s >= seg.count) continue;
       T* const row = static_cast<T*>(b.adj) + seg.row(s) * b.lda;
+      float* const sums_row = b.kv + ((int64_t(part) * a.T + seg.row(s)) * 2 * a.Hk + hk) * a.hd;
 #pragma unroll
       for (int jp = 0; jp < DS; ++jp) {
         if (!klive[kt]) dk[kt][2 * jp] = dk[kt][2 * jp + 1] = dv[kt][2 * jp] = dv[kt][2 * jp + 1] = f4{0.f, 0.f, 0.f, 0.f};
-        put8(row + (a.H + hk) * a.hd, dk[kt][2 * jp], dk[kt][2 * jp + 1], a.scale * back, 32 * jp + 8 * g, a.hd);
-        put8(row + (a.H + a.Hk + hk) * a.hd, dv[kt][2 * jp], dv[kt][2 * jp + 1], 1.f, 32 * jp + 8 * g, a.hd);
+        const int d = 32 * jp + 8 * g;
+        if (parts > 1) {
+          put8(sums_row, dk[kt][2 * jp], dk[kt][2 * jp + 1], a.scale * back, d, a.hd);
+          put8(sums_row + a.Hk * a.hd, dv[kt][2 * jp], dv[kt][2 * jp + 1], 1.f, d, a.hd);
+        } else {
+          put8(row + (a.H + hk) * a.hd, dk[kt][2 * jp], dk[kt][2 * jp + 1], a.scale * back, d, a.hd);
+          put8(row + (a.H + a.Hk + hk) * a.hd, dv[kt][2 * jp], dv[kt][2 * jp + 1], 1.f, d, a.hd);
+        }
       }
     }
   }
@@ -899,8 +913,30 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_q_kernel(Args a, Grads b, in
   }
 }
 
-// cf_adj[n][k] = beta cf_adj[n][k] + (sum over heads in order of cfh[n][h][k]) / cf (keys that count)
-__global__ __launch_bounds__(256) void typed_cf_kernel(Args a, const float* cfh, float* adj, int64_t lda, float beta) {
+// dK and dV of the parts, summed in order and rounded once: a thread has four columns of a token's row.
+template <class T>
+__global__ __launch_bounds__(256) void typed_kv_sum_kernel(Args a, Grads b) {
+  const int width = 2 * a.Hk * a.hd, quads = (width + 3) / 4, parts = b.heads_in * b.queries_in;
+  const int64_t last = int64_t(a.N) + a.off[a.N], rows = last < 0 ? 0 : last < a.T ? last : a.T;
+  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < rows * quads; i += int64_t(gridDim.x) * 256) {
+    const int64_t row = i / quads;
+    const int c = int(i - row * quads) * 4, n = min(4, width - c);
+    float sum[4] = {};
+    for (int p = 0; p < parts; ++p) {
+      const float* const from = b.kv + (int64_t(p) * a.T + row) * width + c;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (e < n) sum[e] += from[e];
+    }
+    T* const to = static_cast<T*>(b.adj) + row * b.lda + a.H * a.hd + c;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < n) to[e] = T(sum[e]);
+  }
+}
+
+// cf_adj[n][k] = beta cf_adj[n][k] + (sum over heads and parts in order of cfh[part][n][h][k]) / cf (keys that count)
+__global__ __launch_bounds__(256) void typed_cf_kernel(Args a, const float* cfh, int parts, float* adj, int64_t lda, float beta) {
   const int64_t all = int64_t(a.N) * a.S;
   for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < all; i += int64_t(gridDim.x) * 256) {
     const int64_t n = i / a.S;
@@ -908,7 +944,8 @@ __global__ __launch_bounds__(256) void typed_cf_kernel(Args a, const float* cfh,
     const Segment seg(a, int(n));
     float sum = 0.f;
     if (seg.key(a, s)) {
-      for (int h = 0; h < a.H; ++h) sum += cfh[(n * a.H + h) * a.S + s];
+      for (int h = 0; h < a.H; ++h)
+        for (int p = 0; p < parts; ++p) sum += cfh[((int64_t(p) * a.N + n) * a.H + h) * a.S + s];
       sum /= seg.cf(a, s);
     }
     float* const to = adj + n * lda + s;
@@ -935,16 +972,39 @@ __global__ __launch_bounds__(1024) void typed_table_kernel(const double* part, i
 
 constexpr size_t aligned(size_t n) { return (n + 255) & ~size_t(255); }
 
+// Tiles of 16 keys a wave of the pass over the keys, by head_dim: two share each read of
+// the staged queries, where their dK and dV leave registers for the rest.
+template <int HD>
+constexpr int kKeyTiles = HD == 128 ? 1 : 2;
+
+// The parts of the pass over the keys: a chip holds two workgroups a CU of it, so with
+// fewer than 512 of them a group's heads, then the queries, are shared out, at the cost of
+// writing and reading fp32 sums.
+struct Parts {
+  int heads = 1, queries = 1;
+  Parts(int N, int S, int H, int Hk, int hd) {
+    if (S <= kShort) return;
+    const int tile = 64 * (hd > 64 ? kKeyTiles<128> : kKeyTiles<64>), G = H / Hk;
+    const int64_t have = std::max<int64_t>(1, int64_t(N) * ((int64_t(S) + tile - 1) / tile) * Hk);
+    const int64_t want = (512 + have - 1) / have;
+    while (heads < G && (heads < want || G % heads != 0)) ++heads;
+    queries = int(std::min<int64_t>((want + heads - 1) / heads, (int64_t(S) + 511) / 512));
+  }
+};
+
 struct Workspace {
-  size_t delta, norms, maxima, cfh, part, bytes;
+  size_t delta, norms, maxima, cfh, part, kv, bytes;
   Workspace(int dtype, const pet_attn_shape& s, int kv_heads, int nb) {
     const size_t T = size_t(s.n_rows), H = size_t(s.heads);
+    const Parts parts(s.n_atoms, s.slots, s.heads, kv_heads, s.head_dim);
     delta = 0;
     norms = delta + aligned(T * H * 4);
     maxima = norms + (dtype == PET_DTYPE_F16 || nb ? aligned(T * (H + size_t(kv_heads)) * 4) : 0);
     cfh = maxima + aligned(nb ? size_t(kMaxima) * 12 : 0);
-    part = cfh + aligned(size_t(s.n_atoms) * H * size_t(s.slots) * 4);
-    bytes = part + aligned(size_t(kMaxSlots) * H * size_t(nb) * 8);
+    part = cfh + aligned(size_t(parts.queries) * size_t(s.n_atoms) * H * size_t(s.slots) * 4);
+    kv = part + aligned(size_t(kMaxSlots) * H * size_t(nb) * 8);
+    const size_t all = size_t(parts.heads) * size_t(parts.queries);
+    bytes = kv + (all > 1 ? aligned(all * T * 2 * size_t(kv_heads) * size_t(s.head_dim) * 4) : 0);
   }
 };
 
@@ -955,7 +1015,8 @@ using namespace pet_tattn;
 
 extern "C" size_t pet_attn_bwd_typed_workspace(int dtype, const pet_attn_shape* shape, int kv_heads, int n_buckets) {
   if (!shape || (dtype != PET_DTYPE_BF16 && dtype != PET_DTYPE_F16) || kv_heads < 1 || shape->heads < 1 ||
-      shape->heads % kv_heads != 0 || shape->n_atoms < 0 || shape->n_rows < 0 || shape->slots < 1 || n_buckets < 0 ||
+      shape->heads % kv_heads != 0 || shape->n_atoms < 0 || shape->n_rows < 0 || shape->slots < 1 || shape->head_dim < 1 ||
+      shape->head_dim > 128 || n_buckets < 0 ||
       n_buckets > PET_BIAS_MAX_BUCKETS)
     return 0;
   return Workspace(dtype, *shape, kv_heads, n_buckets).bytes;
@@ -984,10 +1045,11 @@ extern "C" int pet_attn_bwd_typed(int dtype, const pet_attn_shape* shape, int kv
   char* const base = static_cast<char*>(workspace);
   a.whole = a.whole && narrow(a, ldg) && narrow(a, ldm);
   const bool half = dtype == PET_DTYPE_F16;
+  const Parts parts(a.N, a.S, a.H, a.Hk, a.hd);
   const auto at = [&](size_t offset) { return reinterpret_cast<float*>(base + offset); };
   const Grads b{dmerged, merged, ldg, ldm, ml, qkv_adj, lda, at(ws.delta), half || table_adj ? at(ws.norms) : nullptr,
                 table_adj ? at(ws.maxima) : nullptr, cf_seq_adj ? at(ws.cfh) : nullptr,
-                table_adj ? reinterpret_cast<double*>(base + ws.part) : nullptr};
+                table_adj ? reinterpret_cast<double*>(base + ws.part) : nullptr, parts.heads, parts.queries, at(ws.kv)};
   if (shape->dead && a.T > 0)
     if (const int e = zero_dead(a, qkv_adj, lda, W, st)) return e;
   int slots = 0;
@@ -1023,16 +1085,22 @@ extern "C" int pet_attn_bwd_typed(int dtype, const pet_attn_shape* shape, int kv
           }
         }
         {
-          constexpr int KT = HD == 128 ? 1 : 2;
+          constexpr int KT = kKeyTiles<HD>;
           const auto kernel = typed_bwd_kv_kernel<T, HD, KT, WHOLE, BIAS, DROP>;
           const int blocks = (a.S + KT * 64 - 1) / (KT * 64);
-          const int64_t items = (int64_t(a.N) * blocks + 7) / 8 * 8;
+          const int64_t items = (int64_t(a.N) * blocks * parts.heads * parts.queries + 7) / 8 * 8;
           const size_t bytes = KvLds<HD>::bytes(a, b.part != nullptr);
           if (const int e = pet_attn::raise_lds(reinterpret_cast<const void*>(kernel), bytes)) return e;
           slots = int(std::min<int64_t>(items, b.part ? std::clamp(2048 / a.Hk / 8 * 8, 8, kMaxSlots) : kMaxSlots));
           if (int64_t(slots) * a.Hk * 256 > INT32_MAX) return int(PET_ATTN_EINDEX);
           hipLaunchKernelGGL(kernel, dim3(unsigned(slots * a.Hk)), dim3(256), bytes, st, a, b, blocks);
           if (const int e = launched()) return e;
+          if (parts.heads * parts.queries > 1) {
+            const int64_t quads = int64_t(a.T) * ((2 * a.Hk * a.hd + 3) / 4);
+            hipLaunchKernelGGL(typed_kv_sum_kernel<T>, dim3(unsigned(std::min<int64_t>((quads + 255) / 256, 8192))), dim3(256), 0,
+                               st, a, b);
+            if (const int e = launched()) return e;
+          }
         }
         {
           constexpr int QT = 2;
@@ -1053,7 +1121,7 @@ extern "C" int pet_attn_bwd_typed(int dtype, const pet_attn_shape* shape, int kv
   if (err) return err;
   if (cf_seq_adj && a.N > 0) {
     const int64_t blocks = std::min<int64_t>((int64_t(a.N) * a.S + 255) / 256, 16384);
-    hipLaunchKernelGGL(typed_cf_kernel, dim3(unsigned(blocks)), dim3(256), 0, st, a, b.cfh, cf_seq_adj, ldca, beta);
+    hipLaunchKernelGGL(typed_cf_kernel, dim3(unsigned(blocks)), dim3(256), 0, st, a, b.cfh, parts.queries, cf_seq_adj, ldca, beta);
     if (hipGetLastError() != hipSuccess) return PET_ATTN_ELAUNCH;
   }
   if (table_adj) {
