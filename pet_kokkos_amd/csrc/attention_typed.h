@@ -13,8 +13,7 @@
 // product as the B operand of the next without an exchange: of 32 tokens,
 // instruction t (0, 1) computes those 8a + 4t + r (a, r = 0 .. 3) as its rows 4a + r,
 // so a lane ends with tokens 8g .. 8g + 7, which is what B wants of it. LDS rows lie
-// in that order (lds_row). The same map over pairs of 16-dim tiles gives a lane
-// eight consecutive dims of its token's output: one 16-byte store.
+// in that order (lds_row).
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -60,49 +59,53 @@ __device__ __forceinline__ u2 lds_tr(const T* p) {
   return __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(p)));
 }
 
-// An LDS row's elements: HD dims and 16 bytes of padding, so that the 16 rows that a
-// wave reads at once start in different banks. Of each 32 dims, the pieces of four go
-// 0 2 4 6 1 3 5 7: those that `transposed` reads for one tile lie side by side (apart, its
-// reads took half of the banks twice), and a product over dims has them in any order
-// that both its operands have.
+// An LDS row is a token's HD dims in 16-byte pieces, piece p at p ^ row_key(row): the
+// pieces that a wave reads at once, one of each of 16 rows or two of each of 16, lie in
+// different banks without padding, and rows can be loaded into LDS straight from memory,
+// a wave's 64 pieces in a line.
 template <int HD>
-constexpr int kPitch = HD + 8;
+__device__ __forceinline__ int row_key(int row) {
+  return HD == 128 ? row & 15 : HD == 64 ? row >> 1 & 7 : row >> 2 & 3;
+}
 
 // The most slots whose atoms a workgroup holds whole.
 constexpr int kShort = 128;
 
-// Tokens a stage past that: the registers that hold the next one while the present
-// one is used leave room for the rest at 32 of 128 dims (at 64, 200 to 400 bytes a lane
-// of the kernels' were spilled).
-template <int HD>
-constexpr int kStage = HD == 128 ? 32 : 64;
+// Tokens a stage past that, two stages in LDS.
+constexpr int kStage = 64;
 
-// Where token k of a stage lies: of each 32, tokens 8a + 4t + r at row 16t + 4a + r.
+// Where token k of a stage lies: of each 32, tokens 8a + 4t + r at row 16t + 4a + r; and the token of a row.
 __device__ __forceinline__ int lds_row(int k) {
   return (k & ~31) | (k & 4) << 2 | (k & 24) >> 1 | (k & 3);
 }
+__device__ __forceinline__ int row_token(int row) {
+  return (row & ~31) | (row & 12) << 1 | (row & 16) >> 2 | (row & 3);
+}
 
 // The A operand of a product over 32 staged tokens (rows base .. base + 31): row m of
-// it is dim 32 jp + 8 (m / 4) + 4 t + m % 4.
+// it is dim 16 j + m.
 template <class T, int HD>
-__device__ __forceinline__ u4 transposed(const T* rows, int base, int jp, int t, int lane) {
-  const int i = lane & 15, g = lane >> 4;
-  const T* p = rows + (base + 4 * g + (i >> 2)) * kPitch<HD> + 32 * jp + 16 * t + 4 * (i & 3);
-  const u2 lo = lds_tr(p), hi = lds_tr(p + 16 * kPitch<HD>);
+__device__ __forceinline__ u4 transposed(const T* rows, int base, int j, int lane) {
+  const int i = lane & 15, row = 4 * (lane >> 4) + (i >> 2);
+  const T* p = rows + base * HD + row * HD + ((8 * ((i & 3) >> 1 ^ row_key<HD>(row)) + 4 * (i & 1)) ^ 16 * j);
+  const u2 lo = lds_tr(p), hi = lds_tr(p + 16 * HD);
   return u4{lo[0], lo[1], hi[0], hi[1]};
 }
 // Its plain A operand: rows 16t .. 16t + 15 of the 32 at base, dims 32 step .. + 31.
 template <class T, int HD>
 __device__ __forceinline__ u4 straight(const T* rows, int base, int t, int step, int lane) {
-  return *reinterpret_cast<const u4*>(rows + (base + 16 * t + (lane & 15)) * kPitch<HD> + 32 * step + 8 * (lane >> 4));
+  const int c = lane & 15;
+  return *reinterpret_cast<const u4*>(rows + (base + 16 * t) * HD + c * HD + (8 * (lane >> 4 ^ row_key<HD>(c)) ^ 32 * step));
 }
 // Dims 8 ch .. + 7 of a row into its place.
-template <class T>
-__device__ __forceinline__ void put_piece(T* row, int ch, const u4& x) {
-  T* const at = row + 32 * (ch >> 2) + 4 * (ch & 3);
-  *reinterpret_cast<u2*>(at) = u2{x[0], x[1]};
-  *reinterpret_cast<u2*>(at + 16) = u2{x[2], x[3]};
+template <class T, int HD>
+__device__ __forceinline__ void put_piece(T* rows, int row, int ch, const u4& x) {
+  *reinterpret_cast<u4*>(rows + row * HD + 8 * (ch ^ row_key<HD>(row))) = x;
 }
+
+// Reads ahead of this are sent before what follows, which waits for them one by one: left
+// to itself the compiler reads an operand, waits and multiplies, one after the other.
+__device__ __forceinline__ void reads_first() { __builtin_amdgcn_sched_barrier(0); }
 
 template <class T>
 __device__ __forceinline__ u4 pack8(const float (&x)[8]) {
@@ -193,9 +196,9 @@ __device__ __forceinline__ void stage_pair(const Args& a, T* xs, const T* xsrc, 
   const int nt = blockDim.x, total = n * CH, last = seg.count - 1;
   const Column xc(xsrc, ldx, seg), yc(ysrc, ldy, seg);
   const auto put = [&](int i, const u4& x, const u4& y, bool on, const auto& m) {
-    const int k = i / CH, row = lds_row(k) * kPitch<HD>;
-    put_piece(xs + row, i % CH, x);
-    put_piece(ys + row, i % CH, y);
+    const int k = i / CH, row = lds_row(k);
+    put_piece<T, HD>(xs, row, i % CH, x);
+    put_piece<T, HD>(ys, row, i % CH, y);
     take(k, i % CH, x, y, on, m);
   };
   if constexpr (!WHOLE) {
@@ -225,7 +228,7 @@ __device__ __forceinline__ void stage_pair(const Args& a, T* xs, const T* xsrc, 
       x[j] = __builtin_bit_cast(u4, *reinterpret_cast<const u4e*>(xc.at(at, d)));
       y[j] = __builtin_bit_cast(u4, *reinterpret_cast<const u4e*>(yc.at(at, d)));
       m[j] = more(at, d);
-      on[j] = s <= last && ch < a.hd && (w > 0.f || (QUERY && s == 0));
+      on[j] = (s <= last) & (ch < a.hd) & ((w > 0.f) | (QUERY && s == 0));
     }
 #pragma unroll
     for (int j = 0; j < EACH; ++j)
@@ -233,97 +236,117 @@ __device__ __forceinline__ void stage_pair(const Args& a, T* xs, const T* xsrc, 
   }
 }
 
-// The same for kernels of 256 threads that go over stages of KS slots: the loads of the
-// next stage go out before the present one is used (not WHOLE: they are loaded as they are
-// stored).
-template <class T, int HD, int KS, bool WHOLE, bool QUERY>
+// 16 bytes a lane from memory into LDS, a wave's 64 lanes to dst .. dst + 1 KB in their
+// order (dst one for the wave).
+__device__ __forceinline__ void to_lds(const void* src, void* dst) {
+  __builtin_amdgcn_global_load_lds(src, reinterpret_cast<u4*>(dst), 16, 0, 0);
+}
+// Every load of this wave has landed.
+__device__ __forceinline__ void wait_loads() {
+  __builtin_amdgcn_s_waitcnt(7 << 4 | 15 << 8);  // vmcnt(0) alone
+  asm volatile("" ::: "memory");
+}
+// The workgroup's barrier with this wave's LDS accesses done and its loads still on their
+// way: a fence would wait for those too.
+__device__ __forceinline__ void stage_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(15 | 3 << 14 | 7 << 4);  // lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// Stages of kStage slots of two columns for kernels of 256 threads, loaded into LDS past
+// the registers while the stage before is used: start() sends the loads, land() waits
+// for this thread's and puts zeros over what is left out, and a stage_barrier makes the
+// stage everyone's. (Not WHOLE: land() loads and stores.)
+template <class T, int HD, bool WHOLE, bool QUERY>
 struct Ahead {
-  static constexpr int CH = HD / 8, EACH = KS * CH / 256;
-  u4 x[EACH], y[EACH];
-  bool on[EACH];
-  __device__ __forceinline__ void load(const Args& a, const T* xsrc, int64_t ldx, const T* ysrc, int64_t ldy,
-                                       const Segment& seg, int s0) {
+  static constexpr int CH = HD / 8, EACH = kStage * CH / 256;
+  float w[EACH];
+  __device__ __forceinline__ void start(const Args& a, T* xs, const T* xsrc, int64_t ldx, T* ys, const T* ysrc,
+                                        int64_t ldy, const Segment& seg, int s0) {
     if constexpr (!WHOLE) return;
-    const int last = seg.count - 1;
+    const int last = seg.count - 1, wave = wave_of();
     const Column xc(xsrc, ldx, seg), yc(ysrc, ldy, seg);
 #pragma unroll
     for (int j = 0; j < EACH; ++j) {
-      const int i = threadIdx.x + 256 * j, s = s0 + i / CH, ch = 8 * (i % CH), at = s < last ? s : last;
-      const int d = ch < a.hd ? ch : 0;
-      const float w = seg.cf(a, at);
-      x[j] = __builtin_bit_cast(u4, *reinterpret_cast<const u4e*>(xc.at(at, d)));
-      y[j] = __builtin_bit_cast(u4, *reinterpret_cast<const u4e*>(yc.at(at, d)));
-      on[j] = s <= last && ch < a.hd && (w > 0.f || (QUERY && s == 0));
+      const int i = threadIdx.x + 256 * j, row = i / CH, ch = 8 * (i % CH ^ row_key<HD>(row));
+      const int s = s0 + row_token(row), at = s < last ? s : last, d = ch < a.hd ? ch : 0, to = (64 * wave + 256 * j) * 8;
+      to_lds(xc.at(at, d), xs + to);
+      to_lds(yc.at(at, d), ys + to);
+      w[j] = seg.cf(a, at);
     }
   }
-  __device__ __forceinline__ void store(const Args& a, T* xs, const T* xsrc, int64_t ldx, T* ys, const T* ysrc,
-                                        int64_t ldy, const Segment& seg, int s0) const {
-    if constexpr (!WHOLE) {
+  __device__ __forceinline__ void land(const Args& a, T* xs, const T* xsrc, int64_t ldx, T* ys, const T* ysrc,
+                                       int64_t ldy, const Segment& seg, int s0) const {
+    const u4 none = {0u, 0u, 0u, 0u};
+    if constexpr (WHOLE) {
+      wait_loads();
+#pragma unroll
+      for (int j = 0; j < EACH; ++j) {
+        const int i = threadIdx.x + 256 * j, row = i / CH, ch = 8 * (i % CH ^ row_key<HD>(row)), s = s0 + row_token(row);
+        const bool on = (s < seg.count) & (ch < a.hd) & ((w[j] > 0.f) | (QUERY && s == 0));
+        if (!on) {
+          *reinterpret_cast<u4*>(xs + 8 * i) = none;
+          *reinterpret_cast<u4*>(ys + 8 * i) = none;
+        }
+      }
+    } else {
 #pragma unroll 1
-      for (int i = threadIdx.x; i < KS * CH; i += 256) {
-        const int s = s0 + i / CH, d = 8 * (i % CH), row = lds_row(i / CH) * kPitch<HD>;
-        u4 u = {0u, 0u, 0u, 0u}, v = u;
+      for (int i = threadIdx.x; i < kStage * CH; i += 256) {
+        const int s = s0 + i / CH, d = 8 * (i % CH), row = lds_row(i / CH);
+        u4 u = none, v = none;
         if (QUERY ? seg.query(a, s) : seg.key(a, s)) {
           u = row_chunk(xsrc + seg.row(s) * ldx, d, a.hd);
           v = row_chunk(ysrc + seg.row(s) * ldy, d, a.hd);
         }
-        put_piece(xs + row, i % CH, u);
-        put_piece(ys + row, i % CH, v);
+        put_piece<T, HD>(xs, row, i % CH, u);
+        put_piece<T, HD>(ys, row, i % CH, v);
       }
-      return;
-    }
-#pragma unroll
-    for (int j = 0; j < EACH; ++j) {
-      const int i = threadIdx.x + 256 * j, row = lds_row(i / CH) * kPitch<HD>;
-      put_piece(xs + row, i % CH, where(on[j], x[j]));
-      put_piece(ys + row, i % CH, where(on[j], y[j]));
     }
   }
 };
 
-// A lane's B operands of a token's own columns (slot s, zeros unless live): of dims 32
-// step .. + 31 the pieces that lie at 8g of an LDS row.
+// A lane's B operands of a token's own columns (slot s, zeros unless live): dims 32 step + 8g .. + 7.
 template <class T, bool WHOLE, int DS>
 __device__ __forceinline__ void own_pieces(const Args& a, const T* src, int64_t ld, const Segment& seg, int s, bool live,
                                            int lane, u4 (&out)[DS]) {
-  const int g = lane >> 4, d0 = 16 * (g & 1) + 4 * (g >> 1);
+  const int d0 = 8 * (lane >> 4);
   if constexpr (WHOLE) {
     const Column col(src, ld, seg);
     const int at = s < seg.count ? s : 0;
 #pragma unroll
     for (int step = 0; step < DS; ++step) {
       const int d = 32 * step + d0;
-      const u2 lo = __builtin_bit_cast(u2, *reinterpret_cast<const u2e*>(col.at(at, d < a.hd ? d : 0)));
-      const u2 hi = __builtin_bit_cast(u2, *reinterpret_cast<const u2e*>(col.at(at, d + 8 < a.hd ? d + 8 : 0)));
-      const bool l = live && d < a.hd, h = live && d + 8 < a.hd;
-      out[step] = u4{l ? lo[0] : 0u, l ? lo[1] : 0u, h ? hi[0] : 0u, h ? hi[1] : 0u};
+      const u4 x = __builtin_bit_cast(u4, *reinterpret_cast<const u4e*>(col.at(at, d < a.hd ? d : 0)));
+      out[step] = where(live && d < a.hd, x);
     }
   } else {
     const T* const row = src + (live ? seg.row(s) : 0) * ld;
 #pragma unroll
     for (int step = 0; step < DS; ++step) {
       out[step] = u4{0u, 0u, 0u, 0u};
-      if (live) {
-        const u4 lo = row_chunk(row, 32 * step + d0, a.hd), hi = row_chunk(row, 32 * step + d0 + 8, a.hd);
-        out[step] = u4{lo[0], lo[1], hi[0], hi[1]};
-      }
+      if (live) out[step] = row_chunk(row, 32 * step + d0, a.hd);
     }
   }
 }
 
-// A row's eight dims 32 jp + 8g of a result's tile pair, times f.
+// A row's dims 16 j + 4g .. + 3 of a result's tile, times f.
 template <class T>
-__device__ __forceinline__ void put8(T* row, const f4& lo, const f4& hi, float f, int d, int hd) {
-  if (d >= hd) return;
-  float x[8];
+__device__ __forceinline__ void put4(T* row, const f4& x, float f, int d, int hd) {
+  if (d + 4 <= hd) {
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-  for (int r = 0; r < 4; ++r) x[r] = lo[r] * f, x[4 + r] = hi[r] * f;
-  if constexpr (sizeof(T) == 4) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (e < hd - d) row[d + e] = x[e];
+      for (int r = 0; r < 4; ++r) row[d + r] = x[r] * f;
+    } else {
+      typedef T t4 __attribute__((ext_vector_type(4)));
+      const t4 y = {T(x[0] * f), T(x[1] * f), T(x[2] * f), T(x[3] * f)};
+      *reinterpret_cast<u2e*>(row + d) = __builtin_bit_cast(u2e, y);
+    }
   } else {
-    pet_typed::store<T>(row + d, hd - d, x);
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (d + r < hd) row[d + r] = T(x[r] * f);
   }
 }
 

@@ -19,7 +19,7 @@ namespace pet_tattn {
 namespace {
 
 template <int HD>
-constexpr int fwd_stage_bytes(int keys) { return keys * (2 * kPitch<HD> * 2 + 8); }
+constexpr int fwd_stage_bytes(int keys) { return keys * (2 * HD * 2 + 8); }
 
 // The tiles of 16 queries at q[], QT of them, against staged keys kb .. kb + 32 U - 1
 // (slots k0 + kb ..; those past n_keys do not count): scores, the running maximum and sum,
@@ -27,6 +27,8 @@ constexpr int fwd_stage_bytes(int keys) { return keys * (2 * kPitch<HD> * 2 + 8)
 template <class T, int HD, int QT, int U, bool WHOLE, bool BIAS, bool DROP>
 struct Tiles {
   static constexpr int DS = HD / 32, DT = HD / 16;
+  // Operands read ahead of their products: two waves a SIMD need it, and have the registers.
+  static constexpr bool EAGER = QT > 1;
   u4 qf[QT][DS];
   f4 o[QT][DT];
   float top[QT], base[QT], sum[QT];  // the largest logit, what exponents are taken from, their sum (log2 units)
@@ -48,6 +50,15 @@ struct Tiles {
     }
   }
 
+  // the biases of four keys
+  __device__ __forceinline__ void gather(const Args& a, float (&b)[QT][2][4], int t, const int* kpos, const float* lut) {
+    const i4 kp = *reinterpret_cast<const i4*>(kpos);
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) b[qt][t][r] = lut[pair_index(kp[r], pos[qt], a.reach)];
+  }
+
   __device__ __forceinline__ void keys(const Args& a, const Words& key, int h, const T* ks, const T* vs,
                                        const float* weight, const int* kpos, const float* lut, int k0, int kb, int n_keys,
                                        int lane) {
@@ -60,27 +71,48 @@ struct Tiles {
         for (int qt = 0; qt < QT; ++qt) s[qt][u][0] = s[qt][u][1] = f4{-kInf, -kInf, -kInf, -kInf};
         continue;
       }
+      u4 kf[2][DS];
+      float b[QT][2][4];
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         const int at = kb + 32 * u + 8 * g + 4 * t;
         const f4 w = *reinterpret_cast<const f4*>(weight + at);
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt) s[qt][u][t] = w;
+        if constexpr (EAGER) {
 #pragma unroll
-        for (int d = 0; d < DS; ++d) {
-          const u4 kf = straight<T, HD>(ks, kb + 32 * u, t, d, lane);
-#pragma unroll
-          for (int qt = 0; qt < QT; ++qt) s[qt][u][t] = mfma<T>(kf, qf[qt][d], s[qt][u][t]);
+          for (int d = 0; d < DS; ++d) kf[t][d] = straight<T, HD>(ks, kb + 32 * u, t, d, lane);
+          if constexpr (BIAS) gather(a, b, t, kpos + at, lut);
         }
-        if constexpr (BIAS) {
-          const i4 kp = *reinterpret_cast<const i4*>(kpos + at);
+      }
+      if constexpr (EAGER) reads_first();
+#pragma unroll
+      for (int d = 0; d < DS; ++d)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const u4 k = EAGER ? kf[t][d] : straight<T, HD>(ks, kb + 32 * u, t, d, lane);
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt) s[qt][u][t] = mfma<T>(k, qf[qt][d], s[qt][u][t]);
+        }
+      if constexpr (BIAS)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if constexpr (!EAGER) gather(a, b, t, kpos + kb + 32 * u + 8 * g + 4 * t, lut);
 #pragma unroll
           for (int qt = 0; qt < QT; ++qt)
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-              s[qt][u][t][r] = fmaf(s[qt][u][t][r], a.scale2, lut[pair_index(kp[r], pos[qt], a.reach)]);
+            for (int r = 0; r < 4; ++r) s[qt][u][t][r] = fmaf(s[qt][u][t][r], a.scale2, b[qt][t][r]);
         }
-      }
+    }
+    // the values' operands, on their way while the probabilities are made
+    u4 vt[U][DT];
+    if constexpr (EAGER) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (u == 0 || kb + 32 * u < n_keys)
+#pragma unroll
+          for (int j = 0; j < DT; ++j) vt[u][j] = transposed<T, HD>(vs, kb + 32 * u, j, lane);
+      reads_first();
     }
     const float f = BIAS ? 1.f : a.scale2;
 #pragma unroll
@@ -133,7 +165,7 @@ struct Tiles {
         if (u > 0 && kb + 32 * u >= n_keys) continue;
 #pragma unroll
         for (int j = 0; j < DT; ++j)
-          o[qt][j] = mfma<T>(transposed<T, HD>(vs, kb + 32 * u, j >> 1, j & 1, lane), pf[u], o[qt][j]);
+          o[qt][j] = mfma<T>(EAGER ? vt[u][j] : transposed<T, HD>(vs, kb + 32 * u, j, lane), pf[u], o[qt][j]);
       }
     }
   }
@@ -154,10 +186,9 @@ struct Tiles {
         T* const to = merged + seg.row(s) * ldm + h * a.hd;
         const float f = DROP ? inv * a.drop.scale : inv;
 #pragma unroll
-        for (int jp = 0; jp < DS; ++jp) {
-          f4 lo = o[qt][2 * jp], hi = o[qt][2 * jp + 1];
-          if (!some) lo = hi = f4{0.f, 0.f, 0.f, 0.f};
-          put8(to, lo, hi, f, 32 * jp + 8 * g, a.hd);
+        for (int j = 0; j < DT; ++j) {
+          if (!some) o[qt][j] = f4{0.f, 0.f, 0.f, 0.f};
+          put4(to, o[qt][j], f, 16 * j + 4 * g, a.hd);
         }
       }
     }
@@ -178,8 +209,8 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 4) void typed_fwd_short_kernel
                                                                                 float* ml) {
   extern __shared__ __align__(16) char lds[];
   T* const ks = reinterpret_cast<T*>(lds);
-  T* const vs = ks + keys * kPitch<HD>;
-  float* const weight = reinterpret_cast<float*>(vs + keys * kPitch<HD>);
+  T* const vs = ks + keys * HD;
+  float* const weight = reinterpret_cast<float*>(vs + keys * HD);
   int* const kpos = reinterpret_cast<int*>(weight + keys);
   float* const lut = reinterpret_cast<float*>(kpos + keys);
   const int lane = threadIdx.x & 63, wave = wave_of(), waves = int(blockDim.x >> 6);
@@ -217,16 +248,15 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 4) void typed_fwd_short_kernel
 }
 
 // Past 128 slots: an item is an atom's 128 queries, two tiles a wave, and the keys come in
-// stages, the next one's loads on their way while the present one is used.
+// stages, the next one's loads on their way into LDS while the present one is used.
 template <class T, int HD, bool WHOLE, bool BIAS, bool DROP>
 __global__ __launch_bounds__(256, 2) void typed_fwd_long_kernel(Args a, int qblocks, T* merged, int64_t ldm, float* ml) {
   extern __shared__ __align__(16) char lds[];
-  constexpr int KS = kStage<HD>, QT = 2, per = 4 * QT * 16;
-  T* const ks = reinterpret_cast<T*>(lds);
-  T* const vs = ks + KS * kPitch<HD>;
-  float* const weight = reinterpret_cast<float*>(vs + KS * kPitch<HD>);
-  int* const kpos = reinterpret_cast<int*>(weight + KS);
-  float* const lut = reinterpret_cast<float*>(kpos + KS);
+  constexpr int QT = 2, per = 4 * QT * 16, U = HD == 128 ? 1 : 2;
+  T* const rows = reinterpret_cast<T*>(lds);  // two stages, each K's rows and V's
+  float* const weights = reinterpret_cast<float*>(rows + 4 * kStage * HD);
+  int* const positions = reinterpret_cast<int*>(weights + 2 * kStage);
+  float* const lut = reinterpret_cast<float*>(positions + 2 * kStage);
   const int lane = threadIdx.x & 63, wave = wave_of();
   const Share share(a.H);
   const int h = share.head, hk = h / (a.H / a.Hk);
@@ -242,32 +272,44 @@ __global__ __launch_bounds__(256, 2) void typed_fwd_long_kernel(Args a, int qblo
     const int n = item / qblocks, qb = item - n * qblocks;
     const Segment seg(a, n);
     const int q0 = qb * per + wave * QT * 16;
-    Tiles<T, HD, QT, KS / 32, WHOLE, BIAS, DROP> q;
+    Tiles<T, HD, QT, U, WHOLE, BIAS, DROP> q;
     q.start(a, qcols, seg, q0, lane);
-    Ahead<T, HD, KS, WHOLE, false> ahead;
-    float next_weight = 0.f;
-    int next_pos = 0;
-    const auto load = [&](int k0) {
-      ahead.load(a, kcols, a.ldq, vcols, a.ldq, seg, k0);
-      if (threadIdx.x < KS) {
-        const int k = k0 + int(threadIdx.x);
-        next_weight = k < seg.count ? seg.cf(a, k) : 0.f;
-        if constexpr (BIAS) next_pos = k < seg.count ? a.pos[seg.row(k)] : 0;
-      }
-    };
     if (qb * per < seg.count) {  // (the same for the whole workgroup)
-      load(0);
-      for (int k0 = 0; k0 < seg.count; k0 += KS) {
-        __syncthreads();
-        ahead.store(a, ks, kcols, a.ldq, vs, vcols, a.ldq, seg, k0);
-        if (threadIdx.x < KS) {
-          weight[threadIdx.x] = next_weight > 0.f ? log_weight(next_weight) * a.inv2 : -kInf;
-          if constexpr (BIAS) kpos[threadIdx.x] = next_pos;
+      Ahead<T, HD, WHOLE, false> ahead;
+      float next_weight = 0.f;
+      int next_pos = 0;
+      const auto start = [&](int k0, int to) {
+        T* const ks = rows + to * 2 * kStage * HD;
+        ahead.start(a, ks, kcols, a.ldq, ks + kStage * HD, vcols, a.ldq, seg, k0);
+        if (threadIdx.x < kStage) {
+          const int k = k0 + int(threadIdx.x);
+          next_weight = k < seg.count ? seg.cf(a, k) : 0.f;
+          if constexpr (BIAS) next_pos = k < seg.count ? a.pos[seg.row(k)] : 0;
         }
-        __syncthreads();
-        if (k0 + KS < seg.count) load(k0 + KS);
-        if (q0 < seg.count)
-          q.keys(a, key, h, ks, vs, weight, kpos, lut, k0, 0, min(KS, round_up(seg.count - k0, 32)), lane);
+      };
+      const auto land = [&](int k0, int to) {
+        T* const ks = rows + to * 2 * kStage * HD;
+        ahead.land(a, ks, kcols, a.ldq, ks + kStage * HD, vcols, a.ldq, seg, k0);
+        if (threadIdx.x < kStage) {
+          weights[to * kStage + threadIdx.x] = next_weight > 0.f ? log_weight(next_weight) * a.inv2 : -kInf;
+          if constexpr (BIAS) positions[to * kStage + threadIdx.x] = next_pos;
+        }
+        stage_barrier();
+      };
+      stage_barrier();  // (the last item's stages are done with)
+      start(0, 0);
+      land(0, 0);
+      int at = 0;
+      for (int k0 = 0; k0 < seg.count; k0 += kStage, at ^= 1) {
+        const bool more = k0 + kStage < seg.count;
+        if (more) start(k0 + kStage, at ^ 1);
+        if (q0 < seg.count) {
+          const T* const ks = rows + at * 2 * kStage * HD;
+          const int n_keys = min(kStage, round_up(seg.count - k0, 32));
+          for (int kb = 0; kb < n_keys; kb += 32 * U)
+            q.keys(a, key, h, ks, ks + kStage * HD, weights + at * kStage, positions + at * kStage, lut, k0, kb, n_keys, lane);
+        }
+        if (more) land(k0 + kStage, at ^ 1);
       }
     }
     q.finish(a, seg, h, q0, lane, merged, ldm, ml);
@@ -369,7 +411,7 @@ extern "C" int pet_attn_fwd_typed(int dtype, const pet_attn_shape* shape, int kv
                              keys, static_cast<T*>(merged), ldm, ml);
         } else {
           const auto kernel = typed_fwd_long_kernel<T, HD, WHOLE, BIAS, DROP>;
-          const size_t bytes = size_t(fwd_stage_bytes<HD>(kStage<HD>)) + lut;
+          const size_t bytes = size_t(2 * fwd_stage_bytes<HD>(kStage)) + lut;
           if (const int e = pet_attn::raise_lds(reinterpret_cast<const void*>(kernel), bytes)) return e;
           hipLaunchKernelGGL(kernel, dim3(unsigned(slots * a.H)), dim3(256), bytes, st, a, int(qblocks),
                              static_cast<T*>(merged), ldm, ml);

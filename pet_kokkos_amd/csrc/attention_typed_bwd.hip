@@ -258,7 +258,7 @@ struct ShortLds {
   int rows;       // R: slots to a whole 32
   size_t stats, more, bytes;
   ShortLds(const Args& a, bool hist) : rows(round_up(a.S, 32)) {
-    stats = size_t(2) * rows * kPitch<HD> * 2 + size_t(rows) * size_t(rows + 8) * 2;
+    stats = size_t(2) * rows * HD * 2 + size_t(rows) * size_t(rows + 8) * 2;
     more = stats + size_t(rows) * 12;
     bytes = more + 4 * (64 + 16) + (a.table ? size_t(2 * a.reach + 1) * 8 : 0) + (hist ? size_t(a.nb) * kColumns * 8 : 0);
   }
@@ -293,13 +293,13 @@ template <class T, int HD, int KT, bool GROUP, bool WHOLE, bool BIAS, bool DROP>
 __global__ __launch_bounds__(256, HD == 128 || (HD == 64 && KT == 2 && GROUP) ? 2 : 3) void typed_bwd_short_kernel(Args a, Grads b, int R,
                                                                                            unsigned stats, unsigned more) {
   extern __shared__ __align__(16) char lds[];
-  constexpr int DS = HD / 32, DT = HD / 16, CH = HD / 8, P = kPitch<HD>;
+  constexpr int DS = HD / 32, DT = HD / 16, CH = HD / 8;
   constexpr int AT = GROUP ? KT : 1;  // tiles whose sums are kept: over a group's heads, or one at a time
   constexpr bool HALF = std::is_same<T, _Float16>::value;
   const int lane = threadIdx.x & 63, wave = wave_of(), waves = int(blockDim.x >> 6), c = lane & 15, g = lane >> 4;
   T* const qs = reinterpret_cast<T*>(lds);  // Q's rows, then K's
-  T* const gs = qs + R * P;                 // dO's rows
-  T* const dss = gs + R * P;                // dS, a key's queries a row
+  T* const gs = qs + R * HD;                // dO's rows
+  T* const dss = gs + R * HD;               // dS, a key's queries a row
   const int pitch = R + 8;
   float* const expo = reinterpret_cast<float*>(lds + stats);
   float* const delta = expo + R;
@@ -363,10 +363,10 @@ __global__ __launch_bounds__(256, HD == 128 || (HD == 64 && KT == 2 && GROUP) ? 
       if (s >= seg.count) return;
       T* const row = static_cast<T*>(b.adj) + seg.row(s) * b.lda;
 #pragma unroll
-      for (int jp = 0; jp < DS; ++jp) {
-        if (!klive[kt]) dk[at][2 * jp] = dk[at][2 * jp + 1] = dv[at][2 * jp] = dv[at][2 * jp + 1] = f4{0.f, 0.f, 0.f, 0.f};
-        put8(row + (a.H + hk) * a.hd, dk[at][2 * jp], dk[at][2 * jp + 1], a.scale / sc, 32 * jp + 8 * g, a.hd);
-        put8(row + (a.H + a.Hk + hk) * a.hd, dv[at][2 * jp], dv[at][2 * jp + 1], 1.f, 32 * jp + 8 * g, a.hd);
+      for (int j = 0; j < DT; ++j) {
+        if (!klive[kt]) dk[at][j] = dv[at][j] = f4{0.f, 0.f, 0.f, 0.f};
+        put4(row + (a.H + hk) * a.hd, dk[at][j], a.scale / sc, 16 * j + 4 * g, a.hd);
+        put4(row + (a.H + a.Hk + hk) * a.hd, dv[at][j], 1.f, 16 * j + 4 * g, a.hd);
       }
     };
     if constexpr (GROUP)
@@ -498,8 +498,8 @@ __global__ __launch_bounds__(256, HD == 128 || (HD == 64 && KT == 2 && GROUP) ? 
           *reinterpret_cast<u4*>(dss + (16 * tile + c) * pitch + qb + 8 * g) = df;
 #pragma unroll
           for (int j = 0; j < DT; ++j) {
-            dv[at_tile][j] = mfma<T>(transposed<T, HD>(gs, qb, j >> 1, j & 1, lane), pf, dv[at_tile][j]);
-            dk[at_tile][j] = mfma<T>(transposed<T, HD>(qs, qb, j >> 1, j & 1, lane), df, dk[at_tile][j]);
+            dv[at_tile][j] = mfma<T>(transposed<T, HD>(gs, qb, j, lane), pf, dv[at_tile][j]);
+            dk[at_tile][j] = mfma<T>(transposed<T, HD>(qs, qb, j, lane), df, dk[at_tile][j]);
           }
         }
         if (b.cfh) {
@@ -513,9 +513,8 @@ __global__ __launch_bounds__(256, HD == 128 || (HD == 64 && KT == 2 && GROUP) ? 
       // K's rows in the place of Q's; zeros for the tiles behind the last token's
       const u4 none = {0u, 0u, 0u, 0u};
       const auto put_keys = [&](int tile, const u4 (&k)[DS]) {
-        T* const row = qs + lds_row(16 * tile + c) * P + 8 * g;
 #pragma unroll
-        for (int d = 0; d < DS; ++d) *reinterpret_cast<u4*>(row + 32 * d) = k[d];
+        for (int d = 0; d < DS; ++d) put_piece<T, HD>(qs, lds_row(16 * tile + c), 4 * d + g, k[d]);
         if (16 * tile >= seg.count)
           for (int qb = 0; qb < rows; qb += 32) *reinterpret_cast<u4*>(dss + (16 * tile + c) * pitch + qb + 8 * g) = none;
       };
@@ -536,13 +535,13 @@ __global__ __launch_bounds__(256, HD == 128 || (HD == 64 && KT == 2 && GROUP) ? 
           const u2 lo = lds_tr(at), hi = lds_tr(at + 4 * pitch);
           const u4 df = {lo[0], lo[1], hi[0], hi[1]};
 #pragma unroll
-          for (int j = 0; j < DT; ++j) dq[j] = mfma<T>(transposed<T, HD>(qs, kb, j >> 1, j & 1, lane), df, dq[j]);
+          for (int j = 0; j < DT; ++j) dq[j] = mfma<T>(transposed<T, HD>(qs, kb, j, lane), df, dq[j]);
         }
         const int s = 16 * tile + c;
         if (s < seg.count) {
           T* const row = static_cast<T*>(b.adj) + seg.row(s) * b.lda + h * a.hd;
 #pragma unroll
-          for (int jp = 0; jp < DS; ++jp) put8(row, dq[2 * jp], dq[2 * jp + 1], a.scale * back, 32 * jp + 8 * g, a.hd);
+          for (int j = 0; j < DT; ++j) put4(row, dq[j], a.scale * back, 16 * j + 4 * g, a.hd);
         }
       }
       if (hist && G > 1) flush(i);
@@ -558,7 +557,7 @@ __global__ __launch_bounds__(256, HD == 128 || (HD == 64 && KT == 2 && GROUP) ? 
 
 template <int HD>
 struct KvLds {
-  static constexpr size_t rows = size_t(2) * kStage<HD> * kPitch<HD> * 2, queries = rows + size_t(kStage<HD>) * 12,
+  static constexpr size_t rows = size_t(4) * kStage * HD * 2, queries = rows + size_t(2 * kStage) * 12,
                           waves = queries + 4 * (64 + 16);  // masks and maxima
   // + the bias's entries, the buckets' columns
   static size_t bytes(const Args& a, bool hist) {
@@ -576,13 +575,12 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, i
   constexpr int DS = HD / 32, DT = HD / 16, per = 4 * KT * 16;
   constexpr bool HALF = std::is_same<T, _Float16>::value;
   const int lane = threadIdx.x & 63, wave = wave_of(), c = lane & 15, g = lane >> 4;
-  T* const qs = reinterpret_cast<T*>(lds);
-  T* const gs = qs + kStage<HD> * kPitch<HD>;
-  float* const expo = reinterpret_cast<float*>(gs + kStage<HD> * kPitch<HD>);
-  float* const delta = expo + kStage<HD>;
-  int* const qpos = reinterpret_cast<int*>(delta + kStage<HD>);
-  unsigned char* const exchange = reinterpret_cast<unsigned char*>(qpos + kStage<HD>) + 64 * wave;
-  float* const room = reinterpret_cast<float*>(qpos + kStage<HD> + 64);
+  T* const staged = reinterpret_cast<T*>(lds);  // two stages, each Q's rows and dO's
+  float* const expos = reinterpret_cast<float*>(staged + 4 * kStage * HD);
+  float* const deltas = expos + 2 * kStage;
+  int* const positions = reinterpret_cast<int*>(deltas + 2 * kStage);
+  unsigned char* const exchange = reinterpret_cast<unsigned char*>(positions + 2 * kStage) + 64 * wave;
+  float* const room = reinterpret_cast<float*>(positions + 2 * kStage + 64);
   BiasEntry* const lut = reinterpret_cast<BiasEntry*>(room + 16);
   int64_t* const columns = reinterpret_cast<int64_t*>(lut + (BIAS ? 2 * a.reach + 1 : 0));
   char* const mine = reinterpret_cast<char*>(columns + (lane & (kColumns - 1)));
@@ -620,7 +618,7 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, i
     if (kb * per >= seg.count) continue;
     const int hi = part % b.heads_in, qi = part / b.heads_in;
     const int first_head = hi * (G / b.heads_in), last_head = first_head + G / b.heads_in;
-    const int q_each = round_up((seg.count + b.queries_in - 1) / b.queries_in, kStage<HD>);
+    const int q_each = round_up((seg.count + b.queries_in - 1) / b.queries_in, kStage);
     const int q_first = min(qi * q_each, seg.count), q_last = min(q_first + q_each, seg.count);
     const float sc = adjoint_scale<T>(a, b, seg, hk, room), back = 1.f / sc, counts = hist ? units * back : 0.f;
     const int k0 = kb * per + wave * KT * 16;
@@ -644,18 +642,15 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, i
     for (int i = first_head; i < last_head; ++i) {
       const int h = hk * G + i;
       float cf_sum[KT] = {};
-      if (BIAS && G > 1) {
-        __syncthreads();
-        bias_entries(a, lut, h);
-      }
       const T* const qcols = qkv + h * a.hd;
       const T* const gcols = static_cast<const T*>(b.out_adj) + h * a.hd;
-      Ahead<T, HD, kStage<HD>, WHOLE, true> ahead;
+      Ahead<T, HD, WHOLE, true> ahead;
       float next_expo = 0.f, next_delta = 0.f;
       int next_pos = 0;
-      const auto load = [&](int q0) {
-        ahead.load(a, qcols, a.ldq, gcols, b.ldg, seg, q0);
-        if (threadIdx.x < kStage<HD>) {
+      const auto start = [&](int q0, int to) {
+        T* const qs = staged + to * 2 * kStage * HD;
+        ahead.start(a, qs, qcols, a.ldq, qs + kStage * HD, gcols, b.ldg, seg, q0);
+        if (threadIdx.x < kStage) {
           const int s = q0 + int(threadIdx.x);
           const bool on = seg.query(a, s);
           const int64_t row = on ? seg.row(s) : 0;
@@ -664,22 +659,31 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, i
           if constexpr (BIAS) next_pos = a.pos[row];
         }
       };
-      if (q_first < q_last) load(q_first);
-      for (int q0 = q_first; q0 < q_last; q0 += kStage<HD>) {
-        const int n_queries = min(kStage<HD>, round_up(seg.count - q0, 32));
-        __syncthreads();
-        ahead.store(a, qs, qcols, a.ldq, gs, gcols, b.ldg, seg, q0);
-        if (threadIdx.x < kStage<HD>) {
+      const auto land = [&](int q0, int to) {
+        T* const qs = staged + to * 2 * kStage * HD;
+        ahead.land(a, qs, qcols, a.ldq, qs + kStage * HD, gcols, b.ldg, seg, q0);
+        if (threadIdx.x < kStage) {
+          const int q = to * kStage + int(threadIdx.x);
           // P is scaled by 1 / (1 - p) with its exponent
-          expo[threadIdx.x] = (DROP ? log2f(a.drop.scale) - next_expo : -next_expo) * a.inv2;
-          delta[threadIdx.x] = DROP ? next_delta / a.drop.scale : next_delta;
-          if constexpr (BIAS) qpos[threadIdx.x] = next_pos;
+          expos[q] = (DROP ? log2f(a.drop.scale) - next_expo : -next_expo) * a.inv2;
+          deltas[q] = DROP ? next_delta / a.drop.scale : next_delta;
+          if constexpr (BIAS) positions[q] = next_pos;
         }
-        __syncthreads();
-        if (q0 + kStage<HD> < q_last) load(q0 + kStage<HD>);
-        if (k0 >= seg.count) continue;
+        stage_barrier();
+      };
+      stage_barrier();  // (the stages and the bias of the head before are done with)
+      if (BIAS && G > 1) bias_entries(a, lut, h);
+      if (q_first < q_last) start(q_first, 0), land(q_first, 0);
+      int at_stage = 0;
+      for (int q0 = q_first; q0 < q_last; q0 += kStage, at_stage ^= 1) {
+        const int n_queries = min(kStage, round_up(seg.count - q0, 32));
+        const bool more = q0 + kStage < q_last;
+        if (more) start(q0 + kStage, at_stage ^ 1);
+        const T *const qs = staged + at_stage * 2 * kStage * HD, *const gs = qs + kStage * HD;
+        const float *const expo = expos + at_stage * kStage, *const delta = deltas + at_stage * kStage;
+        const int* const qpos = positions + at_stage * kStage;
         float part_sum[KT] = {};
-        for (int qb = 0; qb < n_queries; qb += 32) {
+        for (int qb = 0; qb < n_queries && k0 < seg.count; qb += 32) {
           u2 bits[KT];
           if constexpr (DROP) {
             const int s = q0 + qb + (lane & 31);
@@ -689,24 +693,35 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, i
           }
           u4 pf[KT], df[KT];
           float p[KT][8], ds[KT][8];
+          f4 s2[2][KT], dp2[2][KT], d2[2];
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
             const int at = qb + 8 * g + 4 * t;
-            f4 s[KT], dp[KT];
-            const f4 e4 = *reinterpret_cast<const f4*>(expo + at), d4 = *reinterpret_cast<const f4*>(delta + at);
+            u4 qf[DS], gf[DS];
+            const f4 e4 = *reinterpret_cast<const f4*>(expo + at);
+            d2[t] = *reinterpret_cast<const f4*>(delta + at);
 #pragma unroll
-            for (int kt = 0; kt < KT; ++kt) s[kt] = e4, dp[kt] = f4{0.f, 0.f, 0.f, 0.f};
+            for (int d = 0; d < DS; ++d) qf[d] = straight<T, HD>(qs, qb, t, d, lane), gf[d] = straight<T, HD>(gs, qb, t, d, lane);
+            reads_first();
 #pragma unroll
-            for (int d = 0; d < DS; ++d) {
-              const u4 qf = straight<T, HD>(qs, qb, t, d, lane), gf = straight<T, HD>(gs, qb, t, d, lane);
+            for (int kt = 0; kt < KT; ++kt) s2[t][kt] = e4, dp2[t][kt] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int d = 0; d < DS; ++d)
 #pragma unroll
               for (int kt = 0; kt < KT; ++kt) {
-                s[kt] = mfma<T>(qf, kf[kt][d], s[kt]);
-                dp[kt] = mfma<T>(gf, vf[kt][d], dp[kt]);
+                s2[t][kt] = mfma<T>(qf[d], kf[kt][d], s2[t][kt]);
+                dp2[t][kt] = mfma<T>(gf[d], vf[kt][d], dp2[t][kt]);
               }
-            }
+          }
+          u4 gt[DT];
+#pragma unroll
+          for (int j = 0; j < DT; ++j) gt[j] = transposed<T, HD>(gs, qb, j, lane);
+          reads_first();
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const f4 d4 = d2[t];
             i4 qp{};
-            if constexpr (BIAS) qp = *reinterpret_cast<const i4*>(qpos + at);
+            if constexpr (BIAS) qp = *reinterpret_cast<const i4*>(qpos + qb + 8 * g + 4 * t);
 #pragma unroll
             for (int kt = 0; kt < KT; ++kt) {
               int column[4] = {};
@@ -720,12 +735,12 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, i
                   w += be.value;
                   column[r] = be.column;
                 }
-                const float e = exp2_fast(fmaf(s[kt][r], a.scale2, w));
+                const float e = exp2_fast(fmaf(s2[t][kt][r], a.scale2, w));
                 float kept = e;
                 if constexpr (DROP) kept = masked(e, bits[kt], t, r);
                 p[kt][4 * t + r] = kept;
                 const float es = HALF ? e * sc : e;
-                const float x = fmaf(HALF ? kept * sc : kept, dp[kt][r], -es * d4[r]);
+                const float x = fmaf(HALF ? kept * sc : kept, dp2[t][kt][r], -es * d4[r]);
                 ds[kt][4 * t + r] = x;
                 part_sum[kt] += x;
                 counted[r] = x * counts;
@@ -735,18 +750,22 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, i
           }
 #pragma unroll
           for (int kt = 0; kt < KT; ++kt) pf[kt] = pack8<T>(p[kt]), df[kt] = pack8<T>(ds[kt]);
+          u4 qt[DT];
 #pragma unroll
-          for (int j = 0; j < DT; ++j) {
-            const u4 gt = transposed<T, HD>(gs, qb, j >> 1, j & 1, lane), qt = transposed<T, HD>(qs, qb, j >> 1, j & 1, lane);
+          for (int j = 0; j < DT; ++j) qt[j] = transposed<T, HD>(qs, qb, j, lane);
+          reads_first();
 #pragma unroll
-            for (int kt = 0; kt < KT; ++kt) {
-              dv[kt][j] = mfma<T>(gt, pf[kt], dv[kt][j]);
-              dk[kt][j] = mfma<T>(qt, df[kt], dk[kt][j]);
-            }
-          }
+          for (int j = 0; j < DT; ++j)
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) dv[kt][j] = mfma<T>(gt[j], pf[kt], dv[kt][j]);
+#pragma unroll
+          for (int j = 0; j < DT; ++j)
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) dk[kt][j] = mfma<T>(qt[j], df[kt], dk[kt][j]);
         }
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt) cf_sum[kt] += part_sum[kt];  // (a stage's sum at a time: its error grows by the stages)
+        if (more) land(q0 + kStage, at_stage ^ 1);
       }
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt) {
@@ -763,15 +782,15 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, i
       T* const row = static_cast<T*>(b.adj) + seg.row(s) * b.lda;
       float* const sums_row = b.kv + ((int64_t(part) * a.T + seg.row(s)) * 2 * a.Hk + hk) * a.hd;
 #pragma unroll
-      for (int jp = 0; jp < DS; ++jp) {
-        if (!klive[kt]) dk[kt][2 * jp] = dk[kt][2 * jp + 1] = dv[kt][2 * jp] = dv[kt][2 * jp + 1] = f4{0.f, 0.f, 0.f, 0.f};
-        const int d = 32 * jp + 8 * g;
+      for (int j = 0; j < DT; ++j) {
+        if (!klive[kt]) dk[kt][j] = dv[kt][j] = f4{0.f, 0.f, 0.f, 0.f};
+        const int d = 16 * j + 4 * g;
         if (parts > 1) {
-          put8(sums_row, dk[kt][2 * jp], dk[kt][2 * jp + 1], a.scale * back, d, a.hd);
-          put8(sums_row + a.Hk * a.hd, dv[kt][2 * jp], dv[kt][2 * jp + 1], 1.f, d, a.hd);
+          put4(sums_row, dk[kt][j], a.scale * back, d, a.hd);
+          put4(sums_row + a.Hk * a.hd, dv[kt][j], 1.f, d, a.hd);
         } else {
-          put8(row + (a.H + hk) * a.hd, dk[kt][2 * jp], dk[kt][2 * jp + 1], a.scale * back, d, a.hd);
-          put8(row + (a.H + a.Hk + hk) * a.hd, dv[kt][2 * jp], dv[kt][2 * jp + 1], 1.f, d, a.hd);
+          put4(row + (a.H + hk) * a.hd, dk[kt][j], a.scale * back, d, a.hd);
+          put4(row + (a.H + a.Hk + hk) * a.hd, dv[kt][j], 1.f, d, a.hd);
         }
       }
     }
@@ -787,11 +806,10 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_q_kernel(Args a, Grads b, in
   constexpr int DS = HD / 32, DT = HD / 16, per = 4 * QT * 16;
   constexpr bool HALF = std::is_same<T, _Float16>::value;
   const int lane = threadIdx.x & 63, wave = wave_of(), c = lane & 15, g = lane >> 4;
-  T* const ks = reinterpret_cast<T*>(lds);
-  T* const vs = ks + kStage<HD> * kPitch<HD>;
-  float* const weight = reinterpret_cast<float*>(vs + kStage<HD> * kPitch<HD>);
-  int* const kpos = reinterpret_cast<int*>(weight + kStage<HD>);
-  float* const room = reinterpret_cast<float*>(kpos + kStage<HD>);
+  T* const staged = reinterpret_cast<T*>(lds);  // two stages, each K's rows and V's
+  float* const weights = reinterpret_cast<float*>(staged + 4 * kStage * HD);
+  int* const positions = reinterpret_cast<int*>(weights + 2 * kStage);
+  float* const room = reinterpret_cast<float*>(positions + 2 * kStage);
   float* const lut = room + 16;
   const Share share(a.H);
   const int h = share.head, hk = h / (a.H / a.Hk);
@@ -832,47 +850,65 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_q_kernel(Args a, Grads b, in
 #pragma unroll
       for (int j = 0; j < DT; ++j) dq[qt][j] = f4{0.f, 0.f, 0.f, 0.f};
     }
-    Ahead<T, HD, kStage<HD>, WHOLE, false> ahead;
+    Ahead<T, HD, WHOLE, false> ahead;
     float next_weight = 0.f;
     int next_pos = 0;
-    const auto load = [&](int k0) {
-      ahead.load(a, kcols, a.ldq, vcols, a.ldq, seg, k0);
-      if (threadIdx.x < kStage<HD>) {
+    const auto start = [&](int k0, int to) {
+      T* const ks = staged + to * 2 * kStage * HD;
+      ahead.start(a, ks, kcols, a.ldq, ks + kStage * HD, vcols, a.ldq, seg, k0);
+      if (threadIdx.x < kStage) {
         const int s = k0 + int(threadIdx.x);
         next_weight = s < seg.count ? seg.cf(a, s) : 0.f;
         if constexpr (BIAS) next_pos = s < seg.count ? a.pos[seg.row(s)] : 0;
       }
     };
-    load(0);
-    for (int k0 = 0; k0 < seg.count; k0 += kStage<HD>) {
-      const int n_keys = min(kStage<HD>, round_up(seg.count - k0, 32));
-      __syncthreads();
-      ahead.store(a, ks, kcols, a.ldq, vs, vcols, a.ldq, seg, k0);
-      if (threadIdx.x < kStage<HD>) {
-        weight[threadIdx.x] = next_weight > 0.f ? log_weight(next_weight) * a.inv2 : -kInf;
-        if constexpr (BIAS) kpos[threadIdx.x] = next_pos;
+    const auto land = [&](int k0, int to) {
+      T* const ks = staged + to * 2 * kStage * HD;
+      ahead.land(a, ks, kcols, a.ldq, ks + kStage * HD, vcols, a.ldq, seg, k0);
+      if (threadIdx.x < kStage) {
+        weights[to * kStage + threadIdx.x] = next_weight > 0.f ? log_weight(next_weight) * a.inv2 : -kInf;
+        if constexpr (BIAS) positions[to * kStage + threadIdx.x] = next_pos;
       }
-      __syncthreads();
-      if (k0 + kStage<HD> < seg.count) load(k0 + kStage<HD>);
-      if (q0 >= seg.count) continue;
-      for (int kb = 0; kb < n_keys; kb += 32) {
+      stage_barrier();
+    };
+    stage_barrier();  // (the last item's stages are done with)
+    start(0, 0);
+    land(0, 0);
+    int at_stage = 0;
+    for (int k0 = 0; k0 < seg.count; k0 += kStage, at_stage ^= 1) {
+      const int n_keys = min(kStage, round_up(seg.count - k0, 32));
+      const bool more = k0 + kStage < seg.count;
+      if (more) start(k0 + kStage, at_stage ^ 1);
+      const T *const ks = staged + at_stage * 2 * kStage * HD, *const vs = ks + kStage * HD;
+      const float* const weight = weights + at_stage * kStage;
+      const int* const kpos = positions + at_stage * kStage;
+      for (int kb = 0; kb < n_keys && q0 < seg.count; kb += 32) {
         float ds[QT][8];
+        f4 s2[2][QT], dp2[2][QT];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          u4 kf[DS], vf[DS];
+          const f4 w4 = *reinterpret_cast<const f4*>(weight + kb + 8 * g + 4 * t);
+#pragma unroll
+          for (int d = 0; d < DS; ++d) kf[d] = straight<T, HD>(ks, kb, t, d, lane), vf[d] = straight<T, HD>(vs, kb, t, d, lane);
+          reads_first();
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt) s2[t][qt] = w4, dp2[t][qt] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int d = 0; d < DS; ++d)
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt) {
+              s2[t][qt] = mfma<T>(kf[d], qf[qt][d], s2[t][qt]);
+              dp2[t][qt] = mfma<T>(vf[d], gf[qt][d], dp2[t][qt]);
+            }
+        }
+        u4 ktr[DT];
+#pragma unroll
+        for (int j = 0; j < DT; ++j) ktr[j] = transposed<T, HD>(ks, kb, j, lane);
+        reads_first();
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           const int at = kb + 8 * g + 4 * t;
-          f4 s[QT], dp[QT];
-          const f4 w4 = *reinterpret_cast<const f4*>(weight + at);
-#pragma unroll
-          for (int qt = 0; qt < QT; ++qt) s[qt] = w4, dp[qt] = f4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int d = 0; d < DS; ++d) {
-            const u4 kf = straight<T, HD>(ks, kb, t, d, lane), vf = straight<T, HD>(vs, kb, t, d, lane);
-#pragma unroll
-            for (int qt = 0; qt < QT; ++qt) {
-              s[qt] = mfma<T>(kf, qf[qt][d], s[qt]);
-              dp[qt] = mfma<T>(vf, gf[qt][d], dp[qt]);
-            }
-          }
           i4 kp{};
           if constexpr (BIAS) kp = *reinterpret_cast<const i4*>(kpos + at);
 #pragma unroll
@@ -884,11 +920,11 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_q_kernel(Args a, Grads b, in
             for (int r = 0; r < 4; ++r) {
               float x = -expo[qt];
               if constexpr (BIAS) x += lut[pair_index(kp[r], qpos[qt], a.reach)];
-              float e = exp2_fast(fmaf(s[qt][r], a.scale2, x));
+              float e = exp2_fast(fmaf(s2[t][qt][r], a.scale2, x));
               if constexpr (HALF) e *= sc;
               float kept = e;
               if constexpr (DROP) kept = Drop::number(w, r) >= a.drop.least ? e : 0.f;
-              ds[qt][4 * t + r] = fmaf(kept, dp[qt][r], -e * delta[qt]);
+              ds[qt][4 * t + r] = fmaf(kept, dp2[t][qt][r], -e * delta[qt]);
             }
           }
         }
@@ -897,9 +933,10 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_q_kernel(Args a, Grads b, in
           const u4 df = pack8<T>(ds[qt]);
 #pragma unroll
           for (int j = 0; j < DT; ++j)
-            dq[qt][j] = mfma<T>(transposed<T, HD>(ks, kb, j >> 1, j & 1, lane), df, dq[qt][j]);
+            dq[qt][j] = mfma<T>(ktr[j], df, dq[qt][j]);
         }
       }
+      if (more) land(k0 + kStage, at_stage ^ 1);
     }
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
@@ -907,8 +944,7 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_q_kernel(Args a, Grads b, in
       if (s >= seg.count) continue;
       T* const row = static_cast<T*>(b.adj) + seg.row(s) * b.lda + h * a.hd;
 #pragma unroll
-      for (int jp = 0; jp < DS; ++jp)
-        put8(row, dq[qt][2 * jp], dq[qt][2 * jp + 1], a.scale * back, 32 * jp + 8 * g, a.hd);
+      for (int j = 0; j < DT; ++j) put4(row, dq[qt][j], a.scale * back, 16 * j + 4 * g, a.hd);
     }
   }
 }
@@ -1106,7 +1142,7 @@ extern "C" int pet_attn_bwd_typed(int dtype, const pet_attn_shape* shape, int kv
           constexpr int QT = 2;
           const auto kernel = typed_bwd_q_kernel<T, HD, QT, WHOLE, BIAS, DROP>;
           const int blocks = (a.S + QT * 64 - 1) / (QT * 64);
-          const size_t bytes = size_t(kStage<HD>) * (2 * kPitch<HD> * 2 + 8) + 64 + (a.table ? size_t(2 * a.reach + 1) * 4 : 0);
+          const size_t bytes = size_t(2 * kStage) * (2 * HD * 2 + 8) + 64 + (a.table ? size_t(2 * a.reach + 1) * 4 : 0);
           if (const int e = pet_attn::raise_lds(reinterpret_cast<const void*>(kernel), bytes)) return e;
           const int64_t q_slots = std::min<int64_t>((int64_t(a.N) * blocks + 7) / 8 * 8, 2048);
           if (q_slots * a.H * 256 > INT32_MAX) return int(PET_ATTN_EINDEX);
