@@ -352,8 +352,9 @@ __device__ __forceinline__ void put4(T* row, const f4& x, float f, int d, int hd
 
 // The offset of a pair in positions as an index 0 .. 2 reach (the difference does not wrap).
 __device__ __forceinline__ int pair_index(int pos_key, int pos_query, int reach) {
-  const int d = __builtin_elementwise_sub_sat(pos_key, pos_query);
-  return (d < -reach ? -reach : d > reach ? reach : d) + reach;
+  int d = __builtin_elementwise_sub_sat(pos_key, pos_query);
+  asm("v_med3_i32 %0, %1, %2, %3" : "=v"(d) : "v"(d), "v"(-reach), "v"(reach));
+  return d + reach;
 }
 __device__ __forceinline__ int bucket_of(const Args& a, int i) {
   const int b = a.buckets[i];

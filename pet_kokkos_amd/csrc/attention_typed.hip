@@ -205,7 +205,7 @@ __device__ __forceinline__ void fill_lut(const Args& a, float* lut, int h) {
 // at one SIMD, and 5 of them, one a tile of 71 slots, left room for no third workgroup
 // on the CU; which wave has the odd tile goes round by the atom).
 template <class T, int HD, bool WHOLE, bool BIAS, bool DROP>
-__global__ __launch_bounds__(256, HD == 128 ? 2 : 4) void typed_fwd_short_kernel(Args a, int keys, T* merged, int64_t ldm,
+__global__ __launch_bounds__(256, HD == 128 ? 2 : HD == 64 && BIAS && DROP ? 3 : 4) void typed_fwd_short_kernel(Args a, int keys, T* merged, int64_t ldm,
                                                                                 float* ml) {
   extern __shared__ __align__(16) char lds[];
   T* const ks = reinterpret_cast<T*>(lds);
