@@ -183,58 +183,70 @@ __device__ __forceinline__ u4 where(bool on, const u4& x) {
   return u4{on ? x[0] : 0u, on ? x[1] : 0u, on ? x[2] : 0u, on ? x[3] : 0u};
 }
 
-// Two columns of slots s0 .. s0 + n - 1 (n a multiple of 32), keys and values or queries
-// and adjoints, into LDS rows, zeros where the slot's weight says that it is left out:
-// nothing that a masked row holds is ever multiplied. EACH pieces of both a thread are
-// loaded at once, without a branch (one that is not wanted is of a place that is there).
-// more(slot, dim): what else is loaded with a piece; take(row k, chunk, x, y, on, that).
-template <class T, int HD, int EACH, bool WHOLE, bool QUERY, class More, class Take>
-__device__ __forceinline__ void stage_pair(const Args& a, T* xs, const T* xsrc, int64_t ldx, T* ys, const T* ysrc,
-                                           int64_t ldy, const Segment& seg, int s0, int n, const More& more,
-                                           const Take& take) {
-  constexpr int CH = HD / 8;
-  const int nt = blockDim.x, total = n * CH, last = seg.count - 1;
-  const Column xc(xsrc, ldx, seg), yc(ysrc, ldy, seg);
-  const auto put = [&](int i, const u4& x, const u4& y, bool on, const auto& m) {
-    const int k = i / CH, row = lds_row(k);
-    put_piece<T, HD>(xs, row, i % CH, x);
-    put_piece<T, HD>(ys, row, i % CH, y);
-    take(k, i % CH, x, y, on, m);
-  };
-  if constexpr (!WHOLE) {
-#pragma unroll 1
-    for (int i = threadIdx.x; i < total; i += nt) {
-      const int s = s0 + i / CH, ch = 8 * (i % CH);
-      const bool on = QUERY ? seg.query(a, s) : seg.key(a, s);
-      u4 x = {0u, 0u, 0u, 0u}, y = x;
-      decltype(more(0, 0)) m = {};
-      if (on) {
-        const int64_t row = seg.row(s);
-        x = row_chunk(xsrc + row * ldx, ch, a.hd), y = row_chunk(ysrc + row * ldy, ch, a.hd);
-        m = more(s, ch);
-      }
-      put(i, x, y, on, m);
-    }
-    return;
-  }
-  for (int i0 = threadIdx.x; i0 < total; i0 += EACH * nt) {
-    u4 x[EACH], y[EACH];
-    bool on[EACH];
-    decltype(more(0, 0)) m[EACH];
+// Columns of slots 0 .. n - 1 (n a multiple of 32), keys and values or queries and
+// adjoints, into LDS rows, zeros where the slot's weight says that it is left out: nothing
+// that a masked row holds is ever multiplied. load() sends a thread's first EACH pieces of
+// both (and of a third column, where there is one), without a branch (a piece that is not
+// wanted is of a place that is there), put() stores them and goes on with the rest.
+// take(row k, chunk, y, z): what else is made of a piece.
+template <class T, int HD, int EACH, bool WHOLE, bool QUERY, bool THIRD>
+struct Staged {
+  static constexpr int CH = HD / 8;
+  u4 x[EACH], y[EACH], z[THIRD ? EACH : 1];
+  float w[EACH];
+
+  __device__ __forceinline__ void load(const Args& a, const T* xsrc, int64_t ldx, const T* ysrc, int64_t ldy,
+                                       const T* zsrc, int64_t ldz, const Segment& seg, int i0) {
+    if constexpr (!WHOLE) return;
+    const int last = seg.count - 1;
+    const Column xc(xsrc, ldx, seg), yc(ysrc, ldy, seg), zc(THIRD ? zsrc : xsrc, ldz, seg);
 #pragma unroll
     for (int j = 0; j < EACH; ++j) {
-      const int i = i0 + j * nt, s = s0 + i / CH, ch = 8 * (i % CH), at = s < last ? s : last, d = ch < a.hd ? ch : 0;
-      const float w = seg.cf(a, at);
+      const int i = i0 + j * int(blockDim.x), s = i / CH, ch = 8 * (i % CH), at = s < last ? s : last, d = ch < a.hd ? ch : 0;
+      w[j] = seg.cf(a, at);
       x[j] = __builtin_bit_cast(u4, *reinterpret_cast<const u4e*>(xc.at(at, d)));
       y[j] = __builtin_bit_cast(u4, *reinterpret_cast<const u4e*>(yc.at(at, d)));
-      m[j] = more(at, d);
-      on[j] = (s <= last) & (ch < a.hd) & ((w > 0.f) | (QUERY && s == 0));
+      if constexpr (THIRD) z[j] = __builtin_bit_cast(u4, *reinterpret_cast<const u4e*>(zc.at(at, d)));
     }
-#pragma unroll
-    for (int j = 0; j < EACH; ++j)
-      if (i0 + j * nt < total) put(i0 + j * nt, where(on[j], x[j]), where(on[j], y[j]), on[j], m[j]);
   }
-}
+  template <class Take>
+  __device__ __forceinline__ void put(const Args& a, T* xs, const T* xsrc, int64_t ldx, T* ys, const T* ysrc, int64_t ldy,
+                                      const T* zsrc, int64_t ldz, const Segment& seg, int n, const Take& take) {
+    const int total = n * CH, step = int(blockDim.x);
+    if constexpr (WHOLE) {
+      for (int i0 = threadIdx.x;;) {
+#pragma unroll
+        for (int j = 0; j < EACH; ++j) {
+          const int i = i0 + j * step, k = i / CH, ch = i % CH;
+          if (i < total) {
+            const bool on = (k < seg.count) & (8 * ch < a.hd) & ((w[j] > 0.f) | (QUERY && k == 0));
+            const u4 u = where(on, x[j]), v = where(on, y[j]);
+            put_piece<T, HD>(xs, lds_row(k), ch, u);
+            put_piece<T, HD>(ys, lds_row(k), ch, v);
+            take(k, ch, v, where(on, z[THIRD ? j : 0]));
+          }
+        }
+        i0 += EACH * step;
+        if (i0 - int(threadIdx.x) >= total) break;  // (the same for the workgroup)
+        load(a, xsrc, ldx, ysrc, ldy, zsrc, ldz, seg, i0);
+      }
+    } else {
+#pragma unroll 1
+      for (int i = threadIdx.x; i < total; i += step) {
+        const int k = i / CH, ch = i % CH;
+        u4 u = {0u, 0u, 0u, 0u}, v = u, q = u;
+        if (QUERY ? seg.query(a, k) : seg.key(a, k)) {
+          const int64_t row = seg.row(k);
+          u = row_chunk(xsrc + row * ldx, 8 * ch, a.hd), v = row_chunk(ysrc + row * ldy, 8 * ch, a.hd);
+          if constexpr (THIRD) q = row_chunk(zsrc + row * ldz, 8 * ch, a.hd);
+        }
+        put_piece<T, HD>(xs, lds_row(k), ch, u);
+        put_piece<T, HD>(ys, lds_row(k), ch, v);
+        take(k, ch, v, q);
+      }
+    }
+  }
+};
 
 // 16 bytes a lane from memory into LDS, a wave's 64 lanes to dst .. dst + 1 KB in their
 // order (dst one for the wave).
@@ -307,28 +319,29 @@ struct Ahead {
   }
 };
 
-// A lane's B operands of a token's own columns (slot s, zeros unless live): dims 32 step + 8g .. + 7.
+// A lane's B operands of a token's own columns: dims 32 step + 8g .. + 7 of slot s, as they
+// lie (own_pieces), and with zeros unless live (own_live). What comes between them is not
+// waited for.
 template <class T, bool WHOLE, int DS>
-__device__ __forceinline__ void own_pieces(const Args& a, const T* src, int64_t ld, const Segment& seg, int s, bool live,
-                                           int lane, u4 (&out)[DS]) {
-  const int d0 = 8 * (lane >> 4);
+__device__ __forceinline__ void own_pieces(const Args& a, const T* src, int64_t ld, const Segment& seg, int s, int lane,
+                                           u4 (&out)[DS]) {
+  const int d0 = 8 * (lane >> 4), at = s < seg.count ? s : 0;
   if constexpr (WHOLE) {
     const Column col(src, ld, seg);
-    const int at = s < seg.count ? s : 0;
 #pragma unroll
     for (int step = 0; step < DS; ++step) {
       const int d = 32 * step + d0;
-      const u4 x = __builtin_bit_cast(u4, *reinterpret_cast<const u4e*>(col.at(at, d < a.hd ? d : 0)));
-      out[step] = where(live && d < a.hd, x);
+      out[step] = __builtin_bit_cast(u4, *reinterpret_cast<const u4e*>(col.at(at, d < a.hd ? d : 0)));
     }
   } else {
-    const T* const row = src + (live ? seg.row(s) : 0) * ld;
 #pragma unroll
-    for (int step = 0; step < DS; ++step) {
-      out[step] = u4{0u, 0u, 0u, 0u};
-      if (live) out[step] = row_chunk(row, 32 * step + d0, a.hd);
-    }
+    for (int step = 0; step < DS; ++step) out[step] = row_chunk(src + seg.row(at) * ld, 32 * step + d0, a.hd);
   }
+}
+template <int DS>
+__device__ __forceinline__ void own_live(const Args& a, bool live, int lane, u4 (&out)[DS]) {
+#pragma unroll
+  for (int step = 0; step < DS; ++step) out[step] = where(live && 32 * step + 8 * (lane >> 4) < a.hd, out[step]);
 }
 
 // A row's dims 16 j + 4g .. + 3 of a result's tile, times f.

@@ -33,17 +33,26 @@ struct Tiles {
   f4 o[QT][DT];
   float top[QT], base[QT], sum[QT];  // the largest logit, what exponents are taken from, their sum (log2 units)
   int64_t row[QT];
+  float cf[QT];
   int pos[QT];
   bool live[QT];
 
-  __device__ __forceinline__ void start(const Args& a, const T* qcols, const Segment& seg, int q0, int lane) {
+  __device__ __forceinline__ void load(const Args& a, const T* qcols, const Segment& seg, int q0, int lane) {
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      const int s = q0 + 16 * qt + (lane & 15), at = s < seg.count ? s : 0;
+      row[qt] = seg.row(at);
+      cf[qt] = seg.cf(a, at);
+      if constexpr (BIAS) pos[qt] = a.pos[row[qt]];
+      own_pieces<T, WHOLE>(a, qcols, a.ldq, seg, s, lane, qf[qt]);
+    }
+  }
+  __device__ __forceinline__ void start(const Args& a, const Segment& seg, int q0, int lane) {
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
       const int s = q0 + 16 * qt + (lane & 15);
-      live[qt] = seg.query(a, s);
-      row[qt] = live[qt] ? seg.row(s) : 0;
-      own_pieces<T, WHOLE>(a, qcols, a.ldq, seg, s, live[qt], lane, qf[qt]);
-      if constexpr (BIAS) pos[qt] = a.pos[row[qt]];
+      live[qt] = (s < seg.count) & ((s == 0) | (cf[qt] > 0.f));
+      own_live(a, live[qt], lane, qf[qt]);
 #pragma unroll
       for (int j = 0; j < DT; ++j) o[qt][j] = f4{0.f, 0.f, 0.f, 0.f};
       top[qt] = base[qt] = -kInf, sum[qt] = 0.f;
@@ -223,26 +232,34 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : HD == 64 && BIAS && DROP ? 3 :
   Words key{};
   if constexpr (DROP) key = a.drop.key();
   if constexpr (BIAS) fill_lut(a, lut, h);
+  const int slots = (a.S + 15) >> 4;
   for (int n = share.slot; n < a.N; n += share.step) {
     const Segment seg(a, n);
-    const int n_keys = round_up(seg.count, 32);
-    __syncthreads();
-    for (int k = threadIdx.x; k < n_keys; k += blockDim.x) {
-      const bool there = k < seg.count;
-      const float w = there ? seg.cf(a, k) : 0.f;
-      weight[k] = w > 0.f ? log_weight(w) * a.inv2 : -kInf;
-      if constexpr (BIAS) kpos[k] = there ? a.pos[seg.row(k)] : 0;
+    const int n_keys = round_up(seg.count, 32), tiles = (seg.count + 15) >> 4;
+    // everything that the atom is read from goes out before any of it is waited for
+    int tile = (wave + n) & (waves - 1);
+    Tiles<T, HD, 1, 2, WHOLE, BIAS, DROP> q;
+    Staged<T, HD, HD == 32 ? 2 : 4, WHOLE, false, false> staged;
+    staged.load(a, kcols, a.ldq, vcols, a.ldq, kcols, a.ldq, seg, threadIdx.x);
+    q.load(a, qcols, seg, 16 * tile, lane);
+    const int k_at = min(int(threadIdx.x), seg.count - 1);  // (threads are more than n_keys)
+    const float w = seg.cf(a, k_at);
+    int p = 0;
+    if constexpr (BIAS) p = a.pos[seg.row(k_at)];
+    stage_barrier();  // (the last atom's rows are done with)
+    if (int(threadIdx.x) < n_keys) {
+      weight[threadIdx.x] = int(threadIdx.x) < seg.count && w > 0.f ? log_weight(w) * a.inv2 : -kInf;
+      if constexpr (BIAS) kpos[threadIdx.x] = p;
     }
-    stage_pair<T, HD, 2, WHOLE, false>(a, ks, kcols, a.ldq, vs, vcols, a.ldq, seg, 0, n_keys, [](int, int) { return 0; },
-                                [](int, int, const u4&, const u4&, bool, int) {});
-    __syncthreads();
-    const int tiles = (seg.count + 15) >> 4, slots = (a.S + 15) >> 4;
-    for (int tile = (wave + n) & (waves - 1); tile < slots; tile += waves) {
-      Tiles<T, HD, 1, 2, WHOLE, BIAS, DROP> q;
-      q.start(a, qcols, seg, 16 * tile, lane);
+    staged.put(a, ks, kcols, a.ldq, vs, vcols, a.ldq, kcols, a.ldq, seg, n_keys, [](int, int, const u4&, const u4&) {});
+    stage_barrier();
+    while (tile < slots) {
+      q.start(a, seg, 16 * tile, lane);
       if (tile < tiles)
         for (int kb = 0; kb < n_keys; kb += 64) q.keys(a, key, h, ks, vs, weight, kpos, lut, 0, kb, n_keys, lane);
       q.finish(a, seg, h, 16 * tile, lane, merged, ldm, ml);
+      tile += waves;
+      if (tile < slots) q.load(a, qcols, seg, 16 * tile, lane);
     }
   }
 }
@@ -273,7 +290,8 @@ __global__ __launch_bounds__(256, 2) void typed_fwd_long_kernel(Args a, int qblo
     const Segment seg(a, n);
     const int q0 = qb * per + wave * QT * 16;
     Tiles<T, HD, QT, U, WHOLE, BIAS, DROP> q;
-    q.start(a, qcols, seg, q0, lane);
+    q.load(a, qcols, seg, q0, lane);
+    q.start(a, seg, q0, lane);
     if (qb * per < seg.count) {  // (the same for the whole workgroup)
       Ahead<T, HD, WHOLE, false> ahead;
       float next_weight = 0.f;

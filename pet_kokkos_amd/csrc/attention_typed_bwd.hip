@@ -340,17 +340,15 @@ __global__ __launch_bounds__(256, HD == 128 || (HD == 64 && (KT == 2 && GROUP ||
     int kpos[KT];
     bool klive[KT];
     unsigned vmax = 0;
+    // everything that the atom is read from goes out before any of it is waited for
+    float kcf[KT];
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) {
-      const int s = 16 * (first + waves * kt) + c;
-      klive[kt] = seg.key(a, s);
-      own_pieces<T, WHOLE>(a, kcols, a.ldq, seg, s, klive[kt], lane, kf[kt]);
-      own_pieces<T, WHOLE>(a, vcols, a.ldq, seg, s, klive[kt], lane, vf[kt]);
-      weight[kt] = klive[kt] ? log_weight(seg.cf(a, s)) : -kInf;
-      if constexpr (BIAS) kpos[kt] = a.pos[klive[kt] ? seg.row(s) : 0];
-      if (HALF || hist)
-#pragma unroll
-        for (int d = 0; d < DS; ++d) onto_magnitude(vmax, vf[kt][d]);
+      const int s = 16 * (first + waves * kt) + c, at = s < seg.count ? s : 0;
+      kcf[kt] = seg.cf(a, at);
+      if constexpr (BIAS) kpos[kt] = a.pos[seg.row(at)];
+      own_pieces<T, WHOLE>(a, kcols, a.ldq, seg, s, lane, kf[kt]);
+      own_pieces<T, WHOLE>(a, vcols, a.ldq, seg, s, lane, vf[kt]);
     }
     const auto clear = [&](int at) {
 #pragma unroll
@@ -377,40 +375,53 @@ __global__ __launch_bounds__(256, HD == 128 || (HD == 64 && (KT == 2 && GROUP ||
       const T* const qcols = qkv + h * a.hd;
       const T* const gcols = static_cast<const T*>(b.out_adj) + h * a.hd;
       const T* const ocols = static_cast<const T*>(b.out) + h * a.hd;
-      __syncthreads();  // (the last head's or atom's rows are done with)
+      Staged<T, HD, KT * CH / 4, WHOLE, true, true> staged;
+      staged.load(a, qcols, a.ldq, gcols, b.ldg, ocols, b.ldm, seg, threadIdx.x);
+      const int q = threadIdx.x, q_at = min(q, seg.count - 1);  // (threads are more than rows)
+      const float q_cf = seg.cf(a, q_at);
+      const float2 q_ml = *reinterpret_cast<const float2*>(b.ml + ((int64_t(n) * a.H + h) * a.S + q_at) * 2);
+      int q_pos = 0;
+      if constexpr (BIAS) q_pos = a.pos[seg.row(q_at)];
+      stage_barrier();  // (the last head's or atom's rows are done with)
+      if (i == 0) {
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) {
+          klive[kt] = (16 * (first + waves * kt) + c < seg.count) & (kcf[kt] > 0.f);
+          own_live(a, klive[kt], lane, kf[kt]);
+          own_live(a, klive[kt], lane, vf[kt]);
+          weight[kt] = klive[kt] ? log_weight(kcf[kt]) : -kInf;
+          if (HALF || hist)
+#pragma unroll
+            for (int d = 0; d < DS; ++d) onto_magnitude(vmax, vf[kt][d]);
+        }
+      }
       if (BIAS && G > 1) bias_entries(a, lut, h);
-      for (int q = threadIdx.x; q < rows; q += blockDim.x) {
-        const bool on = seg.query(a, q);
-        const float e = exponent(a, b, n, h, q, on);
+      if (q < rows) {
+        const bool on = (q < seg.count) & ((q == 0) | (q_cf > 0.f)) & (q_ml.y != 0.f);
+        const float e = on ? q_ml.x * kLog2e - log2f(q_ml.y) : kInf;
         expo[q] = (DROP ? log2f(a.drop.scale) - e : -e) * a.inv2;  // P is scaled by 1 / (1 - p) with its exponent
-        if constexpr (BIAS) qpos[q] = a.pos[on ? seg.row(q) : 0];
+        if constexpr (BIAS) qpos[q] = q_pos;
       }
       unsigned gmax = 0;
       float dmax = 0.f;
-      const Column ocol(ocols, b.ldm, seg);
-      stage_pair<T, HD, 2, WHOLE, true>(
-          a, qs, qcols, a.ldq, gs, gcols, b.ldg, seg, 0, rows,
-          [&](int s, int d) {
-            return WHOLE ? __builtin_bit_cast(u4, *reinterpret_cast<const u4e*>(ocol.at(s, d)))
-                           : row_chunk(ocols + seg.row(s) * b.ldm, d, a.hd);
-          },
-          [&](int k, int ch, const u4&, const u4& y, bool on, const u4& o) {
-            float u[8], v[8], dot = 0.f;
-            pet_typed::unpack<T>(__builtin_bit_cast(u4e, y), u);
-            pet_typed::unpack<T>(__builtin_bit_cast(u4e, where(on, o)), v);
+      staged.put(a, qs, qcols, a.ldq, gs, gcols, b.ldg, ocols, b.ldm, seg, rows,
+                 [&](int k, int ch, const u4& y, const u4& o) {
+                   float u[8], v[8], dot = 0.f;
+                   pet_typed::unpack<T>(__builtin_bit_cast(u4e, y), u);
+                   pet_typed::unpack<T>(__builtin_bit_cast(u4e, o), v);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) dot = fmaf(u[e], v[e], dot);
-            dot = row_sum<CH>(dot);
-            if (ch == 0) delta[k] = DROP ? dot / a.drop.scale : dot;
-            if (HALF || hist) onto_magnitude(gmax, y), dmax = fmaxf(dmax, dot == dot ? fabsf(dot) : kInf);
-          });
+                   for (int e = 0; e < 8; ++e) dot = fmaf(u[e], v[e], dot);
+                   dot = row_sum<CH>(dot);
+                   if (ch == 0) delta[k] = DROP ? dot / a.drop.scale : dot;
+                   if (HALF || hist) onto_magnitude(gmax, y), dmax = fmaxf(dmax, dot == dot ? fabsf(dot) : kInf);
+                 });
       if (HALF || hist) {
         const float m[3] = {wave_max(magnitude<T>(gmax)), wave_max(magnitude<T>(vmax)), wave_max(dmax)};
         if (lane == 0)
 #pragma unroll
           for (int k = 0; k < 3; ++k) room[3 * wave + k] = m[k];
       }
-      __syncthreads();
+      stage_barrier();
       // what brings dS into the range of fp16, and into whole numbers (adjoint_scale, count_in)
       float counts = 0.f;
       if (HALF || hist) {
@@ -509,7 +520,7 @@ __global__ __launch_bounds__(256, HD == 128 || (HD == 64 && (KT == 2 && GROUP ||
         }
         if constexpr (!GROUP) store(kt, 0);
       }
-      __syncthreads();
+      stage_barrier();
       // K's rows in the place of Q's; zeros for the tiles behind the last token's
       const u4 none = {0u, 0u, 0u, 0u};
       const auto put_keys = [&](int tile, const u4 (&k)[DS]) {
@@ -525,7 +536,7 @@ __global__ __launch_bounds__(256, HD == 128 || (HD == 64 && (KT == 2 && GROUP ||
         const u4 zeros[DS] = {};
         put_keys(1, zeros);
       }
-      __syncthreads();
+      stage_barrier();
       for (int tile = first; 16 * tile < seg.count; tile += waves) {
         f4 dq[DT];
 #pragma unroll
@@ -632,8 +643,10 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, i
       const int s = k0 + 16 * kt + c;
       klive[kt] = seg.key(a, s);
       const int64_t row = klive[kt] ? seg.row(s) : 0;
-      own_pieces<T, WHOLE>(a, kcols, a.ldq, seg, s, klive[kt], lane, kf[kt]);
-      own_pieces<T, WHOLE>(a, vcols, a.ldq, seg, s, klive[kt], lane, vf[kt]);
+      own_pieces<T, WHOLE>(a, kcols, a.ldq, seg, s, lane, kf[kt]);
+      own_pieces<T, WHOLE>(a, vcols, a.ldq, seg, s, lane, vf[kt]);
+      own_live(a, klive[kt], lane, kf[kt]);
+      own_live(a, klive[kt], lane, vf[kt]);
       weight[kt] = klive[kt] ? log_weight(seg.cf(a, s)) : -kInf;
       if constexpr (BIAS) kpos[kt] = a.pos[row];
 #pragma unroll
@@ -841,8 +854,10 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_q_kernel(Args a, Grads b, in
       const int s = q0 + 16 * qt + c;
       const bool on = seg.query(a, s);
       qrow[qt] = on ? seg.row(s) : 0;
-      own_pieces<T, WHOLE>(a, qcols, a.ldq, seg, s, on, lane, qf[qt]);
-      own_pieces<T, WHOLE>(a, gcols, b.ldg, seg, s, on, lane, gf[qt]);
+      own_pieces<T, WHOLE>(a, qcols, a.ldq, seg, s, lane, qf[qt]);
+      own_pieces<T, WHOLE>(a, gcols, b.ldg, seg, s, lane, gf[qt]);
+      own_live(a, on, lane, qf[qt]);
+      own_live(a, on, lane, gf[qt]);
       expo[qt] = exponent(a, b, n, h, s, on);
       if constexpr (DROP) expo[qt] -= log2f(a.drop.scale);
       delta[qt] = on ? b.delta[qrow[qt] * a.H + h] / a.drop.scale : 0.f;
