@@ -290,7 +290,7 @@ __device__ __forceinline__ float magnitude(unsigned m) {
 // transposed for dQ^T += K^T dS^T, a tile of queries a wave: every product is formed once,
 // where the two passes past 128 slots form S, dP and their exponentials twice.
 template <class T, int HD, int KT, bool GROUP, bool WHOLE, bool BIAS, bool DROP>
-__global__ __launch_bounds__(256, HD == 128 || (HD == 64 && (KT == 2 && GROUP || BIAS && DROP)) ? 2 : 3) void typed_bwd_short_kernel(Args a, Grads b, int R,
+__global__ __launch_bounds__(256, HD == 128 || (KT == 2 && GROUP && (HD == 64 || BIAS)) || (HD == 64 && (BIAS || KT == 1)) ? 2 : 3) void typed_bwd_short_kernel(Args a, Grads b, int R,
                                                                                            unsigned stats, unsigned more) {
   extern __shared__ __align__(16) char lds[];
   constexpr int DS = HD / 32, DT = HD / 16, CH = HD / 8;
