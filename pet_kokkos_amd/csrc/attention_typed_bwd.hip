@@ -763,14 +763,14 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, i
           }
 #pragma unroll
           for (int kt = 0; kt < KT; ++kt) pf[kt] = pack8<T>(p[kt]), df[kt] = pack8<T>(ds[kt]);
-          u4 qt[DT];
-#pragma unroll
-          for (int j = 0; j < DT; ++j) qt[j] = transposed<T, HD>(qs, qb, j, lane);
-          reads_first();
 #pragma unroll
           for (int j = 0; j < DT; ++j)
 #pragma unroll
             for (int kt = 0; kt < KT; ++kt) dv[kt][j] = mfma<T>(gt[j], pf[kt], dv[kt][j]);
+          u4 qt[DT];
+#pragma unroll
+          for (int j = 0; j < DT; ++j) qt[j] = transposed<T, HD>(qs, qb, j, lane);
+          reads_first();
 #pragma unroll
           for (int j = 0; j < DT; ++j)
 #pragma unroll
