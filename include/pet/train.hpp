@@ -1,7 +1,9 @@
 // pet/train.hpp -- what a training step adds, for a C++ caller: the norm's and a
 // dense layer's parameter gradients, an attention layer's, and the norm and
 // clipping of them all (pet_norm_rows_grads, pet_linear_grads,
-// pet_attention_layer_grads, pet_grad_norm, pet_grad_clip). The reference
+// pet_attention_layer_grads, pet_grad_norm, pet_grad_clip); dropout of rows, and the
+// attention of 16-bit rows with grouped heads, a bias by position and dropout, with its
+// backward (pet_dropout_rows, pet_attn_fwd_typed, pet_attn_bwd_typed). The reference
 // (peterspackman/pet-kokkos) evaluates only, so none of it has a counterpart
 // there; the views, the Workspace that holds the scratch and the exceptions are
 // those of pet/attention.hpp. A Workspace serves one stream at a time, and a call that
@@ -123,6 +125,82 @@ inline void attention_layer_grads(Workspace& ws, const std::string& key, const p
                                   cf_seq.data(), cf_seq.stride(0), w_out.v.data(), tk.off, merged.data(), ml.data(),
                                   scratch, bytes, stream),
         "attention_layer_grads");
+}
+
+// out = residual + M in, M the dropout's mask with its scale (residual may hold no
+// pointer): also its own backward, of the adjoint.
+inline void dropout_rows(const Rows& out, const Rows& in, const Rows& residual, const pet_dropout& dropout,
+                         const int* live = nullptr, hipStream_t stream = nullptr) {
+  check_rows(out, in, "dropout_rows");
+  if (residual.ptr) check_rows(residual, in, "dropout_rows");
+  need(out.rows == in.rows && out.cols == in.cols &&
+           (!residual.ptr || (residual.rows == in.rows && residual.cols == in.cols)),
+       "dropout_rows", "rows of one shape are needed");
+  check(pet_dropout_rows(in.dtype, in.rows, in.cols, out.ptr, out.ld, in.ptr, in.ld, residual.ptr, residual.ld, &dropout,
+                         live, stream),
+        "dropout_rows");
+}
+
+// What a call of the typed attention and its backward share; the bias's arrays, where
+// there is one, are as long as pet_attn_bias says.
+struct TypedAttention {
+  Tokens tk;
+  int S = 0, heads = 0, kv_heads = 0, head_dim = 0;
+  double temperature = 1.0;
+  const pet_attn_bias* bias = nullptr;
+  const pet_dropout* dropout = nullptr;
+};
+
+inline pet_attn_shape typed_shape(const TypedAttention& at, const Rows& qkv, const View2D& cf_seq, const char* what) {
+  need(qkv.cols == (at.heads + 2 * at.kv_heads) * at.head_dim, what, "qkv is not [T, (heads + 2 kv_heads) head_dim]");
+  need(cf_seq.extent(0) == at.tk.N && cf_seq.extent(1) >= at.S, what, "cf_seq is not [N, S] or wider");
+  return make_shape(at.tk, qkv.rows, at.S, at.heads, at.head_dim, at.temperature);
+}
+
+// merged [T, heads head_dim] and ml [N heads S, 2] (may hold none) of qkv's rows (bf16, fp16).
+inline void attn_fwd_typed(const TypedAttention& at, const Rows& merged, View2D ml, const Rows& qkv, View2D cf_seq,
+                           hipStream_t stream = nullptr) {
+  const char* what = "attn_fwd_typed";
+  const pet_attn_shape sh = typed_shape(at, qkv, cf_seq, what);
+  check_rows(merged, qkv, what);
+  need(merged.rows == qkv.rows && merged.cols == at.heads * at.head_dim, what, "merged is not [T, heads head_dim]");
+  check_matrix(ml, at.tk.N * at.heads * at.S, 2, what, "ml is not [N heads S, 2]");
+  need(!ml.data() || ml.stride(0) == 2, what, "a contiguous ml is needed");
+  check(pet_attn_fwd_typed(qkv.dtype, &sh, at.kv_heads, qkv.ptr, qkv.ld, at.tk.off, cf_seq.data(), cf_seq.stride(0),
+                           at.bias, at.dropout, merged.ptr, merged.ld, ml.data(), stream),
+        what);
+}
+
+// Its backward: qkv_adj, and onto beta times themselves cf_seq_adj and table_adj
+// [n_buckets, heads] (each may hold none).
+inline void attn_bwd_typed(Workspace& ws, const TypedAttention& at, const Rows& qkv_adj, View2D cf_seq_adj,
+                           View2D table_adj, const Rows& dmerged, const Rows& qkv, const Rows& merged, View2D ml,
+                           View2D cf_seq, Net beta = 0, hipStream_t stream = nullptr) {
+  const char* what = "attn_bwd_typed";
+  const pet_attn_shape sh = typed_shape(at, qkv, cf_seq, what);
+  check_rows(qkv_adj, qkv, what);
+  check_rows(merged, qkv, what);
+  check_rows(dmerged, qkv, what);
+  need(qkv_adj.rows == qkv.rows && qkv_adj.cols == qkv.cols, what, "qkv_adj is not of qkv's shape");
+  need(merged.rows == qkv.rows && merged.cols == at.heads * at.head_dim && dmerged.rows == qkv.rows &&
+           dmerged.cols == merged.cols,
+       what, "merged and dmerged are not [T, heads head_dim]");
+  need(ml.data() && ml.stride(0) == 2, what, "a contiguous ml is needed");
+  check_matrix(ml, at.tk.N * at.heads * at.S, 2, what, "ml is not [N heads S, 2]");
+  need(!cf_seq_adj.data() || (cf_seq_adj.extent(0) == at.tk.N && cf_seq_adj.extent(1) >= at.S), what,
+       "cf_seq_adj is not [N, S] or wider");
+  need(!table_adj.data() || at.bias, what, "table_adj without a bias");
+  if (table_adj.data()) {
+    check_matrix(table_adj, at.bias->n_buckets, at.heads, what, "table_adj is not [n_buckets, heads]");
+    need(table_adj.stride(0) == at.heads, what, "a contiguous table_adj is needed");
+  }
+  const size_t bytes = pet_attn_bwd_typed_workspace(qkv.dtype, &sh, at.kv_heads, at.bias ? at.bias->n_buckets : 0);
+  void* scratch = ws.bytes("attn_bwd_typed:scratch", bytes);
+  check(pet_attn_bwd_typed(qkv.dtype, &sh, at.kv_heads, qkv.ptr, qkv.ld, at.tk.off, dmerged.ptr, dmerged.ld, merged.ptr,
+                           merged.ld, static_cast<const float*>(ml.data()), cf_seq.data(), cf_seq.stride(0), at.bias,
+                           at.dropout, qkv_adj.ptr, qkv_adj.ld, cf_seq_adj.data(), cf_seq_adj.stride(0),
+                           table_adj.data(), beta, scratch, bytes, stream),
+        what);
 }
 
 // One tensor of a list of gradients: consecutive elements, or rows of a wider matrix.

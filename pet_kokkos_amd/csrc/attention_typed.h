@@ -376,7 +376,7 @@ __device__ __forceinline__ int bucket_of(const Args& a, int i) {
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// log2 of cutoff factors, in units of the scores before their scale
+// A key's part of the exponent in base 2.
 __device__ __forceinline__ float log_weight(float cf) { return log2f(cf); }
 
 // Workgroups go round the XCDs, and so do the items of a head: block b has head

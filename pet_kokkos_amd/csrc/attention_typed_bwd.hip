@@ -207,9 +207,17 @@ struct BiasEntry {
 // wave where its fp32 addition takes 194 (a CU, measured: a lane at a time). A query's
 // |dS| sum to at most about the bound, so a column holds 2^25 queries and more. Four of a
 // lane's dS at a time: under 2^30, as nearly all are, one conversion to 32 bits each.
+// floor(x + 1/2): halves go up. All of them up would shift the sum of 10^7 pairs by 10^-5 of
+// it, so every other one is taken as less floor(1/2 - x), whose halves go down (rounding them
+// to even by an instruction of its own cost a tenth of the whole kernel: 2040 -> 2240 us).
 __device__ __forceinline__ int nearest(float x) {
   int q;
-  asm("v_cvt_rpi_i32_f32 %0, %1" : "=v"(q) : "v"(x));  // floor(x + 1/2)
+  asm("v_cvt_rpi_i32_f32 %0, %1" : "=v"(q) : "v"(x));
+  return q;
+}
+__device__ __forceinline__ int less_nearest(float x) {
+  int q;
+  asm("v_cvt_rpi_i32_f32 %0, -%1" : "=v"(q) : "v"(x));
   return q;
 }
 __device__ __forceinline__ void count_in(char* columns, const int (&column)[4], const float (&x)[4]) {
@@ -217,18 +225,24 @@ __device__ __forceinline__ void count_in(char* columns, const int (&column)[4], 
     __hip_atomic_fetch_add(reinterpret_cast<unsigned long long*>(columns + column[i]), static_cast<unsigned long long>(q),
                            __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
   };
+  const auto take = [&](int i, int64_t q) {
+    __hip_atomic_fetch_sub(reinterpret_cast<unsigned long long*>(columns + column[i]), static_cast<unsigned long long>(q),
+                           __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+  };
   const float m = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
   if (__builtin_expect(__any(m >= 0x1p30f), 0)) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int high = nearest(x[i] * 0x1p-16f);
+      const float low = fmaf(float(high), -0x1p16f, x[i]);
       add(i, int64_t(high) << 16);
-      add(i, nearest(fmaf(float(high), -0x1p16f, x[i])));
+      if (i & 1) take(i, less_nearest(low)); else add(i, nearest(low));
     }
     return;
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) add(i, nearest(x[i]));
+  for (int i = 0; i < 4; ++i)
+    if (i & 1) take(i, less_nearest(x[i])); else add(i, nearest(x[i]));
 }
 // A head's columns summed in units of `unit` onto the workgroup's own row of sums, and cleared.
 __device__ __forceinline__ void flush_columns(int64_t* columns, int nb, double unit, double* sums) {
@@ -678,7 +692,7 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, i
         if (threadIdx.x < kStage) {
           const int q = to * kStage + int(threadIdx.x);
           // P is scaled by 1 / (1 - p) with its exponent
-          expos[q] = (DROP ? log2f(a.drop.scale) - next_expo : -next_expo) * a.inv2;
+          expos[q] = DROP ? log2f(a.drop.scale) - next_expo : -next_expo;
           deltas[q] = DROP ? next_delta / a.drop.scale : next_delta;
           if constexpr (BIAS) positions[q] = next_pos;
         }
@@ -711,13 +725,12 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, i
           for (int t = 0; t < 2; ++t) {
             const int at = qb + 8 * g + 4 * t;
             u4 qf[DS], gf[DS];
-            const f4 e4 = *reinterpret_cast<const f4*>(expo + at);
             d2[t] = *reinterpret_cast<const f4*>(delta + at);
 #pragma unroll
             for (int d = 0; d < DS; ++d) qf[d] = straight<T, HD>(qs, qb, t, d, lane), gf[d] = straight<T, HD>(gs, qb, t, d, lane);
             reads_first();
 #pragma unroll
-            for (int kt = 0; kt < KT; ++kt) s2[t][kt] = e4, dp2[t][kt] = f4{0.f, 0.f, 0.f, 0.f};
+            for (int kt = 0; kt < KT; ++kt) s2[t][kt] = dp2[t][kt] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int d = 0; d < DS; ++d)
 #pragma unroll
@@ -732,7 +745,8 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, i
           reads_first();
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
-            const f4 d4 = d2[t];
+            // (added here: in the products' sums it would round each of them at its own size)
+            const f4 d4 = d2[t], e4 = *reinterpret_cast<const f4*>(expo + qb + 8 * g + 4 * t);
             i4 qp{};
             if constexpr (BIAS) qp = *reinterpret_cast<const i4*>(qpos + qb + 8 * g + 4 * t);
 #pragma unroll
@@ -741,7 +755,7 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, i
               float counted[4];
 #pragma unroll
               for (int r = 0; r < 4; ++r) {
-                float w = weight[kt];
+                float w = weight[kt] + e4[r];
                 BiasEntry be{};
                 if constexpr (BIAS) {
                   be = lut[pair_index(kpos[kt], qp[r], a.reach)];

@@ -112,6 +112,72 @@ def test_tables(device, buckets, reach, group):
     OnDevice(Case([60, 3, 140], 4, 4 // group, 32, BF16, seed=buckets, buckets=buckets, reach=reach), device).check()
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("heads,kv_heads,head_dim,counts,slots", [
+    (1, 1, 32, [700], None), (1, 1, 128, [1100], None), (2, 1, 64, [520, 3], None), (3, 3, 48, [600, 0, 129], None),
+    (4, 2, 33, [150, 300], None), (2, 2, 100, [200, 1], None), (2, 1, 116, [530], None), (2, 1, 32, [3, 0, 40], 1500)])
+def test_long_passes_in_parts(device, dtype, heads, kv_heads, head_dim, counts, slots):
+    """Heads and queries shared out among workgroups, heads in odd pieces, a few tokens in many slots."""
+    OnDevice(Case(counts, heads, kv_heads, head_dim, dtype, seed=head_dim, buckets=9, reach=30, p=0.2, zeros=0.1, dead=4,
+                  slots=slots), device).check()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("counts,heads,kv_heads,head_dim", [(SMALL, 4, 4, 32), ([50, 127, 3], 4, 2, 64), ([200, 17], 4, 1, 128)])
+def test_a_block_forward_and_backward(device, dtype, counts, heads, kv_heads, head_dim):
+    """out = x + M2 attention(qkv) and its adjoints from out's. M2 of p = 1/2 is 0 or 2: the adjoint of merged is
+    exact, and out is off by twice merged's bound and the rounding of itself."""
+    case = Case(counts, heads, kv_heads, head_dim, dtype, seed=3, buckets=12, reach=9, p=0.125, zeros=0.1)
+    out_adj = case.dmerged
+    m2 = rows_mask(*case.state, 8, 0.5, case.T, heads * head_dim)
+    case.dmerged = (m2 * out_adj.double()).to(dtype)
+    d = OnDevice(case, device)
+    x = torch.randn(case.T, heads * head_dim, generator=torch.Generator().manual_seed(1)).to(dtype)
+    after = A.Dropout(0.5, d.drop.state, 8)
+    d.forward()
+    out = x.to(device)
+    L.dropout_rows(out, d.merged, after, out)
+    merged, tol, *_ = case.forward()
+    ref = x.double() + m2 * merged
+    within(out, ref, m2 * tol + half(dtype) * (ref.abs() + m2 * tol) + 2.0 ** -24 * (x.double().abs() + 2 * merged.abs()), "out")
+    d.dmerged.fill_(math.nan)
+    L.dropout_rows(d.dmerged, out_adj.to(device), after)
+    assert torch.equal(d.dmerged.cpu(), case.dmerged)
+    d.backward()
+    for name, (want, bound) in case.backward(d.merged.cpu()).items():
+        within({"qkv_adj": d.adj, "cf_seq_adj": d.cf_adj, "bias_adj": d.table_adj}[name], want, bound, name)
+
+
+@pytest.mark.parametrize("edges,fine,unit", [(63, 26, 2.0 ** -30), (255, 30, 2.0 ** -36)])
+def test_the_tables_sums_do_not_drift(device, edges, fine, unit):
+    """Logits all 0, so P = 1 / tokens, and the values' sum 0, so dO.O = 0 but at the rows that set the sums' unit: every
+    dS is exact, in quarters of a unit. Rounded to whole units each is off by 1/2 at most and by nothing on the mean,
+    so n pairs by 6 * 0.36 sqrt(n) units (0.36: the root of a mean square of 1/8, of quarters as likely as each other)."""
+    rng = np.random.default_rng(0)
+    tokens, N, hd = edges + 1, 8, 8
+    case = Case([edges] * N, 1, 1, hd, BF16, buckets=2, reach=1)
+    qkv, g = torch.zeros(case.T, 3 * hd, dtype=torch.float64), torch.zeros(case.T, hd, dtype=torch.float64)
+    case.table, case.buckets, case.cf = torch.zeros(2, 1), torch.tensor([0, 1, 1]).int(), torch.ones(N, tokens)
+    exact = torch.zeros(2, dtype=torch.float64)
+    for n in range(N):
+        rows = case.rows(n)
+        v = rng.integers(1, 128, tokens // 2)
+        v = np.concatenate([v, -v])
+        w = rng.integers(-127, 128, tokens)
+        w[0] = 0
+        qkv[rows, 2 * hd + 1] = torch.from_numpy(v * 2.0 ** -(fine // 2))
+        qkv[rows[0], 2 * hd] = 1.0
+        g[rows, 1] = torch.from_numpy(w * 2.0 ** -(fine // 2))
+        g[rows[0], 0] = 1.0
+        case.pos[rows] = torch.from_numpy(np.where(v > 0, 10, 0)).int()
+    case.qkv, case.dmerged = qkv.to(BF16), g.to(BF16)
+    d = OnDevice(case, device)
+    d.forward(), d.backward()
+    ref, _ = case.backward(d.merged.cpu())["bias_adj"]
+    pairs = N * tokens ** 2
+    within(d.table_adj, ref, 6 * 0.36 * math.sqrt(pairs) * unit + U * ref.abs(), "bias_adj")
+
+
 def test_many_atoms_share_the_workgroups(device):
     """More items than workgroups: the table's sums run over several atoms in each."""
     rng = np.random.default_rng(3)

@@ -6,11 +6,13 @@ from __future__ import annotations
 
 import ctypes
 import math
+import os
+import subprocess
 
 import pytest
 import torch
 
-from pet_kokkos_amd import _lib, layer
+from pet_kokkos_amd import _lib, build, layer
 from pet_kokkos_amd import attention as A
 from typed_attention import Case, attention_mask, rows_mask, threefry
 
@@ -195,3 +197,11 @@ def test_the_formulas_against_differences():
         x.copy_(keep)
         quotient, along = (ends[0] - ends[1]) * 2.0 ** 9, float((got[name][0] * delta).sum())
         assert abs(quotient - along) <= 2.0 ** -14 * float((got[name][0] * delta).abs().sum()), name
+
+
+def test_cpp_calls_refuse_shapes():
+    """The C++ calls throw for views that do not fit together, before they reach the GPU."""
+    if not os.path.exists(build.CPP_TEST6):
+        pytest.fail(f"{build.CPP_TEST6} is not built (python -m pet_kokkos_amd.build)")
+    res = subprocess.run([build.CPP_TEST6], capture_output=True, text=True, timeout=60)
+    assert res.returncode == 0 and res.stdout == "", res.stdout + res.stderr
