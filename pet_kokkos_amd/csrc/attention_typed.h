@@ -344,10 +344,11 @@ __device__ __forceinline__ void own_live(const Args& a, bool live, int lane, u4 
   for (int step = 0; step < DS; ++step) out[step] = where(live && 32 * step + 8 * (lane >> 4) < a.hd, out[step]);
 }
 
-// A row's dims 16 j + 4g .. + 3 of a result's tile, times f.
-template <class T>
+// A row's dims d = 16 j + 4g .. + 3 of a result's tile, times f. (WHOLE: all of them or none
+// are there: the way for parts of them, present if never taken, costs a store its branches.)
+template <bool WHOLE, class T>
 __device__ __forceinline__ void put4(T* row, const f4& x, float f, int d, int hd) {
-  if (d + 4 <= hd) {
+  if (WHOLE ? d < hd : d + 4 <= hd) {
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) row[d + r] = x[r] * f;
@@ -356,7 +357,7 @@ __device__ __forceinline__ void put4(T* row, const f4& x, float f, int d, int hd
       const t4 y = {T(x[0] * f), T(x[1] * f), T(x[2] * f), T(x[3] * f)};
       *reinterpret_cast<u2e*>(row + d) = __builtin_bit_cast(u2e, y);
     }
-  } else {
+  } else if constexpr (!WHOLE) {
 #pragma unroll
     for (int r = 0; r < 4; ++r)
       if (d + r < hd) row[d + r] = T(x[r] * f);

@@ -6,7 +6,9 @@
 // are staged in LDS, masked ones as zeros with a weight of -inf, and S^T = K Q^T
 // comes with a lane's query in its column, so maxima and sums are the lane's own but
 // for two lane swaps, and P^T is the B operand of O^T += V^T P^T as it lies. log cf
-// is the product's first summand, the bias a gather from LDS by the pair's offset.
+// is the product's first summand, the bias a gather from LDS by the pair's offset. The
+// probabilities are rounded to the row type for their product with V, whose operands are
+// of that type; their sum is of the unrounded ones.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -197,7 +199,8 @@ struct Tiles {
 #pragma unroll
         for (int j = 0; j < DT; ++j) {
           if (!some) o[qt][j] = f4{0.f, 0.f, 0.f, 0.f};
-          put4(to, o[qt][j], f, 16 * j + 4 * g, a.hd);
+          // (at 64 dims with a bias and dropout the short way moved the stores: 711 -> 787 us; at 32, 67 -> 64)
+          put4<WHOLE && HD == 32>(to, o[qt][j], f, 16 * j + 4 * g, a.hd);
         }
       }
     }
@@ -212,10 +215,16 @@ __device__ __forceinline__ void fill_lut(const Args& a, float* lut, int h) {
 // Up to 128 slots: an item is an atom, all of its keys staged at once, its tiles of
 // queries dealt to the workgroup's waves (4 from 33 slots on: a workgroup's waves start
 // at one SIMD, and 5 of them, one a tile of 71 slots, left room for no third workgroup
-// on the CU; which wave has the odd tile goes round by the atom).
+// on the CU; which wave has the odd tile goes round by the atom). 1728 atoms of 71
+// tokens, 8 heads of 32, bf16: 64 us, 4.0 TB/s of Q, K, V and the result, each moved once
+// (a copy reaches 5.0); 11392 of 32 to 71, 8 heads of 64, with bias and dropout: 711 us,
+// 3.4 TB/s, bound by the exponentials, the bias and the random numbers.
+// Three waves a SIMD where four would spill.
+template <int HD, bool BIAS, bool DROP>
+constexpr int kFwdWaves = HD == 128 ? 2 : HD == 64 && BIAS && DROP ? 3 : 4;
 template <class T, int HD, bool WHOLE, bool BIAS, bool DROP>
-__global__ __launch_bounds__(256, HD == 128 ? 2 : HD == 64 && BIAS && DROP ? 3 : 4) void typed_fwd_short_kernel(Args a, int keys, T* merged, int64_t ldm,
-                                                                                float* ml) {
+__global__ __launch_bounds__(256, (kFwdWaves<HD, BIAS, DROP>)) void typed_fwd_short_kernel(Args a, int keys, T* merged,
+                                                                                           int64_t ldm, float* ml) {
   extern __shared__ __align__(16) char lds[];
   T* const ks = reinterpret_cast<T*>(lds);
   T* const vs = ks + keys * HD;
@@ -251,7 +260,8 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : HD == 64 && BIAS && DROP ? 3 :
       weight[threadIdx.x] = int(threadIdx.x) < seg.count && w > 0.f ? log_weight(w) * a.inv2 : -kInf;
       if constexpr (BIAS) kpos[threadIdx.x] = p;
     }
-    staged.put(a, ks, kcols, a.ldq, vs, vcols, a.ldq, kcols, a.ldq, seg, n_keys, [](int, int, const u4&, const u4&) {});
+    staged.put(a, ks, kcols, a.ldq, vs, vcols, a.ldq, kcols, a.ldq, seg, n_keys,
+               [](int, int, const u4&, const u4&) {});
     stage_barrier();
     while (tile < slots) {
       q.start(a, seg, 16 * tile, lane);
@@ -265,7 +275,10 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : HD == 64 && BIAS && DROP ? 3 :
 }
 
 // Past 128 slots: an item is an atom's 128 queries, two tiles a wave, and the keys come in
-// stages, the next one's loads on their way into LDS while the present one is used.
+// stages, the next one's loads on their way into LDS while the present one is used. Two
+// atoms of 3500 to 4096 tokens, 8 heads of 128 over 2, with a bias: 190 us, 650 TFLOP/s
+// (a library's large product: 1143); the exponentials and the bias' gathers stand between
+// the products. Two tiles a wave share each read of K and V.
 template <class T, int HD, bool WHOLE, bool BIAS, bool DROP>
 __global__ __launch_bounds__(256, 2) void typed_fwd_long_kernel(Args a, int qblocks, T* merged, int64_t ldm, float* ml) {
   extern __shared__ __align__(16) char lds[];
@@ -325,7 +338,8 @@ __global__ __launch_bounds__(256, 2) void typed_fwd_long_kernel(Args a, int qblo
           const T* const ks = rows + at * 2 * kStage * HD;
           const int n_keys = min(kStage, round_up(seg.count - k0, 32));
           for (int kb = 0; kb < n_keys; kb += 32 * U)
-            q.keys(a, key, h, ks, ks + kStage * HD, weights + at * kStage, positions + at * kStage, lut, k0, kb, n_keys, lane);
+            q.keys(a, key, h, ks, ks + kStage * HD, weights + at * kStage, positions + at * kStage, lut, k0, kb, n_keys,
+                   lane);
         }
         if (more) land(k0 + kStage, at ^ 1);
       }
@@ -352,7 +366,9 @@ int zero_dead(const Args& a, void* x, int64_t ld, int width, hipStream_t st) {
 }
 
 // Whether a segment's offsets of a matrix are the product of 24-bit numbers under 2^32.
-bool narrow(const Args& a, int64_t ld) { return ld < (1 << 23) && a.S < (1 << 24) && int64_t(a.S) * ld * 2 < INT64_C(1) << 32; }
+bool narrow(const Args& a, int64_t ld) {
+  return ld < (1 << 23) && a.S < (1 << 24) && int64_t(a.S) * ld * 2 < INT64_C(1) << 32;
+}
 
 int check_args(int dtype, const pet_attn_shape* sh, int kv_heads, const void* qkv, int64_t ldq, const int* off,
                const float* cf_seq, int64_t ldc, const pet_attn_bias* bias, const pet_dropout* dropout, Args& a) {
@@ -372,7 +388,8 @@ int check_args(int dtype, const pet_attn_shape* sh, int kv_heads, const void* qk
   a = Args{};
   if (bias) {
     if (!bias->table || !bias->buckets || (sh->n_rows > 0 && !bias->positions)) return PET_ATTN_EINVAL;
-    if (bias->n_buckets < 1 || bias->n_buckets > PET_BIAS_MAX_BUCKETS || bias->reach < 0 || bias->reach > PET_BIAS_MAX_REACH)
+    if (bias->n_buckets < 1 || bias->n_buckets > PET_BIAS_MAX_BUCKETS || bias->reach < 0 ||
+        bias->reach > PET_BIAS_MAX_REACH)
       return PET_ATTN_EINVAL;
     for (const void* p : {static_cast<const void*>(bias->table), static_cast<const void*>(bias->buckets),
                           static_cast<const void*>(bias->positions)})

@@ -302,9 +302,18 @@ __device__ __forceinline__ float magnitude(unsigned m) {
 // operands of dV^T += dO^T P and dK^T += Q^T dS as they lie. dS goes to LDS, a key's
 // queries a row, and once every wave is done with Q's rows and K's lie there, it is read
 // transposed for dQ^T += K^T dS^T, a tile of queries a wave: every product is formed once,
-// where the two passes past 128 slots form S, dP and their exponentials twice.
+// where the two passes past 128 slots form S, dP and their exponentials twice. dS is rounded
+// to the row type for its products with Q and K, as P is for its with dO: the operands'
+// type. 1728 atoms of 71 tokens, 8 heads of 32, bf16: 135 us (209 in two passes' kernels with
+// all sums kept), 3.9 TB/s of what is moved once; 11392 of 32 to 71, 8 heads of 64, with bias,
+// its gradient and dropout: 2000 us, the vector unit half busy, waves waiting 70% of their
+// time at two a SIMD, which registers bound.
+// Two waves a SIMD where three would spill.
+template <int HD, int KT, bool GROUP, bool BIAS>
+constexpr int kShortWaves =
+    HD == 128 || (KT == 2 && GROUP && (HD == 64 || BIAS)) || (HD == 64 && (BIAS || KT == 1)) ? 2 : 3;
 template <class T, int HD, int KT, bool GROUP, bool WHOLE, bool BIAS, bool DROP>
-__global__ __launch_bounds__(256, HD == 128 || (KT == 2 && GROUP && (HD == 64 || BIAS)) || (HD == 64 && (BIAS || KT == 1)) ? 2 : 3) void typed_bwd_short_kernel(Args a, Grads b, int R,
+__global__ __launch_bounds__(256, (kShortWaves<HD, KT, GROUP, BIAS>)) void typed_bwd_short_kernel(Args a, Grads b, int R,
                                                                                            unsigned stats, unsigned more) {
   extern __shared__ __align__(16) char lds[];
   constexpr int DS = HD / 32, DT = HD / 16, CH = HD / 8;
@@ -377,8 +386,8 @@ __global__ __launch_bounds__(256, HD == 128 || (KT == 2 && GROUP && (HD == 64 ||
 #pragma unroll
       for (int j = 0; j < DT; ++j) {
         if (!klive[kt]) dk[at][j] = dv[at][j] = f4{0.f, 0.f, 0.f, 0.f};
-        put4(row + (a.H + hk) * a.hd, dk[at][j], a.scale / sc, 16 * j + 4 * g, a.hd);
-        put4(row + (a.H + a.Hk + hk) * a.hd, dv[at][j], 1.f, 16 * j + 4 * g, a.hd);
+        put4<WHOLE>(row + (a.H + hk) * a.hd, dk[at][j], a.scale / sc, 16 * j + 4 * g, a.hd);
+        put4<WHOLE>(row + (a.H + a.Hk + hk) * a.hd, dv[at][j], 1.f, 16 * j + 4 * g, a.hd);
       }
     };
     if constexpr (GROUP)
@@ -566,7 +575,7 @@ __global__ __launch_bounds__(256, HD == 128 || (KT == 2 && GROUP && (HD == 64 ||
         if (s < seg.count) {
           T* const row = static_cast<T*>(b.adj) + seg.row(s) * b.lda + h * a.hd;
 #pragma unroll
-          for (int j = 0; j < DT; ++j) put4(row, dq[j], a.scale * back, 16 * j + 4 * g, a.hd);
+          for (int j = 0; j < DT; ++j) put4<WHOLE>(row, dq[j], a.scale * back, 16 * j + 4 * g, a.hd);
         }
       }
       if (hist && G > 1) flush(i);
@@ -593,7 +602,11 @@ struct KvLds {
 // dK, dV, the cutoff factors' and the table's adjoints: a wave has KT tiles of 16 keys
 // as B operands, dK^T and dV^T in registers, and goes over all queries of the group's
 // heads, staged in LDS: S = Q K^T and dP = dO V^T with a lane's key in its column, so P
-// and dS are the B operands of dV^T += dO^T P and dK^T += Q^T dS as they lie.
+// and dS are the B operands of dV^T += dO^T P and dK^T += Q^T dS as they lie. Two atoms
+// of 3500 to 4096 tokens, 8 heads of 128 over 2, with a bias and its gradient: 537 us, 460
+// TFLOP/s of its four products. LDS is busy 44% of that (each wave reads Q and dO twice for
+// 16 keys), the vector unit 37%. Two tiles of keys a wave there halve the reads and leave one
+// wave a SIMD: 647 us against 551.
 template <class T, int HD, int KT, bool WHOLE, bool BIAS, bool DROP>
 __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, int kblocks) {
   extern __shared__ __align__(16) char lds[];
@@ -727,7 +740,10 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, i
             u4 qf[DS], gf[DS];
             d2[t] = *reinterpret_cast<const f4*>(delta + at);
 #pragma unroll
-            for (int d = 0; d < DS; ++d) qf[d] = straight<T, HD>(qs, qb, t, d, lane), gf[d] = straight<T, HD>(gs, qb, t, d, lane);
+            for (int d = 0; d < DS; ++d) {
+              qf[d] = straight<T, HD>(qs, qb, t, d, lane);
+              gf[d] = straight<T, HD>(gs, qb, t, d, lane);
+            }
             reads_first();
 #pragma unroll
             for (int kt = 0; kt < KT; ++kt) s2[t][kt] = dp2[t][kt] = f4{0.f, 0.f, 0.f, 0.f};
@@ -791,7 +807,7 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, i
             for (int kt = 0; kt < KT; ++kt) dk[kt][j] = mfma<T>(qt[j], df[kt], dk[kt][j]);
         }
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt) cf_sum[kt] += part_sum[kt];  // (a stage's sum at a time: its error grows by the stages)
+        for (int kt = 0; kt < KT; ++kt) cf_sum[kt] += part_sum[kt];  // (a stage's sum at a time, for its roundings)
         if (more) land(q0 + kStage, at_stage ^ 1);
       }
 #pragma unroll
@@ -813,11 +829,11 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, i
         if (!klive[kt]) dk[kt][j] = dv[kt][j] = f4{0.f, 0.f, 0.f, 0.f};
         const int d = 16 * j + 4 * g;
         if (parts > 1) {
-          put4(sums_row, dk[kt][j], a.scale * back, d, a.hd);
-          put4(sums_row + a.Hk * a.hd, dv[kt][j], 1.f, d, a.hd);
+          put4<WHOLE>(sums_row, dk[kt][j], a.scale * back, d, a.hd);
+          put4<WHOLE>(sums_row + a.Hk * a.hd, dv[kt][j], 1.f, d, a.hd);
         } else {
-          put4(row + (a.H + hk) * a.hd, dk[kt][j], a.scale * back, d, a.hd);
-          put4(row + (a.H + a.Hk + hk) * a.hd, dv[kt][j], 1.f, d, a.hd);
+          put4<WHOLE>(row + (a.H + hk) * a.hd, dk[kt][j], a.scale * back, d, a.hd);
+          put4<WHOLE>(row + (a.H + a.Hk + hk) * a.hd, dv[kt][j], 1.f, d, a.hd);
         }
       }
     }
@@ -826,7 +842,8 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, i
 }
 
 // dQ: a wave has QT tiles of 16 queries as B operands and goes over the keys: S^T and
-// dP^T with a lane's query in its column, dS^T the B operand of dQ^T += K^T dS^T.
+// dP^T with a lane's query in its column, dS^T the B operand of dQ^T += K^T dS^T. The same
+// case: 285 us, 650 TFLOP/s of its three products, the exponentials between them.
 template <class T, int HD, int QT, bool WHOLE, bool BIAS, bool DROP>
 __global__ __launch_bounds__(256, 2) void typed_bwd_q_kernel(Args a, Grads b, int qblocks) {
   extern __shared__ __align__(16) char lds[];
@@ -973,7 +990,7 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_q_kernel(Args a, Grads b, in
       if (s >= seg.count) continue;
       T* const row = static_cast<T*>(b.adj) + seg.row(s) * b.lda + h * a.hd;
 #pragma unroll
-      for (int j = 0; j < DT; ++j) put4(row, dq[qt][j], a.scale * back, 16 * j + 4 * g, a.hd);
+      for (int j = 0; j < DT; ++j) put4<WHOLE>(row, dq[qt][j], a.scale * back, 16 * j + 4 * g, a.hd);
     }
   }
 }
@@ -1081,8 +1098,7 @@ using namespace pet_tattn;
 extern "C" size_t pet_attn_bwd_typed_workspace(int dtype, const pet_attn_shape* shape, int kv_heads, int n_buckets) {
   if (!shape || (dtype != PET_DTYPE_BF16 && dtype != PET_DTYPE_F16) || kv_heads < 1 || shape->heads < 1 ||
       shape->heads % kv_heads != 0 || shape->n_atoms < 0 || shape->n_rows < 0 || shape->slots < 1 || shape->head_dim < 1 ||
-      shape->head_dim > 128 || n_buckets < 0 ||
-      n_buckets > PET_BIAS_MAX_BUCKETS)
+      shape->head_dim > 128 || n_buckets < 0 || n_buckets > PET_BIAS_MAX_BUCKETS)
     return 0;
   return Workspace(dtype, *shape, kv_heads, n_buckets).bytes;
 }
@@ -1096,7 +1112,8 @@ extern "C" int pet_attn_bwd_typed(int dtype, const pet_attn_shape* shape, int kv
   Args a;
   if (const int e = check_args(dtype, shape, kv_heads, qkv, ldq, off, cf_seq, ldc, bias, dropout, a)) return e;
   const int D = a.H * a.hd, W = (a.H + 2 * a.Hk) * a.hd;
-  if ((a.T > 0 && (!dmerged || !merged || !qkv_adj)) || (a.N > 0 && !ml) || ldg < D || ldm < D || lda < W) return PET_ATTN_EINVAL;
+  if ((a.T > 0 && (!dmerged || !merged || !qkv_adj)) || (a.N > 0 && !ml) || ldg < D || ldm < D || lda < W)
+    return PET_ATTN_EINVAL;
   if ((cf_seq_adj && ldca < a.S) || (table_adj && !bias)) return PET_ATTN_EINVAL;
   for (const void* p : {dmerged, merged, static_cast<const void*>(qkv_adj)})
     if (!pet_typed::element_aligned(p, dtype)) return PET_ATTN_EALIGN;
