@@ -306,7 +306,7 @@ __device__ __forceinline__ float magnitude(unsigned m) {
 // to the row type for its products with Q and K, as P is for its with dO: the operands'
 // type. 1728 atoms of 71 tokens, 8 heads of 32, bf16: 135 us (209 in two passes' kernels with
 // all sums kept), 3.9 TB/s of what is moved once; 11392 of 32 to 71, 8 heads of 64, with bias,
-// its gradient and dropout: 2000 us, the vector unit half busy, waves waiting 70% of their
+// its gradient and dropout: 2000 us, the vector unit half busy, waves waiting half of their
 // time at two a SIMD, which registers bound.
 // Two waves a SIMD where three would spill.
 template <int HD, int KT, bool GROUP, bool BIAS>
