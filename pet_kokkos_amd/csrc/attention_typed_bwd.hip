@@ -1017,39 +1017,41 @@ __global__ __launch_bounds__(256) void typed_kv_sum_kernel(Args a, Grads b) {
   }
 }
 
-// cf_adj[n][k] = beta cf_adj[n][k] + (sum over heads and parts in order of cfh[part][n][h][k]) / cf (keys that count)
-__global__ __launch_bounds__(256) void typed_cf_kernel(Args a, const float* cfh, int parts, float* adj, int64_t lda, float beta) {
-  const int64_t all = int64_t(a.N) * a.S;
-  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < all; i += int64_t(gridDim.x) * 256) {
+// What is left to sum, one launch of both: workgroups h < tables take a head's table adjoint,
+// table_adj[b][h] = beta table_adj[b][h] + the passes' workgroups' sums, 16 strips of them in
+// order, in double (1024 threads); the rest the cutoff factors' adjoints, the heads' sums over
+// cf. (Two launches: 4 us more a call.)
+__global__ __launch_bounds__(1024) void typed_sums_kernel(Args a, Grads b, int slots, int tables, float* table_adj,
+                                                          float* cf_adj, int64_t ldc, float beta) {
+  __shared__ double strips[16][64];
+  if (int(blockIdx.x) < tables) {
+    const int h = blockIdx.x, k = threadIdx.x & 63, strip = threadIdx.x >> 6;
+    double sum = 0.0;
+    if (k < a.nb)
+      for (int s = strip; s < slots; s += 16) sum += b.part[(int64_t(s) * a.H + h) * a.nb + k];
+    strips[strip][k] = sum;
+    __syncthreads();
+    if (strip || k >= a.nb) return;
+    sum = 0.0;
+    for (int i = 0; i < 16; ++i) sum += strips[i][k];
+    float* const to = table_adj + int64_t(k) * a.H + h;
+    *to = float(beta == 0.f ? sum : double(beta) * *to + sum);
+    return;
+  }
+  const int64_t all = int64_t(a.N) * a.S, step = int64_t(int(gridDim.x) - tables) * blockDim.x;
+  for (int64_t i = int64_t(int(blockIdx.x) - tables) * blockDim.x + threadIdx.x; i < all; i += step) {
     const int64_t n = i / a.S;
     const int s = int(i - n * a.S);
     const Segment seg(a, int(n));
     float sum = 0.f;
     if (seg.key(a, s)) {
       for (int h = 0; h < a.H; ++h)
-        for (int p = 0; p < parts; ++p) sum += cfh[((int64_t(p) * a.N + n) * a.H + h) * a.S + s];
+        for (int p = 0; p < b.queries_in; ++p) sum += b.cfh[((int64_t(p) * a.N + n) * a.H + h) * a.S + s];
       sum /= seg.cf(a, s);
     }
-    float* const to = adj + n * lda + s;
+    float* const to = cf_adj + n * ldc + s;
     *to = beta == 0.f ? sum : fmaf(beta, *to, sum);
   }
-}
-
-// table_adj[b][h] = beta table_adj[b][h] + the workgroups' sums in order: workgroup h, 16 strips of them in double.
-__global__ __launch_bounds__(1024) void typed_table_kernel(const double* part, int slots, int H, int nb, float* adj,
-                                                           float beta) {
-  __shared__ double strips[16][64];
-  const int h = blockIdx.x, b = threadIdx.x & 63, strip = threadIdx.x >> 6;
-  double sum = 0.0;
-  if (b < nb)
-    for (int s = strip; s < slots; s += 16) sum += part[(int64_t(s) * H + h) * nb + b];
-  strips[strip][b] = sum;
-  __syncthreads();
-  if (strip || b >= nb) return;
-  sum = 0.0;
-  for (int i = 0; i < 16; ++i) sum += strips[i][b];
-  float* const to = adj + int64_t(b) * H + h;
-  *to = float(beta == 0.f ? sum : double(beta) * *to + sum);
 }
 
 constexpr size_t aligned(size_t n) { return (n + 255) & ~size_t(255); }
@@ -1115,6 +1117,7 @@ extern "C" int pet_attn_bwd_typed(int dtype, const pet_attn_shape* shape, int kv
   if ((a.T > 0 && (!dmerged || !merged || !qkv_adj)) || (a.N > 0 && !ml) || ldg < D || ldm < D || lda < W)
     return PET_ATTN_EINVAL;
   if ((cf_seq_adj && ldca < a.S) || (table_adj && !bias)) return PET_ATTN_EINVAL;
+  if (table_adj && a.H > 1 << 20) return PET_ATTN_EINDEX;  // (threads of typed_sums_kernel)
   for (const void* p : {dmerged, merged, static_cast<const void*>(qkv_adj)})
     if (!pet_typed::element_aligned(p, dtype)) return PET_ATTN_EALIGN;
   if ((reinterpret_cast<uintptr_t>(ml) & 7u) != 0 || !pet_typed::element_aligned(cf_seq_adj, PET_DTYPE_F32) ||
@@ -1201,14 +1204,12 @@ extern "C" int pet_attn_bwd_typed(int dtype, const pet_attn_shape* shape, int kv
     });
   });
   if (err) return err;
-  if (cf_seq_adj && a.N > 0) {
-    const int64_t blocks = std::min<int64_t>((int64_t(a.N) * a.S + 255) / 256, 16384);
-    hipLaunchKernelGGL(typed_cf_kernel, dim3(unsigned(blocks)), dim3(256), 0, st, a, b.cfh, parts.queries, cf_seq_adj, ldca, beta);
-    if (hipGetLastError() != hipSuccess) return PET_ATTN_ELAUNCH;
-  }
-  if (table_adj) {
-    hipLaunchKernelGGL(typed_table_kernel, dim3(unsigned(a.H)), dim3(1024), 0, st, b.part, slots, a.H, a.nb, table_adj,
-                       beta);
+  const int tables = table_adj ? a.H : 0, threads = table_adj ? 1024 : 256;
+  const int64_t cfs = cf_seq_adj && a.N > 0
+                          ? std::min<int64_t>((int64_t(a.N) * a.S + threads - 1) / threads, (1 << 22) / threads) : 0;
+  if (tables + cfs > 0) {
+    hipLaunchKernelGGL(typed_sums_kernel, dim3(unsigned(tables + cfs)), dim3(threads), 0, st, a, b, slots, tables, table_adj,
+                       cf_seq_adj, ldca, beta);
     if (hipGetLastError() != hipSuccess) return PET_ATTN_ELAUNCH;
   }
   return PET_ATTN_OK;

@@ -60,6 +60,13 @@ def bwd(dtype=BF16, sh=None, kv=2, qkv=P[0], ldq=128, off=P[1], g=P[5], ldg=64, 
                                           ldca, ta, 0.0, ws, nbytes, None)
 
 
+def test_more_heads_than_a_launch_holds():
+    """The tables' sums are a workgroup of 1024 threads a head."""
+    wide = dict(sh=shape(H=(1 << 20) + 1, hd=1), kv=1, ldq=1 << 40, ldg=1 << 40, ldm=1 << 40, lda=1 << 40, b=bias())
+    assert bwd(ta=P[11], **wide) == _lib.EINDEX
+    assert bwd(ta=P[11], ws=None, **{**wide, "sh": shape(H=1 << 20, hd=1)}) == _lib.EWORKSPACE
+
+
 @pytest.mark.parametrize("call", [fwd, bwd])
 def test_attention_refusals(call):
     assert call(dtype=F32) == call(dtype=3) == call(kv=0) == call(kv=3) == _lib.EINVAL
