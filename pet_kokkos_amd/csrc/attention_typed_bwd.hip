@@ -145,6 +145,15 @@ __device__ __forceinline__ float adjoint_scale(const Args& a, const Grads& b, co
   return scale_to(m[0] * m[1] * a.drop.scale + m[2], 14);
 }
 
+// And a long row's probabilities, or a key's near the cutoff, lie as far under 1: for their
+// product with dO they are scaled by the power of two that brings 1 / (1 - p), the most that
+// P M is, to 2^13 .. 2^14 (P of large logits can be off to past 1), and dV is scaled back.
+// Unscaled, keys of cf 1e-5 among 2500 had no dV at all.
+template <class T>
+__device__ __forceinline__ float probability_scale(const Args& a) {
+  return std::is_same<T, _Float16>::value ? scale_to(a.drop.scale, 13) : 1.f;
+}
+
 // The same maxima over the whole call, a workgroup's at b.maxima[3 block].
 __global__ __launch_bounds__(256) void maxima_kernel(Args a, Grads b) {
   __shared__ float room[12];
@@ -336,6 +345,7 @@ __global__ __launch_bounds__(256, (kShortWaves<HD, KT, GROUP, BIAS>)) void typed
   const Share share(a.Hk);
   const int hk = share.head;
   const bool hist = BIAS && b.part;
+  const float up = probability_scale<T>(a);
   const T* const qkv = static_cast<const T*>(a.qkv);
   const T* const kcols = qkv + (a.H + hk) * a.hd;
   const T* const vcols = qkv + (a.H + a.Hk + hk) * a.hd;
@@ -387,7 +397,7 @@ __global__ __launch_bounds__(256, (kShortWaves<HD, KT, GROUP, BIAS>)) void typed
       for (int j = 0; j < DT; ++j) {
         if (!klive[kt]) dk[at][j] = dv[at][j] = f4{0.f, 0.f, 0.f, 0.f};
         put4<WHOLE>(row + (a.H + hk) * a.hd, dk[at][j], a.scale / sc, 16 * j + 4 * g, a.hd);
-        put4<WHOLE>(row + (a.H + a.Hk + hk) * a.hd, dv[at][j], 1.f, 16 * j + 4 * g, a.hd);
+        put4<WHOLE>(row + (a.H + a.Hk + hk) * a.hd, dv[at][j], 1.f / up, 16 * j + 4 * g, a.hd);
       }
     };
     if constexpr (GROUP)
@@ -478,7 +488,7 @@ __global__ __launch_bounds__(256, (kShortWaves<HD, KT, GROUP, BIAS>)) void typed
         }
         counts = units / sc;
       }
-      const float back = 1.f / sc;
+      const float back = 1.f / sc, down = sc / up;
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt) {
         const int tile = first + waves * kt;
@@ -516,12 +526,13 @@ __global__ __launch_bounds__(256, (kShortWaves<HD, KT, GROUP, BIAS>)) void typed
                 w += be.value;
                 column[r] = be.column;
               }
-              const float e = exp2_fast(fmaf(s[r], a.scale2, w));
+              float e = exp2_fast(fmaf(s[r], a.scale2, w));
+              if constexpr (HALF) e *= up;
               float kept = e;
               if constexpr (DROP) kept = masked(e, bits, t, r);
               p[4 * t + r] = kept;
-              const float es = HALF ? e * sc : e;
-              const float x = fmaf(HALF ? kept * sc : kept, dp[r], -es * d4[r]);
+              float x = fmaf(kept, dp[r], -e * d4[r]);
+              if constexpr (HALF) x *= down;
               ds[4 * t + r] = x;
               cf_sum += x;
               counted[r] = x * counts;
@@ -626,6 +637,7 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, i
   const Share share(a.Hk);
   const int hk = share.head;
   const bool hist = BIAS && b.part;
+  const float up = probability_scale<T>(a);
   const T* const qkv = static_cast<const T*>(a.qkv);
   const T* const kcols = qkv + (a.H + hk) * a.hd;
   const T* const vcols = qkv + (a.H + a.Hk + hk) * a.hd;
@@ -658,7 +670,7 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, i
     const int first_head = hi * (G / b.heads_in), last_head = first_head + G / b.heads_in;
     const int q_each = round_up((seg.count + b.queries_in - 1) / b.queries_in, kStage);
     const int q_first = min(qi * q_each, seg.count), q_last = min(q_first + q_each, seg.count);
-    const float sc = adjoint_scale<T>(a, b, seg, hk, room), back = 1.f / sc, counts = hist ? units * back : 0.f;
+    const float sc = adjoint_scale<T>(a, b, seg, hk, room), back = 1.f / sc, down = sc / up, counts = hist ? units * back : 0.f;
     const int k0 = kb * per + wave * KT * 16;
     u4 kf[KT][DS], vf[KT][DS];
     f4 dk[KT][DT], dv[KT][DT];
@@ -778,12 +790,13 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, i
                   w += be.value;
                   column[r] = be.column;
                 }
-                const float e = exp2_fast(fmaf(s2[t][kt][r], a.scale2, w));
+                float e = exp2_fast(fmaf(s2[t][kt][r], a.scale2, w));
+                if constexpr (HALF) e *= up;
                 float kept = e;
                 if constexpr (DROP) kept = masked(e, bits[kt], t, r);
                 p[kt][4 * t + r] = kept;
-                const float es = HALF ? e * sc : e;
-                const float x = fmaf(HALF ? kept * sc : kept, dp2[t][kt][r], -es * d4[r]);
+                float x = fmaf(kept, dp2[t][kt][r], -e * d4[r]);
+                if constexpr (HALF) x *= down;
                 ds[kt][4 * t + r] = x;
                 part_sum[kt] += x;
                 counted[r] = x * counts;
@@ -830,10 +843,10 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, i
         const int d = 16 * j + 4 * g;
         if (parts > 1) {
           put4<WHOLE>(sums_row, dk[kt][j], a.scale * back, d, a.hd);
-          put4<WHOLE>(sums_row + a.Hk * a.hd, dv[kt][j], 1.f, d, a.hd);
+          put4<WHOLE>(sums_row + a.Hk * a.hd, dv[kt][j], 1.f / up, d, a.hd);
         } else {
           put4<WHOLE>(row + (a.H + hk) * a.hd, dk[kt][j], a.scale * back, d, a.hd);
-          put4<WHOLE>(row + (a.H + a.Hk + hk) * a.hd, dv[kt][j], 1.f, d, a.hd);
+          put4<WHOLE>(row + (a.H + a.Hk + hk) * a.hd, dv[kt][j], 1.f / up, d, a.hd);
         }
       }
     }
