@@ -21,7 +21,6 @@ namespace pet_tattn {
 namespace {
 
 constexpr int kMaxSlots = 1024;    // workgroups a head at most (a partial sum of the table each)
-constexpr int kMaxima = 256;
 constexpr int kColumns = 32;       // columns of a bucket's sum
 
 // What the backward's kernels are given beside Args.
@@ -33,7 +32,7 @@ struct Grads {
   int64_t lda;
   float* delta;   // [T, H]: dO.O
   float* norms;   // [T, H] |dO|, then [T, Hk] |v|: fp16, or a table's gradient
-  float* maxima;  // [kMaxima, 3], with a table's gradient: of |dO|, |v| and |dO.O|
+  float* bounds;  // [N, H], where norms are, past 128 slots: of an atom's and head's |dS|
   float* cfh;     // [queries_in, N, H, S], or null
   double* part;   // [slots, H, nb], with a table's gradient
   // the pass over the keys in parts, of a group's heads by `heads_in`, of the queries by `queries_in`
@@ -44,16 +43,24 @@ struct Grads {
 __device__ __forceinline__ float power_of_two(int e) { return ldexpf(1.f, e); }
 
 // Over groups of `n` lanes (4, 8, 16) within a row of 16.
-template <int n>
-__device__ __forceinline__ float row_sum(float x) {
+template <int n, class Join>
+__device__ __forceinline__ float row_join(float x, const Join& join) {
   const auto swap = [](float v, auto ctrl) {
     return __uint_as_float(__builtin_amdgcn_update_dpp(0u, __float_as_uint(v), decltype(ctrl)::value, 0xf, 0xf, true));
   };
-  x += swap(x, std::integral_constant<int, 0xB1>{});                        // lane ^ 1
-  x += swap(x, std::integral_constant<int, 0x4E>{});                        // lane ^ 2
-  if constexpr (n >= 8) x += swap(x, std::integral_constant<int, 0x141>{});  // 7 - lane of eight
-  if constexpr (n >= 16) x += swap(x, std::integral_constant<int, 0x140>{});  // 15 - lane
+  x = join(x, swap(x, std::integral_constant<int, 0xB1>{}));                        // lane ^ 1
+  x = join(x, swap(x, std::integral_constant<int, 0x4E>{}));                        // lane ^ 2
+  if constexpr (n >= 8) x = join(x, swap(x, std::integral_constant<int, 0x141>{}));  // 7 - lane of eight
+  if constexpr (n >= 16) x = join(x, swap(x, std::integral_constant<int, 0x140>{}));  // 15 - lane
   return x;
+}
+template <int n>
+__device__ __forceinline__ float row_sum(float x) {
+  return row_join<n>(x, [](float a, float b) { return a + b; });
+}
+template <int n>
+__device__ __forceinline__ float row_max(float x) {
+  return row_join<n>(x, [](float a, float b) { return fmaxf(a, b); });
 }
 __device__ __forceinline__ float wave_max(float x) {
   const auto swap = [](float v, auto ctrl) {
@@ -66,6 +73,13 @@ __device__ __forceinline__ float wave_max(float x) {
   return pet_attn::max_g(x);
 }
 
+// The power of two that brings a bound to 2^to .. 2^(to + 1); 1 for 0 and for what is not finite.
+__device__ __forceinline__ float scale_to(float bound, int to) {
+  if (!(bound > 0.f) || !(bound < kInf)) return 1.f;
+  const int e = to - ilogbf(bound);
+  return power_of_two(e > 126 ? 126 : e);
+}
+
 // dO.O of each row and head (and |dO| and |v| where b.norms is there): a group of lanes
 // takes a head's slice, eight elements each.
 template <class T, int LG>
@@ -76,7 +90,7 @@ __global__ __launch_bounds__(256) void delta_kernel(Args a, Grads b) {
     const bool q = i < heads;
     const int64_t j = q ? i : i - heads, per = q ? a.H : a.Hk, row = j / per;
     const int h = int(j - row * per);
-    float x[8], y[8], dot = 0.f, sq = 0.f;
+    float x[8], y[8], dot = 0.f, most = 0.f, sq = 0.f;
     const T* p = q ? static_cast<const T*>(b.out_adj) + row * b.ldg + h * a.hd
                    : static_cast<const T*>(a.qkv) + row * a.ldq + (a.H + a.Hk + h) * a.hd;
     pet_typed::unpack<T>(__builtin_bit_cast(u4e, row_chunk(p, 8 * l, a.hd)), x);
@@ -85,15 +99,25 @@ __global__ __launch_bounds__(256) void delta_kernel(Args a, Grads b) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       if (q) dot = fmaf(x[e], y[e], dot);
-      sq = fmaf(x[e], x[e], sq);
+      most = fmaxf(most, fabsf(x[e]));
     }
     dot = row_sum<LG>(dot);
-    if (b.norms) sq = sqrtf(row_sum<LG>(sq));
+    if (b.norms) {
+      const float to_one = scale_to(row_max<LG>(most), 1);  // (a square's exponent is twice its number's)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sq = fmaf(x[e] * to_one, x[e] * to_one, sq);
+      sq = sqrtf(row_sum<LG>(sq)) / to_one;
+    }
     if (l == 0) {
       if (q) b.delta[i] = dot;
       if (b.norms) b.norms[i] = sq;
     }
   }
+}
+
+// One for the wave, and known to be.
+__device__ __forceinline__ float uniform(float x) {
+  return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x)));
 }
 
 // Three maxima over the workgroup: m of every thread of every wave. room: 3 floats a wave.
@@ -111,38 +135,41 @@ __device__ __forceinline__ void block_max(float (&m)[3], float* room) {
     for (int i = 0; i < 3; ++i) m[i] = fmaxf(m[i], room[3 * w + i]);
 }
 
-// The power of two that brings a bound to 2^to .. 2^(to + 1); 1 for 0 and for what is not finite.
-__device__ __forceinline__ float scale_to(float bound, int to) {
-  if (!(bound > 0.f) || !(bound < kInf)) return 1.f;
-  const int e = to - ilogbf(bound);
-  return power_of_two(e < -110 ? -110 : e > 80 ? 80 : e);
-}
+// A magnitude onto a maximum; a NaN is infinite.
+__device__ __forceinline__ void onto(float& at, float x) { at = fmaxf(at, x == x ? fabsf(x) : kInf); }
 
-// The largest |dO|, |v| and |dO.O| of slot s and the heads of hk onto m, for a token that
-// counts; a NaN is infinite.
-__device__ __forceinline__ void live_maxima(const Args& a, const Grads& b, const Segment& seg, int s, int hk, float (&m)[3]) {
-  if (!seg.query(a, s)) return;
+// A bound of the dS of an atom and head, max |dO| max |v| / (1 - p) + max |dO.O|: a workgroup an
+// atom and head. Infinite or NaN where something of them is.
+__global__ __launch_bounds__(1024) void bounds_kernel(Args a, Grads b) {
+  __shared__ float room[48];
   const int G = a.H / a.Hk;
-  const int64_t row = seg.row(s);
-  const auto onto = [](float& at, float x) { at = fmaxf(at, x == x ? fabsf(x) : kInf); };
-  for (int i = 0; i < G; ++i) {
-    onto(m[0], b.norms[row * a.H + hk * G + i]);
-    onto(m[2], b.delta[row * a.H + hk * G + i]);
+  const int64_t items = int64_t(a.N) * a.H;
+  for (int64_t i = blockIdx.x; i < items; i += gridDim.x) {
+    const int64_t n = i / a.H;
+    const int h = int(i - n * a.H);
+    const Segment seg(a, int(n));
+    float m[3] = {0.f, 0.f, 0.f};
+    for (int s = threadIdx.x; s < seg.count; s += blockDim.x) {
+      if (!seg.query(a, s)) continue;
+      const int64_t row = seg.row(s);
+      onto(m[0], b.norms[row * a.H + h]);
+      onto(m[2], b.delta[row * a.H + h]);
+      if (seg.key(a, s)) onto(m[1], b.norms[int64_t(a.T) * a.H + row * a.Hk + h / G]);
+    }
+    block_max(m, room);
+    if (threadIdx.x == 0) b.bounds[i] = m[0] * m[1] * a.drop.scale + m[2];
   }
-  if (seg.key(a, s)) onto(m[1], b.norms[int64_t(a.T) * a.H + row * a.Hk + hk]);
 }
 
 // fp16 holds down to 2^-14 at full precision, and a long row's dS lie far under the
-// adjoints that they come from: they are scaled by the power of two that brings a bound
-// of them, max |dO| max |v| / (1 - p) + max |dO.O| over the atom and the group of heads,
-// to 2^14 .. 2^15. bf16 has fp32's range, and takes 1.
+// adjoints that they come from: those of `heads` heads from h on are scaled by the power of
+// two that brings their bound to 2^14 .. 2^15. bf16 has fp32's range, and takes 1.
 template <class T>
-__device__ __forceinline__ float adjoint_scale(const Args& a, const Grads& b, const Segment& seg, int hk, float* room) {
+__device__ __forceinline__ float adjoint_scale(const Args& a, const Grads& b, int n, int h, int heads) {
   if constexpr (!std::is_same<T, _Float16>::value) return 1.f;
-  float m[3] = {0.f, 0.f, 0.f};
-  for (int s = threadIdx.x; s < seg.count; s += blockDim.x) live_maxima(a, b, seg, s, hk, m);
-  block_max(m, room);
-  return scale_to(m[0] * m[1] * a.drop.scale + m[2], 14);
+  float bound = 0.f;
+  for (int i = 0; i < heads; ++i) onto(bound, b.bounds[int64_t(n) * a.H + h + i]);
+  return scale_to(uniform(bound), 14);
 }
 
 // And a long row's probabilities, or a key's near the cutoff, lie as far under 1: for their
@@ -152,22 +179,6 @@ __device__ __forceinline__ float adjoint_scale(const Args& a, const Grads& b, co
 template <class T>
 __device__ __forceinline__ float probability_scale(const Args& a) {
   return std::is_same<T, _Float16>::value ? scale_to(a.drop.scale, 13) : 1.f;
-}
-
-// The same maxima over the whole call, a workgroup's at b.maxima[3 block].
-__global__ __launch_bounds__(256) void maxima_kernel(Args a, Grads b) {
-  __shared__ float room[12];
-  float m[3] = {0.f, 0.f, 0.f};
-  const int strips = (a.S + 255) / 256;
-  const int64_t items = int64_t(a.N) * strips;
-  for (int64_t i = blockIdx.x; i < items; i += gridDim.x) {
-    const int64_t n = i / strips;
-    const Segment seg(a, int(n));
-    const int s = int(i - n * strips) * 256 + threadIdx.x;
-    for (int hk = 0; hk < a.Hk && s < seg.count; ++hk) live_maxima(a, b, seg, s, hk, m);
-  }
-  block_max(m, room);
-  if (threadIdx.x < 3) b.maxima[3 * blockIdx.x + threadIdx.x] = m[threadIdx.x];
 }
 
 // A query's exponent: P = 2^(s - this), +inf (P = 0) for one that attends to nothing.
@@ -210,12 +221,16 @@ struct BiasEntry {
 };
 
 // The bias table's gradient, sums of dS by bucket, in whole numbers of a power of two
-// that brings a bound of the dS to 2^33 .. 2^35 (past 128 slots, where probabilities are
-// small, to 2^37): additions in any order give one result, so a bucket's 32 columns are
-// shared by the workgroup's waves, and the LDS adds 64-bit integers to them at 8 cycles a
-// wave where its fp32 addition takes 194 (a CU, measured: a lane at a time). A query's
-// |dS| sum to at most about the bound, so a column holds 2^25 queries and more. Four of a
-// lane's dS at a time: under 2^30, as nearly all are, one conversion to 32 bits each.
+// that brings a bound of the atom's and head's dS to 2^33 .. 2^34 (past 128 slots, where
+// probabilities are small, to 2^36 .. 2^37): additions in any order give one result, so a
+// bucket's 32 columns are shared by the workgroup's waves, and the LDS adds 64-bit integers to
+// them at 8 cycles a wave where its fp32 addition takes 194 (a CU, measured: a lane at a time). A
+// query's |dS| sum to at most about the bound, so a column holds 2^25 queries and more. The
+// unit stays while bounds are within 2^-6 and 2 of it, and the columns are summed in float64
+// before another is taken. A bound past fp32's range, or of what is not finite, has no unit:
+// there every dS is added in float64, a column by one lane of a wave at a time (Columns::real).
+//
+// Four of a lane's dS at a time: under 2^30, as nearly all are, one conversion to 32 bits each.
 // floor(x + 1/2): halves go up. All of them up would shift the sum of 10^7 pairs by 10^-5 of
 // it, so every other one is taken as less floor(1/2 - x), whose halves go down (rounding them
 // to even by an instruction of its own cost a tenth of the whole kernel: 2040 -> 2240 us).
@@ -229,44 +244,86 @@ __device__ __forceinline__ int less_nearest(float x) {
   asm("v_cvt_rpi_i32_f32 %0, -%1" : "=v"(q) : "v"(x));
   return q;
 }
-__device__ __forceinline__ void count_in(char* columns, const int (&column)[4], const float (&x)[4]) {
-  const auto add = [&](int i, int64_t q) {
-    __hip_atomic_fetch_add(reinterpret_cast<unsigned long long*>(columns + column[i]), static_cast<unsigned long long>(q),
-                           __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-  };
-  const auto take = [&](int i, int64_t q) {
-    __hip_atomic_fetch_sub(reinterpret_cast<unsigned long long*>(columns + column[i]), static_cast<unsigned long long>(q),
-                           __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-  };
-  const float m = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
-  if (__builtin_expect(__any(m >= 0x1p30f), 0)) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int high = nearest(x[i] * 0x1p-16f);
-      const float low = fmaf(float(high), -0x1p16f, x[i]);
-      add(i, int64_t(high) << 16);
-      if (i & 1) take(i, less_nearest(low)); else add(i, nearest(low));
-    }
-    return;
+struct Columns {
+  int64_t* at;        // [nb, kColumns]
+  float units = 0.f;  // a dS of 1 counts so much (0: nothing is counted)
+  bool real = false;  // the columns are float64
+
+  __device__ __forceinline__ void clear(int nb) {
+    for (int i = threadIdx.x; i < nb * kColumns; i += blockDim.x) at[i] = 0;
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (i & 1) take(i, less_nearest(x[i])); else add(i, nearest(x[i]));
-}
-// A head's columns summed in units of `unit` onto the workgroup's own row of sums, and cleared.
-__device__ __forceinline__ void flush_columns(int64_t* columns, int nb, double unit, double* sums) {
-  __syncthreads();
-  for (int k = threadIdx.x; k < nb; k += blockDim.x) {
-    int64_t sum = 0;
-    for (int l = 0; l < kColumns; ++l) {
-      int64_t* const at = columns + k * kColumns + ((l + k) & (kColumns - 1));
-      sum += *at;
-      *at = 0;
-    }
-    sums[k] += double(sum) * unit;
+  // For dS under a bound (one for the workgroup); sums: what a flush adds to.
+  __device__ __forceinline__ void fit(float bound, int to, int nb, double* sums) {
+    const bool over = !(bound < kInf);
+    if (!over && !(bound > 0.f)) return;  // (every dS is 0)
+    const float one = over ? 1.f : scale_to(bound, to);
+    if (units > 0.f && (real != over || units >= 4.f * one || one > 64.f * units)) flush(nb, sums);
+    if (units == 0.f) units = one, real = over;
   }
-  __syncthreads();
-}
+  // x: four of a lane's dS in units, onto the buckets whose first columns are at column (bytes).
+  __device__ __forceinline__ void count(const int (&column)[4], const float (&x)[4]) const {
+    char* const columns = reinterpret_cast<char*>(at + (threadIdx.x & (kColumns - 1)));
+    const auto add = [&](int i, int64_t q) {
+      __hip_atomic_fetch_add(reinterpret_cast<unsigned long long*>(columns + column[i]), static_cast<unsigned long long>(q),
+                             __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    };
+    const auto take = [&](int i, int64_t q) {
+      __hip_atomic_fetch_sub(reinterpret_cast<unsigned long long*>(columns + column[i]), static_cast<unsigned long long>(q),
+                             __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    };
+    const float m = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+    if (__builtin_expect(__any(!(m < (real ? -1.f : 0x1p30f))), 0)) {
+      if (real) {
+        count_real(column, x);
+        return;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int high = nearest(x[i] * 0x1p-16f);
+        const float low = fmaf(float(high), -0x1p16f, x[i]);
+        add(i, int64_t(high) << 16);
+        if (i & 1) take(i, less_nearest(low)); else add(i, nearest(low));
+      }
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i & 1) take(i, less_nearest(x[i])); else add(i, nearest(x[i]));
+  }
+  // Eight columns a wave, eight lanes at a time: one lane to a column, in one order.
+  __device__ __forceinline__ void count_real(const int (&column)[4], const float (&x)[4]) const {
+    const int lane = threadIdx.x & 63;
+    char* const columns = reinterpret_cast<char*>(at + 8 * wave_of() + (lane & 7));
+#pragma unroll 1
+    for (int turn = 0; turn < 8; ++turn) {
+      if (lane >> 3 == turn)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          double* const to = reinterpret_cast<double*>(columns + column[i]);
+          const double was = __hip_atomic_load(to, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+          __hip_atomic_store(to, was + double(x[i]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+      __builtin_amdgcn_wave_barrier();
+    }
+  }
+  // The columns summed onto a head's row of the workgroup's own sums, and cleared.
+  __device__ __forceinline__ void flush(int nb, double* sums) {
+    __syncthreads();
+    for (int k = threadIdx.x; k < nb && units > 0.f; k += blockDim.x) {
+      int64_t sum = 0;
+      double float_sum = 0.0;
+      for (int l = 0; l < kColumns; ++l) {
+        int64_t* const column = at + k * kColumns + ((l + k) & (kColumns - 1));
+        if (real) float_sum += __builtin_bit_cast(double, *column); else sum += *column;
+        *column = 0;
+      }
+      sums[k] += real ? float_sum : double(sum) / double(units);
+    }
+    units = 0.f, real = false;
+    __syncthreads();
+  }
+};
 __device__ __forceinline__ void bias_entries(const Args& a, BiasEntry* lut, int h) {
   for (int i = threadIdx.x; i <= 2 * a.reach; i += blockDim.x) {
     const int bucket = bucket_of(a, i);
@@ -340,7 +397,6 @@ __global__ __launch_bounds__(256, (kShortWaves<HD, KT, GROUP, BIAS>)) void typed
   float* const room = reinterpret_cast<float*>(lds + more + 256);
   BiasEntry* const lut = reinterpret_cast<BiasEntry*>(room + 16);
   int64_t* const columns = reinterpret_cast<int64_t*>(lut + (BIAS ? 2 * a.reach + 1 : 0));
-  char* const mine = reinterpret_cast<char*>(columns + (lane & (kColumns - 1)));
   const int G = GROUP ? a.H / a.Hk : 1;
   const Share share(a.Hk);
   const int hk = share.head;
@@ -351,18 +407,14 @@ __global__ __launch_bounds__(256, (kShortWaves<HD, KT, GROUP, BIAS>)) void typed
   const T* const vcols = qkv + (a.H + a.Hk + hk) * a.hd;
   Words key{};
   if constexpr (DROP) key = a.drop.key();
-  float units = 0.f;   // of the table's sums: a power of two, made smaller as larger bounds come (0: none yet)
-  bool beyond = false;  // a dS that no unit holds
+  Columns cols{columns};
   double* const sums = hist ? b.part + (int64_t(share.slot) * a.H + hk * G) * a.nb : nullptr;
   if (hist) {
-    for (int i = threadIdx.x; i < a.nb * kColumns; i += blockDim.x) columns[i] = 0;
+    cols.clear(a.nb);
     for (int k = threadIdx.x; k < a.nb; k += blockDim.x)
       for (int i = 0; i < G; ++i) sums[i * a.nb + k] = 0.0;
   }
   if (BIAS && G == 1) bias_entries(a, lut, hk);
-  const auto flush = [&](int i) {
-    flush_columns(columns, a.nb, beyond ? double(__builtin_nanf("")) : units > 0.f ? 1.0 / double(units) : 0.0, sums + i * a.nb);
-  };
 
   for (int n = share.slot; n < a.N; n += share.step) {
     const Segment seg(a, n);
@@ -455,28 +507,15 @@ __global__ __launch_bounds__(256, (kShortWaves<HD, KT, GROUP, BIAS>)) void typed
           for (int k = 0; k < 3; ++k) room[3 * wave + k] = m[k];
       }
       stage_barrier();
-      // what brings dS into the range of fp16, and into whole numbers (adjoint_scale, count_in)
+      // what brings dS into the range of fp16, and into whole numbers (adjoint_scale, Columns)
       float counts = 0.f;
       if (HALF || hist) {
         float m[3] = {0.f, 0.f, 0.f};
         for (int w = 0; w < waves; ++w)
 #pragma unroll
           for (int k = 0; k < 3; ++k) m[k] = fmaxf(m[k], room[3 * w + k]);
-        const float bound = float(a.hd) * m[0] * m[1] * a.drop.scale + m[2];
-        if (hist) {
-          if (!(bound < kInf)) {
-            beyond = true;
-          } else if (bound > 0.f && (units == 0.f || bound * units > 0x1p35f)) {
-            const float fit = scale_to(bound, 33);
-            if (units > 0.f) {
-              const int by = ilogbf(units) - ilogbf(fit);
-              __syncthreads();
-              for (int k = threadIdx.x; k < a.nb * kColumns; k += blockDim.x) columns[k] = by < 63 ? columns[k] >> by : 0;
-              __syncthreads();
-            }
-            units = fit;
-          }
-        }
+        const float bound = uniform(float(a.hd) * m[0] * m[1] * a.drop.scale + m[2]);
+        if (hist) cols.fit(bound, 33, a.nb, sums + i * a.nb);
         if constexpr (HALF) {
           const float was = sc;
           sc = scale_to(bound, 14);
@@ -486,7 +525,7 @@ __global__ __launch_bounds__(256, (kShortWaves<HD, KT, GROUP, BIAS>)) void typed
 #pragma unroll
               for (int j = 0; j < DT; ++j) dk[at][j] *= sc / was;
         }
-        counts = units / sc;
+        counts = cols.units / sc;
       }
       const float back = 1.f / sc, down = sc / up;
 #pragma unroll
@@ -537,7 +576,7 @@ __global__ __launch_bounds__(256, (kShortWaves<HD, KT, GROUP, BIAS>)) void typed
               cf_sum += x;
               counted[r] = x * counts;
             }
-            if (hist) count_in(mine, column, counted);
+            if (hist) cols.count(column, counted);
           }
           const u4 pf = pack8<T>(p), df = pack8<T>(ds);
           *reinterpret_cast<u4*>(dss + (16 * tile + c) * pitch + qb + 8 * g) = df;
@@ -589,13 +628,13 @@ __global__ __launch_bounds__(256, (kShortWaves<HD, KT, GROUP, BIAS>)) void typed
           for (int j = 0; j < DT; ++j) put4<WHOLE>(row, dq[j], a.scale * back, 16 * j + 4 * g, a.hd);
         }
       }
-      if (hist && G > 1) flush(i);
+      if (hist && G > 1) cols.flush(a.nb, sums + i * a.nb);
     }
     if constexpr (GROUP)
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt) store(kt, kt);
   }
-  if (hist && G == 1) flush(0);
+  if (hist && G == 1) cols.flush(a.nb, sums);
 }
 
 // ---- past 128 slots: a pass over the keys and one over the queries --------------------
@@ -603,7 +642,7 @@ __global__ __launch_bounds__(256, (kShortWaves<HD, KT, GROUP, BIAS>)) void typed
 template <int HD>
 struct KvLds {
   static constexpr size_t rows = size_t(4) * kStage * HD * 2, queries = rows + size_t(2 * kStage) * 12,
-                          waves = queries + 4 * (64 + 16);  // masks and maxima
+                          waves = queries + 4 * 64;  // masks
   // + the bias's entries, the buckets' columns
   static size_t bytes(const Args& a, bool hist) {
     return waves + (a.table ? size_t(2 * a.reach + 1) * 8 : 0) + (hist ? size_t(a.nb) * kColumns * 8 : 0);
@@ -629,10 +668,8 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, i
   float* const deltas = expos + 2 * kStage;
   int* const positions = reinterpret_cast<int*>(deltas + 2 * kStage);
   unsigned char* const exchange = reinterpret_cast<unsigned char*>(positions + 2 * kStage) + 64 * wave;
-  float* const room = reinterpret_cast<float*>(positions + 2 * kStage + 64);
-  BiasEntry* const lut = reinterpret_cast<BiasEntry*>(room + 16);
+  BiasEntry* const lut = reinterpret_cast<BiasEntry*>(positions + 2 * kStage + 64);
   int64_t* const columns = reinterpret_cast<int64_t*>(lut + (BIAS ? 2 * a.reach + 1 : 0));
-  char* const mine = reinterpret_cast<char*>(columns + (lane & (kColumns - 1)));
   const int G = a.H / a.Hk;
   const Share share(a.Hk);
   const int hk = share.head;
@@ -643,19 +680,10 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, i
   const T* const vcols = qkv + (a.H + a.Hk + hk) * a.hd;
   Words key{};
   if constexpr (DROP) key = a.drop.key();
-  // the unit of the table's sums is one for the whole call
-  float units = 1.f;
-  double unit = 1.0;
+  Columns cols{columns};
   double* const sums = hist ? b.part + (int64_t(share.slot) * a.H + hk * G) * a.nb : nullptr;
   if (hist) {
-    float m[3] = {0.f, 0.f, 0.f};
-#pragma unroll
-    for (int k = 0; k < 3; ++k) m[k] = b.maxima[3 * threadIdx.x + k];
-    block_max(m, room);
-    const float bound = m[0] * m[1] * a.drop.scale + m[2];
-    units = scale_to(bound, 36);
-    unit = bound < kInf ? 1.0 / double(units) : double(__builtin_nanf(""));  // (no unit holds an infinite dS)
-    for (int i = threadIdx.x; i < a.nb * kColumns; i += 256) columns[i] = 0;
+    cols.clear(a.nb);
     for (int k = threadIdx.x; k < a.nb; k += 256)
       for (int i = 0; i < G; ++i) sums[i * a.nb + k] = 0.0;
   }
@@ -670,7 +698,7 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, i
     const int first_head = hi * (G / b.heads_in), last_head = first_head + G / b.heads_in;
     const int q_each = round_up((seg.count + b.queries_in - 1) / b.queries_in, kStage);
     const int q_first = min(qi * q_each, seg.count), q_last = min(q_first + q_each, seg.count);
-    const float sc = adjoint_scale<T>(a, b, seg, hk, room), back = 1.f / sc, down = sc / up, counts = hist ? units * back : 0.f;
+    const float sc = adjoint_scale<T>(a, b, n, hk * G, G), back = 1.f / sc, down = sc / up;
     const int k0 = kb * per + wave * KT * 16;
     u4 kf[KT][DS], vf[KT][DS];
     f4 dk[KT][DT], dv[KT][DT];
@@ -724,6 +752,8 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, i
         stage_barrier();
       };
       stage_barrier();  // (the stages and the bias of the head before are done with)
+      if (hist) cols.fit(uniform(b.bounds[int64_t(n) * a.H + h]), 36, a.nb, sums + i * a.nb);
+      const float counts = cols.units * back;
       if (BIAS && G > 1) bias_entries(a, lut, h);
       if (q_first < q_last) start(q_first, 0), land(q_first, 0);
       int at_stage = 0;
@@ -801,7 +831,7 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, i
                 part_sum[kt] += x;
                 counted[r] = x * counts;
               }
-              if (hist) count_in(mine, column, counted);
+              if (hist) cols.count(column, counted);
             }
           }
 #pragma unroll
@@ -829,7 +859,7 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, i
         const int s = k0 + 16 * kt + c;
         if (b.cfh && g == 0 && s < seg.count) b.cfh[((int64_t(qi) * a.N + n) * a.H + h) * a.S + s] = sum;
       }
-      if (hist && G > 1) flush_columns(columns, a.nb, unit, sums + i * a.nb);
+      if (hist && G > 1) cols.flush(a.nb, sums + i * a.nb);
     }
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) {
@@ -851,7 +881,7 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, i
       }
     }
   }
-  if (hist && G == 1) flush_columns(columns, a.nb, unit, sums);
+  if (hist && G == 1) cols.flush(a.nb, sums);
 }
 
 // dQ: a wave has QT tiles of 16 queries as B operands and goes over the keys: S^T and
@@ -866,8 +896,7 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_q_kernel(Args a, Grads b, in
   T* const staged = reinterpret_cast<T*>(lds);  // two stages, each K's rows and V's
   float* const weights = reinterpret_cast<float*>(staged + 4 * kStage * HD);
   int* const positions = reinterpret_cast<int*>(weights + 2 * kStage);
-  float* const room = reinterpret_cast<float*>(positions + 2 * kStage);
-  float* const lut = room + 16;
+  float* const lut = reinterpret_cast<float*>(positions + 2 * kStage);
   const Share share(a.H);
   const int h = share.head, hk = h / (a.H / a.Hk);
   const T* const qkv = static_cast<const T*>(a.qkv);
@@ -886,7 +915,7 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_q_kernel(Args a, Grads b, in
     const int n = item / qblocks, qb = item - n * qblocks;
     const Segment seg(a, n);
     if (qb * per >= seg.count) continue;
-    const float sc = adjoint_scale<T>(a, b, seg, hk, room), back = 1.f / sc;
+    const float sc = adjoint_scale<T>(a, b, n, h, 1), back = 1.f / sc;
     const int q0 = qb * per + wave * QT * 16;
     u4 qf[QT][DS], gf[QT][DS];
     f4 dq[QT][DT];
@@ -1090,14 +1119,14 @@ struct Parts {
 };
 
 struct Workspace {
-  size_t delta, norms, maxima, cfh, part, kv, bytes;
+  size_t delta, norms, bounds, cfh, part, kv, bytes;
   Workspace(int dtype, const pet_attn_shape& s, int kv_heads, int nb) {
     const size_t T = size_t(s.n_rows), H = size_t(s.heads);
     const Parts parts(s.n_atoms, s.slots, s.heads, kv_heads, s.head_dim);
     delta = 0;
     norms = delta + aligned(T * H * 4);
-    maxima = norms + (dtype == PET_DTYPE_F16 || nb ? aligned(T * (H + size_t(kv_heads)) * 4) : 0);
-    cfh = maxima + aligned(nb ? size_t(kMaxima) * 12 : 0);
+    bounds = norms + (dtype == PET_DTYPE_F16 || nb ? aligned(T * (H + size_t(kv_heads)) * 4) : 0);
+    cfh = bounds + aligned((dtype == PET_DTYPE_F16 || nb) && s.slots > kShort ? size_t(s.n_atoms) * H * 4 : 0);
     part = cfh + aligned(size_t(parts.queries) * size_t(s.n_atoms) * H * size_t(s.slots) * 4);
     kv = part + aligned(size_t(kMaxSlots) * H * size_t(nb) * 8);
     const size_t all = size_t(parts.heads) * size_t(parts.queries);
@@ -1146,7 +1175,7 @@ extern "C" int pet_attn_bwd_typed(int dtype, const pet_attn_shape* shape, int kv
   const Parts parts(a.N, a.S, a.H, a.Hk, a.hd);
   const auto at = [&](size_t offset) { return reinterpret_cast<float*>(base + offset); };
   const Grads b{dmerged, merged, ldg, ldm, ml, qkv_adj, lda, at(ws.delta), half || table_adj ? at(ws.norms) : nullptr,
-                table_adj ? at(ws.maxima) : nullptr, cf_seq_adj ? at(ws.cfh) : nullptr,
+                half || table_adj ? at(ws.bounds) : nullptr, cf_seq_adj ? at(ws.cfh) : nullptr,
                 table_adj ? reinterpret_cast<double*>(base + ws.part) : nullptr, parts.heads, parts.queries, at(ws.kv)};
   if (shape->dead && a.T > 0)
     if (const int e = zero_dead(a, qkv_adj, lda, W, st)) return e;
@@ -1177,8 +1206,10 @@ extern "C" int pet_attn_bwd_typed(int dtype, const pet_attn_shape* shape, int kv
           const unsigned blocks = unsigned(std::min<int64_t>((groups * (HD / 8) + 255) / 256, 16384));
           hipLaunchKernelGGL((delta_kernel<T, HD / 8>), dim3(blocks), dim3(256), 0, st, a, b);
           if (const int e = launched()) return e;
-          if (table_adj) {
-            hipLaunchKernelGGL(maxima_kernel, dim3(kMaxima), dim3(256), 0, st, a, b);
+          if (b.norms) {
+            const int64_t items = int64_t(a.N) * a.H;
+            hipLaunchKernelGGL(bounds_kernel, dim3(unsigned(std::min<int64_t>(items, 16384))), dim3(a.S > 512 ? 1024 : 256), 0, st,
+                               a, b);
             if (const int e = launched()) return e;
           }
         }
@@ -1204,7 +1235,7 @@ extern "C" int pet_attn_bwd_typed(int dtype, const pet_attn_shape* shape, int kv
           constexpr int QT = 2;
           const auto kernel = typed_bwd_q_kernel<T, HD, QT, WHOLE, BIAS, DROP>;
           const int blocks = (a.S + QT * 64 - 1) / (QT * 64);
-          const size_t bytes = size_t(2 * kStage) * (2 * HD * 2 + 8) + 64 + (a.table ? size_t(2 * a.reach + 1) * 4 : 0);
+          const size_t bytes = size_t(2 * kStage) * (2 * HD * 2 + 8) + (a.table ? size_t(2 * a.reach + 1) * 4 : 0);
           if (const int e = pet_attn::raise_lds(reinterpret_cast<const void*>(kernel), bytes)) return e;
           const int64_t q_slots = std::min<int64_t>((int64_t(a.N) * blocks + 7) / 8 * 8, 2048);
           if (q_slots * a.H * 256 > INT32_MAX) return int(PET_ATTN_EINDEX);
