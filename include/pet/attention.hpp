@@ -120,6 +120,14 @@ inline pet_attn_shape make_shape(const Tokens& tk, int T, int S, int heads, int 
   return sh;
 }
 
+// Rows of the saves (max, 1/sum), N heads S, which a view counts in int.
+inline int save_rows(int N, int heads, int S, const char* what) {
+  int rows = 0;
+  if (__builtin_mul_overflow(N, heads, &rows) || __builtin_mul_overflow(rows, S, &rows))
+    throw std::runtime_error(std::string("pet: ") + what + ": N heads S passes what a view's int counts");
+  return rows;
+}
+
 // Multi-head attention over each atom's tokens with log(cf) as a per-key bias,
 // then out = merged W_out^T + b_out. `save` keeps what the backward needs under
 // `key`.
@@ -128,8 +136,9 @@ inline void attention(Workspace& ws, const std::string& key, View2D out, View2D 
                       double temperature, bool save, hipStream_t stream = nullptr) {
   const int D = heads * head_dim, T = qkv.extent(0);
   if (cf_seq.extent(1) < S) throw std::runtime_error("pet: cf_seq narrower than S");
+  const int saves = save ? save_rows(tk.N, heads, S, "attention") : 0;
   const View2D merged = ws.n2(save ? key + ":merged" : std::string("attention:tmp"), T, D);
-  float* ml = save ? ws.n2(key + ":ml", tk.N * heads * S, 2).data() : nullptr;
+  float* ml = save ? ws.n2(key + ":ml", saves, 2).data() : nullptr;
   const pet_attn_shape sh = make_shape(tk, T, S, heads, head_dim, temperature);
   check(pet_attention(&sh, out.data(), out.stride(0), qkv.data(), qkv.stride(0), cf_seq.data(), cf_seq.stride(0),
                       w_out.v.data(), b_out.data(), tk.off, merged.data(), ml, stream),
@@ -190,8 +199,9 @@ inline void attention_layer(Workspace& ws, const std::string& key, View2D out, V
                             hipStream_t stream = nullptr) {
   const int D = heads * head_dim, T = tokens.extent(0);
   const pet_attn_shape sh = make_shape(tk, T, S, heads, head_dim, temperature);
+  const int saves = save_rows(tk.N, heads, S, "attention_layer");
   const View2D merged = ws.n2(key + ":merged", T, D);
-  const View2D ml = ws.n2(key + ":ml", tk.N * heads * S, 2);
+  const View2D ml = ws.n2(key + ":ml", saves, 2);
   const size_t need = pet_attention_layer_workspace(&sh);
   void* scratch = ws.bytes("attention_layer:scratch", need);
   check(pet_attention_layer(&sh, out.data(), out.stride(0), tokens.data(), tokens.stride(0), norm_w.data(),

@@ -102,6 +102,7 @@ inline void attention_layer_grads(Workspace& ws, const std::string& key, const p
                                   double temperature, hipStream_t stream = nullptr) {
   const int T = tokens.extent(0), D = heads * head_dim;
   const char* what = "attention_layer_grads";
+  const int saves = save_rows(tk.N, heads, S, what);
   check_matrix(tokens, T, D, what, "tokens are not [T, heads * head_dim]");
   check_matrix(tokens_adj, T, D, what, "tokens_adj is not [T, heads * head_dim]");
   check_matrix(out_adj, T, D, what, "out_adj is not [T, heads * head_dim]");
@@ -116,7 +117,7 @@ inline void attention_layer_grads(Workspace& ws, const std::string& key, const p
   const pet_attn_shape sh = make_shape(tk, T, S, heads, head_dim, temperature);
   const View2D merged = ws.peek2(key + ":merged"), ml = ws.peek2(key + ":ml");
   check_matrix(merged, T, D, what, "the saves under the key are of another shape");
-  check_matrix(ml, tk.N * heads * S, 2, what, "the saves under the key are of another shape");
+  check_matrix(ml, saves, 2, what, "the saves under the key are of another shape");
   const size_t bytes = pet_attention_layer_grads_workspace(&sh);
   void* scratch = ws.bytes("attention_layer_grads:scratch", bytes);
   check(pet_attention_layer_grads(&sh, &grads, tokens_adj.data(), tokens_adj.stride(0), cf_seq_adj.data(),
@@ -152,7 +153,8 @@ struct TypedAttention {
 };
 
 inline pet_attn_shape typed_shape(const TypedAttention& at, const Rows& qkv, const View2D& cf_seq, const char* what) {
-  need(qkv.cols == (at.heads + 2 * at.kv_heads) * at.head_dim, what, "qkv is not [T, (heads + 2 kv_heads) head_dim]");
+  need(at.head_dim <= 128 && qkv.cols == (int64_t(at.heads) + 2 * int64_t(at.kv_heads)) * at.head_dim, what,
+       "qkv is not [T, (heads + 2 kv_heads) head_dim] with heads of at most 128");
   need(cf_seq.extent(0) == at.tk.N && cf_seq.extent(1) >= at.S, what, "cf_seq is not [N, S] or wider");
   return make_shape(at.tk, qkv.rows, at.S, at.heads, at.head_dim, at.temperature);
 }
@@ -163,8 +165,8 @@ inline void attn_fwd_typed(const TypedAttention& at, const Rows& merged, View2D 
   const char* what = "attn_fwd_typed";
   const pet_attn_shape sh = typed_shape(at, qkv, cf_seq, what);
   check_rows(merged, qkv, what);
-  need(merged.rows == qkv.rows && merged.cols == at.heads * at.head_dim, what, "merged is not [T, heads head_dim]");
-  check_matrix(ml, at.tk.N * at.heads * at.S, 2, what, "ml is not [N heads S, 2]");
+  need(merged.rows == qkv.rows && merged.cols == int64_t(at.heads) * at.head_dim, what, "merged is not [T, heads head_dim]");
+  if (ml.data()) check_matrix(ml, save_rows(at.tk.N, at.heads, at.S, what), 2, what, "ml is not [N heads S, 2]");
   need(!ml.data() || ml.stride(0) == 2, what, "a contiguous ml is needed");
   check(pet_attn_fwd_typed(qkv.dtype, &sh, at.kv_heads, qkv.ptr, qkv.ld, at.tk.off, cf_seq.data(), cf_seq.stride(0),
                            at.bias, at.dropout, merged.ptr, merged.ld, ml.data(), stream),
@@ -182,11 +184,11 @@ inline void attn_bwd_typed(Workspace& ws, const TypedAttention& at, const Rows& 
   check_rows(merged, qkv, what);
   check_rows(dmerged, qkv, what);
   need(qkv_adj.rows == qkv.rows && qkv_adj.cols == qkv.cols, what, "qkv_adj is not of qkv's shape");
-  need(merged.rows == qkv.rows && merged.cols == at.heads * at.head_dim && dmerged.rows == qkv.rows &&
+  need(merged.rows == qkv.rows && merged.cols == int64_t(at.heads) * at.head_dim && dmerged.rows == qkv.rows &&
            dmerged.cols == merged.cols,
        what, "merged and dmerged are not [T, heads head_dim]");
   need(ml.data() && ml.stride(0) == 2, what, "a contiguous ml is needed");
-  check_matrix(ml, at.tk.N * at.heads * at.S, 2, what, "ml is not [N heads S, 2]");
+  check_matrix(ml, save_rows(at.tk.N, at.heads, at.S, what), 2, what, "ml is not [N heads S, 2]");
   need(!cf_seq_adj.data() || (cf_seq_adj.extent(0) == at.tk.N && cf_seq_adj.extent(1) >= at.S), what,
        "cf_seq_adj is not [N, S] or wider");
   need(!table_adj.data() || at.bias, what, "table_adj without a bias");

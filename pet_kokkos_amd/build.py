@@ -53,15 +53,18 @@ CPP_TEST5_SRC = os.path.join(ROOT, "tests", "cpp", "train_shapes_test.cpp")
 CPP_TEST5 = os.path.join(ROOT, "tests", "cpp", "train_shapes_test")
 CPP_TEST6_SRC = os.path.join(ROOT, "tests", "cpp", "typed_attention_test.cpp")
 CPP_TEST6 = os.path.join(ROOT, "tests", "cpp", "typed_attention_test")
+CPP_TEST7_SRC = os.path.join(ROOT, "tests", "cpp", "typed_limits_test.cpp")
+CPP_TEST7 = os.path.join(ROOT, "tests", "cpp", "typed_limits_test")
 
 
 def build_cpp_test(verbose: bool = False) -> str:
     """The C++ callers of include/pet/attention.hpp, include/pet/forces.hpp,
     include/pet/model.hpp and include/pet/train.hpp that tests/test_gpu_cpp_api.py,
-    tests/test_gpu_cpp_train.py, tests/test_gpu_cpp_typed.py, tests/test_train_args.py
-    and tests/test_typed_args.py run."""
+    tests/test_gpu_cpp_train.py, tests/test_gpu_cpp_typed.py, tests/test_train_args.py,
+    tests/test_typed_args.py and tests/test_typed_limits.py run."""
     for src, exe in ((CPP_TEST_SRC, CPP_TEST), (CPP_TEST2_SRC, CPP_TEST2), (CPP_TEST3_SRC, CPP_TEST3),
-                     (CPP_TEST4_SRC, CPP_TEST4), (CPP_TEST5_SRC, CPP_TEST5), (CPP_TEST6_SRC, CPP_TEST6)):
+                     (CPP_TEST4_SRC, CPP_TEST4), (CPP_TEST5_SRC, CPP_TEST5), (CPP_TEST6_SRC, CPP_TEST6),
+                     (CPP_TEST7_SRC, CPP_TEST7)):
         cmd = [hipcc(), "--offload-arch=gfx950", "-O2", "-std=c++17", "-I", os.path.join(ROOT, "include"),
                "-o", exe, src, "-L", HERE, "-lpet_attn", "-Wl,-rpath,$ORIGIN/../../pet_kokkos_amd"]
         if verbose:
