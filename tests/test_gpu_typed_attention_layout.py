@@ -1,0 +1,62 @@
+"""What the typed attention writes and what it leaves alone, where offsets promise more
+than there is; heads and layouts that no other test of it has."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from pet_kokkos_amd import _lib
+from pet_kokkos_amd import attention as A
+from test_gpu_typed_attention import BF16, F16, OnDevice, within
+from typed_attention import Case
+
+pytestmark = pytest.mark.gpu
+
+
+class Cut(Case):
+    """A case whose offsets are replaced: an atom's tokens are cut to the slots and the rows."""
+
+    def __init__(self, off, slots, *args, **kwargs):
+        super().__init__(*args, **kwargs)
+        self.off, self.S = np.array(off, dtype=np.int32), slots
+        self.cf = torch.ones((self.N, self.S))
+
+    def rows(self, n):
+        first, last = int(self.off[n]), int(self.off[n + 1])
+        edges = min(last - first, self.S - 1, self.T - self.N - first)
+        return [n] + ([self.N + first + i for i in range(edges)] if first >= 0 else [])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("off,counts,slots,heads,kv_heads", [
+    ([0, 9, 24, 4000], [9, 11, 5], 12, 2, 2), ([-4, 2 ** 30, 7, 7], [9, 11, 5], 12, 2, 2), ([3, 9, 9, 20], [9, 11, 5], 30, 4, 2),
+    ([0, 200, 411, 616], [200, 211, 205], 150, 2, 1), ([0, 200, 411, 4000], [200, 211, 205], 190, 2, 2),
+    ([5, 200, 380, 500], [200, 211, 205], 300, 4, 1), ([-4, 2 ** 30, 7, 7], [200, 211, 205], 212, 2, 2)])
+def test_rows_of_no_atom_are_left_as_they_were(device, dtype, off, counts, slots, heads, kv_heads):
+    """Offsets past the slots or the rows are cut, ones that are no range give an atom its own token; the rows that are
+    then no atom's, the columns beside the rows and what lies around them keep what they held, whatever the scratch holds."""
+    case = Cut(off, slots, counts, heads, kv_heads, 32, dtype, buckets=8, reach=9, p=0.1)
+    d = OnDevice(case, device, pad=5, shift=3)
+    mine = sorted(r for n in range(case.N) for r in case.rows(n))
+    assert len(set(mine)) == len(mine) < case.T
+    others = torch.ones(case.T, dtype=torch.bool)
+    others[mine] = False
+    nbytes = _lib.load().pet_attn_bwd_typed_workspace(A.DTYPES[dtype], A.shape(case.N, case.T, case.S, heads, 32), kv_heads, 8)
+    scratch = torch.full((nbytes + 512,), 255, dtype=torch.uint8, device=device)
+    d.forward(), d.backward(scratch=scratch[:nbytes])
+    assert (scratch[nbytes:] == 255).all()
+    for view in (d.merged, d.adj):
+        assert (view[others.to(device)] == 3).all()
+        whole = torch.as_strided(view, (view.shape[0], view.shape[1] + 5), (view.stride(0), 1))
+        assert torch.isnan(whole[:, view.shape[1]:]).all()
+        before = torch.as_strided(view, (3,), (1,), 0)
+        assert torch.isnan(before).all()
+    out, tol, ml, ml_tol = case.forward()
+    within(d.merged[mine], out[mine], tol[mine], "merged")
+    within(d.ml, ml, ml_tol, "ml")
+    got = {"qkv_adj": d.adj[mine], "cf_seq_adj": d.cf_adj, "bias_adj": d.table_adj}
+    for name, (ref, bound) in case.backward(d.merged.cpu()).items():
+        if name == "qkv_adj":
+            ref, bound = ref[mine], bound[mine]
+        within(got[name], ref, bound, name)
