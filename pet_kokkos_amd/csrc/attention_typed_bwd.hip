@@ -1037,29 +1037,31 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_q_kernel(Args a, Grads b, in
   }
 }
 
-// dK and dV of the parts, summed in order and rounded once: a thread has four columns of a
-// token's row. It goes by atoms and slots as the pass does, so that rows which are no atom's stay.
+// dK and dV of the parts, summed in order and rounded once: a wave has a token's row, a lane four
+// columns of it. It goes by atoms and slots as the pass does, so that rows which are no atom's stay.
 template <class T>
 __global__ __launch_bounds__(256) void typed_kv_sum_kernel(Args a, Grads b) {
-  const int width = 2 * a.Hk * a.hd, quads = (width + 3) / 4, parts = b.heads_in * b.queries_in;
-  const int64_t all = int64_t(a.N) * a.S * quads;
-  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < all; i += int64_t(gridDim.x) * 256) {
-    const int64_t slot = i / quads, n = slot / a.S;
-    const Segment seg(a, int(n));
-    const int s = int(slot - n * a.S), c = int(i - slot * quads) * 4, count = min(4, width - c);
+  const int width = 2 * a.Hk * a.hd, parts = b.heads_in * b.queries_in, lane = threadIdx.x & 63;
+  const int slots = a.N * a.S;  // (parts are of fewer than 512 blocks of slots)
+  for (int slot = int(blockIdx.x) * 4 + wave_of(); slot < slots; slot += int(gridDim.x) * 4) {
+    const int n = slot / a.S, s = slot - n * a.S;
+    const Segment seg(a, n);
     if (s >= seg.count) continue;
     const int64_t row = seg.row(s);
-    float sum[4] = {};
-    for (int p = 0; p < parts; ++p) {
-      const float* const from = b.kv + (int64_t(p) * a.T + row) * width + c;
+    T* const to = static_cast<T*>(b.adj) + row * b.lda + a.H * a.hd;
+    for (int c = 4 * lane; c < width; c += 256) {
+      const int count = min(4, width - c);
+      float sum[4] = {};
+      for (int p = 0; p < parts; ++p) {
+        const float* const from = b.kv + (int64_t(p) * a.T + row) * width + c;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (e < count) sum[e] += from[e];
+      }
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (e < count) sum[e] += from[e];
+        if (e < count) to[c + e] = T(sum[e]);
     }
-    T* const to = static_cast<T*>(b.adj) + row * b.lda + a.H * a.hd + c;
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (e < count) to[e] = T(sum[e]);
   }
 }
 
@@ -1229,8 +1231,8 @@ extern "C" int pet_attn_bwd_typed(int dtype, const pet_attn_shape* shape, int kv
           hipLaunchKernelGGL(kernel, dim3(unsigned(slots * a.Hk)), dim3(256), bytes, st, a, b, blocks);
           if (const int e = launched()) return e;
           if (parts.heads * parts.queries > 1) {
-            const int64_t quads = int64_t(a.N) * a.S * ((2 * a.Hk * a.hd + 3) / 4);
-            hipLaunchKernelGGL(typed_kv_sum_kernel<T>, dim3(unsigned(std::min<int64_t>((quads + 255) / 256, 8192))), dim3(256), 0,
+            const int64_t token_slots = int64_t(a.N) * a.S;
+            hipLaunchKernelGGL(typed_kv_sum_kernel<T>, dim3(unsigned(std::min<int64_t>((token_slots + 3) / 4, 8192))), dim3(256), 0,
                                st, a, b);
             if (const int e = launched()) return e;
           }
