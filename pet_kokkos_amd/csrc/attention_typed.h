@@ -18,6 +18,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 #include <type_traits>
@@ -395,7 +396,12 @@ struct Share {
 
 // ---- the host's half --------------------------------------------------------------
 
-
+// Slots of items of a grid (Share): `items` to a whole 8, `most` at most, and no more than
+// 2^31 threads hold of `heads` heads; 0 where not 8 fit.
+inline int grid_slots(int64_t items, int64_t most, int heads) {
+  const int64_t room = INT32_MAX / 256 / heads / 8 * 8;
+  return int(std::min({(items + 7) / 8 * 8, most, room}));
+}
 
 // Arguments that forward and backward share; fills `a`.
 int check_args(int dtype, const pet_attn_shape* sh, int kv_heads, const void* qkv, int64_t ldq, const int* off,

@@ -435,8 +435,8 @@ extern "C" int pet_attn_fwd_typed(int dtype, const pet_attn_shape* shape, int kv
         constexpr bool BIAS = decltype(bc)::value, DROP = decltype(dc)::value;
         const size_t lut = a.table ? size_t(2 * a.reach + 1) * 4 : 0;
         const int64_t qblocks = a.S <= kShort ? 1 : (int64_t(a.S) + 127) / 128;
-        const int64_t slots = std::min<int64_t>((a.N * qblocks + 7) / 8 * 8, 2048);
-        if (slots * a.H * 256 > INT32_MAX) return int(PET_ATTN_EINDEX);
+        const int slots = grid_slots(a.N * qblocks, 2048, a.H);
+        if (slots == 0) return int(PET_ATTN_EINDEX);
         if (a.S <= kShort) {
           const auto kernel = typed_fwd_short_kernel<T, HD, WHOLE, BIAS, DROP>;
           const int keys = round_up(a.S, 32);

@@ -1200,9 +1200,8 @@ extern "C" int pet_attn_bwd_typed(int dtype, const pet_attn_shape* shape, int kv
                               : a.H > a.Hk ? typed_bwd_short_kernel<T, HD, 2, true, WHOLE, BIAS, DROP>
                                            : typed_bwd_short_kernel<T, HD, 2, false, WHOLE, BIAS, DROP>;
           if (const int e = pet_attn::raise_lds(reinterpret_cast<const void*>(kernel), l.bytes)) return e;
-          const int64_t items = (int64_t(a.N) + 7) / 8 * 8;
-          slots = int(std::min<int64_t>(items, b.part ? std::clamp(4096 / a.Hk / 8 * 8, 8, kMaxSlots) : 4096));
-          if (int64_t(slots) * a.Hk * 256 > INT32_MAX) return int(PET_ATTN_EINDEX);
+          slots = grid_slots(a.N, b.part ? std::clamp(4096 / a.Hk / 8 * 8, 8, kMaxSlots) : 4096, a.Hk);
+          if (slots == 0) return int(PET_ATTN_EINDEX);
           hipLaunchKernelGGL(kernel, dim3(unsigned(slots * a.Hk)), dim3(a.S <= 16 ? 64 : a.S <= 32 ? 128 : 256), l.bytes, st, a, b,
                              l.rows, unsigned(l.stats), unsigned(l.more));
           return launched();
@@ -1223,11 +1222,11 @@ extern "C" int pet_attn_bwd_typed(int dtype, const pet_attn_shape* shape, int kv
           constexpr int KT = kKeyTiles<HD>;
           const auto kernel = typed_bwd_kv_kernel<T, HD, KT, WHOLE, BIAS, DROP>;
           const int blocks = (a.S + KT * 64 - 1) / (KT * 64);
-          const int64_t items = (int64_t(a.N) * blocks * parts.heads * parts.queries + 7) / 8 * 8;
+          const int64_t items = int64_t(a.N) * blocks * parts.heads * parts.queries;
           const size_t bytes = KvLds<HD>::bytes(a, b.part != nullptr);
           if (const int e = pet_attn::raise_lds(reinterpret_cast<const void*>(kernel), bytes)) return e;
-          slots = int(std::min<int64_t>(items, b.part ? std::clamp(2048 / a.Hk / 8 * 8, 8, kMaxSlots) : kMaxSlots));
-          if (int64_t(slots) * a.Hk * 256 > INT32_MAX) return int(PET_ATTN_EINDEX);
+          slots = grid_slots(items, b.part ? std::clamp(2048 / a.Hk / 8 * 8, 8, kMaxSlots) : kMaxSlots, a.Hk);
+          if (slots == 0) return int(PET_ATTN_EINDEX);
           hipLaunchKernelGGL(kernel, dim3(unsigned(slots * a.Hk)), dim3(256), bytes, st, a, b, blocks);
           if (const int e = launched()) return e;
           if (parts.heads * parts.queries > 1) {
@@ -1243,8 +1242,8 @@ extern "C" int pet_attn_bwd_typed(int dtype, const pet_attn_shape* shape, int kv
           const int blocks = (a.S + QT * 64 - 1) / (QT * 64);
           const size_t bytes = size_t(2 * kStage) * (2 * HD * 2 + 8) + (a.table ? size_t(2 * a.reach + 1) * 4 : 0);
           if (const int e = pet_attn::raise_lds(reinterpret_cast<const void*>(kernel), bytes)) return e;
-          const int64_t q_slots = std::min<int64_t>((int64_t(a.N) * blocks + 7) / 8 * 8, 2048);
-          if (q_slots * a.H * 256 > INT32_MAX) return int(PET_ATTN_EINDEX);
+          const int q_slots = grid_slots(int64_t(a.N) * blocks, 2048, a.H);
+          if (q_slots == 0) return int(PET_ATTN_EINDEX);
           hipLaunchKernelGGL(kernel, dim3(unsigned(q_slots * a.H)), dim3(256), bytes, st, a, b, blocks);
           return launched();
         }

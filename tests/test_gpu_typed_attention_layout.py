@@ -60,3 +60,31 @@ def test_rows_of_no_atom_are_left_as_they_were(device, dtype, off, counts, slots
         if name == "qkv_adj":
             ref, bound = ref[mine], bound[mine]
         within(got[name], ref, bound, name)
+
+
+@pytest.mark.parametrize("kv_heads", [1, 4100])
+@pytest.mark.parametrize("buckets", [0, 2])
+def test_more_heads_and_atoms_than_a_grid_holds(device, kv_heads, buckets):
+    """A workgroup goes through as many atoms more as the grid has fewer of them."""
+    OnDevice(Case([0] * 2100, 4100, kv_heads, 1, BF16, buckets=buckets, reach=buckets // 2), device).check()
+
+
+def test_more_heads_and_atoms_than_a_grid_holds_past_128_slots(device):
+    """The bits of a call are those of the calls on its halves, whose grids are whole."""
+    H, N, S = 4100, 1100, 130
+    gen = torch.Generator().manual_seed(0)
+    qkv = torch.randn(N, H + 2, generator=gen).to(BF16).to(device)
+    g = torch.randn(N, H, generator=gen).to(BF16).to(device)
+    cf = torch.zeros(N, S, device=device)
+    cf[:, 0] = 1.0
+
+    def call(at):
+        n = len(range(N)[at])
+        off = torch.zeros(n + 1, dtype=torch.int32, device=device)
+        merged, ml = A.attn_fwd_typed(qkv[at], off, cf[at], H, 1, kv_heads=1)
+        adj, cf_adj, _ = A.attn_bwd_typed(qkv[at], off, g[at], merged, ml, cf[at], H, 1, kv_heads=1,
+                                          cf_seq_adj=torch.empty(n, S, device=device))
+        return merged, adj, cf_adj
+    whole, halves = call(slice(0, N)), [call(slice(0, N // 2)), call(slice(N // 2, N))]
+    for x, *parts in zip(whole, *halves):
+        assert torch.equal(x, torch.cat(parts))
