@@ -429,7 +429,8 @@ typedef struct pet_attn_bias {
  * with V. ml (may be NULL) as pet_attn_fwd's, but (0, 0) where no token or no key is, and
  * 8-byte aligned. A key counts where cf > 0 (a NaN does not); what masked rows hold
  * reaches no result. Any alignment of an element otherwise; head_dim 1..128, any number
- * of slots. Nothing may overlap. No counterpart in the reference. */
+ * of slots. Nothing may overlap (a result at an operand's own address is refused, other
+ * overlaps are the caller's to keep from). No counterpart in the reference. */
 PET_ATTN_API int pet_attn_fwd_typed(int dtype, const pet_attn_shape* shape, int kv_heads, const void* qkv, int64_t ldq,
                                     const int* off, const float* cf_seq, int64_t ldc, const pet_attn_bias* bias,
                                     const pet_dropout* dropout, void* merged, int64_t ldm, float* ml, void* stream);
@@ -442,7 +443,8 @@ PET_ATTN_API size_t pet_attn_bwd_typed_workspace(int dtype, const pet_attn_shape
  * them, the probabilities and the mask made again: qkv_adj [T, (heads + 2 kv_heads)
  * head_dim] (dead rows zeroed when shape->dead), and onto beta times itself cf_seq_adj
  * [N, S] (may be NULL; the whole of it is written) and table_adj [n_buckets, heads]
- * (contiguous; may be NULL). dO.O is formed from merged as it was rounded. workspace
+ * (contiguous; may be NULL). dO.O is formed from merged as it was rounded. Nothing may
+ * overlap, as in the forward. workspace
  * 16-byte aligned, its contents nobody's after the call: calls that may run at once have
  * one each. */
 PET_ATTN_API int pet_attn_bwd_typed(int dtype, const pet_attn_shape* shape, int kv_heads, const void* qkv, int64_t ldq,

@@ -422,6 +422,7 @@ extern "C" int pet_attn_fwd_typed(int dtype, const pet_attn_shape* shape, int kv
   if ((a.T > 0 && !merged) || ldm < D) return PET_ATTN_EINVAL;
   if (!pet_typed::element_aligned(merged, dtype) || (reinterpret_cast<uintptr_t>(ml) & 7u) != 0) return PET_ATTN_EALIGN;
   if (a.T == 0) return PET_ATTN_OK;
+  if (merged == qkv || (ml && ml == cf_seq)) return PET_ATTN_EINVAL;  // in place
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   if (shape->dead)
     if (const int e = zero_dead(a, merged, ldm, D, st)) return e;

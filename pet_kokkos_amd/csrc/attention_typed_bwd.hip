@@ -1165,6 +1165,12 @@ extern "C" int pet_attn_bwd_typed(int dtype, const pet_attn_shape* shape, int kv
   if ((a.T > 0 && (!dmerged || !merged || !qkv_adj)) || (a.N > 0 && !ml) || ldg < D || ldm < D || lda < W)
     return PET_ATTN_EINVAL;
   if ((cf_seq_adj && ldca < a.S) || (table_adj && !bias)) return PET_ATTN_EINVAL;
+  const auto in_place = [](const void* to, std::initializer_list<const void*> from) {
+    return to && std::find(from.begin(), from.end(), to) != from.end();
+  };
+  if ((a.T > 0 && in_place(qkv_adj, {qkv, dmerged, merged})) || in_place(cf_seq_adj, {cf_seq, ml}) ||
+      in_place(table_adj, {a.table, cf_seq, ml}))
+    return PET_ATTN_EINVAL;
   if (table_adj && a.H > 1 << 20) return PET_ATTN_EINDEX;  // (threads of typed_sums_kernel)
   for (const void* p : {dmerged, merged, static_cast<const void*>(qkv_adj)})
     if (!pet_typed::element_aligned(p, dtype)) return PET_ATTN_EALIGN;
