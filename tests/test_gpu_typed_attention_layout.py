@@ -88,3 +88,36 @@ def test_more_heads_and_atoms_than_a_grid_holds_past_128_slots(device):
     whole, halves = call(slice(0, N)), [call(slice(0, N // 2)), call(slice(N // 2, N))]
     for x, *parts in zip(whole, *halves):
         assert torch.equal(x, torch.cat(parts))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("bias,p", [(False, 0.0), (True, 0.0), (False, 0.3), (True, 0.3)])
+@pytest.mark.parametrize("kv_heads", [1, 2])
+@pytest.mark.parametrize("head_dim", [72, 80, 96, 100, 128])
+def test_wide_heads_of_65_to_128_slots(device, dtype, bias, p, kv_heads, head_dim):
+    """Two tiles of keys a wave at 128 dims, with what an atom is staged from in more than one round."""
+    OnDevice(Case([64, 70, 100, 127, 3], 2, kv_heads, head_dim, dtype, seed=head_dim, buckets=20 if bias else 0,
+                  reach=40 if bias else 0, p=p, zeros=0.1, dead=2), device).check()
+
+
+@pytest.mark.parametrize("kv_heads", [1, 2])
+def test_the_most_of_a_workgroups_memory(device, kv_heads):
+    """128 slots of heads of 128, 64 buckets and a reach of 1024."""
+    case = Case([127, 20, 90], 2, kv_heads, 128, BF16, seed=4, buckets=64, reach=1024, p=0.1)
+    OnDevice(case, device).check()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("head_dim", [20, 33, 50, 16, 48, 80, 96])
+@pytest.mark.parametrize("counts", [[70, 127, 2], [140, 300]])
+def test_heads_between_the_instances(device, dtype, head_dim, counts):
+    OnDevice(Case(counts, 4, 2, head_dim, dtype, seed=head_dim, buckets=9, reach=12, p=0.2, zeros=0.1), device).check()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("heads,kv_heads,head_dim", [(4, 4, 32), (8, 2, 128), (6, 3, 20)])
+def test_many_small_molecules(device, dtype, heads, kv_heads, head_dim):
+    """More atoms of up to 16 tokens than workgroups: one wave each, grouped heads and a table in turn."""
+    rng = np.random.default_rng(5)
+    OnDevice(Case(rng.integers(3, 16, 1500), heads, kv_heads, head_dim, dtype, seed=6, buckets=9, reach=7, p=0.1, zeros=0.1,
+                  slots=16), device).check()
