@@ -184,12 +184,18 @@ __device__ __forceinline__ u4 where(bool on, const u4& x) {
   return u4{on ? x[0] : 0u, on ? x[1] : 0u, on ? x[2] : 0u, on ? x[3] : 0u};
 }
 
+__device__ __forceinline__ u4 negate_if(bool on, const u4& x) {
+  const unsigned flip = on ? 0x80008000u : 0u;
+  return x ^ u4{flip, flip, flip, flip};
+}
+
 // Columns of slots 0 .. n - 1 (n a multiple of 32), keys and values or queries and
 // adjoints, into LDS rows, zeros where the slot's weight says that it is left out: nothing
 // that a masked row holds is ever multiplied. load() sends a thread's first EACH pieces of
 // both (and of a third column, where there is one), without a branch (a piece that is not
 // wanted is of a place that is there), put() stores them and goes on with the rest.
-// take(row k, chunk, y, z): what else is made of a piece.
+// take(row k, chunk, y, z): what else is made of a piece. QUERY: queries and adjoints, the
+// adjoints of odd slots negated.
 template <class T, int HD, int EACH, bool WHOLE, bool QUERY, bool THIRD>
 struct Staged {
   static constexpr int CH = HD / 8;
@@ -223,7 +229,7 @@ struct Staged {
             const bool on = (k < seg.count) & (8 * ch < a.hd) & ((w[j] > 0.f) | (QUERY && k == 0));
             const u4 u = where(on, x[j]), v = where(on, y[j]);
             put_piece<T, HD>(xs, lds_row(k), ch, u);
-            put_piece<T, HD>(ys, lds_row(k), ch, v);
+            put_piece<T, HD>(ys, lds_row(k), ch, negate_if(QUERY && (k & 1), v));
             take(k, ch, v, where(on, z[THIRD ? j : 0]));
           }
         }
@@ -242,7 +248,7 @@ struct Staged {
           if constexpr (THIRD) q = row_chunk(zsrc + row * ldz, 8 * ch, a.hd);
         }
         put_piece<T, HD>(xs, lds_row(k), ch, u);
-        put_piece<T, HD>(ys, lds_row(k), ch, v);
+        put_piece<T, HD>(ys, lds_row(k), ch, negate_if(QUERY && (k & 1), v));
         take(k, ch, v, q);
       }
     }

@@ -80,6 +80,15 @@ __device__ __forceinline__ float scale_to(float bound, int to) {
   return power_of_two(e > 126 ? 126 : e);
 }
 
+// Elements of one register in two sums: in one, the compiler takes fp16's dot instruction for
+// them, which drops bits to one side as the matrix instruction does.
+__device__ __forceinline__ float dot8(const float (&x)[8], const float (&y)[8]) {
+  float even = 0.f, odd = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) even = fmaf(x[e], y[e], even), odd = fmaf(x[e + 1], y[e + 1], odd);
+  return even + odd;
+}
+
 // dO.O of each row and head (and |dO| and |v| where b.norms is there): a group of lanes
 // takes a head's slice, eight elements each.
 template <class T, int LG>
@@ -90,18 +99,15 @@ __global__ __launch_bounds__(256) void delta_kernel(Args a, Grads b) {
     const bool q = i < heads;
     const int64_t j = q ? i : i - heads, per = q ? a.H : a.Hk, row = j / per;
     const int h = int(j - row * per);
-    float x[8], y[8], dot = 0.f, most = 0.f, sq = 0.f;
+    float x[8], y[8] = {}, most = 0.f, sq = 0.f;
     const T* p = q ? static_cast<const T*>(b.out_adj) + row * b.ldg + h * a.hd
                    : static_cast<const T*>(a.qkv) + row * a.ldq + (a.H + a.Hk + h) * a.hd;
     pet_typed::unpack<T>(__builtin_bit_cast(u4e, row_chunk(p, 8 * l, a.hd)), x);
     if (q)
       pet_typed::unpack<T>(__builtin_bit_cast(u4e, row_chunk(static_cast<const T*>(b.out) + row * b.ldm + h * a.hd, 8 * l, a.hd)), y);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      if (q) dot = fmaf(x[e], y[e], dot);
-      most = fmaxf(most, fabsf(x[e]));
-    }
-    dot = row_sum<LG>(dot);
+    for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(x[e]));
+    const float dot = row_sum<LG>(dot8(x, y));
     if (b.norms) {
       const float to_one = scale_to(row_max<LG>(most), 1);  // (a square's exponent is twice its number's)
 #pragma unroll
@@ -180,6 +186,18 @@ template <class T>
 __device__ __forceinline__ float probability_scale(const Args& a) {
   return std::is_same<T, _Float16>::value ? scale_to(a.drop.scale, 13) : 1.f;
 }
+
+// The matrix instruction drops what lies some bits under a sum's last, towards minus infinity:
+// 2^-31 of a dP on the mean, which the sum of 10^7 pairs' dS by bucket shows (fp16, 955 atoms up
+// to 202 tokens: the table's adjoint was 1.2e-6 from float64, and is 3.6e-7). So every other
+// dP is formed of negated operands. Up to 128 slots every other query's dO is negated in LDS,
+// and its P for their product, signs that the instructions take for nothing; past them, where
+// dO comes into LDS as it is, the V of every other key, and with it the key's dS, in a lane's
+// own column, whose sums take the sign at their end.
+__device__ __forceinline__ bool negated(int c, int n) { return (c + n) & 1; }
+// dO.O of n queries, and their negatives at + negative(n) (4 further: other banks).
+__device__ __forceinline__ constexpr int negative(int n) { return n + 4; }
+__device__ __forceinline__ void put_delta(float* at, int n, int q, float x) { at[q] = x, at[negative(n) + q] = -x; }
 
 // A query's exponent: P = 2^(s - this), +inf (P = 0) for one that attends to nothing.
 __device__ __forceinline__ float exponent(const Args& a, const Grads& b, int n, int h, int s, bool live) {
@@ -387,7 +405,7 @@ __global__ __launch_bounds__(256, (kShortWaves<HD, KT, GROUP, BIAS>)) void typed
   constexpr bool HALF = std::is_same<T, _Float16>::value;
   const int lane = threadIdx.x & 63, wave = wave_of(), waves = int(blockDim.x >> 6), c = lane & 15, g = lane >> 4;
   T* const qs = reinterpret_cast<T*>(lds);  // Q's rows, then K's
-  T* const gs = qs + R * HD;                // dO's rows
+  T* const gs = qs + R * HD;                // dO's rows, every other one negated
   T* const dss = gs + R * HD;               // dS, a key's queries a row
   const int pitch = R + 8;
   float* const expo = reinterpret_cast<float*>(lds + stats);
@@ -491,12 +509,10 @@ __global__ __launch_bounds__(256, (kShortWaves<HD, KT, GROUP, BIAS>)) void typed
       float dmax = 0.f;
       staged.put(a, qs, qcols, a.ldq, gs, gcols, b.ldg, ocols, b.ldm, seg, rows,
                  [&](int k, int ch, const u4& y, const u4& o) {
-                   float u[8], v[8], dot = 0.f;
+                   float u[8], v[8];
                    pet_typed::unpack<T>(__builtin_bit_cast(u4e, y), u);
                    pet_typed::unpack<T>(__builtin_bit_cast(u4e, o), v);
-#pragma unroll
-                   for (int e = 0; e < 8; ++e) dot = fmaf(u[e], v[e], dot);
-                   dot = row_sum<CH>(dot);
+                   const float dot = row_sum<CH>(dot8(u, v));
                    if (ch == 0) delta[k] = DROP ? dot / a.drop.scale : dot;
                    if (HALF || hist) onto_magnitude(gmax, y), dmax = fmaxf(dmax, dot == dot ? fabsf(dot) : kInf);
                  });
@@ -569,8 +585,8 @@ __global__ __launch_bounds__(256, (kShortWaves<HD, KT, GROUP, BIAS>)) void typed
               if constexpr (HALF) e *= up;
               float kept = e;
               if constexpr (DROP) kept = masked(e, bits, t, r);
-              p[4 * t + r] = kept;
-              float x = fmaf(kept, dp[r], -e * d4[r]);
+              p[4 * t + r] = r & 1 ? -kept : kept;
+              float x = fmaf(kept, r & 1 ? -dp[r] : dp[r], -e * d4[r]);
               if constexpr (HALF) x *= down;
               ds[4 * t + r] = x;
               cf_sum += x;
@@ -641,7 +657,7 @@ __global__ __launch_bounds__(256, (kShortWaves<HD, KT, GROUP, BIAS>)) void typed
 
 template <int HD>
 struct KvLds {
-  static constexpr size_t rows = size_t(4) * kStage * HD * 2, queries = rows + size_t(2 * kStage) * 12,
+  static constexpr size_t rows = size_t(4) * kStage * HD * 2, queries = rows + size_t(2 * kStage) * 8 + size_t(4) * negative(kStage) * 4,
                           waves = queries + 4 * 64;  // masks
   // + the bias's entries, the buckets' columns
   static size_t bytes(const Args& a, bool hist) {
@@ -666,7 +682,7 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, i
   T* const staged = reinterpret_cast<T*>(lds);  // two stages, each Q's rows and dO's
   float* const expos = reinterpret_cast<float*>(staged + 4 * kStage * HD);
   float* const deltas = expos + 2 * kStage;
-  int* const positions = reinterpret_cast<int*>(deltas + 2 * kStage);
+  int* const positions = reinterpret_cast<int*>(deltas + 4 * negative(kStage));
   unsigned char* const exchange = reinterpret_cast<unsigned char*>(positions + 2 * kStage) + 64 * wave;
   BiasEntry* const lut = reinterpret_cast<BiasEntry*>(positions + 2 * kStage + 64);
   int64_t* const columns = reinterpret_cast<int64_t*>(lut + (BIAS ? 2 * a.reach + 1 : 0));
@@ -699,6 +715,8 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, i
     const int q_each = round_up((seg.count + b.queries_in - 1) / b.queries_in, kStage);
     const int q_first = min(qi * q_each, seg.count), q_last = min(q_first + q_each, seg.count);
     const float sc = adjoint_scale<T>(a, b, n, hk * G, G), back = 1.f / sc, down = sc / up;
+    const bool minus = negated(c, n);
+    const float sign = minus ? -1.f : 1.f;
     const int k0 = kb * per + wave * KT * 16;
     u4 kf[KT][DS], vf[KT][DS];
     f4 dk[KT][DT], dv[KT][DT];
@@ -714,6 +732,8 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, i
       own_pieces<T, WHOLE>(a, vcols, a.ldq, seg, s, lane, vf[kt]);
       own_live(a, klive[kt], lane, kf[kt]);
       own_live(a, klive[kt], lane, vf[kt]);
+#pragma unroll
+      for (int d = 0; d < DS; ++d) vf[kt][d] = negate_if(minus, vf[kt][d]);
       weight[kt] = klive[kt] ? log_weight(seg.cf(a, s)) : -kInf;
       if constexpr (BIAS) kpos[kt] = a.pos[row];
 #pragma unroll
@@ -746,14 +766,14 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, i
           const int q = to * kStage + int(threadIdx.x);
           // P is scaled by 1 / (1 - p) with its exponent
           expos[q] = DROP ? log2f(a.drop.scale) - next_expo : -next_expo;
-          deltas[q] = DROP ? next_delta / a.drop.scale : next_delta;
+          put_delta(deltas + to * 2 * negative(kStage), kStage, int(threadIdx.x), DROP ? next_delta / a.drop.scale : next_delta);
           if constexpr (BIAS) positions[q] = next_pos;
         }
         stage_barrier();
       };
       stage_barrier();  // (the stages and the bias of the head before are done with)
       if (hist) cols.fit(uniform(b.bounds[int64_t(n) * a.H + h]), 36, a.nb, sums + i * a.nb);
-      const float counts = cols.units * back;
+      const float counts = sign * cols.units * back;
       if (BIAS && G > 1) bias_entries(a, lut, h);
       if (q_first < q_last) start(q_first, 0), land(q_first, 0);
       int at_stage = 0;
@@ -762,7 +782,7 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, i
         const bool more = q0 + kStage < q_last;
         if (more) start(q0 + kStage, at_stage ^ 1);
         const T *const qs = staged + at_stage * 2 * kStage * HD, *const gs = qs + kStage * HD;
-        const float *const expo = expos + at_stage * kStage, *const delta = deltas + at_stage * kStage;
+        const float *const expo = expos + at_stage * kStage, *const delta = deltas + at_stage * 2 * negative(kStage) + (minus ? negative(kStage) : 0);
         const int* const qpos = positions + at_stage * kStage;
         float part_sum[KT] = {};
         for (int qb = 0; qb < n_queries && k0 < seg.count; qb += 32) {
@@ -855,7 +875,7 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, i
       }
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt) {
-        const float sum = pet_attn::sum_g(cf_sum[kt]) * back;
+        const float sum = pet_attn::sum_g(cf_sum[kt]) * sign * back;
         const int s = k0 + 16 * kt + c;
         if (b.cfh && g == 0 && s < seg.count) b.cfh[((int64_t(qi) * a.N + n) * a.H + h) * a.S + s] = sum;
       }
@@ -872,10 +892,10 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, i
         if (!klive[kt]) dk[kt][j] = dv[kt][j] = f4{0.f, 0.f, 0.f, 0.f};
         const int d = 16 * j + 4 * g;
         if (parts > 1) {
-          put4<WHOLE>(sums_row, dk[kt][j], a.scale * back, d, a.hd);
+          put4<WHOLE>(sums_row, dk[kt][j], sign * a.scale * back, d, a.hd);
           put4<WHOLE>(sums_row + a.Hk * a.hd, dv[kt][j], 1.f / up, d, a.hd);
         } else {
-          put4<WHOLE>(row + (a.H + hk) * a.hd, dk[kt][j], a.scale * back, d, a.hd);
+          put4<WHOLE>(row + (a.H + hk) * a.hd, dk[kt][j], sign * a.scale * back, d, a.hd);
           put4<WHOLE>(row + (a.H + a.Hk + hk) * a.hd, dv[kt][j], 1.f / up, d, a.hd);
         }
       }

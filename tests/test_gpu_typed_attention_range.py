@@ -10,6 +10,7 @@ import numpy as np
 import pytest
 import torch
 
+from pet_kokkos_amd import attention as A
 from test_gpu_typed_attention import BF16, F16, OnDevice, within
 from typed_attention import U, Case, half
 
@@ -199,3 +200,42 @@ def test_what_is_not_finite_stays_in_its_head_and_buckets(device, dtype, bad, wh
     some = check_table(OnDevice(case, device), what)
     gone = heads // kv_heads if what == "value" else 1
     assert int((~some).sum()) == gone and not some[4, head]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("atoms,tokens", [(10000, 128), (600, 512)])
+def test_the_products_roundings_do_not_add_up(device, dtype, atoms, tokens):
+    """1.6e8 pairs of one bucket. Logits are 0, so P is 1 / tokens, a power of two, and exact. Of hd products each dP
+    has at most hd roundings of at most U of its magnitudes' sum; with none of them favoured, their square is a third
+    of that on the mean, and so is that of dO.O's, of dS's own (U of itself) and a unit's half: 6 of their deviations. (The
+    atoms' bounds are within 2 of each other, so a unit is at most twice the fitting one.)"""
+    hd = 32
+    gen = torch.Generator(device).manual_seed(0)
+    T, edges = atoms * tokens, tokens - 1
+    qkv = torch.zeros(T, 3 * hd, dtype=dtype, device=device)
+    qkv[:, 2 * hd:] = (torch.randn(T, hd, generator=gen, device=device).clamp(-3, 3) * 0.7).to(dtype)
+    g = (torch.randn(T, hd, generator=gen, device=device).clamp(-3, 3) * 0.05).to(dtype)
+    off = torch.arange(atoms + 1, dtype=torch.int32, device=device) * edges
+    cf = torch.ones(atoms, tokens, device=device)
+    bias = A.RelativeBias(torch.zeros(1, 1, device=device), torch.zeros(1, dtype=torch.int32, device=device),
+                          torch.zeros(T, dtype=torch.int32, device=device))
+    merged, ml = A.attn_fwd_typed(qkv, off, cf, 1, hd, bias=bias)
+    assert (ml[:, 1] == 1 / tokens).all() and (ml[:, 0] == 0).all()
+    table = torch.zeros(1, 1, device=device)
+    A.attn_bwd_typed(qkv, off, g, merged, ml, cf, 1, hd, bias=bias, bias_adj=table)
+
+    def by_atom(x):  # [atoms, tokens, hd]
+        return torch.cat([x[:atoms, None], x[atoms:].view(atoms, edges, hd)], 1).double()
+    v, do, o = (by_atom(x) for x in (qkv[:, 2 * hd:], g, merged))
+    d, d_mag = (do * o).sum(-1), (do * o).abs().sum(-1)
+    ref = ((do * v.sum(1, keepdim=True)).sum(-1) / tokens - d).sum()
+
+    def squares(x, y):  # of x_i.y_j over all pairs of an atom
+        return (torch.bmm(x.transpose(1, 2).contiguous(), x) * torch.bmm(y.transpose(1, 2).contiguous(), y)).sum()
+    bound = (hd * do.abs().amax((1, 2)) * v.abs().amax((1, 2)) + d.abs().amax(1))
+    assert float(bound.max()) <= 2 * float(bound.min())
+    unit = bound.max() * 2.0 ** (-32 if tokens <= 128 else -35)
+    variance = ((hd / 3) * U ** 2 * squares(do.abs(), v.abs()) + 2 * U ** 2 * (squares(do, v) + tokens * (d ** 2).sum())) / tokens ** 2 \
+        + (hd / 3) * U ** 2 * (d_mag ** 2).sum() + atoms * tokens ** 2 * unit ** 2 / 12
+    error = float(table.double()[0, 0] - ref)
+    assert abs(error) <= 6 * math.sqrt(float(variance)) + U * abs(float(ref)), (error, math.sqrt(float(variance)), float(ref))
