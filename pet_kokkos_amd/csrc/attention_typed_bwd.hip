@@ -270,13 +270,18 @@ struct Columns {
   __device__ __forceinline__ void clear(int nb) {
     for (int i = threadIdx.x; i < nb * kColumns; i += blockDim.x) at[i] = 0;
   }
-  // For dS under a bound (one for the workgroup); sums: what a flush adds to.
-  __device__ __forceinline__ void fit(float bound, int to, int nb, double* sums) {
+  // For dS under a bound (one for the workgroup), brought to 2^TO .. ; sums: what a flush adds to.
+  template <int TO>
+  __device__ __forceinline__ void fit(float bound, int nb, double* sums) {
+    constexpr float most = float(uint64_t(1) << (TO + 2)), least = float(uint64_t(1) << (TO - 6));
+    const float counted = bound * units;
+    if (!real && counted >= least && counted < most) return;
     const bool over = !(bound < kInf);
     if (!over && !(bound > 0.f)) return;  // (every dS is 0)
-    const float one = over ? 1.f : scale_to(bound, to);
-    if (units > 0.f && (real != over || units >= 4.f * one || one > 64.f * units)) flush(nb, sums);
-    if (units == 0.f) units = one, real = over;
+    const float one = over ? 1.f : scale_to(bound, TO);
+    if (one == units && real == over) return;
+    if (units > 0.f) flush(nb, sums);
+    units = one, real = over;
   }
   // x: four of a lane's dS in units, onto the buckets whose first columns are at column (bytes).
   __device__ __forceinline__ void count(const int (&column)[4], const float (&x)[4]) const {
@@ -329,16 +334,18 @@ struct Columns {
   __device__ __forceinline__ void flush(int nb, double* sums) {
     __syncthreads();
     for (int k = threadIdx.x; k < nb && units > 0.f; k += blockDim.x) {
-      int64_t sum = 0;
-      double float_sum = 0.0;
+      int64_t whole = 0;
+      double sum = 0.0;
+#pragma unroll 4
       for (int l = 0; l < kColumns; ++l) {
         int64_t* const column = at + k * kColumns + ((l + k) & (kColumns - 1));
-        if (real) float_sum += __builtin_bit_cast(double, *column); else sum += *column;
+        const int64_t x = *column;
         *column = 0;
+        if (real) sum += __builtin_bit_cast(double, x); else whole += x;
       }
-      sums[k] += real ? float_sum : double(sum) / double(units);
+      if (!real) sum = double(whole) * double(1.f / units);
+      sums[k] += sum;
     }
-    units = 0.f, real = false;
     __syncthreads();
   }
 };
@@ -531,7 +538,7 @@ __global__ __launch_bounds__(256, (kShortWaves<HD, KT, GROUP, BIAS>)) void typed
 #pragma unroll
           for (int k = 0; k < 3; ++k) m[k] = fmaxf(m[k], room[3 * w + k]);
         const float bound = uniform(float(a.hd) * m[0] * m[1] * a.drop.scale + m[2]);
-        if (hist) cols.fit(bound, 33, a.nb, sums + i * a.nb);
+        if (hist) cols.fit<33>(bound, a.nb, sums + i * a.nb);
         if constexpr (HALF) {
           const float was = sc;
           sc = scale_to(bound, 14);
@@ -772,7 +779,7 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, i
         stage_barrier();
       };
       stage_barrier();  // (the stages and the bias of the head before are done with)
-      if (hist) cols.fit(uniform(b.bounds[int64_t(n) * a.H + h]), 36, a.nb, sums + i * a.nb);
+      if (hist) cols.fit<36>(uniform(b.bounds[int64_t(n) * a.H + h]), a.nb, sums + i * a.nb);
       const float counts = sign * cols.units * back;
       if (BIAS && G > 1) bias_entries(a, lut, h);
       if (q_first < q_last) start(q_first, 0), land(q_first, 0);
