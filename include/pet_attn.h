@@ -443,8 +443,14 @@ PET_ATTN_API size_t pet_attn_bwd_typed_workspace(int dtype, const pet_attn_shape
  * them, the probabilities and the mask made again: qkv_adj [T, (heads + 2 kv_heads)
  * head_dim] (dead rows zeroed when shape->dead), and onto beta times itself cf_seq_adj
  * [N, S] (may be NULL; the whole of it is written) and table_adj [n_buckets, heads]
- * (contiguous; may be NULL). dO.O is formed from merged as it was rounded. Nothing may
- * overlap, as in the forward. workspace
+ * (contiguous; may be NULL). dO.O is formed from merged as it was rounded. The probabilities
+ * for dV and the adjoints of the logits for dQ and dK are rounded to the type; in fp16 both
+ * are first scaled by powers of two, the adjoints for the largest of an atom and a key head's
+ * group, which an adjoint or value there that is not finite leaves unscaled. cf_seq_adj and
+ * table_adj are of the unrounded ones: the table's are summed in whole numbers of 2^-27 or
+ * less (past 128 slots 2^-30) of a bound of an atom's and head's, or in float64 where no such
+ * bound is in fp32's range. One that is not finite reaches its own bucket and head alone.
+ * Nothing may overlap, as in the forward. workspace
  * 16-byte aligned, its contents nobody's after the call: calls that may run at once have
  * one each. */
 PET_ATTN_API int pet_attn_bwd_typed(int dtype, const pet_attn_shape* shape, int kv_heads, const void* qkv, int64_t ldq,

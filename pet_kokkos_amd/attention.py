@@ -392,8 +392,8 @@ def attn_bwd_typed(qkv: torch.Tensor, off: torch.Tensor, dmerged: torch.Tensor, 
                    scratch: torch.Tensor | None = None):
     """attn_fwd_typed's backward from the adjoint of merged, merged and ml as it left
     them and its bias and dropout: qkv_adj [T, (heads + 2 kv_heads) * head_dim], and
-    where given, each onto beta times itself, cf_seq_adj [N, S] and bias_adj (the bias
-    table's shape, float32). ``scratch``: pet_attn_bwd_typed_workspace bytes, else
+    where given, each onto beta times itself (0: overwritten, where attn_bwd accumulates),
+    cf_seq_adj [N, S] and bias_adj (the bias table's shape, float32). ``scratch``: pet_attn_bwd_typed_workspace bytes, else
     allocated. Returns (qkv_adj, cf_seq_adj, bias_adj)."""
     sh, kv_heads, ldq, ldc = _typed_call(qkv, off, cf_seq, heads, head_dim, kv_heads, temperature, dead, N)
     dev, dt, T, D, S = qkv.device, qkv.dtype, qkv.shape[0], heads * head_dim, cf_seq.shape[1]

@@ -199,7 +199,8 @@ struct Tiles {
 #pragma unroll
         for (int j = 0; j < DT; ++j) {
           if (!some) o[qt][j] = f4{0.f, 0.f, 0.f, 0.f};
-          // (at 64 dims with a bias and dropout the short way moved the stores: 711 -> 787 us; at 32, 67 -> 64)
+          // (at 64 dims with a bias and dropout the short way moved the stores, 711 -> 787 us; at 32 dims it
+          // took 69 -> 66; past 128 slots at 128 it made no difference)
           put4<WHOLE && HD == 32>(to, o[qt][j], f, 16 * j + 4 * g, a.hd);
         }
       }
@@ -216,10 +217,12 @@ __device__ __forceinline__ void fill_lut(const Args& a, float* lut, int h) {
 // queries dealt to the workgroup's waves (4 from 33 slots on: a workgroup's waves start
 // at one SIMD, and 5 of them, one a tile of 71 slots, left room for no third workgroup
 // on the CU; which wave has the odd tile goes round by the atom). 1728 atoms of 71
-// tokens, 8 heads of 32, bf16: 64 us, 4.0 TB/s of Q, K, V and the result, each moved once
-// (a copy reaches 5.0); 11392 of 32 to 71, 8 heads of 64, with bias and dropout: 711 us,
-// 3.4 TB/s, bound by the exponentials, the bias and the random numbers.
-// Three waves a SIMD where four would spill.
+// tokens, 8 heads of 32, bf16: 66 us, 3.9 TB/s of Q, K, V and the result, each moved once
+// (a copy reaches 5.0), the vector unit issuing 98% of the time; 11392 of 32 to 71, 8 heads of
+// 64, with bias and dropout: 712 us, 3.4 TB/s, the vector unit (exponentials, the bias, the
+// random numbers) 77%.
+// Four waves a SIMD up to 64 dims (with dropout 64 take 24 bytes of scratch a lane); with bias
+// and dropout 64 are compiled for three, which runs the batch in 712 us where four takes 724.
 template <int HD, bool BIAS, bool DROP>
 constexpr int kFwdWaves = HD == 128 ? 2 : HD == 64 && BIAS && DROP ? 3 : 4;
 template <class T, int HD, bool WHOLE, bool BIAS, bool DROP>
@@ -278,7 +281,7 @@ __global__ __launch_bounds__(256, (kFwdWaves<HD, BIAS, DROP>)) void typed_fwd_sh
 // stages, the next one's loads on their way into LDS while the present one is used. Two
 // atoms of 3500 to 4096 tokens, 8 heads of 128 over 2, with a bias: 190 us, 650 TFLOP/s
 // (a library's large product: 1143); the exponentials and the bias' gathers stand between
-// the products. Two tiles a wave share each read of K and V.
+// the products (vector unit 61%, matrix unit 27% of the time). Two tiles a wave share each read of K and V.
 template <class T, int HD, bool WHOLE, bool BIAS, bool DROP>
 __global__ __launch_bounds__(256, 2) void typed_fwd_long_kernel(Args a, int qblocks, T* merged, int64_t ldm, float* ml) {
   extern __shared__ __align__(16) char lds[];

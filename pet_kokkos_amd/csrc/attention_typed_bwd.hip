@@ -5,10 +5,10 @@
 //   dcf_j = sum over heads and i of dS_ij / cf_j,   dtable[b][h] = sum over pairs in bucket b of dS_ij.
 // Keys and values shared by a group of heads sum over it.
 //
-// Nothing is atomic across lanes and every sum has one owner and a fixed order, so
-// results repeat bit for bit: the bias table's gradient goes through a column of LDS
-// of each lane's own (a bucket a row: the lanes' additions never meet, nor do their
-// banks), the columns are summed in order, and so are the workgroups' sums.
+// Results repeat bit for bit. Sums of floats have one owner and a fixed order. The bias
+// table's gradient is summed in LDS by the workgroup's waves at once, 32 columns a bucket,
+// with 64-bit atomic additions of whole numbers, which give one sum in any order
+// (Columns); the columns and then the workgroups' sums are added in order, in float64.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -395,11 +395,14 @@ __device__ __forceinline__ float magnitude(unsigned m) {
 // transposed for dQ^T += K^T dS^T, a tile of queries a wave: every product is formed once,
 // where the two passes past 128 slots form S, dP and their exponentials twice. dS is rounded
 // to the row type for its products with Q and K, as P is for its with dO: the operands'
-// type. 1728 atoms of 71 tokens, 8 heads of 32, bf16: 135 us (209 in two passes' kernels with
-// all sums kept), 3.9 TB/s of what is moved once; 11392 of 32 to 71, 8 heads of 64, with bias,
-// its gradient and dropout: 2000 us, the vector unit half busy, waves waiting half of their
-// time at two a SIMD, which registers bound.
-// Two waves a SIMD where three would spill.
+// type. 1728 atoms of 71 tokens, 8 heads of 32, bf16: 137 us (209 in two passes' kernels with
+// all sums kept), 3.8 TB/s of what is moved once, the vector unit busy two thirds of it; 11392
+// of 32 to 71, 8 heads of 64, with bias, its gradient and dropout: 2030 us, the vector unit half
+// busy, waves waiting half of their time at two a SIMD, which registers bound.
+// Two waves a SIMD, or three where that takes little or no scratch: with dropout 64 dims take 72
+// to 108 bytes a lane at three, 32 dims in groups 72 to 104. At 128 dims, and in groups at 64,
+// two take scratch as well: 156 to 356 bytes, in groups past 64 slots 84 to 200 at 64 dims and
+// 1116 to 1516 at 128, some of it in the pairs' loop.
 template <int HD, int KT, bool GROUP, bool BIAS>
 constexpr int kShortWaves =
     HD == 128 || (KT == 2 && GROUP && (HD == 64 || BIAS)) || (HD == 64 && (BIAS || KT == 1)) ? 2 : 3;
@@ -676,9 +679,9 @@ struct KvLds {
 // as B operands, dK^T and dV^T in registers, and goes over all queries of the group's
 // heads, staged in LDS: S = Q K^T and dP = dO V^T with a lane's key in its column, so P
 // and dS are the B operands of dV^T += dO^T P and dK^T += Q^T dS as they lie. Two atoms
-// of 3500 to 4096 tokens, 8 heads of 128 over 2, with a bias and its gradient: 537 us, 460
+// of 3500 to 4096 tokens, 8 heads of 128 over 2, with a bias and its gradient: 535 us, 460
 // TFLOP/s of its four products. LDS is busy 44% of that (each wave reads Q and dO twice for
-// 16 keys), the vector unit 37%. Two tiles of keys a wave there halve the reads and leave one
+// 16 keys), the vector unit 42%. Two tiles of keys a wave there halve the reads and leave one
 // wave a SIMD: 647 us against 551.
 template <class T, int HD, int KT, bool WHOLE, bool BIAS, bool DROP>
 __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, int kblocks) {
@@ -913,7 +916,8 @@ __global__ __launch_bounds__(256, 2) void typed_bwd_kv_kernel(Args a, Grads b, i
 
 // dQ: a wave has QT tiles of 16 queries as B operands and goes over the keys: S^T and
 // dP^T with a lane's query in its column, dS^T the B operand of dQ^T += K^T dS^T. The same
-// case: 285 us, 650 TFLOP/s of its three products, the exponentials between them.
+// case: 285 us, 650 TFLOP/s of its three products, the exponentials between them (the vector
+// unit is busy 45% of it, the matrix unit 30%).
 template <class T, int HD, int QT, bool WHOLE, bool BIAS, bool DROP>
 __global__ __launch_bounds__(256, 2) void typed_bwd_q_kernel(Args a, Grads b, int qblocks) {
   extern __shared__ __align__(16) char lds[];
